@@ -389,6 +389,68 @@ int mnv_lrn_bwd(const float* bottom, const float* top, const float* scale, const
                 float* bottom_diff, int local_size, float alpha, float beta, int num_images,
                 int num_channels, int height, int width, mnv_stream_t stream);
 
+/* ---- layer norm (no counterpart in the reference, whose only normalisation is the LRN above).
+ * x, y, dy, dx {features, count}; gamma, beta, dgamma, dbeta {features}.  Over each of the `count`
+ * columns, with mean and var = mean((x - mean)^2) of its values:
+ *   xh = (x - mean) / sqrt(var + eps),  y = gamma * xh + beta
+ *   dx = (g - mean(g) - xh * mean(g * xh)) / sqrt(var + eps),  g = gamma * dy
+ *   dgamma = sum over the columns of dy * xh,  dbeta = sum over the columns of dy
+ * eps is finite and not negative.  backward works from x alone (nothing of the forward pass is kept).
+ * Its workspace holds partial sums over columns; with less of it, or none, fewer workgroups run.
+ * The results' bits depend on the sizes, the workspace's size and 16-byte alignment alone. ---- */
+int mnv_layernorm_fwd(const float* x, const float* gamma, const float* beta, float* y, int features,
+                      int count, float eps, mnv_stream_t stream);
+size_t mnv_layernorm_bwd_workspace_bytes(int features, int count);
+int mnv_layernorm_bwd(const float* x, const float* gamma, const float* dy, float* dx, float* dgamma,
+                      float* dbeta, int features, int count, float eps, void* workspace,
+                      size_t workspace_bytes, mnv_stream_t stream);
+
+/* ---- attention of queries to the states of another sequence, or their own (no counterpart in
+ * the reference).  q, out, dout, dq {head_dim, heads, q_len, batch}; k, v, dk, dv {head_dim, kv_heads,
+ * k_len, batch}: head h reads the keys of head h / (heads / kv_heads); head_dim is 1 to 128.
+ *   t_ij = scale * q_i.k_j + bias[j - i + q_len - 1]   for the keys j < lengths[b]
+ *   m_i = max t_ij,  l_i = sum exp(t_ij - m_i),  out_i = sum exp(t_ij - m_i) / l_i * v_j
+ * bias {q_len + k_len - 1, heads}, one value per offset between key and query, or NULL; -inf hides
+ * an offset.  lengths {batch}: whole numbers as floats (from 0 to k_len; others are cut to that, NaN to 0),
+ * or NULL for k_len everywhere; keys from there on are not read.  A query that sees no key
+ * has out 0, m -inf, l 0 and no part in any gradient.  stats {2, heads, q_len, batch}
+ * receives (m, l); backward reads `out` and `stats` as forward wrote them:
+ *   p_ij = exp(t_ij - m_i) / l_i,  ds_ij = p_ij * (dout_i.v_j - dout_i.out_i)
+ *   dq_i = scale * sum_j ds_ij k_j,  dk_j = scale * sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
+ *   dbias[o] = sum of ds_ij with j - i + q_len - 1 = o over the batch
+ * dk and dv sum over the heads that share a key, and are 0 for keys that are not read; dbias is
+ * written unless `bias` is NULL (then dbias is ignored).  An infinity or a NaN among the values that are read
+ * gives NaN where it has a part.  forward's workspace holds the parts of a key range that few
+ * queries are spread over; backward's (`has_bias`: with the bias's gradient) partial sums. ---- */
+size_t mnv_attention_fwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len,
+                                         int head_dim);
+int mnv_attention_fwd(const float* q, const float* k, const float* v, const float* bias,
+                      const float* lengths, float* out, float* stats, int batch, int heads,
+                      int kv_heads, int q_len, int k_len, int head_dim, float scale, void* workspace,
+                      size_t workspace_bytes, mnv_stream_t stream);
+size_t mnv_attention_bwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len,
+                                         int head_dim, int has_bias);
+int mnv_attention_bwd(const float* q, const float* k, const float* v, const float* bias,
+                      const float* lengths, const float* out, const float* stats, const float* dout,
+                      float* dq, float* dk, float* dv, float* dbias, int batch, int heads,
+                      int kv_heads, int q_len, int k_len, int head_dim, float scale, void* workspace,
+                      size_t workspace_bytes, mnv_stream_t stream);
+
+/* ---- learned relative position bias by buckets: the `bias` of the attention above, and its
+ * table's gradient.  table, dtable {heads, buckets}; bias, dbias {q_len + k_len - 1, heads}.
+ * Query i stands at position q_start + i, key j at j:  r = j - i - q_start, and
+ *   bias[j - i + q_len - 1] = table[bucket(r)],  dtable[u] = sum of dbias over the offsets of bucket u.
+ * With n = |r| and c = buckets / 2 (both_ways), r > 0 in the second half of the buckets, or
+ * n = max(0, -r) and c = buckets:  of c buckets the first e = c / 2 (rounded down) hold one distance n each, and the
+ * others the distances from e on, bucket e + u from  e * (max_distance / e)^(u / (c - e))  on; the last
+ * has all that are farther.  buckets is 2 to 256 (both_ways: even, from 4), max_distance above e,
+ * |q_start| at most 2^30.  A bucket without an offset has gradient 0. ---- */
+int mnv_relative_bias_fwd(const float* table, float* bias, int buckets, int heads, int q_len, int k_len,
+                          int q_start, int max_distance, int both_ways, mnv_stream_t stream);
+int mnv_relative_bias_bwd(const float* dbias, float* dtable, int buckets, int heads, int q_len,
+                          int k_len, int q_start, int max_distance, int both_ways,
+                          mnv_stream_t stream);
+
 /* ---- Concat / Slice / Select data movement (reference cuda.cpp:80-155, 644-655).
  * The reference builds Concat and Slice from one CudaPerformCopy (cuda_perform.h:20) per
  * image; here one 2-D copy per input tensor does it: `rows` rows of `row_elems` floats,

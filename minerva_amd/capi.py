@@ -113,6 +113,15 @@ PROTOTYPES["mnv_randn"] = [_P, c_sz, ctypes.c_uint64, c_f, c_f, _S]
 PROTOTYPES["mnv_rand_bernoulli"] = [_P, c_sz, ctypes.c_uint64, c_f, _S]
 PROTOTYPES["mnv_lrn_fwd"] = [_P, _P, _P, _I, c_f, c_f, _I, _I, _I, _I, _S]
 PROTOTYPES["mnv_lrn_bwd"] = [_P, _P, _P, _P, _P, _I, c_f, c_f, _I, _I, _I, _I, _S]
+PROTOTYPES["mnv_layernorm_fwd"] = [_P] * 4 + [_I, _I, c_f, _S]
+PROTOTYPES["mnv_layernorm_bwd_workspace_bytes"] = [_I, _I]
+PROTOTYPES["mnv_layernorm_bwd"] = [_P] * 6 + [_I, _I, c_f, _P, c_sz, _S]
+PROTOTYPES["mnv_attention_fwd_workspace_bytes"] = [_I] * 6
+PROTOTYPES["mnv_attention_fwd"] = [_P] * 7 + [_I] * 6 + [c_f, _P, c_sz, _S]
+PROTOTYPES["mnv_attention_bwd_workspace_bytes"] = [_I] * 7
+PROTOTYPES["mnv_attention_bwd"] = [_P] * 12 + [_I] * 6 + [c_f, _P, c_sz, _S]
+PROTOTYPES["mnv_relative_bias_fwd"] = [_P, _P] + [_I] * 7 + [_S]
+PROTOTYPES["mnv_relative_bias_bwd"] = [_P, _P] + [_I] * 7 + [_S]
 
 _RESTYPES = {
     "mnv_error_string": ctypes.c_char_p,
@@ -122,6 +131,9 @@ _RESTYPES = {
     "mnv_conv_bwd_data_workspace_bytes": c_sz,
     "mnv_conv_bwd_bias_workspace_bytes": c_sz,
     "mnv_select_workspace_bytes": c_sz,
+    "mnv_layernorm_bwd_workspace_bytes": c_sz,
+    "mnv_attention_fwd_workspace_bytes": c_sz,
+    "mnv_attention_bwd_workspace_bytes": c_sz,
 }
 
 
