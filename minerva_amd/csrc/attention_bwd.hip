@@ -6,26 +6,9 @@
 //   dbias[o] = sum of ds_ij with j - i + q_len - 1 = o
 // A row that sees no key has m = -inf, l = 0, out = 0.  The pair (m, l) is kept and not m + ln l: where the bias is the
 // type's lowest value for a whole row, ln l would be lost in the sum.
-#include <math.h>
-
-#include "mnv_common.h"
+#include "attention_core.h"
 
 namespace {
-
-#define MNV_AT_MAX_DIM 128
-
-struct AttentionSizes {
-  int batch, heads, kv_heads, q_len, k_len, dim;
-  float scale;
-};
-
-// Keys of entry b that are read.
-__device__ __forceinline__ int visible(const float* lengths, int b, int k_len) {
-  if (!lengths) return k_len;
-  const float n = lengths[b];
-  if (!(n > 0.f)) return 0;
-  return n >= (float)k_len ? k_len : (int)n;
-}
 
 __device__ __forceinline__ size_t q_row(const AttentionSizes& z, int b, int i, int h) {
   return ((size_t)b * z.q_len + i) * z.heads + h;
@@ -48,47 +31,6 @@ __device__ __forceinline__ float score(const AttentionSizes& z, const float* q, 
 
 // exp(t - m), and 0 for a hidden t = -inf where hidden ones alone leave m at -inf too
 __device__ __forceinline__ float weight(float t, float m) { return expf(t - (m == -INFINITY ? 0.f : m)); }
-// 1 / l, and 0 for a row that sees no key
-__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
-
-// One wavefront per query: its lanes take a key each, then a value of the result each.
-__global__ __launch_bounds__(MNV_WAVE) void mnv_attention_fwd_kernel(const float* __restrict__ q,
-                                                                     const float* __restrict__ k,
-                                                                     const float* __restrict__ v,
-                                                                     const float* __restrict__ bias,
-                                                                     const float* __restrict__ lengths,
-                                                                     float* __restrict__ out, float* __restrict__ stats,
-                                                                     AttentionSizes z) {
-  const int lane = threadIdx.x;
-  const size_t rows = (size_t)z.batch * z.q_len * z.heads;
-  for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int h = (int)(row % z.heads), i = (int)(row / z.heads % z.q_len), b = (int)(row / z.heads / z.q_len);
-    const int kh = h / (z.heads / z.kv_heads), n = visible(lengths, b, z.k_len);
-    const float* qi = q + row * z.dim;
-    float m = -INFINITY;
-    for (int j = lane; j < n; j += MNV_WAVE) m = fmaxf(m, score(z, qi, k + k_row(z, b, j, kh) * z.dim, bias, h, i, j));
-    m = __shfl(mnv_wave_max(m), 0, MNV_WAVE);
-    float l = 0.f;
-    for (int j = lane; j < n; j += MNV_WAVE) l += weight(score(z, qi, k + k_row(z, b, j, kh) * z.dim, bias, h, i, j), m);
-    l = __shfl(mnv_wave_sum(l), 0, MNV_WAVE);
-    float acc[2] = {0.f, 0.f};
-    for (int j0 = 0; j0 < n; j0 += MNV_WAVE) {
-      const int j = j0 + lane;
-      const float p = j < n ? weight(score(z, qi, k + k_row(z, b, j, kh) * z.dim, bias, h, i, j), m) : 0.f;
-      for (int u = 0; u < MNV_WAVE && j0 + u < n; ++u) {
-        const float pu = __shfl(p, u, MNV_WAVE);
-        const float* vj = v + k_row(z, b, j0 + u, kh) * z.dim;
-        if (lane < z.dim) acc[0] = fmaf(pu, vj[lane], acc[0]);
-        if (lane + MNV_WAVE < z.dim) acc[1] = fmaf(pu, vj[lane + MNV_WAVE], acc[1]);
-      }
-    }
-    const float inv = inverse(l);
-    for (int u = 0; u < 2; ++u)
-      if (lane + u * MNV_WAVE < z.dim) out[row * z.dim + lane + u * MNV_WAVE] = acc[u] * inv;
-    if (lane < 2) stats[row * 2 + lane] = lane ? l : m;
-  }
-}
-
 struct AttentionGrads {
   const float *q, *k, *v, *bias, *lengths, *out, *stats, *dout;
 };
@@ -98,7 +40,7 @@ __device__ __forceinline__ void pair(const AttentionSizes& z, const AttentionGra
                                      float* p, float* ds) {
   const size_t row = q_row(z, b, i, h), key = k_row(z, b, j, kh);
   const float e = weight(score(z, a.q + row * z.dim, a.k + key * z.dim, a.bias, h, i, j), a.stats[2 * row]);
-  *p = e * inverse(a.stats[2 * row + 1]);
+  *p = e * mnv_inverse(a.stats[2 * row + 1]);
   *ds = *p * (dot(a.dout + row * z.dim, a.v + key * z.dim, z.dim) - dot(a.dout + row * z.dim, a.out + row * z.dim, z.dim));
 }
 
@@ -109,7 +51,7 @@ __global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dq_kernel(AttentionGra
   const size_t rows = (size_t)z.batch * z.q_len * z.heads;
   for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const int h = (int)(row % z.heads), i = (int)(row / z.heads % z.q_len), b = (int)(row / z.heads / z.q_len);
-    const int kh = h / (z.heads / z.kv_heads), n = visible(a.lengths, b, z.k_len);
+    const int kh = h / (z.heads / z.kv_heads), n = mnv_visible(a.lengths, b, z.k_len);
     float acc[2] = {0.f, 0.f};
     for (int j0 = 0; j0 < n; j0 += MNV_WAVE) {
       float p = 0.f, ds = 0.f;
@@ -135,7 +77,7 @@ __global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dkv_kernel(AttentionGr
   for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const int kh = (int)(row % z.kv_heads), j = (int)(row / z.kv_heads % z.k_len), b = (int)(row / z.kv_heads / z.k_len);
     float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
-    const int queries = j < visible(a.lengths, b, z.k_len) ? z.q_len : 0;
+    const int queries = j < mnv_visible(a.lengths, b, z.k_len) ? z.q_len : 0;
     for (int h = kh * group; h < (kh + 1) * group; ++h)
       for (int i0 = 0; i0 < queries; i0 += MNV_WAVE) {
         float p = 0.f, ds = 0.f;
@@ -169,7 +111,7 @@ __global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dbias_kernel(Attention
     const int kh = h / (z.heads / z.kv_heads);
     float s = 0.f;
     for (int b = 0; b < z.batch; ++b) {
-      const int n = visible(a.lengths, b, z.k_len);
+      const int n = mnv_visible(a.lengths, b, z.k_len);
       for (int i = threadIdx.x; i < z.q_len; i += MNV_WAVE) {
         const int j = o + i - (z.q_len - 1);
         if (j < 0 || j >= n) continue;
@@ -183,32 +125,11 @@ __global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dbias_kernel(Attention
   }
 }
 
-bool sizes_ok(const AttentionSizes& z) {
-  if (z.batch < 1 || z.heads < 1 || z.kv_heads < 1 || z.q_len < 1 || z.k_len < 1 || z.dim < 1) return false;
-  if (z.dim > MNV_AT_MAX_DIM || z.heads % z.kv_heads) return false;
-  const long long most = 0x7fffffffLL, d = z.dim > 2 ? z.dim : 2;  // stats has two values where out has dim
-  if ((long long)z.batch * z.heads > most || (long long)z.batch * z.heads * z.q_len > most / d) return false;
-  if ((long long)z.batch * z.kv_heads * z.k_len > most / z.dim) return false;
-  return ((long long)z.q_len + z.k_len - 1) * z.heads <= most && fabsf(z.scale) <= 3e38f;
-}
-
 unsigned row_grid(size_t rows) { return (unsigned)(rows < (1u << 20) ? rows : (1u << 20)); }
 
 }  // namespace
 
 extern "C" {
-
-size_t mnv_attention_fwd_workspace_bytes(int, int, int, int, int, int) { return 0; }
-
-int mnv_attention_fwd(const float* q, const float* k, const float* v, const float* bias, const float* lengths,
-                      float* out, float* stats, int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim,
-                      float scale, void*, size_t, mnv_stream_t stream) {
-  const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, scale};
-  if (!q || !k || !v || !out || !stats || !sizes_ok(z)) return MNV_ERR_INVALID;
-  hipLaunchKernelGGL(mnv_attention_fwd_kernel, dim3(row_grid((size_t)batch * q_len * heads)), dim3(MNV_WAVE), 0,
-                     mnv_stream(stream), q, k, v, bias, lengths, out, stats, z);
-  return MNV_LAUNCH_STATUS();
-}
 
 size_t mnv_attention_bwd_workspace_bytes(int, int, int, int, int, int, int) { return 0; }
 
@@ -217,7 +138,7 @@ int mnv_attention_bwd(const float* q, const float* k, const float* v, const floa
                       float* dbias, int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim, float scale,
                       void*, size_t, mnv_stream_t stream) {
   const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, scale};
-  if (!q || !k || !v || !out || !stats || !dout || !dq || !dk || !dv || (bias && !dbias) || !sizes_ok(z))
+  if (!q || !k || !v || !out || !stats || !dout || !dq || !dk || !dv || (bias && !dbias) || !mnv_attention_sizes_ok(z))
     return MNV_ERR_INVALID;
   const hipStream_t s = mnv_stream(stream);
   const AttentionGrads a = {q, k, v, bias, lengths, out, stats, dout};

@@ -1,0 +1,275 @@
+// What the attention kernels share: sizes, tiles of a sequence in LDS, and products of them on the matrix cores.
+//
+// Every product is one of a tile that streams through LDS (32 or 64 rows of two matrices, by the whole
+// workgroup) and an operand that a wavefront holds in registers for its own 32 columns: 32 queries in the
+// forward pass and for dq, 32 keys for dk and dv.  fp32 values are cut into three bf16 parts and six of
+// the nine part products are summed (gemm_split.h): the bf16 matrix instruction at 6 products per value
+// has 2.6 times the fp32 one's rate.
+//
+// The 32 x 32 x 16 instruction gives lane l the column l % 32 and the rows 8 (r / 4) + 4 (l / 32) + r % 4 of
+// the result, r = 0..15.  As an operand, lane l holds the 8 contraction places 8 (l / 32)... of column (or
+// row) l % 32.  Which rows stand in which contraction places is free as long as both operands agree, so a
+// result (scores, weights) becomes the next product's operand without leaving its lane: places 8 h + e
+// of step s hold the rows 16 s + 4 h + e (e < 4) and 16 s + 8 + 4 h + e - 4, and the other operand's tile is
+// written to LDS in that order (`place`).  So the softmax's sums run over a lane's own registers and one exchange
+// between the two half wavefronts.
+#pragma once
+#include <math.h>
+
+#include "gemm_split.h"
+
+#define MNV_AT_MAX_DIM 128
+
+struct AttentionSizes {
+  int batch, heads, kv_heads, q_len, k_len, dim;
+  float scale;
+  __host__ __device__ int group() const { return heads / kv_heads; }
+  __host__ __device__ size_t offsets() const { return (size_t)q_len + k_len - 1; }
+  __host__ __device__ size_t q_rows() const { return (size_t)batch * q_len * heads; }
+};
+
+static inline bool mnv_attention_sizes_ok(const AttentionSizes& z) {
+  if (z.batch < 1 || z.heads < 1 || z.kv_heads < 1 || z.q_len < 1 || z.k_len < 1 || z.dim < 1) return false;
+  if (z.dim > MNV_AT_MAX_DIM || z.heads % z.kv_heads) return false;
+  const long long most = 0x7fffffffLL, d = z.dim > 2 ? z.dim : 2;  // stats has two values where out has dim
+  if ((long long)z.batch * z.heads > most || (long long)z.batch * z.heads * z.q_len > most / d) return false;
+  if ((long long)z.batch * z.kv_heads * z.k_len > most / z.dim) return false;
+  return ((long long)z.q_len + z.k_len - 1) * z.heads <= most && fabsf(z.scale) <= 3e38f;
+}
+
+#ifdef __HIPCC__
+#define MNV_LOG2E 1.4426950408889634f
+
+typedef float mnv_f16 __attribute__((ext_vector_type(16)));
+
+// Keys of entry b that are read.
+__device__ __forceinline__ int mnv_visible(const float* lengths, int b, int k_len) {
+  if (!lengths) return k_len;
+  const float n = lengths[b];
+  if (!(n > 0.f)) return 0;
+  return n >= (float)k_len ? k_len : (int)n;
+}
+
+// exp(t - m), and 0 for a hidden t = -inf where hidden ones alone leave m at -inf too (m: see mnv_finite_max).
+// The difference is taken before the factor: at the type's lowest value t * log2(e) would be infinite.
+__device__ __forceinline__ float mnv_weight(float t, float m) { return __builtin_amdgcn_exp2f((t - m) * MNV_LOG2E); }
+__device__ __forceinline__ float mnv_finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+// 1 / l, and 0 for a row that sees no key
+__device__ __forceinline__ float mnv_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// Eight values of one operand as three parts.
+struct MnvParts {
+  mnv_bf8 p[3];
+};
+__device__ __forceinline__ MnvParts mnv_cut8(const float* x) {
+  mnv_u4 u[3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned t[3];
+    mnv_split_pair(x[2 * i], x[2 * i + 1], 1.f, t);
+    u[0][i] = t[0];
+    u[1][i] = t[1];
+    u[2][i] = t[2];
+  }
+  MnvParts r;
+#pragma unroll
+  for (int c = 0; c < 3; ++c) r.p[c] = __builtin_bit_cast(mnv_bf8, u[c]);
+  return r;
+}
+
+// acc[n] += a[n] * b for N tiles at once (independent sums between dependent ones), the smallest terms first.
+template <int N>
+__device__ __forceinline__ void mnv_mul(mnv_f16* acc, const MnvParts (&a)[N], const MnvParts& b) {
+  constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
+#pragma unroll
+  for (int t = 0; t < 6; ++t)
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[n].p[PA[t]], b.p[PB[t]], acc[n], 0, 0, 0);
+}
+
+// Row of result register r, for lanes of half h.
+__device__ __forceinline__ constexpr int mnv_acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
+
+// ROWS consecutive rows of two matrices (of up to DP columns, `pitch` floats from row to row) on their way
+// from memory to LDS: fetched into registers a tile ahead, then cut into planes of parts, by rows (FORM & 1), for
+// products that contract the columns, by columns (FORM & 2), for those that contract the rows, or both.
+// A thread takes blocks of 4 x 4 values, so that both forms are written 8 bytes at a time; the
+// four row blocks and 16 column blocks of a wavefront reach all banks in either.
+template <int DP, int ROWS, int NT, int FORM0, int FORM1>
+struct MnvStage {
+  static constexpr int DQ = DP / 4, QUADS = ROWS / 4 * DQ, SLOTS = (2 * QUADS + NT - 1) / NT;
+  static constexpr int RP = DP + 8, CP = ROWS + 8;  // bf16 from row to row, and from column to column
+  static constexpr int ROW_BYTES = 3 * ROWS * RP * 2, COL_BYTES = 3 * DP * CP * 2;
+  static constexpr int ROWS0 = 0, COLS0 = ROWS0 + (FORM0 & 1 ? ROW_BYTES : 0);
+  static constexpr int ROWS1 = COLS0 + (FORM0 & 2 ? COL_BYTES : 0), COLS1 = ROWS1 + (FORM1 & 1 ? ROW_BYTES : 0);
+  static constexpr int BYTES = COLS1 + (FORM1 & 2 ? COL_BYTES : 0);
+  static_assert(QUADS % MNV_WAVE == 0, "a wavefront's blocks are all of one matrix");
+
+  float v[SLOTS][4][4];
+
+  struct At {
+    bool any, second;
+    int row, col;
+  };
+  __device__ static At at(int s) {
+    int q = s * NT + (int)threadIdx.x;
+    At a;
+    a.any = 2 * QUADS % NT == 0 || q < 2 * QUADS;
+    a.second = q >= QUADS;
+    if (a.second) q -= QUADS;
+    a.row = 4 * (q % 4 + 4 * (q / 4 / DQ));
+    a.col = 4 * (q / 4 % DQ);
+    return a;
+  }
+
+  // rows >= 1 of the tile exist; those behind them and the columns from dim on become 0.
+  __device__ void fetch(const float* m0, const float* m1, size_t pitch, int rows, int dim) {
+    const bool whole = rows >= ROWS && dim == DP;
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const At a = at(s);
+      if (!a.any) continue;
+      const float* m = a.second ? m1 : m0;
+      if (whole) {
+        const float* p = m + a.row * pitch + a.col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const mnv_f4 t = mnv_ldx4u<false>(p + i * pitch);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[s][i][c] = t[c];
+        }
+      } else if (dim % 4 == 0) {
+        const int col = a.col < dim ? a.col : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = a.row + i < rows ? a.row + i : rows - 1;
+          const mnv_f4 t = mnv_ldx4u<false>(m + r * pitch + col);
+          const bool in = a.row + i < rows && a.col < dim;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[s][i][c] = in ? t[c] : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = a.row + i < rows ? a.row + i : rows - 1;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float t = m[r * pitch + (a.col + c < dim ? a.col + c : 0)];
+            v[s][i][c] = a.row + i < rows && a.col + c < dim ? t : 0.f;
+          }
+        }
+      }
+    }
+  }
+
+  // Place of row `row` (a multiple of 4) and its three successors in a column.
+  __device__ static int place(int row) { return row / 16 * 16 + (row / 4 % 2) * 8 + (row / 8 % 2) * 4; }
+
+  // scale0: factor of the first matrix
+  __device__ void store(char* lds, float scale0) {
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const At a = at(s);
+      if (!a.any) continue;
+      const float f = a.second ? 1.f : scale0;
+      unsigned w[3][4][2];  // [part][row][pair of columns]
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          unsigned t[3];
+          mnv_split_pair(v[s][i][2 * h] * f, v[s][i][2 * h + 1] * f, 1.f, t);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) w[p][i][h] = t[p];
+        }
+      if (a.second ? FORM1 & 1 : FORM0 & 1) {
+        char* to = lds + (a.second ? ROWS1 : ROWS0) + (a.row * RP + a.col) * 2;
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<mnv_u2*>(to + (p * ROWS + i) * RP * 2) = mnv_u2{w[p][i][0], w[p][i][1]};
+      }
+      if (a.second ? FORM1 & 2 : FORM0 & 2) {
+        char* to = lds + (a.second ? COLS1 : COLS0) + (a.col * CP + place(a.row)) * 2;
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const unsigned sel = c % 2 ? 0x07060302u : 0x05040100u;
+            *reinterpret_cast<mnv_u2*>(to + (p * DP + c) * CP * 2) =
+                mnv_u2{__builtin_amdgcn_perm(w[p][1][c / 2], w[p][0][c / 2], sel),
+                       __builtin_amdgcn_perm(w[p][3][c / 2], w[p][2][c / 2], sel)};
+          }
+      }
+    }
+  }
+
+  // Operands of the 32 rows from `row` on, columns 16 s ... of step s; and of the 32 columns from `col` on, rows 16 s...
+  __device__ static MnvParts by_rows(const char* plane, int row, int s) {
+    const int lane = threadIdx.x % MNV_WAVE;
+    const char* p = plane + ((row + lane % 32) * RP + s * 16 + lane / 32 * 8) * 2;
+    MnvParts r;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * ROWS * RP * 2);
+    return r;
+  }
+  __device__ static MnvParts by_cols(const char* plane, int col, int s) {
+    const int lane = threadIdx.x % MNV_WAVE;
+    const char* p = plane + ((col + lane % 32) * CP + s * 16 + lane / 32 * 8) * 2;
+    MnvParts r;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * DP * CP * 2);
+    return r;
+  }
+};
+
+// The columns 16 s + 8 (l / 32)... of one row (the lane's own) as an operand, times `scale`; 0 from dim on.
+template <int DP>
+__device__ __forceinline__ void mnv_load8(const float* row, int s, int dim, float (&x)[8]) {
+  const int d0 = s * 16 + (int)threadIdx.x % MNV_WAVE / 32 * 8;
+  if (dim == DP) {
+    const mnv_f4 a = mnv_ldx4u<false>(row + d0), b = mnv_ldx4u<false>(row + d0 + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = a[e];
+      x[4 + e] = b[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = row[d0 + e < dim ? d0 + e : 0];
+      x[e] = d0 + e < dim ? t : 0.f;
+    }
+  }
+}
+
+// Writes the lane's column of a [DP x 32] result, times f, to the dim values of `row`.
+template <int DP>
+__device__ __forceinline__ void mnv_store_column(const mnv_f16 (&acc)[DP / 32], float f, float* row, int dim) {
+  const int half = (int)threadIdx.x % MNV_WAVE / 32;
+#pragma unroll
+  for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int d = n * 32 + 8 * u + 4 * half;
+      mnv_f4 t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = acc[n][4 * u + e] * f;
+      if (d + 4 <= dim) {
+        *reinterpret_cast<mnv_f4u*>(row + d) = t;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < dim) row[d + e] = t[e];
+      }
+    }
+}
+
+// Consecutive work items go to one of the 8 dies, whose L2 then holds what they share.
+__device__ __forceinline__ unsigned mnv_by_die(unsigned id, unsigned total) {
+  const unsigned each = total / 8;
+  return id < each * 8 ? id % 8 * each + id / 8 : id;
+}
+#endif

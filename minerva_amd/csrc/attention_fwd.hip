@@ -1,0 +1,190 @@
+// Attention of queries to the states of another sequence (or their own), forward.
+//   t_ij = scale * q_i.k_j + bias[j - i + q_len - 1] (j < lengths[b]),  m_i = max t_ij,  l_i = sum exp(t_ij - m_i)
+//   out_i = sum_j exp(t_ij - m_i) / l_i * v_j
+// One pass over the keys with the running maximum and sum of each query: a workgroup of four wavefronts
+// has 128 queries, 32 per wavefront, and tiles of 32 or 64 keys stream through LDS.  t^T = K Q^T, so a lane
+// has one query and a quarter of the tile's keys; exp(t - m) goes on as the operand of out^T += V^T P^T from
+// the registers it stands in (attention_core.h).  Heads that share keys are rows of the same workgroup: row r is query
+// r / group, head r % group of the key head, so their keys are read and cut once.
+// A row that sees no key has m = -inf, l = 0, out = 0.  The pair (m, l) is kept and not m + ln l: where the bias is the
+// type's lowest value for a whole row, ln l would be lost in the sum.
+#include "attention_core.h"
+
+namespace {
+
+struct FwdArgs {
+  const float *q, *k, *v, *bias, *lengths;
+  float *out, *stats;
+  AttentionSizes z;
+  int rows;        // q_len * group
+  int row_tiles;   // per entry and key head
+  MnvFastDiv by_group;
+};
+
+template <int DP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
+  constexpr int BK = DP <= 64 ? 64 : 32, KB = BK / 32, NB = DP / 32;
+  using Stage = MnvStage<DP, BK, 256, 1, 2>;  // keys by rows, values by columns
+  __shared__ __align__(16) char lds[Stage::BYTES];
+  const AttentionSizes& z = a.z;
+  const unsigned id = mnv_by_die(blockIdx.x, gridDim.x);
+  const int tile = (int)(id % a.row_tiles);
+  const unsigned pair = id / a.row_tiles;
+  const int kh = (int)(pair % z.kv_heads), b = (int)(pair / z.kv_heads);
+  const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
+  const int n = mnv_visible(a.lengths, b, z.k_len);
+
+  const int r = tile * 128 + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
+  const int rc = r < a.rows ? r : a.rows - 1;
+  const int i = mnv_fastdiv(rc, a.by_group), h = kh * z.group() + (rc - i * z.group());
+  const size_t row = ((size_t)b * z.q_len + i) * z.heads + h;
+
+  mnv_f16 acc[NB];
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[c][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  if (n > 0) {
+    MnvParts qp[DP / 16];
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      float x[8];
+      mnv_load8<DP>(a.q + row * z.dim, s, z.dim, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= z.scale;
+      qp[s] = mnv_cut8(x);
+    }
+    const size_t pitch = (size_t)z.kv_heads * z.dim;
+    const float* kb = a.k + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
+    const float* vb = a.v + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
+    const float* bias = BIAS ? a.bias + h * z.offsets() + (z.q_len - 1 - i) : nullptr;
+
+    Stage stage;
+    stage.fetch(kb, vb, pitch, n, z.dim);
+    stage.store(lds, 1.f);
+    for (int j0 = 0; j0 < n; j0 += BK) {
+      __syncthreads();
+      const bool more = j0 + BK < n;
+      if (more) stage.fetch(kb + (j0 + BK) * pitch, vb + (j0 + BK) * pitch, pitch, n - j0 - BK, z.dim);
+
+      mnv_f16 t[KB];
+#pragma unroll
+      for (int c = 0; c < KB; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[c][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s) {
+        MnvParts kp[KB];
+#pragma unroll
+        for (int c = 0; c < KB; ++c) kp[c] = Stage::by_rows(lds + Stage::ROWS0, c * 32, s);
+        mnv_mul(t, kp, qp[s]);
+      }
+      const bool whole = j0 + BK <= n;
+      if (BIAS) {
+#pragma unroll
+        for (int c = 0; c < KB; ++c)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int j = j0 + c * 32 + 8 * u + 4 * half;
+            if (whole) {
+              const mnv_f4 add = mnv_ldx4u<false>(bias + j);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t[c][4 * u + e] += add[e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t[c][4 * u + e] += bias[j + e < n ? j + e : n - 1];
+            }
+          }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int c = 0; c < KB; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (j0 + c * 32 + mnv_acc_row(e, half) >= n) t[c][e] = -INFINITY;
+      }
+      float top = t[0][0];
+#pragma unroll
+      for (int c = 0; c < KB; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, t[c][e]);
+      top = fmaxf(top, __shfl_xor(top, 32, MNV_WAVE));
+      const float next = fmaxf(m, top);
+      const float base = mnv_finite_max(next);
+      if (__any(next > m)) {
+        const float shrink = mnv_weight(m, base);
+        l *= shrink;
+#pragma unroll
+        for (int c = 0; c < NB; ++c)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c][e] *= shrink;
+        m = next;
+      }
+#pragma unroll
+      for (int s = 0; s < BK / 16; ++s) {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = mnv_weight(t[s / 2][s % 2 * 8 + e], base);
+          l += p[e];
+        }
+        const MnvParts pp = mnv_cut8(p);
+#pragma unroll
+        for (int c = 0; c + 2 <= NB; c += 2) {
+          const MnvParts vp[2] = {Stage::by_cols(lds + Stage::COLS1, c * 32, s),
+                                  Stage::by_cols(lds + Stage::COLS1, c * 32 + 32, s)};
+          mnv_mul(acc + c, vp, pp);
+        }
+        if (NB % 2) {
+          const MnvParts vp[1] = {Stage::by_cols(lds + Stage::COLS1, NB * 32 - 32, s)};
+          mnv_mul(acc + NB - 1, vp, pp);
+        }
+      }
+      __syncthreads();
+      if (more) stage.store(lds, 1.f);
+    }
+    l += __shfl_xor(l, 32, MNV_WAVE);
+  }
+  if (r < a.rows) {
+    mnv_store_column<DP>(acc, mnv_inverse(l), a.out + row * z.dim, z.dim);
+    if (half == 0) {
+      a.stats[2 * row] = m;
+      a.stats[2 * row + 1] = l;
+    }
+  }
+}
+
+template <int DP>
+int launch(const FwdArgs& a, unsigned grid, hipStream_t s) {
+  if (a.bias)
+    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, true>), dim3(grid), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, false>), dim3(grid), dim3(256), 0, s, a);
+  return MNV_LAUNCH_STATUS();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mnv_attention_fwd_workspace_bytes(int, int, int, int, int, int) { return 0; }
+
+int mnv_attention_fwd(const float* q, const float* k, const float* v, const float* bias, const float* lengths,
+                      float* out, float* stats, int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim,
+                      float scale, void*, size_t, mnv_stream_t stream) {
+  const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, scale};
+  if (!q || !k || !v || !out || !stats || !mnv_attention_sizes_ok(z)) return MNV_ERR_INVALID;
+  FwdArgs a = {q, k, v, bias, lengths, out, stats, z, q_len * z.group(), 0, mnv_fastdiv_make(z.group())};
+  a.row_tiles = (int)mnv_ceil_div(a.rows, 128);
+  const long long grid = (long long)a.row_tiles * batch * kv_heads;
+  if (grid > 0x7fffffffLL) return MNV_ERR_INVALID;
+  const hipStream_t s = mnv_stream(stream);
+  if (head_dim <= 32) return launch<32>(a, (unsigned)grid, s);
+  if (head_dim <= 64) return launch<64>(a, (unsigned)grid, s);
+  if (head_dim <= 96) return launch<96>(a, (unsigned)grid, s);
+  return launch<128>(a, (unsigned)grid, s);
+}
+
+}  // extern "C"
