@@ -1,157 +1,472 @@
-// Attention of queries to the states of another sequence (or their own), forward and backward.
-//   t_ij = scale * q_i.k_j + bias[j - i + q_len - 1] (j < lengths[b]),  m_i = max t_ij,  l_i = sum exp(t_ij - m_i)
-//   out_i = sum_j exp(t_ij - m_i) / l_i * v_j
-//   p_ij = exp(t_ij - m_i) / l_i,  ds_ij = p_ij * (dout_i.v_j - dout_i.out_i)
+// Attention, backward: dq, dk, dv and the bias's gradient from what the forward pass kept (m and l of each row).
+//   p_ij = exp(t_ij - m_i) / l_i,  ds_ij = p_ij * (dout_i.v_j - delta_i),  delta_i = dout_i.out_i
 //   dq_i = scale * sum_j ds_ij k_j,  dk_j = scale * sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
 //   dbias[o] = sum of ds_ij with j - i + q_len - 1 = o
-// A row that sees no key has m = -inf, l = 0, out = 0.  The pair (m, l) is kept and not m + ln l: where the bias is the
-// type's lowest value for a whole row, ln l would be lost in the sum.
+// Scores are computed again, twice: once with a workgroup's 128 keys in registers while queries and their
+// gradients stream through LDS (dk, dv, dbias), once with its 128 rows of queries in registers while keys and
+// values do (dq).  That is 7 products where 5 would do, but every gradient is summed by one wavefront
+// in one order: no atomics, and no partial gradients in memory.  delta waits in the first value of each row of
+// dq, which the last kernel overwrites, so no workspace is needed for it.
 #include "attention_core.h"
 
 namespace {
 
-__device__ __forceinline__ size_t q_row(const AttentionSizes& z, int b, int i, int h) {
-  return ((size_t)b * z.q_len + i) * z.heads + h;
-}
-__device__ __forceinline__ size_t k_row(const AttentionSizes& z, int b, int j, int h) {
-  return ((size_t)b * z.k_len + j) * z.kv_heads + h;
+struct BwdArgs {
+  const float *q, *k, *v, *bias, *lengths, *out, *stats, *dout;
+  float *dq, *dk, *dv;
+  float* parts;         // sums of ds along the diagonals of each wavefront's 32 keys, or NULL
+  AttentionSizes z;
+  int tiles;            // workgroups per entry and key head
+  unsigned first_pair;  // the launch's first (entry, key head)
+  int rows;             // q_len * group
+  MnvFastDiv by_group;
+};
+
+// dq[row][0] = dout_row . out_row; 16 lanes per row.
+__global__ __launch_bounds__(256) void mnv_attention_delta_kernel(const float* __restrict__ dout,
+                                                                  const float* __restrict__ out,
+                                                                  float* __restrict__ dq, size_t rows, int dim) {
+  const size_t row = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
+  if (row >= rows) return;
+  float s = 0.f;
+  for (int d = threadIdx.x % 16; d < dim; d += 16) s = fmaf(dout[row * dim + d], out[row * dim + d], s);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 16);
+  if (threadIdx.x % 16 == 0) dq[row * dim] = s;
 }
 
+// Floats of one wavefront's partial diagonal sums: those of 32 keys and the queries in tiles of 32.
+__host__ __device__ inline size_t diagonal_pitch(int q_len) { return ((size_t)q_len + 31) / 32 * 32 + 32; }
+__host__ __device__ inline size_t key_tiles(int k_len) { return ((size_t)k_len + 31) / 32; }
+
+template <int DP, bool BIAS>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
+  constexpr int NB = DP / 32, KS = DP / 16;
+  using Stage = MnvStage<DP, 32, 256, 3, 3>;  // queries (times scale) and their gradients, either way
+  __shared__ __align__(16) char lds[Stage::BYTES];
+  __shared__ __align__(16) float row_m[32], row_inverse[32], row_delta[32];
+  __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
+  const AttentionSizes& z = a.z;
+  const unsigned id = mnv_by_die(blockIdx.x, gridDim.x);
+  const int tile = (int)(id % a.tiles);
+  const unsigned pair = a.first_pair + id / a.tiles;
+  const int kh = (int)(pair % z.kv_heads), b = (int)(pair / z.kv_heads), group = z.group();
+  const int wave = threadIdx.x / MNV_WAVE, lane = threadIdx.x % MNV_WAVE, half = lane / 32;
+  const int n = mnv_visible(a.lengths, b, z.k_len);
+
+  const int j = tile * 128 + wave * 32 + lane % 32;
+  const size_t key = ((size_t)b * z.k_len + (j < z.k_len ? j : z.k_len - 1)) * z.kv_heads + kh;
+  mnv_f16 dk[NB], dv[NB];
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dk[c][e] = dv[c][e] = 0.f;
+
+  if (tile * 128 < n) {
+    if (BIAS)
+      for (int e = threadIdx.x; e < 4 * 16 * 48; e += 256) turned[e] = 0.f;
+    const bool shown = j < n;
+    MnvParts kp[KS], vp[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float x[8], y[8];
+      // a key that is not read may hold anything: another one stands in for it, and its weights are 0
+      const size_t at = ((size_t)b * z.k_len + (shown ? j : n - 1)) * z.kv_heads + kh;
+      mnv_load8<DP>(a.k + at * z.dim, s, z.dim, x);
+      mnv_load8<DP>(a.v + at * z.dim, s, z.dim, y);
+      kp[s] = mnv_cut8(x);
+      vp[s] = mnv_cut8(y);
+    }
+    const size_t pitch = (size_t)z.heads * z.dim;
+    const int jb = shown ? j : n - 1;
+    for (int g = 0; g < group; ++g) {
+      const int h = kh * group + g;
+      const size_t row0 = (size_t)b * z.q_len * z.heads + h;  // rows of the head are z.heads apart
+      const float* qb = a.q + row0 * z.dim;
+      const float* ob = a.dout + row0 * z.dim;
+      const float* bias = BIAS ? a.bias + h * z.offsets() + (jb + z.q_len - 1) : nullptr;
+      float* parts = nullptr;
+      if (BIAS && a.parts && tile * 128 + wave * 32 < n)  // no others are read
+        parts = a.parts + (((size_t)(pair - a.first_pair) * group + g) * key_tiles(z.k_len) + tile * 4 + wave) *
+                              diagonal_pitch(z.q_len);
+      float carry = 0.f;
+      Stage stage;
+      float next_m = 0.f, next_l = 0.f, next_delta = 0.f;
+      auto fetch = [&](int i0) {
+        stage.fetch(qb + i0 * pitch, ob + i0 * pitch, pitch, z.q_len - i0, z.dim);
+        if (threadIdx.x < 32) {
+          const int i = i0 + (int)threadIdx.x;
+          const size_t row = row0 + (size_t)(i < z.q_len ? i : z.q_len - 1) * z.heads;
+          next_m = mnv_finite_max(a.stats[2 * row]);
+          next_l = i < z.q_len ? mnv_inverse(a.stats[2 * row + 1]) : 0.f;
+          next_delta = i < z.q_len ? a.dq[row * z.dim] : 0.f;
+        }
+      };
+      auto store = [&] {
+        stage.store(lds, z.scale);
+        if (threadIdx.x < 32) {
+          row_m[threadIdx.x] = next_m;
+          row_inverse[threadIdx.x] = next_l;
+          row_delta[threadIdx.x] = next_delta;
+        }
+      };
+      fetch(0);
+      store();
+      for (int i0 = 0; i0 < z.q_len; i0 += 32) {
+        __syncthreads();
+        const bool more = i0 + 32 < z.q_len;
+        if (more) fetch(i0 + 32);
+
+        mnv_f16 t[1], dp[1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) t[0][e] = dp[0][e] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const MnvParts qp[1] = {Stage::by_rows(lds + Stage::ROWS0, 0, s)};
+          mnv_mul(t, qp, kp[s]);
+          const MnvParts op[1] = {Stage::by_rows(lds + Stage::ROWS1, 0, s)};
+          mnv_mul(dp, op, vp[s]);
+        }
+        if (BIAS) {
+          const bool whole = i0 + 32 <= z.q_len;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int i = i0 + 8 * u + 4 * half;
+            if (whole) {
+              const mnv_f4 add = mnv_ldx4u<false>(bias - (i + 3));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t[0][4 * u + e] += add[3 - e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t[0][4 * u + e] += bias[-(i + e < z.q_len ? i + e : z.q_len - 1)];
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int at = 8 * u + 4 * half;
+          const mnv_f4 m = *reinterpret_cast<const mnv_f4*>(row_m + at);
+          const mnv_f4 il = *reinterpret_cast<const mnv_f4*>(row_inverse + at);
+          const mnv_f4 delta = *reinterpret_cast<const mnv_f4*>(row_delta + at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = shown ? mnv_weight(t[0][4 * u + e], m[e]) * il[e] : 0.f;
+            t[0][4 * u + e] = p;
+            dp[0][4 * u + e] = shown ? p * (dp[0][4 * u + e] - delta[e]) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float x[8], y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            x[e] = t[0][8 * s + e];
+            y[e] = dp[0][8 * s + e];
+          }
+          const MnvParts pp = mnv_cut8(x), sp = mnv_cut8(y);
+#pragma unroll
+          for (int c = 0; c < NB; ++c) {
+            const MnvParts op[1] = {Stage::by_cols(lds + Stage::COLS1, c * 32, s)};
+            mnv_mul(dv + c, op, pp);
+            const MnvParts qp[1] = {Stage::by_cols(lds + Stage::COLS0, c * 32, s)};
+            mnv_mul(dk + c, qp, sp);
+          }
+        }
+        if (BIAS && parts) {
+          // Lane u sums the diagonal key - query = u - 31 of the 32 x 32 tile: 16 queries at a time go to LDS,
+          // each shifted by its number, so that a diagonal is a column; what a row does not reach stays 0.  The
+          // next tile's diagonals lie 32 lower, so those below 0 go on in the lane 32 higher; the others
+          // are whole, and written.
+          float* mine = turned + wave * 16 * 48;
+          float sum = carry;
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int i = mnv_acc_row(e, half);
+              mine[i * 47 + 15 + lane % 32] = dp[0][8 * part + e];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int u = part == 0 ? lane - 16 : lane;
+            const bool in = u >= 0 && u < 47;
+            const float* column = mine + (in ? u : 0);
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x += column[i * 48];
+            sum += in ? x : 0.f;
+            __builtin_amdgcn_wave_barrier();
+          }
+          const size_t at = diagonal_pitch(z.q_len) - 64 - i0 + lane;  // place of the diagonal key - query = lane - 31
+          if (lane >= 31 && lane < 63) parts[at] = sum;
+          if (!more && lane < 31) parts[at] = sum;
+          carry = __shfl(sum, lane - 32, MNV_WAVE);
+          carry = lane >= 32 && lane < 63 ? carry : 0.f;
+        }
+        __syncthreads();
+        if (more) store();
+      }
+    }
+  }
+  if (j < z.k_len) {
+    mnv_store_column<DP>(dk, j < n ? 1.f : 0.f, a.dk + key * z.dim, z.dim);
+    mnv_store_column<DP>(dv, j < n ? 1.f : 0.f, a.dv + key * z.dim, z.dim);
+  }
+}
+
+template <int DP, bool BIAS>
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
+  constexpr int NB = DP / 32, KS = DP / 16;
+  using Stage = MnvStage<DP, 32, 256, 3, 1>;  // keys either way, values by rows
+  __shared__ __align__(16) char lds[Stage::BYTES];
+  const AttentionSizes& z = a.z;
+  const unsigned id = mnv_by_die(blockIdx.x, gridDim.x);
+  const int tile = (int)(id % a.tiles);
+  const unsigned pair = id / a.tiles;
+  const int kh = (int)(pair % z.kv_heads), b = (int)(pair / z.kv_heads);
+  const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
+  const int n = mnv_visible(a.lengths, b, z.k_len);
+
+  const int r = tile * 128 + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
+  const int rc = r < a.rows ? r : a.rows - 1;
+  const int i = mnv_fastdiv(rc, a.by_group), h = kh * z.group() + (rc - i * z.group());
+  const size_t row = ((size_t)b * z.q_len + i) * z.heads + h;
+
+  mnv_f16 dq[NB];
+#pragma unroll
+  for (int c = 0; c < NB; ++c)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) dq[c][e] = 0.f;
+
+  if (n > 0) {
+    MnvParts qp[KS], op[KS];
+    float delta = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float x[8], y[8], o[8];
+      mnv_load8<DP>(a.q + row * z.dim, s, z.dim, x);
+      mnv_load8<DP>(a.dout + row * z.dim, s, z.dim, y);
+      mnv_load8<DP>(a.out + row * z.dim, s, z.dim, o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] *= z.scale;
+        delta = fmaf(y[e], o[e], delta);
+      }
+      qp[s] = mnv_cut8(x);
+      op[s] = mnv_cut8(y);
+    }
+    delta += __shfl_xor(delta, 32, MNV_WAVE);
+    const float m = mnv_finite_max(a.stats[2 * row]), il = mnv_inverse(a.stats[2 * row + 1]);
+    const size_t pitch = (size_t)z.kv_heads * z.dim;
+    const float* kb = a.k + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
+    const float* vb = a.v + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
+    const float* bias = BIAS ? a.bias + h * z.offsets() + (z.q_len - 1 - i) : nullptr;
+
+    Stage stage;
+    stage.fetch(kb, vb, pitch, n, z.dim);
+    stage.store(lds, 1.f);
+    for (int j0 = 0; j0 < n; j0 += 32) {
+      __syncthreads();
+      const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
+      if (more) stage.fetch(kb + (j0 + 32) * pitch, vb + (j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
+
+      mnv_f16 t[1], dp[1];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t[0][e] = dp[0][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const MnvParts kp[1] = {Stage::by_rows(lds + Stage::ROWS0, 0, s)};
+        mnv_mul(t, kp, qp[s]);
+        const MnvParts vp[1] = {Stage::by_rows(lds + Stage::ROWS1, 0, s)};
+        mnv_mul(dp, vp, op[s]);
+      }
+      if (BIAS) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = j0 + 8 * u + 4 * half;
+          if (whole) {
+            const mnv_f4 add = mnv_ldx4u<false>(bias + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[0][4 * u + e] += add[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[0][4 * u + e] += bias[j + e < n ? j + e : n - 1];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[0][e] = mnv_weight(t[0][e], m) * il * (dp[0][e] - delta);
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (j0 + mnv_acc_row(e, half) >= n) dp[0][e] = 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = dp[0][8 * s + e];
+        const MnvParts sp = mnv_cut8(x);
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {
+          const MnvParts kp[1] = {Stage::by_cols(lds + Stage::COLS0, c * 32, s)};
+          mnv_mul(dq + c, kp, sp);
+        }
+      }
+      __syncthreads();
+      if (more) stage.store(lds, 1.f);
+    }
+  }
+  if (r < a.rows) mnv_store_column<DP>(dq, z.scale, a.dq + row * z.dim, z.dim);
+}
+
+// dbias[o] += the parts of o: of every entry among the launch's pairs and every 32 keys that have the diagonal.
+__global__ __launch_bounds__(256) void mnv_attention_dbias_kernel(const float* __restrict__ parts,
+                                                                  const float* __restrict__ lengths,
+                                                                  float* __restrict__ dbias, AttentionSizes z,
+                                                                  unsigned first_pair, unsigned pairs, bool first) {
+  const size_t offsets = z.offsets();
+  const size_t o = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (o >= offsets) return;
+  const size_t pitch = diagonal_pitch(z.q_len), per_key = key_tiles(z.k_len);
+  const int group = z.group(), padded = (int)pitch - 32;
+  for (int h = blockIdx.y; h < z.heads; h += gridDim.y) {
+    float s = first ? 0.f : dbias[h * offsets + o];
+    const int kh = h / group;
+    for (unsigned p = 0; p < pairs; ++p) {
+      const unsigned pair = first_pair + p;
+      if (pair % z.kv_heads != (unsigned)kh) continue;
+      const int n = mnv_visible(lengths, pair / z.kv_heads, z.k_len);
+      // key kt + c and query 32 s + r of the part: place o - kt + padded - q_len
+      const long long place = (long long)o + padded - z.q_len;
+      long long from = place - (padded + 30);
+      from = from <= 0 ? 0 : (from + 31) / 32 * 32;
+      const float* mine = parts + ((size_t)p * group + h % group) * per_key * pitch;
+      for (long long kt = from; kt < n && kt <= place; kt += 32) s += mine[kt / 32 * pitch + (place - kt)];
+    }
+    dbias[h * offsets + o] = s;
+  }
+}
+
+// The bias's gradient without a workspace: one wavefront per head and offset goes through all its pairs of
+// a query and a key and computes their scores again, one after the other.
 __device__ __forceinline__ float dot(const float* a, const float* b, int n) {
   float s = 0.f;
   for (int d = 0; d < n; ++d) s = fmaf(a[d], b[d], s);
   return s;
 }
-
-__device__ __forceinline__ float score(const AttentionSizes& z, const float* q, const float* k, const float* bias,
-                                       int h, int i, int j) {
-  const float t = z.scale * dot(q, k, z.dim);
-  return bias ? t + bias[(size_t)h * ((size_t)z.q_len + z.k_len - 1) + (j - i + z.q_len - 1)] : t;
-}
-
-// exp(t - m), and 0 for a hidden t = -inf where hidden ones alone leave m at -inf too
-__device__ __forceinline__ float weight(float t, float m) { return expf(t - (m == -INFINITY ? 0.f : m)); }
-struct AttentionGrads {
-  const float *q, *k, *v, *bias, *lengths, *out, *stats, *dout;
-};
-
-// p_ij and ds_ij of one query and one visible key
-__device__ __forceinline__ void pair(const AttentionSizes& z, const AttentionGrads& a, int b, int h, int kh, int i, int j,
-                                     float* p, float* ds) {
-  const size_t row = q_row(z, b, i, h), key = k_row(z, b, j, kh);
-  const float e = weight(score(z, a.q + row * z.dim, a.k + key * z.dim, a.bias, h, i, j), a.stats[2 * row]);
-  *p = e * mnv_inverse(a.stats[2 * row + 1]);
-  *ds = *p * (dot(a.dout + row * z.dim, a.v + key * z.dim, z.dim) - dot(a.dout + row * z.dim, a.out + row * z.dim, z.dim));
-}
-
-// One wavefront per query.
-__global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dq_kernel(AttentionGrads a, float* __restrict__ dq,
-                                                                    AttentionSizes z) {
-  const int lane = threadIdx.x;
-  const size_t rows = (size_t)z.batch * z.q_len * z.heads;
-  for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int h = (int)(row % z.heads), i = (int)(row / z.heads % z.q_len), b = (int)(row / z.heads / z.q_len);
-    const int kh = h / (z.heads / z.kv_heads), n = mnv_visible(a.lengths, b, z.k_len);
-    float acc[2] = {0.f, 0.f};
-    for (int j0 = 0; j0 < n; j0 += MNV_WAVE) {
-      float p = 0.f, ds = 0.f;
-      if (j0 + lane < n) pair(z, a, b, h, kh, i, j0 + lane, &p, &ds);
-      for (int u = 0; u < MNV_WAVE && j0 + u < n; ++u) {
-        const float du = __shfl(ds, u, MNV_WAVE);
-        const float* kj = a.k + k_row(z, b, j0 + u, kh) * z.dim;
-        if (lane < z.dim) acc[0] = fmaf(du, kj[lane], acc[0]);
-        if (lane + MNV_WAVE < z.dim) acc[1] = fmaf(du, kj[lane + MNV_WAVE], acc[1]);
-      }
-    }
-    for (int u = 0; u < 2; ++u)
-      if (lane + u * MNV_WAVE < z.dim) dq[row * z.dim + lane + u * MNV_WAVE] = z.scale * acc[u];
-  }
-}
-
-// One wavefront per key.
-__global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dkv_kernel(AttentionGrads a, float* __restrict__ dk,
-                                                                     float* __restrict__ dv, AttentionSizes z) {
-  const int lane = threadIdx.x;
-  const size_t rows = (size_t)z.batch * z.k_len * z.kv_heads;
-  const int group = z.heads / z.kv_heads;
-  for (size_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int kh = (int)(row % z.kv_heads), j = (int)(row / z.kv_heads % z.k_len), b = (int)(row / z.kv_heads / z.k_len);
-    float sk[2] = {0.f, 0.f}, sv[2] = {0.f, 0.f};
-    const int queries = j < mnv_visible(a.lengths, b, z.k_len) ? z.q_len : 0;
-    for (int h = kh * group; h < (kh + 1) * group; ++h)
-      for (int i0 = 0; i0 < queries; i0 += MNV_WAVE) {
-        float p = 0.f, ds = 0.f;
-        if (i0 + lane < queries) pair(z, a, b, h, kh, i0 + lane, j, &p, &ds);
-        for (int u = 0; u < MNV_WAVE && i0 + u < queries; ++u) {
-          const float pu = __shfl(p, u, MNV_WAVE), du = __shfl(ds, u, MNV_WAVE);
-          const size_t at = q_row(z, b, i0 + u, h) * z.dim;
-          for (int c = 0; c < 2; ++c) {
-            const int d = lane + c * MNV_WAVE;
-            if (d >= z.dim) continue;
-            sv[c] = fmaf(pu, a.dout[at + d], sv[c]);
-            sk[c] = fmaf(du, a.q[at + d], sk[c]);
-          }
-        }
-      }
-    for (int c = 0; c < 2; ++c) {
-      const int d = lane + c * MNV_WAVE;
-      if (d >= z.dim) continue;
-      dk[row * z.dim + d] = z.scale * sk[c];
-      dv[row * z.dim + d] = sv[c];
-    }
-  }
-}
-
-// One wavefront per head and offset.
-__global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dbias_kernel(AttentionGrads a, float* __restrict__ dbias,
-                                                                       AttentionSizes z) {
-  const long long offsets = (long long)z.q_len + z.k_len - 1;
-  for (long long at = blockIdx.x; at < offsets * z.heads; at += gridDim.x) {
-    const int h = (int)(at / offsets), o = (int)(at % offsets);
-    const int kh = h / (z.heads / z.kv_heads);
-    float s = 0.f;
+__global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dbias_alone_kernel(BwdArgs a, float* __restrict__ dbias) {
+  const AttentionSizes& z = a.z;
+  const size_t offsets = z.offsets();
+  for (size_t at = blockIdx.x; at < offsets * z.heads; at += gridDim.x) {
+    const int h = (int)(at / offsets), o = (int)(at % offsets), kh = h / z.group();
+    float sum = 0.f;
     for (int b = 0; b < z.batch; ++b) {
       const int n = mnv_visible(a.lengths, b, z.k_len);
       for (int i = threadIdx.x; i < z.q_len; i += MNV_WAVE) {
         const int j = o + i - (z.q_len - 1);
         if (j < 0 || j >= n) continue;
-        float p, ds;
-        pair(z, a, b, h, kh, i, j, &p, &ds);
-        s += ds;
+        const size_t row = ((size_t)b * z.q_len + i) * z.heads + h;
+        const float* kj = a.k + (((size_t)b * z.k_len + j) * z.kv_heads + kh) * z.dim;
+        const float* vj = a.v + (((size_t)b * z.k_len + j) * z.kv_heads + kh) * z.dim;
+        const float* oi = a.dout + row * z.dim;
+        const float t = z.scale * dot(a.q + row * z.dim, kj, z.dim) + a.bias[at];
+        const float p = mnv_weight(t, mnv_finite_max(a.stats[2 * row])) * mnv_inverse(a.stats[2 * row + 1]);
+        sum += p * (dot(oi, vj, z.dim) - dot(oi, a.out + row * z.dim, z.dim));
       }
     }
-    s = mnv_wave_sum(s);
-    if (threadIdx.x == 0) dbias[at] = s;
+    sum = mnv_wave_sum(sum);
+    if (threadIdx.x == 0) dbias[at] = sum;
   }
 }
 
-unsigned row_grid(size_t rows) { return (unsigned)(rows < (1u << 20) ? rows : (1u << 20)); }
+// Bytes of the partial diagonal sums of one entry and key head.
+size_t pair_bytes(const AttentionSizes& z) {
+  return (size_t)z.group() * key_tiles(z.k_len) * diagonal_pitch(z.q_len) * sizeof(float);
+}
+#define MNV_AT_PARTS_BYTES ((size_t)256 << 20)  // of partial sums at a time, where there are more
+
+template <int DP>
+int launch_dkv(const BwdArgs& a, unsigned grid, hipStream_t s) {
+  if (a.bias)
+    hipLaunchKernelGGL((mnv_attention_dkv_kernel<DP, true>), dim3(grid), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((mnv_attention_dkv_kernel<DP, false>), dim3(grid), dim3(256), 0, s, a);
+  return MNV_LAUNCH_STATUS();
+}
+template <int DP>
+int launch_dq(const BwdArgs& a, unsigned grid, hipStream_t s) {
+  if (a.bias)
+    hipLaunchKernelGGL((mnv_attention_dq_kernel<DP, true>), dim3(grid), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((mnv_attention_dq_kernel<DP, false>), dim3(grid), dim3(256), 0, s, a);
+  return MNV_LAUNCH_STATUS();
+}
+int by_dim(int dim, int (*f32)(const BwdArgs&, unsigned, hipStream_t), int (*f64)(const BwdArgs&, unsigned, hipStream_t),
+           int (*f96)(const BwdArgs&, unsigned, hipStream_t), int (*f128)(const BwdArgs&, unsigned, hipStream_t),
+           const BwdArgs& a, unsigned grid, hipStream_t s) {
+  return (dim <= 32 ? f32 : dim <= 64 ? f64 : dim <= 96 ? f96 : f128)(a, grid, s);
+}
 
 }  // namespace
 
 extern "C" {
 
-size_t mnv_attention_bwd_workspace_bytes(int, int, int, int, int, int, int) { return 0; }
+size_t mnv_attention_bwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim,
+                                         int has_bias) {
+  const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, 1.f};
+  if (!has_bias || !mnv_attention_sizes_ok(z)) return 0;
+  const size_t one = pair_bytes(z), all = one * batch * kv_heads;
+  if (all <= MNV_AT_PARTS_BYTES) return all;
+  return one > MNV_AT_PARTS_BYTES ? one : MNV_AT_PARTS_BYTES / one * one;
+}
 
 int mnv_attention_bwd(const float* q, const float* k, const float* v, const float* bias, const float* lengths,
                       const float* out, const float* stats, const float* dout, float* dq, float* dk, float* dv,
                       float* dbias, int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim, float scale,
-                      void*, size_t, mnv_stream_t stream) {
+                      void* workspace, size_t workspace_bytes, mnv_stream_t stream) {
   const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, scale};
   if (!q || !k || !v || !out || !stats || !dout || !dq || !dk || !dv || (bias && !dbias) || !mnv_attention_sizes_ok(z))
     return MNV_ERR_INVALID;
   const hipStream_t s = mnv_stream(stream);
-  const AttentionGrads a = {q, k, v, bias, lengths, out, stats, dout};
-  hipLaunchKernelGGL(mnv_attention_dq_kernel, dim3(row_grid((size_t)batch * q_len * heads)), dim3(MNV_WAVE), 0, s, a,
-                     dq, z);
+  BwdArgs a = {q, k, v, bias, lengths, out, stats, dout, dq, dk, dv, nullptr, z, 0, 0, q_len * z.group(),
+               mnv_fastdiv_make(z.group())};
+  const unsigned pairs = (unsigned)batch * kv_heads;
+  hipLaunchKernelGGL(mnv_attention_delta_kernel, dim3((unsigned)mnv_ceil_div(z.q_rows(), 16)), dim3(256), 0, s, dout,
+                     out, dq, z.q_rows(), head_dim);
   MNV_HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(mnv_attention_dkv_kernel, dim3(row_grid((size_t)batch * k_len * kv_heads)), dim3(MNV_WAVE), 0, s,
-                     a, dk, dv, z);
-  MNV_HIP_TRY(hipGetLastError());
-  if (bias)
-    hipLaunchKernelGGL(mnv_attention_dbias_kernel, dim3(row_grid(((size_t)q_len + k_len - 1) * heads)), dim3(MNV_WAVE),
-                       0, s, a, dbias, z);
-  return MNV_LAUNCH_STATUS();
+
+  // keys, with the bias's gradient as many pairs of an entry and a key head at a time as the workspace holds
+  size_t at_once = pairs;
+  if (bias) {
+    at_once = workspace ? workspace_bytes / pair_bytes(z) : 0;
+    if (at_once > pairs) at_once = pairs;
+    if (at_once) a.parts = static_cast<float*>(workspace);
+  }
+  BwdArgs ka = a;
+  if (bias && !at_once) at_once = pairs;
+  ka.tiles = (int)mnv_ceil_div(k_len, 128);
+  if ((unsigned long long)ka.tiles * at_once > 0x7fffffffULL) return MNV_ERR_INVALID;
+  for (unsigned p = 0; p < pairs; p += (unsigned)at_once) {
+    const unsigned now = pairs - p < at_once ? pairs - p : (unsigned)at_once;
+    ka.first_pair = p;
+    const int rc = by_dim(head_dim, launch_dkv<32>, launch_dkv<64>, launch_dkv<96>, launch_dkv<128>, ka, now * ka.tiles, s);
+    if (rc) return rc;
+    if (!a.parts) continue;
+    const dim3 grid((unsigned)mnv_ceil_div(z.offsets(), 256), heads < 65535 ? heads : 65535);
+    hipLaunchKernelGGL(mnv_attention_dbias_kernel, grid, dim3(256), 0, s, a.parts, lengths, dbias, z, p, now, p == 0);
+    MNV_HIP_TRY(hipGetLastError());
+  }
+  if (bias && !a.parts) {
+    const size_t work = z.offsets() * heads;
+    hipLaunchKernelGGL(mnv_attention_dbias_alone_kernel, dim3((unsigned)(work < (1u << 20) ? work : (1u << 20))),
+                       dim3(MNV_WAVE), 0, s, a, dbias);
+    MNV_HIP_TRY(hipGetLastError());
+  }
+  a.tiles = (int)mnv_ceil_div(a.rows, 128);
+  if ((unsigned long long)a.tiles * pairs > 0x7fffffffULL) return MNV_ERR_INVALID;
+  return by_dim(head_dim, launch_dq<32>, launch_dq<64>, launch_dq<96>, launch_dq<128>, a, a.tiles * pairs, s);
 }
 
 }  // extern "C"
