@@ -47,12 +47,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
   __shared__ __align__(16) float row_m[32], row_inverse[32], row_delta[32];
   __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
   const AttentionSizes& z = a.z;
-  const unsigned id = mnv_by_die(blockIdx.x, gridDim.x);
-  const int tile = (int)(id % a.tiles);
-  const unsigned pair = a.first_pair + id / a.tiles;
-  const int kh = (int)(pair % z.kv_heads), b = (int)(pair / z.kv_heads), group = z.group();
-  const int wave = threadIdx.x / MNV_WAVE, lane = threadIdx.x % MNV_WAVE, half = lane / 32;
-  const int n = mnv_visible(a.lengths, b, z.k_len);
+  const MnvAttentionPlace place = mnv_attention_place(a.tiles, a.first_pair, z, a.lengths);
+  const int tile = place.tile, b = place.b, kh = place.kh, n = place.n, group = z.group();
+  const int wave = mnv_uniform(threadIdx.x / MNV_WAVE), lane = threadIdx.x % MNV_WAVE, half = lane / 32;
 
   const int j = tile * 128 + wave * 32 + lane % 32;
   const size_t key = ((size_t)b * z.k_len + (j < z.k_len ? j : z.k_len - 1)) * z.kv_heads + kh;
@@ -70,14 +67,14 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       float x[8], y[8];
-      // a key that is not read may hold anything: another one stands in for it, and its weights are 0
+      // a key that is not read may hold anything: another one stands in for it, and 0 is stored
       const size_t at = ((size_t)b * z.k_len + (shown ? j : n - 1)) * z.kv_heads + kh;
       mnv_load8<DP>(a.k + at * z.dim, s, z.dim, x);
       mnv_load8<DP>(a.v + at * z.dim, s, z.dim, y);
       kp[s] = mnv_cut8(x);
       vp[s] = mnv_cut8(y);
     }
-    const size_t pitch = (size_t)z.heads * z.dim;
+    const unsigned pitch = (unsigned)z.heads * z.dim;
     const int jb = shown ? j : n - 1;
     for (int g = 0; g < group; ++g) {
       const int h = kh * group + g;
@@ -87,46 +84,45 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
       const float* bias = BIAS ? a.bias + h * z.offsets() + (jb + z.q_len - 1) : nullptr;
       float* parts = nullptr;
       if (BIAS && a.parts && tile * 128 + wave * 32 < n)  // no others are read
-        parts = a.parts + (((size_t)(pair - a.first_pair) * group + g) * key_tiles(z.k_len) + tile * 4 + wave) *
+        parts = a.parts + (((size_t)place.pair * group + g) * key_tiles(z.k_len) + tile * 4 + wave) *
                               diagonal_pitch(z.q_len);
       float carry = 0.f;
-      Stage stage;
-      float next_m = 0.f, next_l = 0.f, next_delta = 0.f;
-      auto fetch = [&](int i0) {
-        stage.fetch(qb + i0 * pitch, ob + i0 * pitch, pitch, z.q_len - i0, z.dim);
+      struct Rows {
+        Stage stage;
+        float m, inverse, delta;
+      };
+      auto fetch = [&](Rows& next, int i0) __attribute__((always_inline)) {
+        next.stage.fetch(qb + (size_t)i0 * pitch, ob + (size_t)i0 * pitch, pitch, z.q_len - i0, z.dim);
         if (threadIdx.x < 32) {
           const int i = i0 + (int)threadIdx.x;
           const size_t row = row0 + (size_t)(i < z.q_len ? i : z.q_len - 1) * z.heads;
-          next_m = mnv_finite_max(a.stats[2 * row]);
-          next_l = i < z.q_len ? mnv_inverse(a.stats[2 * row + 1]) : 0.f;
-          next_delta = i < z.q_len ? a.dq[row * z.dim] : 0.f;
+          next.m = mnv_finite_max(a.stats[2 * row]);
+          next.inverse = i < z.q_len ? mnv_inverse(a.stats[2 * row + 1]) : 0.f;
+          next.delta = a.dq[row * z.dim];
         }
       };
-      auto store = [&] {
-        stage.store(lds, z.scale);
+      auto store = [&](Rows& next) __attribute__((always_inline)) {
+        next.stage.store(lds, z.scale);
         if (threadIdx.x < 32) {
-          row_m[threadIdx.x] = next_m;
-          row_inverse[threadIdx.x] = next_l;
-          row_delta[threadIdx.x] = next_delta;
+          row_m[threadIdx.x] = next.m;
+          row_inverse[threadIdx.x] = next.inverse;
+          row_delta[threadIdx.x] = next.delta;
         }
       };
-      fetch(0);
-      store();
+      {
+        Rows first;
+        fetch(first, 0);
+        store(first);
+      }
       for (int i0 = 0; i0 < z.q_len; i0 += 32) {
         __syncthreads();
         const bool more = i0 + 32 < z.q_len;
-        if (more) fetch(i0 + 32);
+        Rows next;
+        if (more) fetch(next, i0 + 32);
 
         mnv_f16 t[1], dp[1];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t[0][e] = dp[0][e] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const MnvParts qp[1] = {Stage::by_rows(lds + Stage::ROWS0, 0, s)};
-          mnv_mul(t, qp, kp[s]);
-          const MnvParts op[1] = {Stage::by_rows(lds + Stage::ROWS1, 0, s)};
-          mnv_mul(dp, op, vp[s]);
-        }
+        Stage::product(t, lds + Stage::ROWS0, kp);
+        Stage::product(dp, lds + Stage::ROWS1, vp);
         if (BIAS) {
           const bool whole = i0 + 32 <= z.q_len;
 #pragma unroll
@@ -150,9 +146,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           const mnv_f4 delta = *reinterpret_cast<const mnv_f4*>(row_delta + at);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = shown ? mnv_weight(t[0][4 * u + e], m[e]) * il[e] : 0.f;
+            const float p = mnv_weight(t[0][4 * u + e], m[e]) * il[e];
             t[0][4 * u + e] = p;
-            dp[0][4 * u + e] = shown ? p * (dp[0][4 * u + e] - delta[e]) : 0.f;
+            dp[0][4 * u + e] = p * (dp[0][4 * u + e] - delta[e]);
           }
         }
 #pragma unroll
@@ -185,7 +181,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int i = mnv_acc_row(e, half);
-              mine[i * 47 + 15 + lane % 32] = dp[0][8 * part + e];
+              mine[i * 47 + 15 + lane % 32] = shown ? dp[0][8 * part + e] : 0.f;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -205,13 +201,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           carry = lane >= 32 && lane < 63 ? carry : 0.f;
         }
         __syncthreads();
-        if (more) store();
+        if (more) store(next);
       }
     }
   }
   if (j < z.k_len) {
-    mnv_store_column<DP>(dk, j < n ? 1.f : 0.f, a.dk + key * z.dim, z.dim);
-    mnv_store_column<DP>(dv, j < n ? 1.f : 0.f, a.dv + key * z.dim, z.dim);
+    mnv_store_column<DP>(dk, 1.f, j < n, a.dk + key * z.dim, z.dim);
+    mnv_store_column<DP>(dv, 1.f, j < n, a.dv + key * z.dim, z.dim);
   }
 }
 
@@ -221,12 +217,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
   using Stage = MnvStage<DP, 32, 256, 3, 1>;  // keys either way, values by rows
   __shared__ __align__(16) char lds[Stage::BYTES];
   const AttentionSizes& z = a.z;
-  const unsigned id = mnv_by_die(blockIdx.x, gridDim.x);
-  const int tile = (int)(id % a.tiles);
-  const unsigned pair = id / a.tiles;
-  const int kh = (int)(pair % z.kv_heads), b = (int)(pair / z.kv_heads);
+  const MnvAttentionPlace place = mnv_attention_place(a.tiles, 0, z, a.lengths);
+  const int tile = place.tile, b = place.b, kh = place.kh, n = place.n;
   const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
-  const int n = mnv_visible(a.lengths, b, z.k_len);
 
   const int r = tile * 128 + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
   const int rc = r < a.rows ? r : a.rows - 1;
@@ -258,29 +251,25 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     }
     delta += __shfl_xor(delta, 32, MNV_WAVE);
     const float m = mnv_finite_max(a.stats[2 * row]), il = mnv_inverse(a.stats[2 * row + 1]);
-    const size_t pitch = (size_t)z.kv_heads * z.dim;
+    const unsigned pitch = (unsigned)z.kv_heads * z.dim;
     const float* kb = a.k + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
     const float* vb = a.v + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
     const float* bias = BIAS ? a.bias + h * z.offsets() + (z.q_len - 1 - i) : nullptr;
 
-    Stage stage;
-    stage.fetch(kb, vb, pitch, n, z.dim);
-    stage.store(lds, 1.f);
+    {
+      Stage first;
+      first.fetch(kb, vb, pitch, n, z.dim);
+      first.store(lds, 1.f);
+    }
     for (int j0 = 0; j0 < n; j0 += 32) {
       __syncthreads();
       const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
-      if (more) stage.fetch(kb + (j0 + 32) * pitch, vb + (j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
+      Stage stage;
+      if (more) stage.fetch(kb + (size_t)(j0 + 32) * pitch, vb + (size_t)(j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
 
       mnv_f16 t[1], dp[1];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) t[0][e] = dp[0][e] = 0.f;
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const MnvParts kp[1] = {Stage::by_rows(lds + Stage::ROWS0, 0, s)};
-        mnv_mul(t, kp, qp[s]);
-        const MnvParts vp[1] = {Stage::by_rows(lds + Stage::ROWS1, 0, s)};
-        mnv_mul(dp, vp, op[s]);
-      }
+      Stage::product(t, lds + Stage::ROWS0, qp);
+      Stage::product(dp, lds + Stage::ROWS1, op);
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -298,6 +287,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
 #pragma unroll
       for (int e = 0; e < 16; ++e) dp[0][e] = mnv_weight(t[0][e], m) * il * (dp[0][e] - delta);
       if (!whole) {
+        MNV_KEEP_BRANCH();
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (j0 + mnv_acc_row(e, half) >= n) dp[0][e] = 0.f;
@@ -318,7 +308,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
       if (more) stage.store(lds, 1.f);
     }
   }
-  if (r < a.rows) mnv_store_column<DP>(dq, z.scale, a.dq + row * z.dim, z.dim);
+  if (r < a.rows) mnv_store_column<DP>(dq, z.scale, true, a.dq + row * z.dim, z.dim);
 }
 
 // dbias[o] += the parts of o: of every entry among the launch's pairs and every 32 keys that have the diagonal.

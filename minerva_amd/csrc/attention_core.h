@@ -19,6 +19,7 @@
 #include "gemm_split.h"
 
 #define MNV_AT_MAX_DIM 128
+#define MNV_AT_MAX_PITCH (1 << 24)  // heads * dim: 64 rows of it are less than 2^32 bytes
 
 struct AttentionSizes {
   int batch, heads, kv_heads, q_len, k_len, dim;
@@ -30,7 +31,7 @@ struct AttentionSizes {
 
 static inline bool mnv_attention_sizes_ok(const AttentionSizes& z) {
   if (z.batch < 1 || z.heads < 1 || z.kv_heads < 1 || z.q_len < 1 || z.k_len < 1 || z.dim < 1) return false;
-  if (z.dim > MNV_AT_MAX_DIM || z.heads % z.kv_heads) return false;
+  if (z.dim > MNV_AT_MAX_DIM || z.heads % z.kv_heads || z.heads > MNV_AT_MAX_PITCH / z.dim) return false;
   const long long most = 0x7fffffffLL, d = z.dim > 2 ? z.dim : 2;  // stats has two values where out has dim
   if ((long long)z.batch * z.heads > most || (long long)z.batch * z.heads * z.q_len > most / d) return false;
   if ((long long)z.batch * z.kv_heads * z.k_len > most / z.dim) return false;
@@ -42,12 +43,45 @@ static inline bool mnv_attention_sizes_ok(const AttentionSizes& z) {
 
 typedef float mnv_f16 __attribute__((ext_vector_type(16)));
 
+// A value that is the same in all lanes, in a scalar register: so are the addresses made from it.
+__device__ __forceinline__ int mnv_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// In a branch that few tiles take: without it, its selections run for all.
+#define MNV_KEEP_BRANCH() asm volatile("")
+
 // Keys of entry b that are read.
 __device__ __forceinline__ int mnv_visible(const float* lengths, int b, int k_len) {
   if (!lengths) return k_len;
   const float n = lengths[b];
   if (!(n > 0.f)) return 0;
   return n >= (float)k_len ? k_len : (int)n;
+}
+
+// The workgroup's place.  Workgroups go to the 8 dies in turn: all of one entry and key head go to one die, whose
+// L2 then holds the keys they share, and neighbouring heads to different ones, so that entries of different lengths
+// load all dies alike.
+struct MnvAttentionPlace {
+  int tile, b, kh;
+  unsigned pair;  // entry and key head, from the launch's first on
+  int n;          // keys of the entry
+};
+__device__ __forceinline__ MnvAttentionPlace mnv_attention_place(unsigned tiles, unsigned first_pair,
+                                                                 const AttentionSizes& z, const float* lengths) {
+  MnvAttentionPlace p;
+  const unsigned even = gridDim.x / tiles / 8 * 8 * tiles;  // workgroups of the pairs that fill all dies
+  if (blockIdx.x < even) {
+    const unsigned row = mnv_uniform(blockIdx.x / 8 / tiles);
+    p.pair = row * 8 + blockIdx.x % 8;
+    p.tile = blockIdx.x / 8 - row * tiles;
+  } else {
+    p.pair = mnv_uniform(blockIdx.x / tiles);
+    p.tile = blockIdx.x - p.pair * tiles;
+  }
+  const unsigned pair = first_pair + p.pair;
+  p.b = mnv_uniform(pair / z.kv_heads);
+  p.kh = pair - p.b * z.kv_heads;
+  p.n = mnv_uniform(mnv_visible(lengths, p.b, z.k_len));
+  return p;
 }
 
 // exp(t - m), and 0 for a hidden t = -inf where hidden ones alone leave m at -inf too (m: see mnv_finite_max).
@@ -77,12 +111,13 @@ __device__ __forceinline__ MnvParts mnv_cut8(const float* x) {
   return r;
 }
 
-// acc[n] += a[n] * b for N tiles at once (independent sums between dependent ones), the smallest terms first.
-template <int N>
+// acc[n] += a[n] * b for N tiles at once (independent sums between dependent ones), the smallest terms first:
+// part products FROM to TO - 1.
+template <int N, int FROM = 0, int TO = 6>
 __device__ __forceinline__ void mnv_mul(mnv_f16* acc, const MnvParts (&a)[N], const MnvParts& b) {
   constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
-  for (int t = 0; t < 6; ++t)
+  for (int t = FROM; t < TO; ++t)
 #pragma unroll
     for (int n = 0; n < N; ++n)
       acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[n].p[PA[t]], b.p[PB[t]], acc[n], 0, 0, 0);
@@ -106,68 +141,73 @@ struct MnvStage {
   static constexpr int BYTES = COLS1 + (FORM1 & 2 ? COL_BYTES : 0);
   static_assert(QUADS % MNV_WAVE == 0, "a wavefront's blocks are all of one matrix");
 
-  float v[SLOTS][4][4];
+  mnv_f4 v[SLOTS][4];
 
   struct At {
-    bool any, second;
+    bool any, second;  // the same for the whole wavefront
     int row, col;
   };
-  __device__ static At at(int s) {
-    int q = s * NT + (int)threadIdx.x;
+  __device__ static __forceinline__ At at(int s) {
+    const unsigned first = s * NT + mnv_uniform(threadIdx.x / MNV_WAVE) * MNV_WAVE;
     At a;
-    a.any = 2 * QUADS % NT == 0 || q < 2 * QUADS;
-    a.second = q >= QUADS;
-    if (a.second) q -= QUADS;
+    a.any = 2 * QUADS % NT == 0 || first < 2 * QUADS;
+    a.second = QUADS % NT == 0 ? s >= QUADS / NT : first >= QUADS;
+    const unsigned q = first % QUADS + threadIdx.x % MNV_WAVE;
     a.row = 4 * (q % 4 + 4 * (q / 4 / DQ));
     a.col = 4 * (q / 4 % DQ);
     return a;
   }
 
-  // rows >= 1 of the tile exist; those behind them and the columns from dim on become 0.
-  __device__ void fetch(const float* m0, const float* m1, size_t pitch, int rows, int dim) {
-    const bool whole = rows >= ROWS && dim == DP;
+  // Fetches the tile from rows >= 1 rows that exist.  In place of a row behind them comes the last one, and in place
+  // of a column behind dim another of the row: what they are multiplied by is 0, and they hold nothing that
+  // has no part in the result anyway, so no value is selected and nothing waits before `store`.  Byte
+  // offsets within a tile fit 32 bits (MNV_AT_MAX_PITCH).
+  __device__ __forceinline__ void fetch(const float* m0, const float* m1, unsigned pitch, int rows, int dim) {
+    if (dim % 4 == 0 && rows >= ROWS) {
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      const At a = at(s);
-      if (!a.any) continue;
-      const float* m = a.second ? m1 : m0;
-      if (whole) {
-        const float* p = m + a.row * pitch + a.col;
+      for (int s = 0; s < SLOTS; ++s) {
+        const At a = at(s);
+        if (!a.any) continue;
+        const unsigned off = ((unsigned)a.row * pitch + (unsigned)(a.col < dim - 4 ? a.col : dim - 4)) * 4;
+        const float* m = a.second ? m1 : m0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[s][i] = get(m + (size_t)i * pitch, off);
+      }
+    } else if (dim % 4 == 0) {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) {
+        const At a = at(s);
+        if (!a.any) continue;
+        const unsigned col = (unsigned)(a.col < dim - 4 ? a.col : dim - 4);
+        const float* m = a.second ? m1 : m0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[s][i] = get(m, ((unsigned)(a.row + i < rows ? a.row + i : rows - 1) * pitch + col) * 4);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) {
+        const At a = at(s);
+        if (!a.any) continue;
+        const float* m = a.second ? m1 : m0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const mnv_f4 t = mnv_ldx4u<false>(p + i * pitch);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[s][i][c] = t[c];
-        }
-      } else if (dim % 4 == 0) {
-        const int col = a.col < dim ? a.col : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = a.row + i < rows ? a.row + i : rows - 1;
-          const mnv_f4 t = mnv_ldx4u<false>(m + r * pitch + col);
-          const bool in = a.row + i < rows && a.col < dim;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) v[s][i][c] = in ? t[c] : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = a.row + i < rows ? a.row + i : rows - 1;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const float t = m[r * pitch + (a.col + c < dim ? a.col + c : 0)];
-            v[s][i][c] = a.row + i < rows && a.col + c < dim ? t : 0.f;
-          }
+          const float* p = m + (unsigned)(a.row + i < rows ? a.row + i : rows - 1) * pitch;
+          v[s][i] = mnv_f4{p[a.col < dim ? a.col : dim - 1], p[a.col + 1 < dim ? a.col + 1 : dim - 1],
+                           p[a.col + 2 < dim ? a.col + 2 : dim - 1], p[a.col + 3 < dim ? a.col + 3 : dim - 1]};
         }
       }
     }
   }
+  __device__ static __forceinline__ mnv_f4 get(const float* m, unsigned off) {
+    return mnv_ldx4u<false>(reinterpret_cast<const float*>(reinterpret_cast<const char*>(m) + off));
+  }
 
   // Place of row `row` (a multiple of 4) and its three successors in a column.
-  __device__ static int place(int row) { return row / 16 * 16 + (row / 4 % 2) * 8 + (row / 8 % 2) * 4; }
+  __device__ static __forceinline__ int place(int row) { return row / 16 * 16 + (row / 4 % 2) * 8 + (row / 8 % 2) * 4; }
 
-  // scale0: factor of the first matrix
-  __device__ void store(char* lds, float scale0) {
+  // Cuts the tile into its planes.  scale0: factor of the first matrix.
+  __device__ __forceinline__ void store(char* lds, float scale0) {
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const At a = at(s);
@@ -179,7 +219,7 @@ struct MnvStage {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           unsigned t[3];
-          mnv_split_pair(v[s][i][2 * h] * f, v[s][i][2 * h + 1] * f, 1.f, t);
+          mnv_split_pair(v[s][i][2 * h], v[s][i][2 * h + 1], f, t);
 #pragma unroll
           for (int p = 0; p < 3; ++p) w[p][i][h] = t[p];
         }
@@ -207,21 +247,50 @@ struct MnvStage {
   }
 
   // Operands of the 32 rows from `row` on, columns 16 s ... of step s; and of the 32 columns from `col` on, rows 16 s...
-  __device__ static MnvParts by_rows(const char* plane, int row, int s) {
+  template <int PARTS = 3>
+  __device__ static __forceinline__ MnvParts by_rows(const char* plane, int row, int s) {
     const int lane = threadIdx.x % MNV_WAVE;
     const char* p = plane + ((row + lane % 32) * RP + s * 16 + lane / 32 * 8) * 2;
     MnvParts r;
 #pragma unroll
-    for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * ROWS * RP * 2);
+    for (int c = 0; c < PARTS; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * ROWS * RP * 2);
     return r;
   }
-  __device__ static MnvParts by_cols(const char* plane, int col, int s) {
+  __device__ static __forceinline__ MnvParts by_cols(const char* plane, int col, int s) {
     const int lane = threadIdx.x % MNV_WAVE;
     const char* p = plane + ((col + lane % 32) * CP + s * 16 + lane / 32 * 8) * 2;
     MnvParts r;
 #pragma unroll
     for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * DP * CP * 2);
     return r;
+  }
+
+  // acc[n] = the 32 rows from 32 n on, by rows, times the operand b over all columns.  The matrix instruction
+  // rounds its sums down, by up to a step of the larger of the sum and the terms: with the five small part
+  // products of all steps before the first large one only the DP / 16 last instructions do so at the full
+  // sum's size.  (In the order of the steps the scores' gradients are off by the same sign everywhere, 2^-27 of
+  // them: nothing to a value, but a bucket's gradient sums 10^5 that cancel.  12 heads of 512 x 512: table's
+  // gradient off by 4.0e-6.)
+  template <int N>
+  __device__ static __forceinline__ void product(mnv_f16 (&acc)[N], const char* plane, const MnvParts (&b)[DP / 16]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      MnvParts a[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) a[n] = by_rows(plane, 32 * n, s);
+      mnv_mul<N, 0, 5>(acc, a, b[s]);
+    }
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      MnvParts a[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) a[n] = by_rows<1>(plane, 32 * n, s);
+      mnv_mul<N, 5, 6>(acc, a, b[s]);
+    }
   }
 };
 
@@ -245,9 +314,10 @@ __device__ __forceinline__ void mnv_load8(const float* row, int s, int dim, floa
   }
 }
 
-// Writes the lane's column of a [DP x 32] result, times f, to the dim values of `row`.
+// Writes the lane's column of a [DP x 32] result, times f, to the dim values of `row`; 0 where it is not wanted.
 template <int DP>
-__device__ __forceinline__ void mnv_store_column(const mnv_f16 (&acc)[DP / 32], float f, float* row, int dim) {
+__device__ __forceinline__ void mnv_store_column(const mnv_f16 (&acc)[DP / 32], float f, bool wanted, float* row,
+                                                 int dim) {
   const int half = (int)threadIdx.x % MNV_WAVE / 32;
 #pragma unroll
   for (int n = 0; n < DP / 32; ++n)
@@ -256,7 +326,7 @@ __device__ __forceinline__ void mnv_store_column(const mnv_f16 (&acc)[DP / 32], 
       const int d = n * 32 + 8 * u + 4 * half;
       mnv_f4 t;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = acc[n][4 * u + e] * f;
+      for (int e = 0; e < 4; ++e) t[e] = wanted ? acc[n][4 * u + e] * f : 0.f;
       if (d + 4 <= dim) {
         *reinterpret_cast<mnv_f4u*>(row + d) = t;
       } else {
@@ -267,9 +337,4 @@ __device__ __forceinline__ void mnv_store_column(const mnv_f16 (&acc)[DP / 32], 
     }
 }
 
-// Consecutive work items go to one of the 8 dies, whose L2 then holds what they share.
-__device__ __forceinline__ unsigned mnv_by_die(unsigned id, unsigned total) {
-  const unsigned each = total / 8;
-  return id < each * 8 ? id % 8 * each + id / 8 : id;
-}
 #endif

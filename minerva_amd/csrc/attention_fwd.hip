@@ -27,12 +27,9 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   using Stage = MnvStage<DP, BK, 256, 1, 2>;  // keys by rows, values by columns
   __shared__ __align__(16) char lds[Stage::BYTES];
   const AttentionSizes& z = a.z;
-  const unsigned id = mnv_by_die(blockIdx.x, gridDim.x);
-  const int tile = (int)(id % a.row_tiles);
-  const unsigned pair = id / a.row_tiles;
-  const int kh = (int)(pair % z.kv_heads), b = (int)(pair / z.kv_heads);
+  const MnvAttentionPlace place = mnv_attention_place(a.row_tiles, 0, z, a.lengths);
+  const int tile = place.tile, b = place.b, kh = place.kh, n = place.n;
   const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
-  const int n = mnv_visible(a.lengths, b, z.k_len);
 
   const int r = tile * 128 + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
   const int rc = r < a.rows ? r : a.rows - 1;
@@ -56,31 +53,24 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
       for (int e = 0; e < 8; ++e) x[e] *= z.scale;
       qp[s] = mnv_cut8(x);
     }
-    const size_t pitch = (size_t)z.kv_heads * z.dim;
+    const unsigned pitch = (unsigned)z.kv_heads * z.dim;
     const float* kb = a.k + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
     const float* vb = a.v + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
     const float* bias = BIAS ? a.bias + h * z.offsets() + (z.q_len - 1 - i) : nullptr;
 
-    Stage stage;
-    stage.fetch(kb, vb, pitch, n, z.dim);
-    stage.store(lds, 1.f);
+    {
+      Stage first;
+      first.fetch(kb, vb, pitch, n, z.dim);
+      first.store(lds, 1.f);
+    }
     for (int j0 = 0; j0 < n; j0 += BK) {
       __syncthreads();
       const bool more = j0 + BK < n;
-      if (more) stage.fetch(kb + (j0 + BK) * pitch, vb + (j0 + BK) * pitch, pitch, n - j0 - BK, z.dim);
+      Stage stage;
+      if (more) stage.fetch(kb + (size_t)(j0 + BK) * pitch, vb + (size_t)(j0 + BK) * pitch, pitch, n - j0 - BK, z.dim);
 
       mnv_f16 t[KB];
-#pragma unroll
-      for (int c = 0; c < KB; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) t[c][e] = 0.f;
-#pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-        MnvParts kp[KB];
-#pragma unroll
-        for (int c = 0; c < KB; ++c) kp[c] = Stage::by_rows(lds + Stage::ROWS0, c * 32, s);
-        mnv_mul(t, kp, qp[s]);
-      }
+      Stage::product(t, lds + Stage::ROWS0, qp);
       const bool whole = j0 + BK <= n;
       if (BIAS) {
 #pragma unroll
@@ -99,6 +89,7 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
           }
       }
       if (!whole) {
+        MNV_KEEP_BRANCH();
 #pragma unroll
         for (int c = 0; c < KB; ++c)
 #pragma unroll
@@ -148,7 +139,7 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
     l += __shfl_xor(l, 32, MNV_WAVE);
   }
   if (r < a.rows) {
-    mnv_store_column<DP>(acc, mnv_inverse(l), a.out + row * z.dim, z.dim);
+    mnv_store_column<DP>(acc, mnv_inverse(l), true, a.out + row * z.dim, z.dim);
     if (half == 0) {
       a.stats[2 * row] = m;
       a.stats[2 * row + 1] = l;
