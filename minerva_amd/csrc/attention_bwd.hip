@@ -42,9 +42,9 @@ __host__ __device__ inline size_t key_tiles(int k_len) { return ((size_t)k_len +
 template <int DP, bool BIAS>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  using Stage = MnvStage<DP, 32, 256, 3, 3>;  // queries (times scale) and their gradients, either way
-  __shared__ __align__(16) char lds[Stage::BYTES];
-  __shared__ __align__(16) float row_m[32], row_inverse[32], row_delta[32];
+  using Stage = MnvStage<DP, 256>;  // queries (times scale) and their gradients
+  __shared__ __align__(16) char lds[2 * Stage::BYTES];
+  __shared__ __align__(16) float row_stats[2][3][32];  // m, 1 / l, delta of the tile's queries
   __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
   const AttentionSizes& z = a.z;
   const MnvAttentionPlace place = mnv_attention_place(a.tiles, a.first_pair, z, a.lengths);
@@ -96,33 +96,36 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
         if (threadIdx.x < 32) {
           const int i = i0 + (int)threadIdx.x;
           const size_t row = row0 + (size_t)(i < z.q_len ? i : z.q_len - 1) * z.heads;
+          const float sign = i % 2 ? -1.f : 1.f;
           next.m = mnv_finite_max(a.stats[2 * row]);
-          next.inverse = i < z.q_len ? mnv_inverse(a.stats[2 * row + 1]) : 0.f;
-          next.delta = a.dq[row * z.dim];
+          next.inverse = i < z.q_len ? sign * mnv_inverse(a.stats[2 * row + 1]) : 0.f;
+          next.delta = sign * a.dq[row * z.dim];
         }
       };
-      auto store = [&](Rows& next) __attribute__((always_inline)) {
-        next.stage.store(lds, z.scale);
+      auto store = [&](const Rows& next, int turn) __attribute__((always_inline)) {
+        next.stage.template store<true>(lds + turn * Stage::BYTES, z.scale);
         if (threadIdx.x < 32) {
-          row_m[threadIdx.x] = next.m;
-          row_inverse[threadIdx.x] = next.inverse;
-          row_delta[threadIdx.x] = next.delta;
+          row_stats[turn][0][threadIdx.x] = next.m;
+          row_stats[turn][1][threadIdx.x] = next.inverse;
+          row_stats[turn][2][threadIdx.x] = next.delta;
         }
       };
       {
         Rows first;
         fetch(first, 0);
-        store(first);
+        store(first, 0);
       }
+      __syncthreads();
+      int turn = 0;
       for (int i0 = 0; i0 < z.q_len; i0 += 32) {
-        __syncthreads();
         const bool more = i0 + 32 < z.q_len;
         Rows next;
         if (more) fetch(next, i0 + 32);
+        const char* now = lds + turn * Stage::BYTES;
 
-        mnv_f16 t[1], dp[1];
-        Stage::product(t, lds + Stage::ROWS0, kp);
-        Stage::product(dp, lds + Stage::ROWS1, vp);
+        mnv_f16 t, dp;
+        Stage::product(t, now, kp);
+        Stage::product(dp, now + Stage::MATRIX, vp);
         if (BIAS) {
           const bool whole = i0 + 32 <= z.q_len;
 #pragma unroll
@@ -131,24 +134,23 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
             if (whole) {
               const mnv_f4 add = mnv_ldx4u<false>(bias - (i + 3));
 #pragma unroll
-              for (int e = 0; e < 4; ++e) t[0][4 * u + e] += add[3 - e];
+              for (int e = 0; e < 4; ++e) t[4 * u + e] += add[3 - e];
             } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) t[0][4 * u + e] += bias[-(i + e < z.q_len ? i + e : z.q_len - 1)];
+              for (int e = 0; e < 4; ++e) t[4 * u + e] += bias[-(i + e < z.q_len ? i + e : z.q_len - 1)];
             }
           }
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int at = 8 * u + 4 * half;
-          const mnv_f4 m = *reinterpret_cast<const mnv_f4*>(row_m + at);
-          const mnv_f4 il = *reinterpret_cast<const mnv_f4*>(row_inverse + at);
-          const mnv_f4 delta = *reinterpret_cast<const mnv_f4*>(row_delta + at);
+          const mnv_f4 m = *reinterpret_cast<const mnv_f4*>(row_stats[turn][0] + at);
+          const mnv_f4 il = *reinterpret_cast<const mnv_f4*>(row_stats[turn][1] + at);
+          const mnv_f4 delta = *reinterpret_cast<const mnv_f4*>(row_stats[turn][2] + at);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float p = mnv_weight(t[0][4 * u + e], m[e]) * il[e];
-            t[0][4 * u + e] = p;
-            dp[0][4 * u + e] = p * (dp[0][4 * u + e] - delta[e]);
+            t[4 * u + e] = mnv_weight(t[4 * u + e], m[e]) * il[e];
+            dp[4 * u + e] = t[4 * u + e] * (dp[4 * u + e] - delta[e]);
           }
         }
 #pragma unroll
@@ -156,17 +158,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           float x[8], y[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            x[e] = t[0][8 * s + e];
-            y[e] = dp[0][8 * s + e];
+            x[e] = t[8 * s + e];
+            y[e] = dp[8 * s + e];
           }
-          const MnvParts pp = mnv_cut8(x), sp = mnv_cut8(y);
-#pragma unroll
-          for (int c = 0; c < NB; ++c) {
-            const MnvParts op[1] = {Stage::by_cols(lds + Stage::COLS1, c * 32, s)};
-            mnv_mul(dv + c, op, pp);
-            const MnvParts qp[1] = {Stage::by_cols(lds + Stage::COLS0, c * 32, s)};
-            mnv_mul(dk + c, qp, sp);
-          }
+          Stage::add_columns(dv, now + Stage::MATRIX, s, mnv_cut8(x));
+          Stage::add_columns(dk, now, s, mnv_cut8(y));
         }
         if (BIAS && parts) {
           // Lane u sums the diagonal key - query = u - 31 of the 32 x 32 tile: 16 queries at a time go to LDS,
@@ -181,7 +177,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const int i = mnv_acc_row(e, half);
-              mine[i * 47 + 15 + lane % 32] = shown ? dp[0][8 * part + e] : 0.f;
+              mine[i * 47 + 15 + lane % 32] = shown ? dp[8 * part + e] : 0.f;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -200,8 +196,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           carry = __shfl(sum, lane - 32, MNV_WAVE);
           carry = lane >= 32 && lane < 63 ? carry : 0.f;
         }
+        turn ^= 1;
+        if (more) store(next, turn);
         __syncthreads();
-        if (more) store(next);
       }
     }
   }
@@ -214,8 +211,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
 template <int DP, bool BIAS>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  using Stage = MnvStage<DP, 32, 256, 3, 1>;  // keys either way, values by rows
-  __shared__ __align__(16) char lds[Stage::BYTES];
+  using Stage = MnvStage<DP, 256>;  // keys and values
+  __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
   const MnvAttentionPlace place = mnv_attention_place(a.tiles, 0, z, a.lengths);
   const int tile = place.tile, b = place.b, kh = place.kh, n = place.n;
@@ -259,17 +256,18 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     {
       Stage first;
       first.fetch(kb, vb, pitch, n, z.dim);
-      first.store(lds, 1.f);
+      first.template store<false>(lds, 1.f);
     }
+    __syncthreads();
+    char* now = lds;
     for (int j0 = 0; j0 < n; j0 += 32) {
-      __syncthreads();
       const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
       Stage stage;
       if (more) stage.fetch(kb + (size_t)(j0 + 32) * pitch, vb + (size_t)(j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
 
-      mnv_f16 t[1], dp[1];
-      Stage::product(t, lds + Stage::ROWS0, qp);
-      Stage::product(dp, lds + Stage::ROWS1, op);
+      mnv_f16 t, dp;
+      Stage::product(t, now, qp);
+      Stage::product(dp, now + Stage::MATRIX, op);
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -277,35 +275,31 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
           if (whole) {
             const mnv_f4 add = mnv_ldx4u<false>(bias + j);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[0][4 * u + e] += add[e];
+            for (int e = 0; e < 4; ++e) t[4 * u + e] += add[e];
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[0][4 * u + e] += bias[j + e < n ? j + e : n - 1];
+            for (int e = 0; e < 4; ++e) t[4 * u + e] += bias[j + e < n ? j + e : n - 1];
           }
         }
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dp[0][e] = mnv_weight(t[0][e], m) * il * (dp[0][e] - delta);
+      for (int e = 0; e < 16; ++e) dp[e] = mnv_weight(t[e], m) * il * (dp[e] - delta);
       if (!whole) {
         MNV_KEEP_BRANCH();
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (j0 + mnv_acc_row(e, half) >= n) dp[0][e] = 0.f;
+          if (j0 + mnv_acc_row(e, half) >= n) dp[e] = 0.f;
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = dp[0][8 * s + e];
-        const MnvParts sp = mnv_cut8(x);
-#pragma unroll
-        for (int c = 0; c < NB; ++c) {
-          const MnvParts kp[1] = {Stage::by_cols(lds + Stage::COLS0, c * 32, s)};
-          mnv_mul(dq + c, kp, sp);
-        }
+        for (int e = 0; e < 8; ++e) x[e] = dp[8 * s + e];
+        Stage::add_columns(dq, now, s, mnv_cut8(x));
       }
+      now = lds + (now == lds ? Stage::BYTES : 0);
+      if (more) stage.template store<false>(now, 1.f);
       __syncthreads();
-      if (more) stage.store(lds, 1.f);
     }
   }
   if (r < a.rows) mnv_store_column<DP>(dq, z.scale, true, a.dq + row * z.dim, z.dim);

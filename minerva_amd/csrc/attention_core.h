@@ -1,18 +1,18 @@
 // What the attention kernels share: sizes, tiles of a sequence in LDS, and products of them on the matrix cores.
 //
-// Every product is one of a tile that streams through LDS (32 or 64 rows of two matrices, by the whole
-// workgroup) and an operand that a wavefront holds in registers for its own 32 columns: 32 queries in the
-// forward pass and for dq, 32 keys for dk and dv.  fp32 values are cut into three bf16 parts and six of
-// the nine part products are summed (gemm_split.h): the bf16 matrix instruction at 6 products per value
-// has 2.6 times the fp32 one's rate.
+// Every product is one of a tile of 32 rows that streams through LDS (two matrices, fetched and cut by the whole
+// workgroup, two tiles in turn, so that one is cut while the other is multiplied) and an operand that a
+// wavefront holds in registers for its own 32 columns: 32 queries in the forward pass and for dq, 32 keys for dk
+// and dv.  fp32 values are cut into three bf16 parts and six of the nine part products are summed
+// (gemm_split.h): the bf16 matrix instruction at 6 products per value has 2.6 times the fp32 one's rate.
 //
 // The 32 x 32 x 16 instruction gives lane l the column l % 32 and the rows 8 (r / 4) + 4 (l / 32) + r % 4 of
 // the result, r = 0..15.  As an operand, lane l holds the 8 contraction places 8 (l / 32)... of column (or
 // row) l % 32.  Which rows stand in which contraction places is free as long as both operands agree, so a
 // result (scores, weights) becomes the next product's operand without leaving its lane: places 8 h + e
-// of step s hold the rows 16 s + 4 h + e (e < 4) and 16 s + 8 + 4 h + e - 4, and the other operand's tile is
-// written to LDS in that order (`place`).  So the softmax's sums run over a lane's own registers and one exchange
-// between the two half wavefronts.
+// of step s hold the rows 16 s + 4 h + e (e < 4) and 16 s + 4 h + 8 + e - 4, and the other operand, the tile by
+// columns, is read in that order: the transposing LDS read gives each of 16 lanes four rows of its column.
+// So the softmax's sums run over a lane's own registers and one exchange between the two half wavefronts.
 #pragma once
 #include <math.h>
 
@@ -111,37 +111,27 @@ __device__ __forceinline__ MnvParts mnv_cut8(const float* x) {
   return r;
 }
 
-// acc[n] += a[n] * b for N tiles at once (independent sums between dependent ones), the smallest terms first:
-// part products FROM to TO - 1.
-template <int N, int FROM = 0, int TO = 6>
-__device__ __forceinline__ void mnv_mul(mnv_f16* acc, const MnvParts (&a)[N], const MnvParts& b) {
+// acc += a * b, the smallest terms first.
+__device__ __forceinline__ void mnv_mul(mnv_f16& acc, const MnvParts& a, const MnvParts& b) {
   constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
-  for (int t = FROM; t < TO; ++t)
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-      acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[n].p[PA[t]], b.p[PB[t]], acc[n], 0, 0, 0);
+  for (int t = 0; t < 6; ++t) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[PA[t]], b.p[PB[t]], acc, 0, 0, 0);
 }
 
 // Row of result register r, for lanes of half h.
 __device__ __forceinline__ constexpr int mnv_acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
 
-// ROWS consecutive rows of two matrices (of up to DP columns, `pitch` floats from row to row) on their way
-// from memory to LDS: fetched into registers a tile ahead, then cut into planes of parts, by rows (FORM & 1), for
-// products that contract the columns, by columns (FORM & 2), for those that contract the rows, or both.
-// A thread takes blocks of 4 x 4 values, so that both forms are written 8 bytes at a time; the
-// four row blocks and 16 column blocks of a wavefront reach all banks in either.
-template <int DP, int ROWS, int NT, int FORM0, int FORM1>
+// 32 consecutive rows of two matrices (of up to DP columns, `pitch` floats from row to row) on their way from
+// memory to LDS: fetched into registers a tile ahead, then cut into planes of parts.  Rows lie DP + 16 bf16
+// apart: an odd multiple of 8 banks' words, so that 8 rows of 16 bytes (by rows) and 4 rows of 32
+// (by columns) are in different banks.
+template <int DP, int NT>
 struct MnvStage {
-  static constexpr int DQ = DP / 4, QUADS = ROWS / 4 * DQ, SLOTS = (2 * QUADS + NT - 1) / NT;
-  static constexpr int RP = DP + 8, CP = ROWS + 8;  // bf16 from row to row, and from column to column
-  static constexpr int ROW_BYTES = 3 * ROWS * RP * 2, COL_BYTES = 3 * DP * CP * 2;
-  static constexpr int ROWS0 = 0, COLS0 = ROWS0 + (FORM0 & 1 ? ROW_BYTES : 0);
-  static constexpr int ROWS1 = COLS0 + (FORM0 & 2 ? COL_BYTES : 0), COLS1 = ROWS1 + (FORM1 & 1 ? ROW_BYTES : 0);
-  static constexpr int BYTES = COLS1 + (FORM1 & 2 ? COL_BYTES : 0);
-  static_assert(QUADS % MNV_WAVE == 0, "a wavefront's blocks are all of one matrix");
+  static constexpr int CHUNKS = DP / 8, UNITS = 32 * CHUNKS, SLOTS = (2 * UNITS + NT - 1) / NT;
+  static constexpr int PITCH = (DP + 16) * 2, PLANE = 32 * PITCH, MATRIX = 3 * PLANE, BYTES = 2 * MATRIX;
+  static_assert(UNITS % MNV_WAVE == 0, "a wavefront's units are all of one matrix");
 
-  mnv_f4 v[SLOTS][4];
+  mnv_f4 v[SLOTS][2];  // a unit is eight values of a row
 
   struct At {
     bool any, second;  // the same for the whole wavefront
@@ -150,11 +140,11 @@ struct MnvStage {
   __device__ static __forceinline__ At at(int s) {
     const unsigned first = s * NT + mnv_uniform(threadIdx.x / MNV_WAVE) * MNV_WAVE;
     At a;
-    a.any = 2 * QUADS % NT == 0 || first < 2 * QUADS;
-    a.second = QUADS % NT == 0 ? s >= QUADS / NT : first >= QUADS;
-    const unsigned q = first % QUADS + threadIdx.x % MNV_WAVE;
-    a.row = 4 * (q % 4 + 4 * (q / 4 / DQ));
-    a.col = 4 * (q / 4 % DQ);
+    a.any = 2 * UNITS % NT == 0 || first < 2 * UNITS;
+    a.second = UNITS % NT == 0 ? s >= UNITS / NT : first >= UNITS;
+    const unsigned u = first % UNITS + threadIdx.x % MNV_WAVE;
+    a.row = u / CHUNKS;
+    a.col = u % CHUNKS * 8;
     return a;
   }
 
@@ -163,38 +153,38 @@ struct MnvStage {
   // has no part in the result anyway, so no value is selected and nothing waits before `store`.  Byte
   // offsets within a tile fit 32 bits (MNV_AT_MAX_PITCH).
   __device__ __forceinline__ void fetch(const float* m0, const float* m1, unsigned pitch, int rows, int dim) {
-    if (dim % 4 == 0 && rows >= ROWS) {
+    if (dim == DP && rows >= 32) {
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s) {
         const At a = at(s);
         if (!a.any) continue;
-        const unsigned off = ((unsigned)a.row * pitch + (unsigned)(a.col < dim - 4 ? a.col : dim - 4)) * 4;
+        const unsigned off = ((unsigned)a.row * pitch + (unsigned)a.col) * 4;
         const float* m = a.second ? m1 : m0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[s][i] = get(m + (size_t)i * pitch, off);
+        v[s][0] = get(m, off);
+        v[s][1] = get(m + 4, off);
       }
     } else if (dim % 4 == 0) {
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s) {
         const At a = at(s);
         if (!a.any) continue;
-        const unsigned col = (unsigned)(a.col < dim - 4 ? a.col : dim - 4);
+        const unsigned row = (unsigned)(a.row < rows ? a.row : rows - 1) * pitch;
         const float* m = a.second ? m1 : m0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[s][i] = get(m, ((unsigned)(a.row + i < rows ? a.row + i : rows - 1) * pitch + col) * 4);
+        for (int h = 0; h < 2; ++h)
+          v[s][h] = get(m, (row + (unsigned)(a.col + 4 * h < dim - 4 ? a.col + 4 * h : dim - 4)) * 4);
       }
     } else {
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s) {
         const At a = at(s);
         if (!a.any) continue;
-        const float* m = a.second ? m1 : m0;
+        const float* p = (a.second ? m1 : m0) + (unsigned)(a.row < rows ? a.row : rows - 1) * pitch;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float* p = m + (unsigned)(a.row + i < rows ? a.row + i : rows - 1) * pitch;
-          v[s][i] = mnv_f4{p[a.col < dim ? a.col : dim - 1], p[a.col + 1 < dim ? a.col + 1 : dim - 1],
-                           p[a.col + 2 < dim ? a.col + 2 : dim - 1], p[a.col + 3 < dim ? a.col + 3 : dim - 1]};
+        for (int h = 0; h < 2; ++h) {
+          const int c = a.col + 4 * h;
+          v[s][h] = mnv_f4{p[c < dim ? c : dim - 1], p[c + 1 < dim ? c + 1 : dim - 1], p[c + 2 < dim ? c + 2 : dim - 1],
+                           p[c + 3 < dim ? c + 3 : dim - 1]};
         }
       }
     }
@@ -203,94 +193,66 @@ struct MnvStage {
     return mnv_ldx4u<false>(reinterpret_cast<const float*>(reinterpret_cast<const char*>(m) + off));
   }
 
-  // Place of row `row` (a multiple of 4) and its three successors in a column.
-  __device__ static __forceinline__ int place(int row) { return row / 16 * 16 + (row / 4 % 2) * 8 + (row / 8 % 2) * 4; }
-
-  // Cuts the tile into its planes.  scale0: factor of the first matrix.
-  __device__ __forceinline__ void store(char* lds, float scale0) {
+  // Cuts the tile into its planes: the first matrix times `scale`; of the second, ODD_MINUS, the odd rows
+  // times -1.
+  template <bool ODD_MINUS>
+  __device__ __forceinline__ void store(char* lds, float scale) const {
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const At a = at(s);
       if (!a.any) continue;
-      const float f = a.second ? 1.f : scale0;
-      unsigned w[3][4][2];  // [part][row][pair of columns]
+      const float f = !a.second ? scale : ODD_MINUS && a.row % 2 ? -1.f : 1.f;
+      mnv_u4 w[3];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int h = 0; h < 4; ++h) {
+        unsigned t[3];
+        mnv_split_pair(v[s][h / 2][h % 2 * 2], v[s][h / 2][h % 2 * 2 + 1], f, t);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          unsigned t[3];
-          mnv_split_pair(v[s][i][2 * h], v[s][i][2 * h + 1], f, t);
-#pragma unroll
-          for (int p = 0; p < 3; ++p) w[p][i][h] = t[p];
-        }
-      if (a.second ? FORM1 & 1 : FORM0 & 1) {
-        char* to = lds + (a.second ? ROWS1 : ROWS0) + (a.row * RP + a.col) * 2;
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<mnv_u2*>(to + (p * ROWS + i) * RP * 2) = mnv_u2{w[p][i][0], w[p][i][1]};
+        for (int p = 0; p < 3; ++p) w[p][h] = t[p];
       }
-      if (a.second ? FORM1 & 2 : FORM0 & 2) {
-        char* to = lds + (a.second ? COLS1 : COLS0) + (a.col * CP + place(a.row)) * 2;
+      char* to = lds + (a.second ? MATRIX : 0) + a.row * PITCH + a.col * 2;
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const unsigned sel = c % 2 ? 0x07060302u : 0x05040100u;
-            *reinterpret_cast<mnv_u2*>(to + (p * DP + c) * CP * 2) =
-                mnv_u2{__builtin_amdgcn_perm(w[p][1][c / 2], w[p][0][c / 2], sel),
-                       __builtin_amdgcn_perm(w[p][3][c / 2], w[p][2][c / 2], sel)};
-          }
-      }
+      for (int p = 0; p < 3; ++p) *reinterpret_cast<mnv_u4*>(to + p * PLANE) = w[p];
     }
   }
 
-  // Operands of the 32 rows from `row` on, columns 16 s ... of step s; and of the 32 columns from `col` on, rows 16 s...
-  template <int PARTS = 3>
-  __device__ static __forceinline__ MnvParts by_rows(const char* plane, int row, int s) {
+  // Operand of the 32 rows, columns 16 s ... of step s, from the planes of one matrix.
+  __device__ static __forceinline__ MnvParts by_rows(const char* planes, int s) {
     const int lane = threadIdx.x % MNV_WAVE;
-    const char* p = plane + ((row + lane % 32) * RP + s * 16 + lane / 32 * 8) * 2;
+    const char* p = planes + lane % 32 * PITCH + (s * 16 + lane / 32 * 8) * 2;
     MnvParts r;
 #pragma unroll
-    for (int c = 0; c < PARTS; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * ROWS * RP * 2);
+    for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * PLANE);
     return r;
   }
-  __device__ static __forceinline__ MnvParts by_cols(const char* plane, int col, int s) {
+  // Operand of the 32 columns from `col` on, rows 16 s ... of step s.
+  __device__ static __forceinline__ MnvParts by_cols(const char* planes, int col, int s) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4* lds_s4;
     const int lane = threadIdx.x % MNV_WAVE;
-    const char* p = plane + ((col + lane % 32) * CP + s * 16 + lane / 32 * 8) * 2;
+    const char* p = planes + (s * 16 + lane / 32 * 4 + lane % 16 / 4) * PITCH + (col + lane / 16 % 2 * 16 + lane % 4 * 4) * 2;
     MnvParts r;
 #pragma unroll
-    for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * DP * CP * 2);
+    for (int c = 0; c < 3; ++c) {
+      const s4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + c * PLANE));
+      const s4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + c * PLANE + 8 * PITCH));
+      r.p[c] = __builtin_bit_cast(mnv_bf8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
     return r;
   }
 
-  // acc[n] = the 32 rows from 32 n on, by rows, times the operand b over all columns.  The matrix instruction
-  // rounds its sums down, by up to a step of the larger of the sum and the terms: with the five small part
-  // products of all steps before the first large one only the DP / 16 last instructions do so at the full
-  // sum's size.  (In the order of the steps the scores' gradients are off by the same sign everywhere, 2^-27 of
-  // them: nothing to a value, but a bucket's gradient sums 10^5 that cancel.  12 heads of 512 x 512: table's
-  // gradient off by 4.0e-6.)
-  template <int N>
-  __device__ static __forceinline__ void product(mnv_f16 (&acc)[N], const char* plane, const MnvParts (&b)[DP / 16]) {
+  // acc = the tile's rows times the operand b, over all columns.
+  __device__ static __forceinline__ void product(mnv_f16& acc, const char* planes, const MnvParts (&b)[DP / 16]) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[n][e] = 0.f;
+    for (int s = 0; s < DP / 16; ++s) mnv_mul(acc, by_rows(planes, s), b[s]);
+  }
+  // acc += the tile's columns times the operand of step s, over 16 rows.
+  __device__ static __forceinline__ void add_columns(mnv_f16 (&acc)[DP / 32], const char* planes, int s, const MnvParts& b) {
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      MnvParts a[N];
-#pragma unroll
-      for (int n = 0; n < N; ++n) a[n] = by_rows(plane, 32 * n, s);
-      mnv_mul<N, 0, 5>(acc, a, b[s]);
-    }
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      MnvParts a[N];
-#pragma unroll
-      for (int n = 0; n < N; ++n) a[n] = by_rows<1>(plane, 32 * n, s);
-      mnv_mul<N, 5, 6>(acc, a, b[s]);
-    }
+    for (int c = 0; c < DP / 32; ++c) mnv_mul(acc[c], by_cols(planes, c * 32, s), b);
   }
 };
 

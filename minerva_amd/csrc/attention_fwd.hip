@@ -1,8 +1,8 @@
 // Attention of queries to the states of another sequence (or their own), forward.
 //   t_ij = scale * q_i.k_j + bias[j - i + q_len - 1] (j < lengths[b]),  m_i = max t_ij,  l_i = sum exp(t_ij - m_i)
 //   out_i = sum_j exp(t_ij - m_i) / l_i * v_j
-// One pass over the keys with the running maximum and sum of each query: a workgroup of four wavefronts
-// has 128 queries, 32 per wavefront, and tiles of 32 or 64 keys stream through LDS.  t^T = K Q^T, so a lane
+// One pass over the keys with the running maximum and sum of each query: a workgroup of four or eight wavefronts
+// has 32 queries per wavefront, and tiles of 32 keys stream through LDS.  t^T = K Q^T, so a lane
 // has one query and a quarter of the tile's keys; exp(t - m) goes on as the operand of out^T += V^T P^T from
 // the registers it stands in (attention_core.h).  Heads that share keys are rows of the same workgroup: row r is query
 // r / group, head r % group of the key head, so their keys are read and cut once.
@@ -21,17 +21,17 @@ struct FwdArgs {
   MnvFastDiv by_group;
 };
 
-template <int DP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
-  constexpr int BK = DP <= 64 ? 64 : 32, KB = BK / 32, NB = DP / 32;
-  using Stage = MnvStage<DP, BK, 256, 1, 2>;  // keys by rows, values by columns
-  __shared__ __align__(16) char lds[Stage::BYTES];
+template <int DP, int NW, bool BIAS>
+__global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
+  constexpr int NB = DP / 32;
+  using Stage = MnvStage<DP, 64 * NW>;
+  __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
   const MnvAttentionPlace place = mnv_attention_place(a.row_tiles, 0, z, a.lengths);
   const int tile = place.tile, b = place.b, kh = place.kh, n = place.n;
   const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
 
-  const int r = tile * 128 + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
+  const int r = tile * (32 * NW) + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
   const int rc = r < a.rows ? r : a.rows - 1;
   const int i = mnv_fastdiv(rc, a.by_group), h = kh * z.group() + (rc - i * z.group());
   const size_t row = ((size_t)b * z.q_len + i) * z.heads + h;
@@ -61,46 +61,40 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
     {
       Stage first;
       first.fetch(kb, vb, pitch, n, z.dim);
-      first.store(lds, 1.f);
+      first.template store<false>(lds, 1.f);
     }
-    for (int j0 = 0; j0 < n; j0 += BK) {
-      __syncthreads();
-      const bool more = j0 + BK < n;
+    __syncthreads();
+    char* now = lds;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+      const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
       Stage stage;
-      if (more) stage.fetch(kb + (size_t)(j0 + BK) * pitch, vb + (size_t)(j0 + BK) * pitch, pitch, n - j0 - BK, z.dim);
+      if (more) stage.fetch(kb + (size_t)(j0 + 32) * pitch, vb + (size_t)(j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
 
-      mnv_f16 t[KB];
-      Stage::product(t, lds + Stage::ROWS0, qp);
-      const bool whole = j0 + BK <= n;
+      mnv_f16 t;
+      Stage::product(t, now, qp);
       if (BIAS) {
 #pragma unroll
-        for (int c = 0; c < KB; ++c)
+        for (int u = 0; u < 4; ++u) {
+          const int j = j0 + 8 * u + 4 * half;
+          if (whole) {
+            const mnv_f4 add = mnv_ldx4u<false>(bias + j);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int j = j0 + c * 32 + 8 * u + 4 * half;
-            if (whole) {
-              const mnv_f4 add = mnv_ldx4u<false>(bias + j);
+            for (int e = 0; e < 4; ++e) t[4 * u + e] += add[e];
+          } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) t[c][4 * u + e] += add[e];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t[c][4 * u + e] += bias[j + e < n ? j + e : n - 1];
-            }
+            for (int e = 0; e < 4; ++e) t[4 * u + e] += bias[j + e < n ? j + e : n - 1];
           }
+        }
       }
       if (!whole) {
         MNV_KEEP_BRANCH();
 #pragma unroll
-        for (int c = 0; c < KB; ++c)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (j0 + c * 32 + mnv_acc_row(e, half) >= n) t[c][e] = -INFINITY;
+        for (int e = 0; e < 16; ++e)
+          if (j0 + mnv_acc_row(e, half) >= n) t[e] = -INFINITY;
       }
-      float top = t[0][0];
+      float top = t[0];
 #pragma unroll
-      for (int c = 0; c < KB; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, t[c][e]);
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, t[e]);
       top = fmaxf(top, __shfl_xor(top, 32, MNV_WAVE));
       const float next = fmaxf(m, top);
       const float base = mnv_finite_max(next);
@@ -114,27 +108,18 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
         m = next;
       }
 #pragma unroll
-      for (int s = 0; s < BK / 16; ++s) {
+      for (int s = 0; s < 2; ++s) {
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          p[e] = mnv_weight(t[s / 2][s % 2 * 8 + e], base);
+          p[e] = mnv_weight(t[s * 8 + e], base);
           l += p[e];
         }
-        const MnvParts pp = mnv_cut8(p);
-#pragma unroll
-        for (int c = 0; c + 2 <= NB; c += 2) {
-          const MnvParts vp[2] = {Stage::by_cols(lds + Stage::COLS1, c * 32, s),
-                                  Stage::by_cols(lds + Stage::COLS1, c * 32 + 32, s)};
-          mnv_mul(acc + c, vp, pp);
-        }
-        if (NB % 2) {
-          const MnvParts vp[1] = {Stage::by_cols(lds + Stage::COLS1, NB * 32 - 32, s)};
-          mnv_mul(acc + NB - 1, vp, pp);
-        }
+        Stage::add_columns(acc, now + Stage::MATRIX, s, mnv_cut8(p));
       }
+      now = lds + (now == lds ? Stage::BYTES : 0);
+      if (more) stage.template store<false>(now, 1.f);
       __syncthreads();
-      if (more) stage.store(lds, 1.f);
     }
     l += __shfl_xor(l, 32, MNV_WAVE);
   }
@@ -147,12 +132,15 @@ __global__ __launch_bounds__(256, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   }
 }
 
-template <int DP>
-int launch(const FwdArgs& a, unsigned grid, hipStream_t s) {
+template <int DP, int NW>
+int launch(FwdArgs& a, hipStream_t s) {
+  a.row_tiles = (int)mnv_ceil_div(a.rows, 32 * NW);
+  const size_t grid = (size_t)a.row_tiles * a.z.batch * a.z.kv_heads;
+  if (grid > 0x7fffffff) return MNV_ERR_INVALID;
   if (a.bias)
-    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, true>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, true>), dim3((unsigned)grid), dim3(64 * NW), 0, s, a);
   else
-    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, false>), dim3(grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, false>), dim3((unsigned)grid), dim3(64 * NW), 0, s, a);
   return MNV_LAUNCH_STATUS();
 }
 
@@ -168,14 +156,11 @@ int mnv_attention_fwd(const float* q, const float* k, const float* v, const floa
   const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, scale};
   if (!q || !k || !v || !out || !stats || !mnv_attention_sizes_ok(z)) return MNV_ERR_INVALID;
   FwdArgs a = {q, k, v, bias, lengths, out, stats, z, q_len * z.group(), 0, mnv_fastdiv_make(z.group())};
-  a.row_tiles = (int)mnv_ceil_div(a.rows, 128);
-  const long long grid = (long long)a.row_tiles * batch * kv_heads;
-  if (grid > 0x7fffffffLL) return MNV_ERR_INVALID;
   const hipStream_t s = mnv_stream(stream);
-  if (head_dim <= 32) return launch<32>(a, (unsigned)grid, s);
-  if (head_dim <= 64) return launch<64>(a, (unsigned)grid, s);
-  if (head_dim <= 96) return launch<96>(a, (unsigned)grid, s);
-  return launch<128>(a, (unsigned)grid, s);
+  if (head_dim <= 32) return launch<32, 4>(a, s);
+  if (head_dim <= 64) return launch<64, 4>(a, s);
+  if (head_dim <= 96) return launch<96, 8>(a, s);
+  return launch<128, 8>(a, s);
 }
 
 }  // extern "C"
