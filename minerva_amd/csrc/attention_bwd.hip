@@ -40,7 +40,7 @@ __host__ __device__ inline size_t diagonal_pitch(int q_len) { return ((size_t)q_
 __host__ __device__ inline size_t key_tiles(int k_len) { return ((size_t)k_len + 31) / 32; }
 
 template <int DP, bool BIAS>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 256>;  // queries (times scale) and their gradients
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
@@ -102,8 +102,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           next.delta = sign * a.dq[row * z.dim];
         }
       };
-      auto store = [&](const Rows& next, int turn) __attribute__((always_inline)) {
-        next.stage.template store<true>(lds + turn * Stage::BYTES, z.scale);
+      auto store_rows = [&](const Rows& next, int turn) __attribute__((always_inline)) {
         if (threadIdx.x < 32) {
           row_stats[turn][0][threadIdx.x] = next.m;
           row_stats[turn][1][threadIdx.x] = next.inverse;
@@ -113,57 +112,107 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
       {
         Rows first;
         fetch(first, 0);
-        store(first, 0);
+        first.stage.template store<true>(lds, z.scale);
+        store_rows(first, 0);
       }
       __syncthreads();
       int turn = 0;
       for (int i0 = 0; i0 < z.q_len; i0 += 32) {
         const bool more = i0 + 32 < z.q_len;
-        Rows next;
-        if (more) fetch(next, i0 + 32);
+        Rows next;  // behind the last tile that one again: no branch parts what follows
+        fetch(next, more ? i0 + 32 : i0);
         const char* now = lds + turn * Stage::BYTES;
-
-        mnv_f16 t, dp;
-        Stage::product(t, now, kp);
-        Stage::product(dp, now + Stage::MATRIX, vp);
+        mnv_f4 add[4];
         if (BIAS) {
-          const bool whole = i0 + 32 <= z.q_len;
+          if (i0 + 32 <= z.q_len) {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int i = i0 + 8 * u + 4 * half;
-            if (whole) {
-              const mnv_f4 add = mnv_ldx4u<false>(bias - (i + 3));
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t[4 * u + e] += add[3 - e];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) t[4 * u + e] += bias[-(i + e < z.q_len ? i + e : z.q_len - 1)];
+            for (int u = 0; u < 4; ++u) {
+              const mnv_f4 x = mnv_ldx4u<false>(bias - (i0 + 8 * u + 4 * half + 3));
+              add[u] = mnv_f4{x.w, x.z, x.y, x.x};
             }
+          } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int i = i0 + 8 * u + 4 * half + e;
+                add[u][e] = bias[-(i < z.q_len ? i : z.q_len - 1)];
+              }
           }
         }
+
+        // Four products in a row, a step per operand: the scores; dout v, under which the weights are made
+        // of the scores and cut; dv, under which ds is; dk, under which the next tile is cut.
+        mnv_f16 t, dp;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int at = 8 * u + 4 * half;
-          const mnv_f4 m = *reinterpret_cast<const mnv_f4*>(row_stats[turn][0] + at);
-          const mnv_f4 il = *reinterpret_cast<const mnv_f4*>(row_stats[turn][1] + at);
-          const mnv_f4 delta = *reinterpret_cast<const mnv_f4*>(row_stats[turn][2] + at);
+        for (int e = 0; e < 16; ++e) t[e] = dp[e] = 0.f;
+        MnvCutting pc[2], sc[2];
+        auto operand = [&](int k) __attribute__((always_inline)) {
+          const int s = k % KS;
+          return k < KS       ? Stage::by_rows(now, s)
+                 : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s)
+                 : k < 3 * KS ? Stage::by_cols(now + Stage::MATRIX, s % NB * 32, s / NB)
+                              : Stage::by_cols(now, s % NB * 32, s / NB);
+        };
+        // the numbers of two queries (a pair of result registers) that a step needs, read in the step before
+        constexpr int MOST = (8 + KS - 1) / KS;
+        mnv_f2 rows[2][MOST];
+        auto read_rows = [&](int k) __attribute__((always_inline)) {
+          if (k < KS || k >= 3 * KS) return;
+          const int first = k % KS * 8 / KS;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            t[4 * u + e] = mnv_weight(t[4 * u + e], m[e]) * il[e];
-            dp[4 * u + e] = t[4 * u + e] * (dp[4 * u + e] - delta[e]);
+          for (int pair = first; pair < (k % KS + 1) * 8 / KS; ++pair)
+#pragma unroll
+            for (int c = 0; c < (k < 2 * KS ? 2 : 1); ++c)
+              rows[c][pair - first] = *reinterpret_cast<const mnv_f2*>(row_stats[turn][k < 2 * KS ? c : 2] + mnv_acc_row(2 * pair, half));
+        };
+        MnvParts cur = operand(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 4 * KS; ++k) {
+          const int s = k % KS;
+          MnvParts ahead = cur;
+          if (k + 1 < 4 * KS) ahead = operand(k + 1);
+          mnv_f2 mine[2][MOST];
+#pragma unroll
+          for (int c = 0; c < MOST; ++c) {
+            mine[0][c] = rows[0][c];
+            mine[1][c] = rows[1][c];
           }
-        }
+          read_rows(k + 1);
+          if (k < KS) {
+            mnv_mul(t, cur, kp[s]);
+          } else if (k < 2 * KS) {
+            mnv_mul(dp, cur, vp[s]);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          float x[8], y[8];
+            for (int pair = s * 8 / KS; pair < (s + 1) * 8 / KS; ++pair) {
+              const mnv_f2 m = mine[0][pair - s * 8 / KS], il = mine[1][pair - s * 8 / KS];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = t[8 * s + e];
-            y[e] = dp[8 * s + e];
+              for (int e = 0; e < 2; ++e) {
+                const int r = 2 * pair + e;
+                if (BIAS) t[r] += add[r / 4][r % 4];
+                t[r] = mnv_weight(t[r], m[e]) * il[e];
+              }
+              pc[pair / 4].pair(pair % 4, t[2 * pair], t[2 * pair + 1]);
+            }
+          } else if (k < 3 * KS) {
+            mnv_mul(dv[s % NB], cur, pc[s / NB].parts());
+#pragma unroll
+            for (int pair = s * 8 / KS; pair < (s + 1) * 8 / KS; ++pair) {
+              const mnv_f2 delta = mine[0][pair - s * 8 / KS];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) dp[2 * pair + e] = t[2 * pair + e] * (dp[2 * pair + e] - delta[e]);
+              sc[pair / 4].pair(pair % 4, dp[2 * pair], dp[2 * pair + 1]);
+            }
+          } else {
+            mnv_mul(dk[s % NB], cur, sc[s / NB].parts());
+            next.stage.template store_piece<true>(s, lds + (turn ^ 1) * Stage::BYTES, z.scale);
           }
-          Stage::add_columns(dv, now + Stage::MATRIX, s, mnv_cut8(x));
-          Stage::add_columns(dk, now, s, mnv_cut8(y));
+          MNV_STEP_ORDER(6);
+          cur = ahead;
         }
+        turn ^= 1;
+        store_rows(next, turn);
         if (BIAS && parts) {
           // Lane u sums the diagonal key - query = u - 31 of the 32 x 32 tile: 16 queries at a time go to LDS,
           // each shifted by its number, so that a diagonal is a column; what a row does not reach stays 0.  The
@@ -196,8 +245,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           carry = __shfl(sum, lane - 32, MNV_WAVE);
           carry = lane >= 32 && lane < 63 ? carry : 0.f;
         }
-        turn ^= 1;
-        if (more) store(next, turn);
         __syncthreads();
       }
     }
@@ -209,7 +256,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
 }
 
 template <int DP, bool BIAS>
-__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 256>;  // keys and values
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
@@ -262,43 +309,75 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     char* now = lds;
     for (int j0 = 0; j0 < n; j0 += 32) {
       const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
-      Stage stage;
-      if (more) stage.fetch(kb + (size_t)(j0 + 32) * pitch, vb + (size_t)(j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
-
-      mnv_f16 t, dp;
-      Stage::product(t, now, qp);
-      Stage::product(dp, now + Stage::MATRIX, op);
+      Stage stage;  // behind the last tile that one again: no branch parts what follows
+      const int j1 = more ? j0 + 32 : j0;
+      stage.fetch(kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
+      mnv_f4 add[4];
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int j = j0 + 8 * u + 4 * half;
           if (whole) {
-            const mnv_f4 add = mnv_ldx4u<false>(bias + j);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[4 * u + e] += add[e];
+            add[u] = mnv_ldx4u<false>(bias + j);
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[4 * u + e] += bias[j + e < n ? j + e : n - 1];
+            for (int e = 0; e < 4; ++e) add[u][e] = bias[j + e < n ? j + e : n - 1];
           }
         }
       }
+      // keys of the tile that are read: the others' weights become 0
+      const int left = n - j0 - 4 * half;
+
+      // Three products in a row: the scores; dout v, under which the weights are made of the scores; dq, under
+      // which the second half of ds is made and the next tile cut.
+      mnv_f16 t, dp;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dp[e] = mnv_weight(t[e], m) * il * (dp[e] - delta);
-      if (!whole) {
-        MNV_KEEP_BRANCH();
+      for (int e = 0; e < 16; ++e) t[e] = dp[e] = 0.f;
+      MnvCutting sc[2];
+      auto cut_ds = [&](int pair) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (j0 + mnv_acc_row(e, half) >= n) dp[e] = 0.f;
+        for (int e = 0; e < 2; ++e) dp[2 * pair + e] = t[2 * pair + e] * (dp[2 * pair + e] - delta);
+        sc[pair / 4].pair(pair % 4, dp[2 * pair], dp[2 * pair + 1]);
+      };
+      auto operand = [&](int k) __attribute__((always_inline)) {
+        const int s = k % KS;
+        return k < KS       ? Stage::by_rows(now, s)
+               : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s)
+                            : Stage::by_cols(now, s % NB * 32, s / NB);
+      };
+      char* then = lds + (now == lds ? Stage::BYTES : 0);
+      MnvParts cur = operand(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < 3 * KS; ++k) {
+        const int s = k % KS;
+        MnvParts ahead = cur;
+        if (k + 1 < 3 * KS) ahead = operand(k + 1);
+        if (k < KS) {
+          mnv_mul(t, cur, qp[s]);
+        } else if (k < 2 * KS) {
+          mnv_mul(dp, cur, op[s]);
+#pragma unroll
+          for (int r = s * 16 / KS; r < (s + 1) * 16 / KS; ++r) {
+            if (BIAS) t[r] += add[r / 4][r % 4];
+            t[r] = mnv_acc_row(r, 0) < left ? mnv_weight(t[r], m) * il : 0.f;
+          }
+        } else {
+          if (s == 0) {
+#pragma unroll
+            for (int pair = 0; pair < 4; ++pair) cut_ds(pair);
+          }
+          mnv_mul(dq[s % NB], cur, sc[s / NB].parts());
+          if (s < NB) {
+#pragma unroll
+            for (int pair = 4 + s * 4 / NB; pair < 4 + (s + 1) * 4 / NB; ++pair) cut_ds(pair);
+          }
+          stage.template store_piece<false>(s, then, 1.f);
+        }
+        MNV_STEP_ORDER(6);
+        cur = ahead;
       }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = dp[8 * s + e];
-        Stage::add_columns(dq, now, s, mnv_cut8(x));
-      }
-      now = lds + (now == lds ? Stage::BYTES : 0);
-      if (more) stage.template store<false>(now, 1.f);
+      now = then;
       __syncthreads();
     }
   }

@@ -42,6 +42,7 @@ static inline bool mnv_attention_sizes_ok(const AttentionSizes& z) {
 #define MNV_LOG2E 1.4426950408889634f
 
 typedef float mnv_f16 __attribute__((ext_vector_type(16)));
+typedef float mnv_f2 __attribute__((ext_vector_type(2)));
 
 // A value that is the same in all lanes, in a scalar register: so are the addresses made from it.
 __device__ __forceinline__ int mnv_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -117,6 +118,37 @@ __device__ __forceinline__ void mnv_mul(mnv_f16& acc, const MnvParts& a, const M
 #pragma unroll
   for (int t = 0; t < 6; ++t) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[PA[t]], b.p[PB[t]], acc, 0, 0, 0);
 }
+
+// The order of instructions.  A 32 x 32 x 16 instruction holds its matrix core for 32 cycles and the issue for 8,
+// so what else a wavefront has to do (exponentials, cutting) is free if it stands between them, six vector
+// instructions to one; left alone, the compiler puts all matrix instructions of a product in a row and reads
+// each operand right before its use.  So a tile's work is written as steps of one operand, six matrix instructions,
+// that read the operand of the next step first and take a share of the other work between them.
+// MNV_STEP_ORDER closes a step; others: vector instructions to a matrix instruction.
+#define MNV_STEP_ORDER(others)                                 \
+  do {                                                         \
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);         \
+    _Pragma("unroll") for (int g_ = 0; g_ < 6; ++g_) {         \
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
+      __builtin_amdgcn_sched_group_barrier(0x002, others, 0);  \
+    }                                                          \
+    __builtin_amdgcn_sched_barrier(0);                         \
+  } while (0)
+
+// Eight values as an operand, cut pair by pair.
+struct MnvCutting {
+  mnv_u4 u[3];
+  __device__ __forceinline__ void pair(int i, float x, float y) {
+    unsigned t[3];
+    mnv_split_pair(x, y, 1.f, t);
+    u[0][i] = t[0];
+    u[1][i] = t[1];
+    u[2][i] = t[2];
+  }
+  __device__ __forceinline__ MnvParts parts() const {
+    return {{__builtin_bit_cast(mnv_bf8, u[0]), __builtin_bit_cast(mnv_bf8, u[1]), __builtin_bit_cast(mnv_bf8, u[2])}};
+  }
+};
 
 // Row of result register r, for lanes of half h.
 __device__ __forceinline__ constexpr int mnv_acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
@@ -194,26 +226,33 @@ struct MnvStage {
   }
 
   // Cuts the tile into its planes: the first matrix times `scale`; of the second, ODD_MINUS, the odd rows
-  // times -1.
+  // times -1.  In pieces of two pairs of values, each unit written with its last: a piece for each step
+  // of a product over all columns (or of all columns).
+  static constexpr int PIECES = DP / 16;
+  mnv_u4 w[3];
   template <bool ODD_MINUS>
-  __device__ __forceinline__ void store(char* lds, float scale) const {
+  __device__ __forceinline__ void store_piece(int piece, char* lds, float scale) {
+    const int s = piece / 2;
+    if (s >= SLOTS) return;
+    const At a = at(s);
+    if (!a.any) return;
+    const float f = !a.second ? scale : ODD_MINUS && a.row % 2 ? -1.f : 1.f;
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      const At a = at(s);
-      if (!a.any) continue;
-      const float f = !a.second ? scale : ODD_MINUS && a.row % 2 ? -1.f : 1.f;
-      mnv_u4 w[3];
+    for (int h = piece % 2 * 2; h < piece % 2 * 2 + 2; ++h) {
+      unsigned t[3];
+      mnv_split_pair(v[s][h / 2][h % 2 * 2], v[s][h / 2][h % 2 * 2 + 1], f, t);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        unsigned t[3];
-        mnv_split_pair(v[s][h / 2][h % 2 * 2], v[s][h / 2][h % 2 * 2 + 1], f, t);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) w[p][h] = t[p];
-      }
-      char* to = lds + (a.second ? MATRIX : 0) + a.row * PITCH + a.col * 2;
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<mnv_u4*>(to + p * PLANE) = w[p];
+      for (int p = 0; p < 3; ++p) w[p][h] = t[p];
     }
+    if (piece % 2 == 0) return;
+    char* to = lds + (a.second ? MATRIX : 0) + a.row * PITCH + a.col * 2;
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<mnv_u4*>(to + p * PLANE) = w[p];
+  }
+  template <bool ODD_MINUS>
+  __device__ __forceinline__ void store(char* lds, float scale) {
+#pragma unroll
+    for (int piece = 0; piece < PIECES; ++piece) store_piece<ODD_MINUS>(piece, lds, scale);
   }
 
   // Operand of the 32 rows, columns 16 s ... of step s, from the planes of one matrix.
@@ -240,19 +279,6 @@ struct MnvStage {
       r.p[c] = __builtin_bit_cast(mnv_bf8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     return r;
-  }
-
-  // acc = the tile's rows times the operand b, over all columns.
-  __device__ static __forceinline__ void product(mnv_f16& acc, const char* planes, const MnvParts (&b)[DP / 16]) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s) mnv_mul(acc, by_rows(planes, s), b[s]);
-  }
-  // acc += the tile's columns times the operand of step s, over 16 rows.
-  __device__ static __forceinline__ void add_columns(mnv_f16 (&acc)[DP / 32], const char* planes, int s, const MnvParts& b) {
-#pragma unroll
-    for (int c = 0; c < DP / 32; ++c) mnv_mul(acc[c], by_cols(planes, c * 32, s), b);
   }
 };
 

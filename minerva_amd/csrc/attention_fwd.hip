@@ -23,7 +23,7 @@ struct FwdArgs {
 
 template <int DP, int NW, bool BIAS>
 __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
-  constexpr int NB = DP / 32;
+  constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 64 * NW>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
@@ -67,11 +67,22 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
     char* now = lds;
     for (int j0 = 0; j0 < n; j0 += 32) {
       const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
-      Stage stage;
-      if (more) stage.fetch(kb + (size_t)(j0 + 32) * pitch, vb + (size_t)(j0 + 32) * pitch, pitch, n - j0 - 32, z.dim);
+      Stage stage;  // behind the last tile that one again: no branch parts what follows
+      const int j1 = more ? j0 + 32 : j0;
+      stage.fetch(kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
 
       mnv_f16 t;
-      Stage::product(t, now, qp);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) t[e] = 0.f;
+      MnvParts cur = Stage::by_rows(now, 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const MnvParts ahead = s + 1 < KS ? Stage::by_rows(now, s + 1) : Stage::by_cols(now + Stage::MATRIX, 0, 0);
+        mnv_mul(t, cur, qp[s]);
+        MNV_STEP_ORDER(6);
+        cur = ahead;
+      }
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -107,18 +118,34 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
           for (int e = 0; e < 16; ++e) acc[c][e] *= shrink;
         m = next;
       }
+      // the second half of the weights is made, and the next tile cut, under the products of the first
+      MnvCutting pc[2];
+      auto cut_p = [&](int pair) __attribute__((always_inline)) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          p[e] = mnv_weight(t[s * 8 + e], base);
-          l += p[e];
+        for (int e = 0; e < 2; ++e) {
+          t[2 * pair + e] = mnv_weight(t[2 * pair + e], base);
+          l += t[2 * pair + e];
         }
-        Stage::add_columns(acc, now + Stage::MATRIX, s, mnv_cut8(p));
+        pc[pair / 4].pair(pair % 4, t[2 * pair], t[2 * pair + 1]);
+      };
+#pragma unroll
+      for (int pair = 0; pair < 4; ++pair) cut_p(pair);
+      char* then = lds + (now == lds ? Stage::BYTES : 0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        MnvParts ahead = cur;
+        if (s + 1 < KS) ahead = Stage::by_cols(now + Stage::MATRIX, (s + 1) % NB * 32, (s + 1) / NB);
+        mnv_mul(acc[s % NB], cur, pc[s / NB].parts());
+        if (s < NB) {
+#pragma unroll
+          for (int pair = 4 + s * 4 / NB; pair < 4 + (s + 1) * 4 / NB; ++pair) cut_p(pair);
+        }
+        stage.template store_piece<false>(s, then, 1.f);
+        MNV_STEP_ORDER(6);
+        cur = ahead;
       }
-      now = lds + (now == lds ? Stage::BYTES : 0);
-      if (more) stage.template store<false>(now, 1.f);
+      now = then;
       __syncthreads();
     }
     l += __shfl_xor(l, 32, MNV_WAVE);
