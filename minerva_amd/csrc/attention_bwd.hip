@@ -89,31 +89,31 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
       float carry = 0.f;
       struct Rows {
         Stage stage;
-        float m, inverse, delta;
+        float m, l, delta;
       };
       auto fetch = [&](Rows& next, int i0) __attribute__((always_inline)) {
         next.stage.fetch(qb + (size_t)i0 * pitch, ob + (size_t)i0 * pitch, pitch, z.q_len - i0, z.dim);
         if (threadIdx.x < 32) {
           const int i = i0 + (int)threadIdx.x;
           const size_t row = row0 + (size_t)(i < z.q_len ? i : z.q_len - 1) * z.heads;
-          const float sign = i % 2 ? -1.f : 1.f;
-          next.m = mnv_finite_max(a.stats[2 * row]);
-          next.inverse = i < z.q_len ? sign * mnv_inverse(a.stats[2 * row + 1]) : 0.f;
-          next.delta = sign * a.dq[row * z.dim];
+          next.m = a.stats[2 * row];
+          next.l = a.stats[2 * row + 1];
+          next.delta = a.dq[row * z.dim];
         }
       };
-      auto store_rows = [&](const Rows& next, int turn) __attribute__((always_inline)) {
+      auto store_rows = [&](const Rows& next, int i0, int turn) __attribute__((always_inline)) {
         if (threadIdx.x < 32) {
-          row_stats[turn][0][threadIdx.x] = next.m;
-          row_stats[turn][1][threadIdx.x] = next.inverse;
-          row_stats[turn][2][threadIdx.x] = next.delta;
+          const float sign = threadIdx.x % 2 ? -1.f : 1.f;
+          row_stats[turn][0][threadIdx.x] = mnv_finite_max(next.m);
+          row_stats[turn][1][threadIdx.x] = i0 + (int)threadIdx.x < z.q_len ? sign * mnv_inverse(next.l) : 0.f;
+          row_stats[turn][2][threadIdx.x] = sign * next.delta;
         }
       };
       {
         Rows first;
         fetch(first, 0);
         first.stage.template store<true>(lds, z.scale);
-        store_rows(first, 0);
+        store_rows(first, 0, 0);
       }
       __syncthreads();
       int turn = 0;
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
           cur = ahead;
         }
         turn ^= 1;
-        store_rows(next, turn);
+        store_rows(next, i0 + 32, turn);
         if (BIAS && parts) {
           // Lane u sums the diagonal key - query = u - 31 of the 32 x 32 tile: 16 queries at a time go to LDS,
           // each shifted by its number, so that a diagonal is a column; what a row does not reach stays 0.  The

@@ -154,13 +154,14 @@ struct MnvCutting {
 __device__ __forceinline__ constexpr int mnv_acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
 
 // 32 consecutive rows of two matrices (of up to DP columns, `pitch` floats from row to row) on their way from
-// memory to LDS: fetched into registers a tile ahead, then cut into planes of parts.  Rows lie DP + 16 bf16
-// apart: an odd multiple of 8 banks' words, so that 8 rows of 16 bytes (by rows) and 4 rows of 32
-// (by columns) are in different banks.
+// memory to LDS: fetched into registers a tile ahead, then cut into planes of parts.  A row's 16-byte chunks
+// are permuted among themselves (`swap`), so that 16 chunks of one number (read by rows) and 4 rows of 64 bytes
+// (read by columns) lie in different banks; with rows padded instead, one of the two reads has conflicts
+// (16 bytes: 2 extra cycles on 4 by columns; 32 bytes: 4 extra on 8 by rows).
 template <int DP, int NT>
 struct MnvStage {
   static constexpr int CHUNKS = DP / 8, UNITS = 32 * CHUNKS, SLOTS = (2 * UNITS + NT - 1) / NT;
-  static constexpr int PITCH = (DP + 16) * 2, PLANE = 32 * PITCH, MATRIX = 3 * PLANE, BYTES = 2 * MATRIX;
+  static constexpr int PITCH = DP * 2, PLANE = 32 * PITCH, MATRIX = 3 * PLANE, BYTES = 2 * MATRIX;
   static_assert(UNITS % MNV_WAVE == 0, "a wavefront's units are all of one matrix");
 
   mnv_f4 v[SLOTS][2];  // a unit is eight values of a row
@@ -245,7 +246,7 @@ struct MnvStage {
       for (int p = 0; p < 3; ++p) w[p][h] = t[p];
     }
     if (piece % 2 == 0) return;
-    char* to = lds + (a.second ? MATRIX : 0) + a.row * PITCH + a.col * 2;
+    char* to = lds + (a.second ? MATRIX : 0) + a.row * PITCH + ((a.col / 8) ^ swap(a.row)) * 16;
 #pragma unroll
     for (int p = 0; p < 3; ++p) *reinterpret_cast<mnv_u4*>(to + p * PLANE) = w[p];
   }
@@ -255,10 +256,19 @@ struct MnvStage {
     for (int piece = 0; piece < PIECES; ++piece) store_piece<ODD_MINUS>(piece, lds, scale);
   }
 
+  // What a row's chunk numbers are xored with.  4 rows of 64 bytes: 128 columns put all in the same banks, 64
+  // two and two, 32 and 96 none.
+  static constexpr int SWAPPED = DP == 128 ? 15 : DP == 64 ? 7 : 3;  // bits of a chunk's number that change
+  __device__ static __forceinline__ int swap(int row) {
+    return row / 4 % 4 + (DP == 128 ? row % 4 * 4 : DP == 64 ? row / 2 % 2 * 4 : 0);
+  }
+
   // Operand of the 32 rows, columns 16 s ... of step s, from the planes of one matrix.
   __device__ static __forceinline__ MnvParts by_rows(const char* planes, int s) {
-    const int lane = threadIdx.x % MNV_WAVE;
-    const char* p = planes + lane % 32 * PITCH + (s * 16 + lane / 32 * 8) * 2;
+    const int lane = threadIdx.x % MNV_WAVE, row = lane % 32;
+    // chunk 2 s + lane / 32
+    const int at = row * PITCH + (swap(row) ^ (lane / 32)) * 16;
+    const char* p = planes + (at ^ (2 * s & SWAPPED) * 16) + (2 * s & ~SWAPPED) * 16;
     MnvParts r;
 #pragma unroll
     for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * PLANE);
@@ -269,14 +279,17 @@ struct MnvStage {
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef short s8 __attribute__((ext_vector_type(8)));
     typedef __attribute__((address_space(3))) s4* lds_s4;
-    const int lane = threadIdx.x % MNV_WAVE;
-    const char* p = planes + (s * 16 + lane / 32 * 4 + lane % 16 / 4) * PITCH + (col + lane / 16 % 2 * 16 + lane % 4 * 4) * 2;
+    const int lane = threadIdx.x % MNV_WAVE, row = lane / 32 * 4 + lane % 16 / 4;
+    // chunk col / 8 + 2 (lane / 16 % 2) + lane % 4 / 2 of rows `row` and row + 8, whose numbers are swapped by 2 more
+    const int at = row * PITCH + (swap(row) ^ (lane / 16 % 2 * 2 + lane % 4 / 2)) * 16 + lane % 2 * 8;
+    const char* p = planes + s * 16 * PITCH + (col / 8 & ~SWAPPED) * 16;
+    const int low = at ^ (col / 8 & SWAPPED) * 16, high = (low ^ 32) + 8 * PITCH;
     MnvParts r;
 #pragma unroll
     for (int c = 0; c < 3; ++c) {
-      const s4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + c * PLANE));
-      const s4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + c * PLANE + 8 * PITCH));
-      r.p[c] = __builtin_bit_cast(mnv_bf8, __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7));
+      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + low + c * PLANE));
+      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + high + c * PLANE));
+      r.p[c] = __builtin_bit_cast(mnv_bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     return r;
   }
