@@ -39,10 +39,10 @@ __global__ __launch_bounds__(256) void mnv_attention_delta_kernel(const float* _
 __host__ __device__ inline size_t diagonal_pitch(int q_len) { return ((size_t)q_len + 31) / 32 * 32 + 32; }
 __host__ __device__ inline size_t key_tiles(int k_len) { return ((size_t)k_len + 31) / 32; }
 
-template <int DP, bool BIAS>
+template <int DP, bool BIAS, bool VEC>
 __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  using Stage = MnvStage<DP, 256>;  // queries (times scale) and their gradients
+  using Stage = MnvStage<DP, 256, VEC>;  // queries (times scale) and their gradients
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   __shared__ __align__(16) float row_stats[2][3][32];  // m, 1 / l, delta of the tile's queries
   __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
@@ -91,8 +91,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
         Stage stage;
         float m, l, delta;
       };
-      auto fetch = [&](Rows& next, int i0) __attribute__((always_inline)) {
-        next.stage.fetch(qb + (size_t)i0 * pitch, ob + (size_t)i0 * pitch, pitch, z.q_len - i0, z.dim);
+      auto fetch_rows = [&](Rows& next, int i0) __attribute__((always_inline)) {
         if (threadIdx.x < 32) {
           const int i = i0 + (int)threadIdx.x;
           const size_t row = row0 + (size_t)(i < z.q_len ? i : z.q_len - 1) * z.heads;
@@ -111,7 +110,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
       };
       {
         Rows first;
-        fetch(first, 0);
+        fetch_rows(first, 0);
+        first.stage.fetch(qb, ob, pitch, z.q_len, z.dim);
         first.stage.template store<true>(lds, z.scale);
         store_rows(first, 0, 0);
       }
@@ -120,7 +120,8 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
       for (int i0 = 0; i0 < z.q_len; i0 += 32) {
         const bool more = i0 + 32 < z.q_len;
         Rows next;  // behind the last tile that one again: no branch parts what follows
-        fetch(next, more ? i0 + 32 : i0);
+        const int i1 = more ? i0 + 32 : i0;
+        fetch_rows(next, i1);
         const char* now = lds + turn * Stage::BYTES;
         mnv_f4 add[4];
         if (BIAS) {
@@ -141,7 +142,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
           }
         }
 
-        // Four products in a row, a step per operand: the scores; dout v, under which the weights are made
+        // Four products in a row, a step per operand: the scores, under which the next tile is fetched; dout v, under which the weights are made
         // of the scores and cut; dv, under which ds is; dk, under which the next tile is cut.
         mnv_f16 t, dp;
 #pragma unroll
@@ -182,6 +183,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
           read_rows(k + 1);
           if (k < KS) {
             mnv_mul(t, cur, kp[s]);
+            next.stage.fetch_piece(s, qb + (size_t)i1 * pitch, ob + (size_t)i1 * pitch, pitch, z.q_len - i1, z.dim);
           } else if (k < 2 * KS) {
             mnv_mul(dp, cur, vp[s]);
 #pragma unroll
@@ -255,10 +257,10 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
   }
 }
 
-template <int DP, bool BIAS>
+template <int DP, bool BIAS, bool VEC>
 __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  using Stage = MnvStage<DP, 256>;  // keys and values
+  using Stage = MnvStage<DP, 256, VEC>;  // keys and values
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
   const MnvAttentionPlace place = mnv_attention_place(a.tiles, 0, z, a.lengths);
@@ -311,7 +313,6 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
       const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
       Stage stage;  // behind the last tile that one again: no branch parts what follows
       const int j1 = more ? j0 + 32 : j0;
-      stage.fetch(kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
       mnv_f4 add[4];
       if (BIAS) {
 #pragma unroll
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
       // keys of the tile that are read: the others' weights become 0
       const int left = n - j0 - 4 * half;
 
-      // Three products in a row: the scores; dout v, under which the weights are made of the scores; dq, under
+      // Three products in a row: the scores, under which the next tile is fetched; dout v, under which the weights are made of the scores; dq, under
       // which the second half of ds is made and the next tile cut.
       mnv_f16 t, dp;
 #pragma unroll
@@ -355,6 +356,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
         if (k + 1 < 3 * KS) ahead = operand(k + 1);
         if (k < KS) {
           mnv_mul(t, cur, qp[s]);
+          stage.fetch_piece(s, kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
         } else if (k < 2 * KS) {
           mnv_mul(dp, cur, op[s]);
 #pragma unroll
@@ -450,21 +452,23 @@ size_t pair_bytes(const AttentionSizes& z) {
 }
 #define MNV_AT_PARTS_BYTES ((size_t)256 << 20)  // of partial sums at a time, where there are more
 
+#define MNV_AT_LAUNCH(kernel)                                                                              \
+  do {                                                                                                     \
+    const dim3 g(grid), b(256);                                                                            \
+    const bool vec = a.z.dim % 4 == 0;                                                                     \
+    if (a.bias && vec) hipLaunchKernelGGL((kernel<DP, true, true>), g, b, 0, s, a);                        \
+    else if (a.bias) hipLaunchKernelGGL((kernel<DP, true, false>), g, b, 0, s, a);                         \
+    else if (vec) hipLaunchKernelGGL((kernel<DP, false, true>), g, b, 0, s, a);                            \
+    else hipLaunchKernelGGL((kernel<DP, false, false>), g, b, 0, s, a);                                    \
+    return MNV_LAUNCH_STATUS();                                                                            \
+  } while (0)
 template <int DP>
 int launch_dkv(const BwdArgs& a, unsigned grid, hipStream_t s) {
-  if (a.bias)
-    hipLaunchKernelGGL((mnv_attention_dkv_kernel<DP, true>), dim3(grid), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((mnv_attention_dkv_kernel<DP, false>), dim3(grid), dim3(256), 0, s, a);
-  return MNV_LAUNCH_STATUS();
+  MNV_AT_LAUNCH(mnv_attention_dkv_kernel);
 }
 template <int DP>
 int launch_dq(const BwdArgs& a, unsigned grid, hipStream_t s) {
-  if (a.bias)
-    hipLaunchKernelGGL((mnv_attention_dq_kernel<DP, true>), dim3(grid), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((mnv_attention_dq_kernel<DP, false>), dim3(grid), dim3(256), 0, s, a);
-  return MNV_LAUNCH_STATUS();
+  MNV_AT_LAUNCH(mnv_attention_dq_kernel);
 }
 int by_dim(int dim, int (*f32)(const BwdArgs&, unsigned, hipStream_t), int (*f64)(const BwdArgs&, unsigned, hipStream_t),
            int (*f96)(const BwdArgs&, unsigned, hipStream_t), int (*f128)(const BwdArgs&, unsigned, hipStream_t),

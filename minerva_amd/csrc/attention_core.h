@@ -89,6 +89,14 @@ __device__ __forceinline__ MnvAttentionPlace mnv_attention_place(unsigned tiles,
 // The difference is taken before the factor: at the type's lowest value t * log2(e) would be infinite.
 __device__ __forceinline__ float mnv_weight(float t, float m) { return __builtin_amdgcn_exp2f((t - m) * MNV_LOG2E); }
 __device__ __forceinline__ float mnv_finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+// The larger of a value and that of the lane 32 away.
+__device__ __forceinline__ float mnv_max_of_halves(float x) {
+  unsigned u = __builtin_bit_cast(unsigned, x), w = u;
+  asm volatile("" : "+v"(w));  // of equal operands the compiler takes both results for the same
+  const auto r = __builtin_amdgcn_permlane32_swap(u, w, false, false);
+  unsigned low = r[0], high = r[1];
+  return fmaxf(__builtin_bit_cast(float, low), __builtin_bit_cast(float, high));
+}
 // 1 / l, and 0 for a row that sees no key
 __device__ __forceinline__ float mnv_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
@@ -158,7 +166,8 @@ __device__ __forceinline__ constexpr int mnv_acc_row(int r, int h) { return 8 * 
 // are permuted among themselves (`swap`), so that 16 chunks of one number (read by rows) and 4 rows of 64 bytes
 // (read by columns) lie in different banks; with rows padded instead, one of the two reads has conflicts
 // (16 bytes: 2 extra cycles on 4 by columns; 32 bytes: 4 extra on 8 by rows).
-template <int DP, int NT>
+// VEC: dim is a multiple of 4 (else values are fetched one by one).
+template <int DP, int NT, bool VEC>
 struct MnvStage {
   static constexpr int CHUNKS = DP / 8, UNITS = 32 * CHUNKS, SLOTS = (2 * UNITS + NT - 1) / NT;
   static constexpr int PITCH = DP * 2, PLANE = 32 * PITCH, MATRIX = 3 * PLANE, BYTES = 2 * MATRIX;
@@ -181,55 +190,36 @@ struct MnvStage {
     return a;
   }
 
-  // Fetches the tile from rows >= 1 rows that exist.  In place of a row behind them comes the last one, and in place
-  // of a column behind dim another of the row: what they are multiplied by is 0, and they hold nothing that
-  // has no part in the result anyway, so no value is selected and nothing waits before `store`.  Byte
-  // offsets within a tile fit 32 bits (MNV_AT_MAX_PITCH).
-  __device__ __forceinline__ void fetch(const float* m0, const float* m1, unsigned pitch, int rows, int dim) {
-    if (dim == DP && rows >= 32) {
-#pragma unroll
-      for (int s = 0; s < SLOTS; ++s) {
-        const At a = at(s);
-        if (!a.any) continue;
-        const unsigned off = ((unsigned)a.row * pitch + (unsigned)a.col) * 4;
-        const float* m = a.second ? m1 : m0;
-        v[s][0] = get(m, off);
-        v[s][1] = get(m + 4, off);
-      }
-    } else if (dim % 4 == 0) {
-#pragma unroll
-      for (int s = 0; s < SLOTS; ++s) {
-        const At a = at(s);
-        if (!a.any) continue;
-        const unsigned row = (unsigned)(a.row < rows ? a.row : rows - 1) * pitch;
-        const float* m = a.second ? m1 : m0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          v[s][h] = get(m, (row + (unsigned)(a.col + 4 * h < dim - 4 ? a.col + 4 * h : dim - 4)) * 4);
-      }
+  // Fetches the tile from rows >= 1 rows that exist, in PIECES pieces.  In place of a row behind them comes the last
+  // one, and in place of a column behind dim another of the row: what they are multiplied by is 0, and they
+  // hold nothing that has no part in the result anyway, so no value is selected and nothing waits before
+  // `store`.  Byte offsets within a tile fit 32 bits (MNV_AT_MAX_PITCH).
+  static constexpr int PIECES = 2 * SLOTS;
+  __device__ __forceinline__ void fetch_piece(int piece, const float* m0, const float* m1, unsigned pitch, int rows,
+                                              int dim) {
+    const int s = piece / 2;
+    if (s >= SLOTS) return;
+    const At a = at(s);
+    if (!a.any) return;
+    const float* m = a.second ? m1 : m0;
+    const unsigned mine = (unsigned)a.row * pitch, last = (unsigned)(rows - 1) * pitch, row = mine < last ? mine : last;
+    const int c = a.col + piece % 2 * 4;
+    if (VEC) {
+      const unsigned off = (row + (unsigned)(c < dim - 4 ? c : dim - 4)) * 4;
+      v[s][piece % 2] = mnv_ldx4u<false>(reinterpret_cast<const float*>(reinterpret_cast<const char*>(m) + off));
     } else {
-#pragma unroll
-      for (int s = 0; s < SLOTS; ++s) {
-        const At a = at(s);
-        if (!a.any) continue;
-        const float* p = (a.second ? m1 : m0) + (unsigned)(a.row < rows ? a.row : rows - 1) * pitch;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int c = a.col + 4 * h;
-          v[s][h] = mnv_f4{p[c < dim ? c : dim - 1], p[c + 1 < dim ? c + 1 : dim - 1], p[c + 2 < dim ? c + 2 : dim - 1],
-                           p[c + 3 < dim ? c + 3 : dim - 1]};
-        }
-      }
+      const float* p = m + row;
+      v[s][piece % 2] = mnv_f4{p[c < dim ? c : dim - 1], p[c + 1 < dim ? c + 1 : dim - 1],
+                               p[c + 2 < dim ? c + 2 : dim - 1], p[c + 3 < dim ? c + 3 : dim - 1]};
     }
   }
-  __device__ static __forceinline__ mnv_f4 get(const float* m, unsigned off) {
-    return mnv_ldx4u<false>(reinterpret_cast<const float*>(reinterpret_cast<const char*>(m) + off));
+  __device__ __forceinline__ void fetch(const float* m0, const float* m1, unsigned pitch, int rows, int dim) {
+#pragma unroll
+    for (int piece = 0; piece < PIECES; ++piece) fetch_piece(piece, m0, m1, pitch, rows, dim);
   }
 
   // Cuts the tile into its planes: the first matrix times `scale`; of the second, ODD_MINUS, the odd rows
-  // times -1.  In pieces of two pairs of values, each unit written with its last: a piece for each step
-  // of a product over all columns (or of all columns).
-  static constexpr int PIECES = DP / 16;
+  // times -1.  In as many pieces, each unit written with its last.
   mnv_u4 w[3];
   template <bool ODD_MINUS>
   __device__ __forceinline__ void store_piece(int piece, char* lds, float scale) {

@@ -8,6 +8,8 @@
 // r / group, head r % group of the key head, so their keys are read and cut once.
 // A row that sees no key has m = -inf, l = 0, out = 0.  The pair (m, l) is kept and not m + ln l: where the bias is the
 // type's lowest value for a whole row, ln l would be lost in the sum.
+#include <type_traits>
+
 #include "attention_core.h"
 
 namespace {
@@ -21,10 +23,10 @@ struct FwdArgs {
   MnvFastDiv by_group;
 };
 
-template <int DP, int NW, bool BIAS>
+template <int DP, int NW, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  using Stage = MnvStage<DP, 64 * NW>;
+  using Stage = MnvStage<DP, 64 * NW, VEC>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
   const MnvAttentionPlace place = mnv_attention_place(a.row_tiles, 0, z, a.lengths);
@@ -64,25 +66,35 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
       first.template store<false>(lds, 1.f);
     }
     __syncthreads();
-    char* now = lds;
-    for (int j0 = 0; j0 < n; j0 += 32) {
-      const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
-      Stage stage;  // behind the last tile that one again: no branch parts what follows
-      const int j1 = more ? j0 + 32 : j0;
-      stage.fetch(kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
 
-      mnv_f16 t;
+    // Two phases to a tile, each the other half's when there are eight wavefronts: while four multiply queries and
+    // keys, the four that share their matrix cores have soft-max to do.
+    const bool late = NW == 8 && mnv_uniform(threadIdx.x / MNV_WAVE) >= 4;
+    mnv_f16 t;
+    Stage stage;
+    auto fetch = [&](int piece, int j1) __attribute__((always_inline)) {
+      stage.fetch_piece(piece, kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
+    };
+    // scores of the tile in `now`; FETCH: the tile from j1 on is fetched, else that in `stage` is cut to `then`
+    auto scores = [&](auto fetches, const char* now, char* then, int j1) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) t[e] = 0.f;
       MnvParts cur = Stage::by_rows(now, 0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const MnvParts ahead = s + 1 < KS ? Stage::by_rows(now, s + 1) : Stage::by_cols(now + Stage::MATRIX, 0, 0);
+        MnvParts ahead = cur;
+        if (s + 1 < KS) ahead = Stage::by_rows(now, s + 1);
         mnv_mul(t, cur, qp[s]);
+        if (decltype(fetches)::value) fetch(s, j1);
+        else stage.template store_piece<false>(s, then, 1.f);
         MNV_STEP_ORDER(6);
         cur = ahead;
       }
+    };
+    auto results = [&](auto fetches, const char* now, char* then, int j0, int j1) __attribute__((always_inline)) {
+      const bool whole = j0 + 32 <= n;
+      MnvParts cur = Stage::by_cols(now + Stage::MATRIX, 0, 0);
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -106,8 +118,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
       float top = t[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, t[e]);
-      top = fmaxf(top, __shfl_xor(top, 32, MNV_WAVE));
-      const float next = fmaxf(m, top);
+      const float next = fmaxf(m, mnv_max_of_halves(top));
       const float base = mnv_finite_max(next);
       if (__any(next > m)) {
         const float shrink = mnv_weight(m, base);
@@ -130,7 +141,6 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
       };
 #pragma unroll
       for (int pair = 0; pair < 4; ++pair) cut_p(pair);
-      char* then = lds + (now == lds ? Stage::BYTES : 0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -141,12 +151,41 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
 #pragma unroll
           for (int pair = 4 + s * 4 / NB; pair < 4 + (s + 1) * 4 / NB; ++pair) cut_p(pair);
         }
-        stage.template store_piece<false>(s, then, 1.f);
+        if (decltype(fetches)::value) fetch(s, j1);
+        else stage.template store_piece<false>(s, then, 1.f);
         MNV_STEP_ORDER(6);
         cur = ahead;
       }
-      now = then;
+    };
+    const std::true_type fetches;
+    const std::false_type cuts;
+    const int last = (n - 1) / 32 * 32;  // behind it that tile again: no branch parts a phase
+    char *now = lds, *then = lds + Stage::BYTES;
+    if (!late) {
+      for (int j0 = 0; j0 < n; j0 += 32) {
+        scores(fetches, now, then, j0 < last ? j0 + 32 : last);
+        if (NW == 8) __syncthreads();
+        results(cuts, now, then, j0, 0);
+        __syncthreads();
+        char* t_ = now;
+        now = then;
+        then = t_;
+      }
+      if (NW == 8) __syncthreads();
+    } else {
+      // one phase behind: cuts a tile while it makes scores, which is when the others do
+#pragma unroll
+      for (int piece = 0; piece < Stage::PIECES; ++piece) fetch(piece, last < 32 ? last : 32);
       __syncthreads();
+      for (int j0 = 0; j0 < n; j0 += 32) {
+        scores(cuts, now, then, 0);
+        __syncthreads();
+        results(fetches, now, then, j0, j0 + 64 < last ? j0 + 64 : last);
+        __syncthreads();
+        char* t_ = now;
+        now = then;
+        then = t_;
+      }
     }
     l += __shfl_xor(l, 32, MNV_WAVE);
   }
@@ -164,10 +203,12 @@ int launch(FwdArgs& a, hipStream_t s) {
   a.row_tiles = (int)mnv_ceil_div(a.rows, 32 * NW);
   const size_t grid = (size_t)a.row_tiles * a.z.batch * a.z.kv_heads;
   if (grid > 0x7fffffff) return MNV_ERR_INVALID;
-  if (a.bias)
-    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, true>), dim3((unsigned)grid), dim3(64 * NW), 0, s, a);
-  else
-    hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, false>), dim3((unsigned)grid), dim3(64 * NW), 0, s, a);
+  const dim3 g((unsigned)grid), b(64 * NW);
+  const bool vec = a.z.dim % 4 == 0;
+  if (a.bias && vec) hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, true, true>), g, b, 0, s, a);
+  else if (a.bias) hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, true, false>), g, b, 0, s, a);
+  else if (vec) hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, false, true>), g, b, 0, s, a);
+  else hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, false, false>), g, b, 0, s, a);
   return MNV_LAUNCH_STATUS();
 }
 
