@@ -20,6 +20,11 @@ struct BwdArgs {
   unsigned first_pair;  // the launch's first (entry, key head)
   int rows;             // q_len * group
   MnvFastDiv by_group;
+  // The loop of a workgroup (dk, dv: over a group's heads and their tiles of queries; dq: over tiles of keys) in
+  // `splits` parts of `chunk` tiles each; with more than one, sums by part in `sums`: [part][row][DP], and for
+  // dk and dv those of dv behind those of dk
+  int splits, chunk;
+  float* sums;
 };
 
 // dq[row][0] = dout_row . out_row; 16 lanes per row.
@@ -47,8 +52,11 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
   __shared__ __align__(16) float row_stats[2][3][32];  // m, 1 / l, delta of the tile's queries
   __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
   const AttentionSizes& z = a.z;
-  const MnvAttentionPlace place = mnv_attention_place(a.tiles, a.first_pair, z, a.lengths);
-  const int tile = place.tile, b = place.b, kh = place.kh, n = place.n, group = z.group();
+  const MnvAttentionPlace place = mnv_attention_place(a.tiles * a.splits, a.first_pair, z, a.lengths);
+  const int split = mnv_uniform(place.tile / a.tiles), tile = place.tile - split * a.tiles;
+  const int b = place.b, kh = place.kh, n = place.n, group = z.group();
+  const int q_tiles = (z.q_len + 31) / 32, begin = split * a.chunk;
+  const int end = begin + a.chunk < group * q_tiles ? begin + a.chunk : group * q_tiles;
   const int wave = mnv_uniform(threadIdx.x / MNV_WAVE), lane = threadIdx.x % MNV_WAVE, half = lane / 32;
 
   const int j = tile * 128 + wave * 32 + lane % 32;
@@ -76,7 +84,10 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
     }
     const unsigned pitch = (unsigned)z.heads * z.dim;
     const int jb = shown ? j : n - 1;
-    for (int g = 0; g < group; ++g) {
+    const int first_g = mnv_uniform(begin / q_tiles), last_g = mnv_uniform((end - 1) / q_tiles);
+    for (int g = first_g; g <= last_g; ++g) {
+      const int from = g == first_g ? (begin - g * q_tiles) * 32 : 0;
+      const int to = g == last_g && (end - g * q_tiles) * 32 < z.q_len ? (end - g * q_tiles) * 32 : z.q_len;
       const int h = kh * group + g;
       const size_t row0 = (size_t)b * z.q_len * z.heads + h;  // rows of the head are z.heads apart
       const float* qb = a.q + row0 * z.dim;
@@ -110,15 +121,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
       };
       {
         Rows first;
-        fetch_rows(first, 0);
-        first.stage.fetch(qb, ob, pitch, z.q_len, z.dim);
+        fetch_rows(first, from);
+        first.stage.fetch(qb + (size_t)from * pitch, ob + (size_t)from * pitch, pitch, z.q_len - from, z.dim);
         first.stage.template store<true>(lds, z.scale);
-        store_rows(first, 0, 0);
+        store_rows(first, from, 0);
       }
       __syncthreads();
       int turn = 0;
-      for (int i0 = 0; i0 < z.q_len; i0 += 32) {
-        const bool more = i0 + 32 < z.q_len;
+      for (int i0 = from; i0 < to; i0 += 32) {
+        const bool more = i0 + 32 < to;
         Rows next;  // behind the last tile that one again: no branch parts what follows
         const int i1 = more ? i0 + 32 : i0;
         fetch_rows(next, i1);
@@ -251,7 +262,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
       }
     }
   }
-  if (j < z.k_len) {
+  if (j < z.k_len && a.splits > 1) {
+    // of keys that are not read, nothing: mnv_attention_sum_kernel knows them
+    const size_t keys = (size_t)z.batch * z.k_len * z.kv_heads;
+    float* to = a.sums + (split * keys + key) * DP;
+    if (j < n) {
+      mnv_store_column<DP>(dk, 1.f, true, to, DP);
+      mnv_store_column<DP>(dv, 1.f, true, to + a.splits * keys * DP, DP);
+    }
+  } else if (j < z.k_len) {
     mnv_store_column<DP>(dk, 1.f, j < n, a.dk + key * z.dim, z.dim);
     mnv_store_column<DP>(dv, 1.f, j < n, a.dv + key * z.dim, z.dim);
   }
@@ -263,8 +282,10 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
   using Stage = MnvStage<DP, 256, VEC>;  // keys and values
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
-  const MnvAttentionPlace place = mnv_attention_place(a.tiles, 0, z, a.lengths);
-  const int tile = place.tile, b = place.b, kh = place.kh, n = place.n;
+  const MnvAttentionPlace place = mnv_attention_place(a.tiles * a.splits, 0, z, a.lengths);
+  const int split = mnv_uniform(place.tile / a.tiles), tile = place.tile - split * a.tiles, b = place.b, kh = place.kh;
+  // the part's keys
+  const int begin = split * a.chunk * 32, n = place.n < begin + a.chunk * 32 ? place.n : begin + a.chunk * 32;
   const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
 
   const int r = tile * 128 + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
@@ -278,7 +299,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[c][e] = 0.f;
 
-  if (n > 0) {
+  if (n > begin) {
     MnvParts qp[KS], op[KS];
     float delta = 0.f;
 #pragma unroll
@@ -304,12 +325,12 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
 
     {
       Stage first;
-      first.fetch(kb, vb, pitch, n, z.dim);
+      first.fetch(kb + (size_t)begin * pitch, vb + (size_t)begin * pitch, pitch, n - begin, z.dim);
       first.template store<false>(lds, 1.f);
     }
     __syncthreads();
     char* now = lds;
-    for (int j0 = 0; j0 < n; j0 += 32) {
+    for (int j0 = begin; j0 < n; j0 += 32) {
       const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
       Stage stage;  // behind the last tile that one again: no branch parts what follows
       const int j1 = more ? j0 + 32 : j0;
@@ -383,7 +404,37 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
       __syncthreads();
     }
   }
-  if (r < a.rows) mnv_store_column<DP>(dq, z.scale, true, a.dq + row * z.dim, z.dim);
+  if (r >= a.rows) return;
+  if (a.splits == 1)
+    mnv_store_column<DP>(dq, z.scale, true, a.dq + row * z.dim, z.dim);
+  else if (n > begin)  // of a part without keys, nothing
+    mnv_store_column<DP>(dq, 1.f, true, a.sums + (split * z.q_rows() + row) * DP, DP);
+}
+
+// out[row] = f * the sums of a row's parts, 0 for none; 16 lanes to a row.  Of queries (per_row = heads, q_len to an entry) the
+// parts that have keys count, `chunk` keys to each; of keys all, and those that are read.
+__global__ __launch_bounds__(256) void mnv_attention_sum_kernel(const float* __restrict__ sums, float* __restrict__ out,
+                                                                const float* __restrict__ lengths, AttentionSizes z,
+                                                                bool queries, int splits, int chunk, int pitch, float f) {
+  const size_t rows = queries ? z.q_rows() : (size_t)z.batch * z.k_len * z.kv_heads;
+  const size_t row = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
+  if (row >= rows) return;
+  const size_t per_entry = queries ? (size_t)z.q_len * z.heads : (size_t)z.k_len * z.kv_heads;
+  const int n = mnv_visible(lengths, (int)(row / per_entry), z.k_len);
+  int parts = splits;
+  if (queries) parts = n < splits * chunk ? (n + chunk - 1) / chunk : splits;
+  else if ((int)(row % per_entry / z.kv_heads) >= n) parts = 0;
+  for (int d = threadIdx.x % 16 * 4; d < z.dim; d += 64) {
+    mnv_f4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < parts; ++s) {
+      const mnv_f4 t = *reinterpret_cast<const mnv_f4*>(sums + (s * rows + row) * pitch + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += t[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (d + e < z.dim) out[row * z.dim + d + e] = acc[e] * f;
+  }
 }
 
 // dbias[o] += the parts of o: of every entry among the launch's pairs and every 32 keys that have the diagonal.
@@ -450,7 +501,42 @@ __global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dbias_alone_kernel(Bwd
 size_t pair_bytes(const AttentionSizes& z) {
   return (size_t)z.group() * key_tiles(z.k_len) * diagonal_pitch(z.q_len) * sizeof(float);
 }
-#define MNV_AT_PARTS_BYTES ((size_t)256 << 20)  // of partial sums at a time, where there are more
+#define MNV_AT_PARTS_BYTES ((size_t)256 << 20)  // of partial sums of diagonals at a time, where there are more
+
+// How a call uses its workspace: the diagonals' partial sums of `pairs` pairs of an entry and a key head at a
+// time (0: none) first, the parts' sums behind them.  dq's come after dk's and dv's are added up.
+struct BwdPlan {
+  size_t pairs, diagonal_bytes;
+  int key_splits, query_splits;
+  size_t bytes;
+};
+BwdPlan make_plan(const AttentionSizes& z, bool has_bias, size_t workspace_bytes) {
+  BwdPlan p = {0, 0, 1, 1, 0};
+  const size_t pairs = (size_t)z.batch * z.kv_heads, dp = mnv_attention_padded(z.dim);
+  if (has_bias) {
+    const size_t one = pair_bytes(z), most = workspace_bytes < MNV_AT_PARTS_BYTES ? workspace_bytes : MNV_AT_PARTS_BYTES;
+    p.pairs = most / one;
+    if (p.pairs == 0 && workspace_bytes >= one) p.pairs = 1;
+    if (p.pairs > pairs) p.pairs = pairs;
+    p.diagonal_bytes = mnv_ceil_div(p.pairs * one, 16) * 16;
+    if (p.diagonal_bytes > workspace_bytes) p.diagonal_bytes = p.pairs * one;
+  }
+  const size_t left = workspace_bytes - p.diagonal_bytes, places = (size_t)mnv_cu_count() * (dp <= 32 ? 2 : 1);
+  // a head's diagonals are summed by one workgroup
+  const size_t key_part = 2 * (size_t)z.batch * z.k_len * z.kv_heads * dp * sizeof(float);
+  const size_t q_tiles = mnv_ceil_div(z.q_len, 32);
+  const bool whole_heads = p.pairs > 0;
+  if (p.pairs == 0 || p.pairs == pairs)
+    p.key_splits = mnv_attention_parts(mnv_ceil_div(z.k_len, 128) * pairs, places, whole_heads ? z.group() : q_tiles * z.group(),
+                                       whole_heads ? 1 : 2, key_part, left);
+  const size_t query_part = z.q_rows() * dp * sizeof(float);
+  p.query_splits = mnv_attention_parts(mnv_ceil_div((size_t)z.q_len * z.group(), 128) * pairs, places, mnv_ceil_div(z.k_len, 32),
+                                       2, query_part, workspace_bytes);
+  const size_t keys = p.diagonal_bytes + (p.key_splits > 1 ? p.key_splits * key_part : 0);
+  const size_t queries = p.query_splits > 1 ? p.query_splits * query_part : 0;
+  p.bytes = keys > queries ? keys : queries;
+  return p;
+}
 
 #define MNV_AT_LAUNCH(kernel)                                                                              \
   do {                                                                                                     \
@@ -483,10 +569,7 @@ extern "C" {
 size_t mnv_attention_bwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim,
                                          int has_bias) {
   const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, 1.f};
-  if (!has_bias || !mnv_attention_sizes_ok(z)) return 0;
-  const size_t one = pair_bytes(z), all = one * batch * kv_heads;
-  if (all <= MNV_AT_PARTS_BYTES) return all;
-  return one > MNV_AT_PARTS_BYTES ? one : MNV_AT_PARTS_BYTES / one * one;
+  return mnv_attention_sizes_ok(z) ? make_plan(z, has_bias != 0, MNV_AT_ANY_WORKSPACE).bytes : 0;
 }
 
 int mnv_attention_bwd(const float* q, const float* k, const float* v, const float* bias, const float* lengths,
@@ -497,43 +580,63 @@ int mnv_attention_bwd(const float* q, const float* k, const float* v, const floa
   if (!q || !k || !v || !out || !stats || !dout || !dq || !dk || !dv || (bias && !dbias) || !mnv_attention_sizes_ok(z))
     return MNV_ERR_INVALID;
   const hipStream_t s = mnv_stream(stream);
-  BwdArgs a = {q, k, v, bias, lengths, out, stats, dout, dq, dk, dv, nullptr, z, 0, 0, q_len * z.group(),
-               mnv_fastdiv_make(z.group())};
-  const unsigned pairs = (unsigned)batch * kv_heads;
-  hipLaunchKernelGGL(mnv_attention_delta_kernel, dim3((unsigned)mnv_ceil_div(z.q_rows(), 16)), dim3(256), 0, s, dout,
-                     out, dq, z.q_rows(), head_dim);
+  const BwdPlan plan = make_plan(z, bias != nullptr, workspace && mnv_aligned16(workspace) ? workspace_bytes : 0);
+  const int dp = mnv_attention_padded(head_dim), group = z.group();
+  const size_t pairs = (size_t)batch * kv_heads, q_rows = z.q_rows(), k_rows = pairs * k_len;
+  BwdArgs a = {q, k, v, bias, lengths, out, stats, dout, dq, dk, dv, nullptr, z, 0, 0, q_len * group,
+               mnv_fastdiv_make(group), 1, 0, nullptr};
+  hipLaunchKernelGGL(mnv_attention_delta_kernel, dim3((unsigned)mnv_ceil_div(q_rows, 16)), dim3(256), 0, s, dout, out, dq,
+                     q_rows, head_dim);
   MNV_HIP_TRY(hipGetLastError());
 
-  // keys, with the bias's gradient as many pairs of an entry and a key head at a time as the workspace holds
-  size_t at_once = pairs;
-  if (bias) {
-    at_once = workspace ? workspace_bytes / pair_bytes(z) : 0;
-    if (at_once > pairs) at_once = pairs;
-    if (at_once) a.parts = static_cast<float*>(workspace);
-  }
+  // keys, and with them the bias's gradient as far as the workspace holds its parts
   BwdArgs ka = a;
-  if (bias && !at_once) at_once = pairs;
   ka.tiles = (int)mnv_ceil_div(k_len, 128);
-  if ((unsigned long long)ka.tiles * at_once > 0x7fffffffULL) return MNV_ERR_INVALID;
-  for (unsigned p = 0; p < pairs; p += (unsigned)at_once) {
-    const unsigned now = pairs - p < at_once ? pairs - p : (unsigned)at_once;
-    ka.first_pair = p;
-    const int rc = by_dim(head_dim, launch_dkv<32>, launch_dkv<64>, launch_dkv<96>, launch_dkv<128>, ka, now * ka.tiles, s);
+  const int q_tiles = (int)mnv_ceil_div(q_len, 32), units = plan.pairs ? group : group * q_tiles;
+  ka.chunk = (int)mnv_ceil_div(units, plan.key_splits) * (plan.pairs ? q_tiles : 1);
+  ka.splits = plan.key_splits;
+  ka.parts = plan.pairs ? static_cast<float*>(workspace) : nullptr;
+  ka.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.diagonal_bytes);
+  const size_t at_once = plan.pairs ? plan.pairs : pairs;
+  if (ka.tiles * ka.splits * at_once > 0x7fffffff) return MNV_ERR_INVALID;
+  for (size_t p = 0; p < pairs; p += at_once) {
+    const unsigned now = (unsigned)(pairs - p < at_once ? pairs - p : at_once);
+    ka.first_pair = (unsigned)p;
+    const int rc = by_dim(head_dim, launch_dkv<32>, launch_dkv<64>, launch_dkv<96>, launch_dkv<128>, ka,
+                          now * ka.tiles * ka.splits, s);
     if (rc) return rc;
-    if (!a.parts) continue;
+    if (!ka.parts) continue;
     const dim3 grid((unsigned)mnv_ceil_div(z.offsets(), 256), heads < 65535 ? heads : 65535);
-    hipLaunchKernelGGL(mnv_attention_dbias_kernel, grid, dim3(256), 0, s, a.parts, lengths, dbias, z, p, now, p == 0);
+    hipLaunchKernelGGL(mnv_attention_dbias_kernel, grid, dim3(256), 0, s, ka.parts, lengths, dbias, z, (unsigned)p, now,
+                       p == 0);
     MNV_HIP_TRY(hipGetLastError());
   }
-  if (bias && !a.parts) {
+  if (ka.splits > 1) {
+    const dim3 grid((unsigned)mnv_ceil_div(k_rows, 16));
+    hipLaunchKernelGGL(mnv_attention_sum_kernel, grid, dim3(256), 0, s, ka.sums, dk, lengths, z, false, ka.splits, 0, dp, 1.f);
+    MNV_HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(mnv_attention_sum_kernel, grid, dim3(256), 0, s, ka.sums + ka.splits * k_rows * dp, dv, lengths, z,
+                       false, ka.splits, 0, dp, 1.f);
+    MNV_HIP_TRY(hipGetLastError());
+  }
+  if (bias && !ka.parts) {
     const size_t work = z.offsets() * heads;
     hipLaunchKernelGGL(mnv_attention_dbias_alone_kernel, dim3((unsigned)(work < (1u << 20) ? work : (1u << 20))),
                        dim3(MNV_WAVE), 0, s, a, dbias);
     MNV_HIP_TRY(hipGetLastError());
   }
+
   a.tiles = (int)mnv_ceil_div(a.rows, 128);
-  if ((unsigned long long)a.tiles * pairs > 0x7fffffffULL) return MNV_ERR_INVALID;
-  return by_dim(head_dim, launch_dq<32>, launch_dq<64>, launch_dq<96>, launch_dq<128>, a, a.tiles * pairs, s);
+  a.splits = plan.query_splits;
+  a.chunk = (int)mnv_ceil_div(mnv_ceil_div(k_len, 32), a.splits);
+  a.sums = static_cast<float*>(workspace);
+  if (a.tiles * a.splits * pairs > 0x7fffffff) return MNV_ERR_INVALID;
+  const int rc = by_dim(head_dim, launch_dq<32>, launch_dq<64>, launch_dq<96>, launch_dq<128>, a,
+                        (unsigned)(a.tiles * a.splits * pairs), s);
+  if (rc || a.splits == 1) return rc;
+  hipLaunchKernelGGL(mnv_attention_sum_kernel, dim3((unsigned)mnv_ceil_div(q_rows, 16)), dim3(256), 0, s, a.sums, dq, lengths,
+                     z, true, a.splits, a.chunk * 32, dp, scale);
+  return MNV_LAUNCH_STATUS();
 }
 
 }  // extern "C"

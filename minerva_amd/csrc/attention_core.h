@@ -38,6 +38,23 @@ static inline bool mnv_attention_sizes_ok(const AttentionSizes& z) {
   return ((long long)z.q_len + z.k_len - 1) * z.heads <= most && fabsf(z.scale) <= 3e38f;
 }
 
+// Columns that the kernels' products have.
+static inline int mnv_attention_padded(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128; }
+
+// Parts that a workgroup's loop over `tiles` tiles is cut into where `blocks` workgroups leave places of the chip
+// empty: as many as fill them, with `least` tiles or more to a part, and no more than the workspace holds.
+static inline int mnv_attention_parts(size_t blocks, size_t places, size_t tiles, size_t least, size_t part_bytes,
+                                      size_t workspace_bytes) {
+  size_t parts = blocks ? places / blocks : 1;
+  if (parts > tiles / least) parts = tiles / least;
+  if (parts > MNV_WAVE) parts = MNV_WAVE;
+  if (parts > workspace_bytes / part_bytes) parts = workspace_bytes / part_bytes;
+  if (parts < 2) return 1;
+  const size_t each = mnv_ceil_div(tiles, parts);
+  return (int)mnv_ceil_div(tiles, each);
+}
+#define MNV_AT_ANY_WORKSPACE ((size_t)-1)  // for the queries
+
 #ifdef __HIPCC__
 #define MNV_LOG2E 1.4426950408889634f
 

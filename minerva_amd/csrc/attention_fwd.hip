@@ -21,16 +21,21 @@ struct FwdArgs {
   int rows;        // q_len * group
   int row_tiles;   // per entry and key head
   MnvFastDiv by_group;
+  int chunk;       // keys of a part, a multiple of 32
+  int parts;       // 1: the result itself is written
+  float *part_out, *part_stats;  // [part][row of q][DP], and [2]: sums without the division by l
 };
 
 template <int DP, int NW, bool BIAS, bool VEC>
-__global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 64 * NW, VEC>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
-  const MnvAttentionPlace place = mnv_attention_place(a.row_tiles, 0, z, a.lengths);
-  const int tile = place.tile, b = place.b, kh = place.kh, n = place.n;
+  const MnvAttentionPlace place = mnv_attention_place(a.row_tiles * a.parts, 0, z, a.lengths);
+  const int part = mnv_uniform(place.tile / a.row_tiles), tile = place.tile - part * a.row_tiles, b = place.b, kh = place.kh;
+  // the part's keys
+  const int begin = part * a.chunk, n = place.n < begin + a.chunk ? place.n : begin + a.chunk;
   const int lane = threadIdx.x % MNV_WAVE, half = lane / 32;
 
   const int r = tile * (32 * NW) + (int)threadIdx.x / MNV_WAVE * 32 + lane % 32;
@@ -45,7 +50,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
     for (int e = 0; e < 16; ++e) acc[c][e] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  if (n > 0) {
+  if (n > begin) {
     MnvParts qp[DP / 16];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
@@ -62,7 +67,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
 
     {
       Stage first;
-      first.fetch(kb, vb, pitch, n, z.dim);
+      first.fetch(kb + (size_t)begin * pitch, vb + (size_t)begin * pitch, pitch, n - begin, z.dim);
       first.template store<false>(lds, 1.f);
     }
     __syncthreads();
@@ -75,7 +80,16 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
     auto fetch = [&](int piece, int j1) __attribute__((always_inline)) {
       stage.fetch_piece(piece, kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
     };
-    // scores of the tile in `now`; FETCH: the tile from j1 on is fetched, else that in `stage` is cut to `then`
+    // a step's share of the next tile's fetching or cutting
+    auto share = [&](auto fetches, int s, char* then, int j1) __attribute__((always_inline)) {
+      constexpr int EACH = (Stage::PIECES + KS - 1) / KS;
+#pragma unroll
+      for (int piece = s * EACH; piece < (s + 1) * EACH && piece < Stage::PIECES; ++piece) {
+        if (decltype(fetches)::value) fetch(piece, j1);
+        else stage.template store_piece<false>(piece, then, 1.f);
+      }
+    };
+    // scores of the tile in `now`; `fetches`: the tile from j1 on is fetched, else that in `stage` is cut into `then`
     auto scores = [&](auto fetches, const char* now, char* then, int j1) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) t[e] = 0.f;
@@ -86,8 +100,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
         MnvParts ahead = cur;
         if (s + 1 < KS) ahead = Stage::by_rows(now, s + 1);
         mnv_mul(t, cur, qp[s]);
-        if (decltype(fetches)::value) fetch(s, j1);
-        else stage.template store_piece<false>(s, then, 1.f);
+        share(fetches, s, then, j1);
         MNV_STEP_ORDER(6);
         cur = ahead;
       }
@@ -151,18 +164,17 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
 #pragma unroll
           for (int pair = 4 + s * 4 / NB; pair < 4 + (s + 1) * 4 / NB; ++pair) cut_p(pair);
         }
-        if (decltype(fetches)::value) fetch(s, j1);
-        else stage.template store_piece<false>(s, then, 1.f);
+        share(fetches, s, then, j1);
         MNV_STEP_ORDER(6);
         cur = ahead;
       }
     };
     const std::true_type fetches;
     const std::false_type cuts;
-    const int last = (n - 1) / 32 * 32;  // behind it that tile again: no branch parts a phase
+    const int last = begin + (n - begin - 1) / 32 * 32;  // behind it that tile again: no branch parts a phase
     char *now = lds, *then = lds + Stage::BYTES;
     if (!late) {
-      for (int j0 = 0; j0 < n; j0 += 32) {
+      for (int j0 = begin; j0 < n; j0 += 32) {
         scores(fetches, now, then, j0 < last ? j0 + 32 : last);
         if (NW == 8) __syncthreads();
         results(cuts, now, then, j0, 0);
@@ -175,9 +187,9 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
     } else {
       // one phase behind: cuts a tile while it makes scores, which is when the others do
 #pragma unroll
-      for (int piece = 0; piece < Stage::PIECES; ++piece) fetch(piece, last < 32 ? last : 32);
+      for (int piece = 0; piece < Stage::PIECES; ++piece) fetch(piece, last < begin + 32 ? last : begin + 32);
       __syncthreads();
-      for (int j0 = 0; j0 < n; j0 += 32) {
+      for (int j0 = begin; j0 < n; j0 += 32) {
         scores(cuts, now, then, 0);
         __syncthreads();
         results(fetches, now, then, j0, j0 + 64 < last ? j0 + 64 : last);
@@ -189,19 +201,94 @@ __global__ __launch_bounds__(64 * NW, 2) void mnv_attention_fwd_kernel(FwdArgs a
     }
     l += __shfl_xor(l, 32, MNV_WAVE);
   }
-  if (r < a.rows) {
-    mnv_store_column<DP>(acc, mnv_inverse(l), true, a.out + row * z.dim, z.dim);
+  if (r >= a.rows) return;
+  if (a.parts > 1) {
+    const size_t at = part * z.q_rows() + row;
+    if (n > begin) mnv_store_column<DP>(acc, 1.f, true, a.part_out + at * DP, DP);
     if (half == 0) {
-      a.stats[2 * row] = m;
-      a.stats[2 * row + 1] = l;
+      a.part_stats[2 * at] = m;
+      a.part_stats[2 * at + 1] = l;
+    }
+    return;
+  }
+  mnv_store_column<DP>(acc, mnv_inverse(l), true, a.out + row * z.dim, z.dim);
+  if (half == 0) {
+    a.stats[2 * row] = m;
+    a.stats[2 * row + 1] = l;
+  }
+}
+
+// out and stats of up to 64 parts: m = max m_s, l = sum l_s exp(m_s - m), out = sum out_s exp(m_s - m) / l.  A part that
+// saw no key has l_s = 0, and wrote no sums.  A wavefront to a row: a lane to a part's numbers, then 16 lanes
+// to the sums of every fourth part.
+__global__ __launch_bounds__(256) void mnv_attention_join_kernel(const float* __restrict__ part_out,
+                                                                 const float* __restrict__ part_stats,
+                                                                 float* __restrict__ out, float* __restrict__ stats,
+                                                                 size_t rows, int parts, int dim, int pitch) {
+  const size_t row = (size_t)blockIdx.x * 4 + threadIdx.x / MNV_WAVE;
+  if (row >= rows) return;
+  const int lane = threadIdx.x % MNV_WAVE;
+  float ms = -INFINITY, ls = 0.f;
+  if (lane < parts) {
+    ms = part_stats[2 * (lane * rows + row)];
+    ls = part_stats[2 * (lane * rows + row) + 1];
+  }
+  float m = ms;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, MNV_WAVE));
+  const float w = ls == 0.f ? 0.f : mnv_weight(ms, mnv_finite_max(m));
+  float l = ls * w;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, MNV_WAVE);
+  const float f = mnv_inverse(l);
+  const unsigned long long shown = __ballot(ls != 0.f);
+  for (int d = lane % 16 * 4; d < pitch; d += 64) {
+    mnv_f4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 16) {
+      mnv_f4 t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = s0 + 4 * u + lane / 16;
+        t[u] = mnv_f4{0.f, 0.f, 0.f, 0.f};
+        if (s < parts && (shown >> s & 1)) t[u] = *reinterpret_cast<const mnv_f4*>(part_out + (s * rows + row) * pitch + d);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int s = s0 + 4 * u + lane / 16;
+        const float ws = __shfl(w, s < parts ? s : 0, MNV_WAVE);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(t[u][e], ws, acc[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[e] += __shfl_xor(acc[e], 16, MNV_WAVE);
+      acc[e] += __shfl_xor(acc[e], 32, MNV_WAVE);
+      if (lane < 16 && d + e < dim) out[row * dim + d + e] = acc[e] * f;
     }
   }
+  if (lane < 2) stats[2 * row + lane] = lane ? l : m;
+}
+
+// Wavefronts of a workgroup: one for up to 32 rows of an entry and key head; eight, in two halves, where a
+// workgroup has the CU to itself and rows enough.
+int wavefronts(const AttentionSizes& z) {
+  const long long rows = (long long)z.q_len * z.group();
+  return rows <= 32 ? 1 : z.dim > 64 && rows > 128 ? 8 : 4;
+}
+size_t part_bytes(const AttentionSizes& z) { return z.q_rows() * (mnv_attention_padded(z.dim) + 2) * sizeof(float); }
+int parts(const AttentionSizes& z, size_t workspace_bytes) {
+  const int nw = wavefronts(z);
+  const size_t blocks = mnv_ceil_div((size_t)z.q_len * z.group(), 32 * nw) * z.batch * z.kv_heads;
+  // workgroups that a CU holds, by LDS and registers
+  const size_t places = (size_t)mnv_cu_count() * (nw == 1 ? (z.dim <= 64 ? 3 : 1) : nw == 4 && z.dim <= 64 ? 2 : 1);
+  return mnv_attention_parts(blocks, places, mnv_ceil_div(z.k_len, 32), nw == 1 ? 2 : 4, part_bytes(z), workspace_bytes);
 }
 
 template <int DP, int NW>
 int launch(FwdArgs& a, hipStream_t s) {
   a.row_tiles = (int)mnv_ceil_div(a.rows, 32 * NW);
-  const size_t grid = (size_t)a.row_tiles * a.z.batch * a.z.kv_heads;
+  const size_t grid = (size_t)a.row_tiles * a.parts * a.z.batch * a.z.kv_heads;
   if (grid > 0x7fffffff) return MNV_ERR_INVALID;
   const dim3 g((unsigned)grid), b(64 * NW);
   const bool vec = a.z.dim % 4 == 0;
@@ -212,23 +299,44 @@ int launch(FwdArgs& a, hipStream_t s) {
   return MNV_LAUNCH_STATUS();
 }
 
+template <int DP>
+int launch_width(FwdArgs& a, int nw, hipStream_t s) {
+  if (nw == 1) return launch<DP, 1>(a, s);
+  if (DP > 64 && nw == 8) return launch<DP, DP <= 64 ? 4 : 8>(a, s);
+  return launch<DP, 4>(a, s);
+}
+
 }  // namespace
 
 extern "C" {
 
-size_t mnv_attention_fwd_workspace_bytes(int, int, int, int, int, int) { return 0; }
+size_t mnv_attention_fwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim) {
+  const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, 1.f};
+  if (!mnv_attention_sizes_ok(z)) return 0;
+  const int n = parts(z, MNV_AT_ANY_WORKSPACE);
+  return n > 1 ? n * part_bytes(z) : 0;
+}
 
 int mnv_attention_fwd(const float* q, const float* k, const float* v, const float* bias, const float* lengths,
                       float* out, float* stats, int batch, int heads, int kv_heads, int q_len, int k_len, int head_dim,
-                      float scale, void*, size_t, mnv_stream_t stream) {
+                      float scale, void* workspace, size_t workspace_bytes, mnv_stream_t stream) {
   const AttentionSizes z = {batch, heads, kv_heads, q_len, k_len, head_dim, scale};
   if (!q || !k || !v || !out || !stats || !mnv_attention_sizes_ok(z)) return MNV_ERR_INVALID;
-  FwdArgs a = {q, k, v, bias, lengths, out, stats, z, q_len * z.group(), 0, mnv_fastdiv_make(z.group())};
+  FwdArgs a = {q, k, v, bias, lengths, out, stats, z, q_len * z.group(), 0, mnv_fastdiv_make(z.group()), 0, 1, nullptr, nullptr};
+  a.parts = parts(z, workspace && mnv_aligned16(workspace) ? workspace_bytes : 0);
+  a.chunk = (int)mnv_ceil_div(mnv_ceil_div(k_len, 32), a.parts) * 32;
+  a.part_out = static_cast<float*>(workspace);
+  a.part_stats = a.part_out + (a.parts > 1 ? a.parts * z.q_rows() * mnv_attention_padded(head_dim) : 0);
   const hipStream_t s = mnv_stream(stream);
-  if (head_dim <= 32) return launch<32, 4>(a, s);
-  if (head_dim <= 64) return launch<64, 4>(a, s);
-  if (head_dim <= 96) return launch<96, 8>(a, s);
-  return launch<128, 8>(a, s);
+  const int nw = wavefronts(z), dp = mnv_attention_padded(head_dim);
+  const int rc = dp == 32   ? launch_width<32>(a, nw, s)
+                 : dp == 64 ? launch_width<64>(a, nw, s)
+                 : dp == 96 ? launch_width<96>(a, nw, s)
+                            : launch_width<128>(a, nw, s);
+  if (rc || a.parts == 1) return rc;
+  hipLaunchKernelGGL(mnv_attention_join_kernel, dim3((unsigned)mnv_ceil_div(z.q_rows(), 4)), dim3(256), 0, s, a.part_out,
+                     a.part_stats, out, stats, z.q_rows(), a.parts, head_dim, dp);
+  return MNV_LAUNCH_STATUS();
 }
 
 }  // extern "C"
