@@ -29,6 +29,7 @@ struct FwdArgs {
 template <int DP, int NW, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
+  constexpr bool AHEAD = NW != 8;
   using Stage = MnvStage<DP, 64 * NW, VEC>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
@@ -93,21 +94,24 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
     auto scores = [&](auto fetches, const char* now, char* then, int j1) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) t[e] = 0.f;
-      MnvParts cur = Stage::by_rows(now, 0);
+      MnvParts cur;
+      if (AHEAD) cur = Stage::by_rows(now, 0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         MnvParts ahead = cur;
-        if (s + 1 < KS) ahead = Stage::by_rows(now, s + 1);
+        if (!AHEAD) cur = Stage::by_rows(now, s);
+        else if (s + 1 < KS) ahead = Stage::by_rows(now, s + 1);
         mnv_mul(t, cur, qp[s]);
         share(fetches, s, then, j1);
         MNV_STEP_ORDER(6);
-        cur = ahead;
+        if (AHEAD) cur = ahead;
       }
     };
     auto results = [&](auto fetches, const char* now, char* then, int j0, int j1) __attribute__((always_inline)) {
       const bool whole = j0 + 32 <= n;
-      MnvParts cur = Stage::by_cols(now + Stage::MATRIX, 0, 0);
+      MnvParts cur;
+      if (AHEAD) cur = Stage::by_cols(now + Stage::MATRIX, 0, 0);
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -158,7 +162,8 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         MnvParts ahead = cur;
-        if (s + 1 < KS) ahead = Stage::by_cols(now + Stage::MATRIX, (s + 1) % NB * 32, (s + 1) / NB);
+        if (!AHEAD) cur = Stage::by_cols(now + Stage::MATRIX, s % NB * 32, s / NB);
+        else if (s + 1 < KS) ahead = Stage::by_cols(now + Stage::MATRIX, (s + 1) % NB * 32, (s + 1) / NB);
         mnv_mul(acc[s % NB], cur, pc[s / NB].parts());
         if (s < NB) {
 #pragma unroll
@@ -166,7 +171,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
         }
         share(fetches, s, then, j1);
         MNV_STEP_ORDER(6);
-        cur = ahead;
+        if (AHEAD) cur = ahead;
       }
     };
     const std::true_type fetches;
@@ -274,7 +279,7 @@ __global__ __launch_bounds__(256) void mnv_attention_join_kernel(const float* __
 // workgroup has the CU to itself and rows enough.
 int wavefronts(const AttentionSizes& z) {
   const long long rows = (long long)z.q_len * z.group();
-  return rows <= 32 ? 1 : z.dim > 64 && rows > 128 ? 8 : 4;
+  return rows <= 32 ? 1 : z.dim > 64 && mnv_ceil_div(rows, 256) * z.batch * z.kv_heads >= (size_t)mnv_cu_count() / 2 ? 8 : 4;
 }
 size_t part_bytes(const AttentionSizes& z) { return z.q_rows() * (mnv_attention_padded(z.dim) + 2) * sizeof(float); }
 int parts(const AttentionSizes& z, size_t workspace_bytes) {
@@ -282,7 +287,7 @@ int parts(const AttentionSizes& z, size_t workspace_bytes) {
   const size_t blocks = mnv_ceil_div((size_t)z.q_len * z.group(), 32 * nw) * z.batch * z.kv_heads;
   // workgroups that a CU holds, by LDS and registers
   const size_t places = (size_t)mnv_cu_count() * (nw == 1 ? (z.dim <= 64 ? 3 : 1) : nw == 4 && z.dim <= 64 ? 2 : 1);
-  return mnv_attention_parts(blocks, places, mnv_ceil_div(z.k_len, 32), nw == 1 ? 2 : 4, part_bytes(z), workspace_bytes);
+  return mnv_attention_parts(blocks, places, mnv_ceil_div(z.k_len, 32), 2, part_bytes(z), workspace_bytes);
 }
 
 template <int DP, int NW>
