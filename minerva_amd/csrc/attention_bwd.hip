@@ -45,7 +45,7 @@ __host__ __device__ inline size_t diagonal_pitch(int q_len) { return ((size_t)q_
 __host__ __device__ inline size_t key_tiles(int k_len) { return ((size_t)k_len + 31) / 32; }
 
 template <int DP, bool BIAS, bool VEC>
-__global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 256, VEC>;  // queries (times scale) and their gradients
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
@@ -159,12 +159,12 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
 #pragma unroll
         for (int e = 0; e < 16; ++e) t[e] = dp[e] = 0.f;
         MnvCutting pc[2], sc[2];
-        auto operand = [&](int k) __attribute__((always_inline)) {
+        auto operand = [&](int k, int c) __attribute__((always_inline)) {
           const int s = k % KS;
-          return k < KS       ? Stage::by_rows(now, s)
-                 : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s)
-                 : k < 3 * KS ? Stage::by_cols(now + Stage::MATRIX, s % NB * 32, s / NB)
-                              : Stage::by_cols(now, s % NB * 32, s / NB);
+          return k < KS       ? Stage::by_rows(now, s, c)
+                 : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s, c)
+                 : k < 3 * KS ? Stage::by_cols(now + Stage::MATRIX, s % NB * 32, s / NB, c)
+                              : Stage::by_cols(now, s % NB * 32, s / NB, c);
         };
         // the numbers of two queries (a pair of result registers) that a step needs, read in the step before
         constexpr int MOST = (8 + KS - 1) / KS;
@@ -173,18 +173,23 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
           if (k < KS || k >= 3 * KS) return;
           const int first = k % KS * 8 / KS;
 #pragma unroll
-          for (int pair = first; pair < (k % KS + 1) * 8 / KS; ++pair)
-#pragma unroll
-            for (int c = 0; c < (k < 2 * KS ? 2 : 1); ++c)
-              rows[c][pair - first] = *reinterpret_cast<const mnv_f2*>(row_stats[turn][k < 2 * KS ? c : 2] + mnv_acc_row(2 * pair, half));
+          for (int u = 0; u < MOST; ++u) {
+            const int pair = first + u;
+            if (pair >= (k % KS + 1) * 8 / KS) continue;
+            rows[0][u] = *reinterpret_cast<const mnv_f2*>(row_stats[turn][k < 2 * KS ? 0 : 2] + mnv_acc_row(2 * pair, half));
+            if (k < 2 * KS) rows[1][u] = *reinterpret_cast<const mnv_f2*>(row_stats[turn][1] + mnv_acc_row(2 * pair, half));
+          }
         };
-        MnvParts cur = operand(0);
+        MnvParts cur = {{operand(0, 0), operand(0, 1), operand(0, 2)}};
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < 4 * KS; ++k) {
           const int s = k % KS;
-          MnvParts ahead = cur;
-          if (k + 1 < 4 * KS) ahead = operand(k + 1);
+          auto step = [&](mnv_f16& acc, const MnvParts& b) __attribute__((always_inline)) {
+            auto after = [&](int c) __attribute__((always_inline)) { return operand(k + 1, c); };
+            if (k + 1 < 4 * KS) mnv_step<false>(acc, cur, b, after);
+            else mnv_step<true>(acc, cur, b, after);
+          };
           mnv_f2 mine[2][MOST];
 #pragma unroll
           for (int c = 0; c < MOST; ++c) {
@@ -193,13 +198,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
           }
           read_rows(k + 1);
           if (k < KS) {
-            mnv_mul(t, cur, kp[s]);
+            step(t, kp[s]);
             next.stage.fetch_piece(s, qb + (size_t)i1 * pitch, ob + (size_t)i1 * pitch, pitch, z.q_len - i1, z.dim);
           } else if (k < 2 * KS) {
-            mnv_mul(dp, cur, vp[s]);
+            step(dp, vp[s]);
 #pragma unroll
-            for (int pair = s * 8 / KS; pair < (s + 1) * 8 / KS; ++pair) {
-              const mnv_f2 m = mine[0][pair - s * 8 / KS], il = mine[1][pair - s * 8 / KS];
+            for (int u = 0; u < MOST; ++u) {
+              const int pair = s * 8 / KS + u;
+              if (pair >= (s + 1) * 8 / KS) continue;
+              const mnv_f2 m = mine[0][u], il = mine[1][u];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int r = 2 * pair + e;
@@ -209,20 +216,21 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
               pc[pair / 4].pair(pair % 4, t[2 * pair], t[2 * pair + 1]);
             }
           } else if (k < 3 * KS) {
-            mnv_mul(dv[s % NB], cur, pc[s / NB].parts());
+            step(dv[s % NB], pc[s / NB].parts());
 #pragma unroll
-            for (int pair = s * 8 / KS; pair < (s + 1) * 8 / KS; ++pair) {
-              const mnv_f2 delta = mine[0][pair - s * 8 / KS];
+            for (int u = 0; u < MOST; ++u) {
+              const int pair = s * 8 / KS + u;
+              if (pair >= (s + 1) * 8 / KS) continue;
+              const mnv_f2 delta = mine[0][u];
 #pragma unroll
               for (int e = 0; e < 2; ++e) dp[2 * pair + e] = t[2 * pair + e] * (dp[2 * pair + e] - delta[e]);
               sc[pair / 4].pair(pair % 4, dp[2 * pair], dp[2 * pair + 1]);
             }
           } else {
-            mnv_mul(dk[s % NB], cur, sc[s / NB].parts());
+            step(dk[s % NB], sc[s / NB].parts());
             next.stage.template store_piece<true>(s, lds + (turn ^ 1) * Stage::BYTES, z.scale);
           }
           MNV_STEP_ORDER(6);
-          cur = ahead;
         }
         turn ^= 1;
         store_rows(next, i0 + 32, turn);
@@ -277,7 +285,7 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dkv_kerne
 }
 
 template <int DP, bool BIAS, bool VEC>
-__global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 256, VEC>;  // keys and values
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
@@ -361,27 +369,32 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
         for (int e = 0; e < 2; ++e) dp[2 * pair + e] = t[2 * pair + e] * (dp[2 * pair + e] - delta);
         sc[pair / 4].pair(pair % 4, dp[2 * pair], dp[2 * pair + 1]);
       };
-      auto operand = [&](int k) __attribute__((always_inline)) {
+      auto operand = [&](int k, int c) __attribute__((always_inline)) {
         const int s = k % KS;
-        return k < KS       ? Stage::by_rows(now, s)
-               : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s)
-                            : Stage::by_cols(now, s % NB * 32, s / NB);
+        return k < KS       ? Stage::by_rows(now, s, c)
+               : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s, c)
+                            : Stage::by_cols(now, s % NB * 32, s / NB, c);
       };
       char* then = lds + (now == lds ? Stage::BYTES : 0);
-      MnvParts cur = operand(0);
+      MnvParts cur = {{operand(0, 0), operand(0, 1), operand(0, 2)}};
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < 3 * KS; ++k) {
         const int s = k % KS;
-        MnvParts ahead = cur;
-        if (k + 1 < 3 * KS) ahead = operand(k + 1);
+        auto step = [&](mnv_f16& acc, const MnvParts& b) __attribute__((always_inline)) {
+          auto after = [&](int c) __attribute__((always_inline)) { return operand(k + 1, c); };
+          if (k + 1 < 3 * KS) mnv_step<false>(acc, cur, b, after);
+          else mnv_step<true>(acc, cur, b, after);
+        };
         if (k < KS) {
-          mnv_mul(t, cur, qp[s]);
+          step(t, qp[s]);
           stage.fetch_piece(s, kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
         } else if (k < 2 * KS) {
-          mnv_mul(dp, cur, op[s]);
+          step(dp, op[s]);
 #pragma unroll
-          for (int r = s * 16 / KS; r < (s + 1) * 16 / KS; ++r) {
+          for (int u = 0; u < (16 + KS - 1) / KS; ++u) {
+            const int r = s * 16 / KS + u;
+            if (r >= (s + 1) * 16 / KS) continue;
             if (BIAS) t[r] += add[r / 4][r % 4];
             t[r] = mnv_acc_row(r, 0) < left ? mnv_weight(t[r], m) * il : 0.f;
           }
@@ -390,15 +403,15 @@ __global__ __launch_bounds__(256, DP <= 32 ? 2 : 1) void mnv_attention_dq_kernel
 #pragma unroll
             for (int pair = 0; pair < 4; ++pair) cut_ds(pair);
           }
-          mnv_mul(dq[s % NB], cur, sc[s / NB].parts());
+          step(dq[s % NB], sc[s / NB].parts());
           if (s < NB) {
 #pragma unroll
-            for (int pair = 4 + s * 4 / NB; pair < 4 + (s + 1) * 4 / NB; ++pair) cut_ds(pair);
+            for (int u = 0; u < (4 + NB - 1) / NB; ++u)
+            if (4 + s * 4 / NB + u < 4 + (s + 1) * 4 / NB) cut_ds(4 + s * 4 / NB + u);
           }
           stage.template store_piece<false>(s, then, 1.f);
         }
         MNV_STEP_ORDER(6);
-        cur = ahead;
       }
       now = then;
       __syncthreads();

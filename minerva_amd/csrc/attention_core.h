@@ -137,24 +137,32 @@ __device__ __forceinline__ MnvParts mnv_cut8(const float* x) {
   return r;
 }
 
-// acc += a * b, the smallest terms first.
-__device__ __forceinline__ void mnv_mul(mnv_f16& acc, const MnvParts& a, const MnvParts& b) {
-  constexpr int PA[6] = {2, 1, 0, 1, 0, 0}, PB[6] = {0, 1, 2, 0, 1, 0};
-#pragma unroll
-  for (int t = 0; t < 6; ++t) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[PA[t]], b.p[PB[t]], acc, 0, 0, 0);
-}
-
 // The order of instructions.  A 32 x 32 x 16 instruction holds its matrix core for 32 cycles and the issue for 8,
 // so what else a wavefront has to do (exponentials, cutting) is free if it stands between them, six vector
 // instructions to one; left alone, the compiler puts all matrix instructions of a product in a row and reads
 // each operand right before its use.  So a tile's work is written as steps of one operand, six matrix instructions,
-// that read the operand of the next step first and take a share of the other work between them.
-// MNV_STEP_ORDER closes a step; others: vector instructions to a matrix instruction.
+// each of which reads the next step's parts as its own are done with and takes a share of the other work.
+//
+// acc += a * b; a becomes the next step's operand, part c of which is next(c).  The smallest terms come first as far as
+// the parts' turns allow: the third part is read five matrix instructions before its use, the second four, the first three.
+template <bool LAST, class Next>
+__device__ __forceinline__ void mnv_step(mnv_f16& acc, MnvParts& a, const MnvParts& b, Next&& next) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[2], b.p[0], acc, 0, 0, 0);
+  if (!LAST) a.p[2] = next(2);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[1], b.p[0], acc, 0, 0, 0);
+  if (!LAST) a.p[1] = next(1);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[2], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[1], acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], acc, 0, 0, 0);
+  if (!LAST) a.p[0] = next(0);
+}
+// Closes a step: others: vector instructions to a matrix instruction.
 #define MNV_STEP_ORDER(others)                                 \
   do {                                                         \
-    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);         \
     _Pragma("unroll") for (int g_ = 0; g_ < 6; ++g_) {         \
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);       \
+      if (g_ == 0 || g_ == 2 || g_ == 5) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); \
       __builtin_amdgcn_sched_group_barrier(0x002, others, 0);  \
     }                                                          \
     __builtin_amdgcn_sched_barrier(0);                         \
@@ -218,7 +226,7 @@ struct MnvStage {
     if (s >= SLOTS) return;
     const At a = at(s);
     if (!a.any) return;
-    const float* m = a.second ? m1 : m0;
+    const float* m = UNITS % NT == 0 ? (a.second ? m1 : m0) : m0 + (ptrdiff_t)a.second * (m1 - m0);
     const unsigned mine = (unsigned)a.row * pitch, last = (unsigned)(rows - 1) * pitch, row = mine < last ? mine : last;
     const int c = a.col + piece % 2 * 4;
     if (VEC) {
@@ -244,7 +252,9 @@ struct MnvStage {
     if (s >= SLOTS) return;
     const At a = at(s);
     if (!a.any) return;
-    const float f = !a.second ? scale : ODD_MINUS && a.row % 2 ? -1.f : 1.f;
+    // 96 columns: a unit's matrix is known at run time only; no branch
+    const float second = a.second, sign = ODD_MINUS && a.row % 2 ? -1.f : 1.f;
+    const float f = UNITS % NT == 0 ? (a.second ? sign : scale) : second * sign + (1.f - second) * scale;
 #pragma unroll
     for (int h = piece % 2 * 2; h < piece % 2 * 2 + 2; ++h) {
       unsigned t[3];
@@ -253,7 +263,7 @@ struct MnvStage {
       for (int p = 0; p < 3; ++p) w[p][h] = t[p];
     }
     if (piece % 2 == 0) return;
-    char* to = lds + (a.second ? MATRIX : 0) + a.row * PITCH + ((a.col / 8) ^ swap(a.row)) * 16;
+    char* to = lds + (int)a.second * MATRIX + a.row * PITCH + ((a.col / 8) ^ swap(a.row)) * 16;
 #pragma unroll
     for (int p = 0; p < 3; ++p) *reinterpret_cast<mnv_u4*>(to + p * PLANE) = w[p];
   }
@@ -270,35 +280,25 @@ struct MnvStage {
     return row / 4 % 4 + (DP == 128 ? row % 4 * 4 : DP == 64 ? row / 2 % 2 * 4 : 0);
   }
 
-  // Operand of the 32 rows, columns 16 s ... of step s, from the planes of one matrix.
-  __device__ static __forceinline__ MnvParts by_rows(const char* planes, int s) {
+  // Part c of the operand of the 32 rows, columns 16 s ... of step s, from the planes of one matrix.
+  __device__ static __forceinline__ mnv_bf8 by_rows(const char* planes, int s, int c) {
     const int lane = threadIdx.x % MNV_WAVE, row = lane % 32;
     // chunk 2 s + lane / 32
     const int at = row * PITCH + (swap(row) ^ (lane / 32)) * 16;
-    const char* p = planes + (at ^ (2 * s & SWAPPED) * 16) + (2 * s & ~SWAPPED) * 16;
-    MnvParts r;
-#pragma unroll
-    for (int c = 0; c < 3; ++c) r.p[c] = *reinterpret_cast<const mnv_bf8*>(p + c * PLANE);
-    return r;
+    return *reinterpret_cast<const mnv_bf8*>(planes + (at ^ (2 * s & SWAPPED) * 16) + (2 * s & ~SWAPPED) * 16 + c * PLANE);
   }
-  // Operand of the 32 columns from `col` on, rows 16 s ... of step s.
-  __device__ static __forceinline__ MnvParts by_cols(const char* planes, int col, int s) {
+  // Part c of the operand of the 32 columns from `col` on, rows 16 s ... of step s.
+  __device__ static __forceinline__ mnv_bf8 by_cols(const char* planes, int col, int s, int c) {
     typedef short s4 __attribute__((ext_vector_type(4)));
-    typedef short s8 __attribute__((ext_vector_type(8)));
     typedef __attribute__((address_space(3))) s4* lds_s4;
     const int lane = threadIdx.x % MNV_WAVE, row = lane / 32 * 4 + lane % 16 / 4;
     // chunk col / 8 + 2 (lane / 16 % 2) + lane % 4 / 2 of rows `row` and row + 8, whose numbers are swapped by 2 more
     const int at = row * PITCH + (swap(row) ^ (lane / 16 % 2 * 2 + lane % 4 / 2)) * 16 + lane % 2 * 8;
-    const char* p = planes + s * 16 * PITCH + (col / 8 & ~SWAPPED) * 16;
+    const char* p = planes + s * 16 * PITCH + (col / 8 & ~SWAPPED) * 16 + c * PLANE;
     const int low = at ^ (col / 8 & SWAPPED) * 16, high = (low ^ 32) + 8 * PITCH;
-    MnvParts r;
-#pragma unroll
-    for (int c = 0; c < 3; ++c) {
-      const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + low + c * PLANE));
-      const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + high + c * PLANE));
-      r.p[c] = __builtin_bit_cast(mnv_bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
-    }
-    return r;
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + low));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + high));
+    return __builtin_bit_cast(mnv_bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
 

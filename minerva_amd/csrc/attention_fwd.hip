@@ -29,7 +29,6 @@ struct FwdArgs {
 template <int DP, int NW, bool BIAS, bool VEC>
 __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  constexpr bool AHEAD = NW != 8;
   using Stage = MnvStage<DP, 64 * NW, VEC>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
@@ -94,24 +93,24 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
     auto scores = [&](auto fetches, const char* now, char* then, int j1) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) t[e] = 0.f;
-      MnvParts cur;
-      if (AHEAD) cur = Stage::by_rows(now, 0);
+      auto operand = [&](int s, int c) __attribute__((always_inline)) { return Stage::by_rows(now, s, c); };
+      MnvParts cur = {{operand(0, 0), operand(0, 1), operand(0, 2)}};
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        MnvParts ahead = cur;
-        if (!AHEAD) cur = Stage::by_rows(now, s);
-        else if (s + 1 < KS) ahead = Stage::by_rows(now, s + 1);
-        mnv_mul(t, cur, qp[s]);
+        auto next = [&](int c) __attribute__((always_inline)) { return operand(s + 1, c); };
+        if (s + 1 < KS) mnv_step<false>(t, cur, qp[s], next);
+        else mnv_step<true>(t, cur, qp[s], next);
         share(fetches, s, then, j1);
         MNV_STEP_ORDER(6);
-        if (AHEAD) cur = ahead;
       }
     };
     auto results = [&](auto fetches, const char* now, char* then, int j0, int j1) __attribute__((always_inline)) {
       const bool whole = j0 + 32 <= n;
-      MnvParts cur;
-      if (AHEAD) cur = Stage::by_cols(now + Stage::MATRIX, 0, 0);
+      auto operand = [&](int s, int c) __attribute__((always_inline)) {
+        return Stage::by_cols(now + Stage::MATRIX, s % NB * 32, s / NB, c);
+      };
+      MnvParts cur = {{operand(0, 0), operand(0, 1), operand(0, 2)}};
       if (BIAS) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -161,17 +160,16 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        MnvParts ahead = cur;
-        if (!AHEAD) cur = Stage::by_cols(now + Stage::MATRIX, s % NB * 32, s / NB);
-        else if (s + 1 < KS) ahead = Stage::by_cols(now + Stage::MATRIX, (s + 1) % NB * 32, (s + 1) / NB);
-        mnv_mul(acc[s % NB], cur, pc[s / NB].parts());
+        auto next = [&](int c) __attribute__((always_inline)) { return operand(s + 1, c); };
+        if (s + 1 < KS) mnv_step<false>(acc[s % NB], cur, pc[s / NB].parts(), next);
+        else mnv_step<true>(acc[s % NB], cur, pc[s / NB].parts(), next);
         if (s < NB) {
 #pragma unroll
-          for (int pair = 4 + s * 4 / NB; pair < 4 + (s + 1) * 4 / NB; ++pair) cut_p(pair);
+          for (int u = 0; u < (4 + NB - 1) / NB; ++u)
+            if (4 + s * 4 / NB + u < 4 + (s + 1) * 4 / NB) cut_p(4 + s * 4 / NB + u);
         }
         share(fetches, s, then, j1);
         MNV_STEP_ORDER(6);
-        if (AHEAD) cur = ahead;
       }
     };
     const std::true_type fetches;
