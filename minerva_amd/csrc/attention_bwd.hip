@@ -424,14 +424,17 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     mnv_store_column<DP>(dq, 1.f, true, a.sums + (split * z.q_rows() + row) * DP, DP);
 }
 
-// out[row] = f * the sums of a row's parts, 0 for none; 16 lanes to a row.  Of queries (per_row = heads, q_len to an entry) the
+// out[row] = f * the sums of a row's parts, 0 for none; 16 lanes to a row.  blockIdx.y: dk and dv.  Of queries (per_row = heads, q_len to an entry) the
 // parts that have keys count, `chunk` keys to each; of keys all, and those that are read.
-__global__ __launch_bounds__(256) void mnv_attention_sum_kernel(const float* __restrict__ sums, float* __restrict__ out,
+__global__ __launch_bounds__(256) void mnv_attention_sum_kernel(const float* __restrict__ sums, float* __restrict__ out0,
+                                                                float* __restrict__ out1,
                                                                 const float* __restrict__ lengths, AttentionSizes z,
                                                                 bool queries, int splits, int chunk, int pitch, float f) {
   const size_t rows = queries ? z.q_rows() : (size_t)z.batch * z.k_len * z.kv_heads;
   const size_t row = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
   if (row >= rows) return;
+  float* out = blockIdx.y ? out1 : out0;
+  sums += (size_t)blockIdx.y * splits * rows * pitch;
   const size_t per_entry = queries ? (size_t)z.q_len * z.heads : (size_t)z.k_len * z.kv_heads;
   const int n = mnv_visible(lengths, (int)(row / per_entry), z.k_len);
   int parts = splits;
@@ -439,10 +442,16 @@ __global__ __launch_bounds__(256) void mnv_attention_sum_kernel(const float* __r
   else if ((int)(row % per_entry / z.kv_heads) >= n) parts = 0;
   for (int d = threadIdx.x % 16 * 4; d < z.dim; d += 64) {
     mnv_f4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < parts; ++s) {
-      const mnv_f4 t = *reinterpret_cast<const mnv_f4*>(sums + (s * rows + row) * pitch + d);
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+      mnv_f4 t[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += t[e];
+      for (int u = 0; u < 4; ++u)
+        t[u] = s0 + u < parts ? *reinterpret_cast<const mnv_f4*>(sums + ((s0 + u) * rows + row) * pitch + d)
+                              : mnv_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += t[u][e];
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -450,31 +459,41 @@ __global__ __launch_bounds__(256) void mnv_attention_sum_kernel(const float* __r
   }
 }
 
-// dbias[o] += the parts of o: of every entry among the launch's pairs and every 32 keys that have the diagonal.
-__global__ __launch_bounds__(256) void mnv_attention_dbias_kernel(const float* __restrict__ parts,
-                                                                  const float* __restrict__ lengths,
-                                                                  float* __restrict__ dbias, AttentionSizes z,
-                                                                  unsigned first_pair, unsigned pairs, bool first) {
+// dbias[o] += the parts of o: of every entry among the launch's pairs and every 32 keys that have the diagonal.  64 offsets to a
+// workgroup, 16 threads to an offset, each with every 16th 32 keys.
+__global__ __launch_bounds__(1024) void mnv_attention_dbias_kernel(const float* __restrict__ parts,
+                                                                   const float* __restrict__ lengths,
+                                                                   float* __restrict__ dbias, AttentionSizes z,
+                                                                   unsigned first_pair, unsigned pairs, bool first) {
+  __shared__ float lds[16][64];
   const size_t offsets = z.offsets();
-  const size_t o = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (o >= offsets) return;
+  const int lane = threadIdx.x % 64, slice = threadIdx.x / 64;
+  const size_t o = (size_t)blockIdx.x * 64 + lane;
   const size_t pitch = diagonal_pitch(z.q_len), per_key = key_tiles(z.k_len);
   const int group = z.group(), padded = (int)pitch - 32;
   for (int h = blockIdx.y; h < z.heads; h += gridDim.y) {
-    float s = first ? 0.f : dbias[h * offsets + o];
-    const int kh = h / group;
-    for (unsigned p = 0; p < pairs; ++p) {
-      const unsigned pair = first_pair + p;
-      if (pair % z.kv_heads != (unsigned)kh) continue;
-      const int n = mnv_visible(lengths, pair / z.kv_heads, z.k_len);
-      // key kt + c and query 32 s + r of the part: place o - kt + padded - q_len
-      const long long place = (long long)o + padded - z.q_len;
-      long long from = place - (padded + 30);
-      from = from <= 0 ? 0 : (from + 31) / 32 * 32;
-      const float* mine = parts + ((size_t)p * group + h % group) * per_key * pitch;
-      for (long long kt = from; kt < n && kt <= place; kt += 32) s += mine[kt / 32 * pitch + (place - kt)];
+    float s = 0.f;
+    // the pairs of the head's key head: one to an entry
+    const unsigned kh = h / group, from_pair = (kh + z.kv_heads - first_pair % z.kv_heads) % z.kv_heads;
+    // key kt + c and query 32 s + r of the part: place o - kt + padded - q_len
+    const long long place = (long long)o + padded - z.q_len;
+    long long from = place - (padded + 30);
+    from = (from <= 0 ? 0 : (from + 31) / 32 * 32) + 32 * slice;
+    if (o < offsets)
+      for (unsigned p = from_pair; p < pairs; p += z.kv_heads) {
+        const int n = mnv_visible(lengths, (first_pair + p) / z.kv_heads, z.k_len);
+        const float* mine = parts + ((size_t)p * group + h % group) * per_key * pitch;
+        for (long long kt = from; kt < n && kt <= place; kt += 32 * 16) s += mine[kt / 32 * pitch + (place - kt)];
+      }
+    __syncthreads();
+    lds[slice][lane] = s;
+    __syncthreads();
+    if (slice == 0 && o < offsets) {
+      s = first ? 0.f : dbias[h * offsets + o];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) s += lds[u][lane];
+      dbias[h * offsets + o] = s;
     }
-    dbias[h * offsets + o] = s;
   }
 }
 
@@ -619,17 +638,14 @@ int mnv_attention_bwd(const float* q, const float* k, const float* v, const floa
                           now * ka.tiles * ka.splits, s);
     if (rc) return rc;
     if (!ka.parts) continue;
-    const dim3 grid((unsigned)mnv_ceil_div(z.offsets(), 256), heads < 65535 ? heads : 65535);
-    hipLaunchKernelGGL(mnv_attention_dbias_kernel, grid, dim3(256), 0, s, ka.parts, lengths, dbias, z, (unsigned)p, now,
+    const dim3 grid((unsigned)mnv_ceil_div(z.offsets(), 64), heads < 65535 ? heads : 65535);
+    hipLaunchKernelGGL(mnv_attention_dbias_kernel, grid, dim3(1024), 0, s, ka.parts, lengths, dbias, z, (unsigned)p, now,
                        p == 0);
     MNV_HIP_TRY(hipGetLastError());
   }
   if (ka.splits > 1) {
-    const dim3 grid((unsigned)mnv_ceil_div(k_rows, 16));
-    hipLaunchKernelGGL(mnv_attention_sum_kernel, grid, dim3(256), 0, s, ka.sums, dk, lengths, z, false, ka.splits, 0, dp, 1.f);
-    MNV_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(mnv_attention_sum_kernel, grid, dim3(256), 0, s, ka.sums + ka.splits * k_rows * dp, dv, lengths, z,
-                       false, ka.splits, 0, dp, 1.f);
+    hipLaunchKernelGGL(mnv_attention_sum_kernel, dim3((unsigned)mnv_ceil_div(k_rows, 16), 2), dim3(256), 0, s, ka.sums, dk, dv,
+                       lengths, z, false, ka.splits, 0, dp, 1.f);
     MNV_HIP_TRY(hipGetLastError());
   }
   if (bias && !ka.parts) {
@@ -647,8 +663,8 @@ int mnv_attention_bwd(const float* q, const float* k, const float* v, const floa
   const int rc = by_dim(head_dim, launch_dq<32>, launch_dq<64>, launch_dq<96>, launch_dq<128>, a,
                         (unsigned)(a.tiles * a.splits * pairs), s);
   if (rc || a.splits == 1) return rc;
-  hipLaunchKernelGGL(mnv_attention_sum_kernel, dim3((unsigned)mnv_ceil_div(q_rows, 16)), dim3(256), 0, s, a.sums, dq, lengths,
-                     z, true, a.splits, a.chunk * 32, dp, scale);
+  hipLaunchKernelGGL(mnv_attention_sum_kernel, dim3((unsigned)mnv_ceil_div(q_rows, 16)), dim3(256), 0, s, a.sums, dq,
+                     nullptr, lengths, z, true, a.splits, a.chunk * 32, dp, scale);
   return MNV_LAUNCH_STATUS();
 }
 
