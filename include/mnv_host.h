@@ -100,6 +100,11 @@ int mnvh_runtime_profile_read(void* runtime, char* text_out, size_t capacity);
  *   "matmult_bias" [relu]                         inputs: a, b, bias {m,1}
  *   "matmult_relu_backward"                       inputs: a, b, bottom
  *   "sgd_update" [scale]                          inputs: w, g
+ * and of the operators of networks over sequences (minerva_amd/host/hip_sequence_ops.h) those with one result:
+ *   "layer_norm_forward" [eps]                    inputs: x, gamma, beta
+ *   "relative_bias_forward" [q_len, k_len, q_start, max_distance, both_ways]      inputs: table
+ *   "relative_bias_backward" [buckets, q_len, k_len, q_start, max_distance, both_ways]
+ *                                                 inputs: the bias's gradient
  * Enum values follow minerva/op/closure.h:8-24 and narray/convolution_info.h:19-57
  * (arithmetic 0 add 1 sub 2 mult 3 div; elewise 0 exp 1 ln 2 negative; reduction 0 sum
  * 1 max; softmax 0 instance 1 channel; activation 0 sigmoid 1 relu 2 tanh; pooling 0 max
@@ -117,6 +122,16 @@ int mnvh_op(void* runtime, const char* op, const mnvh_tensor* inputs, int n_inpu
 int mnvh_tensor_create(void* runtime, const mnvh_tensor* host, void** tensor);
 int mnvh_tensor_op(void* runtime, const char* op, void* const* inputs, int n_inputs,
                    const double* params, int n_params, void** out);
+/* The same for an operator of any number of results: those of mnvh_tensor_op, one of each, and
+ *   "layer_norm_backward" [eps]       inputs: diff, x, gamma; results: dx, dgamma, dbeta
+ *   "attention_forward" [scale, has_bias, has_lengths]
+ *                                     inputs: q, k, v [, bias] [, lengths]; results: out, stats
+ *   "attention_backward" [scale, has_bias, has_lengths]
+ *                                     inputs: diff, q, k, v, out, stats [, bias] [, lengths];
+ *                                     results: dq, dk, dv [, dbias]
+ * (extents as in mnv_hip.h).  `outs` has room for `capacity` handles; *n_outs are written. */
+int mnvh_tensor_op_list(void* runtime, const char* op, void* const* inputs, int n_inputs,
+                        const double* params, int n_params, void** outs, int capacity, int* n_outs);
 int mnvh_tensor_info(void* tensor, int* ndims, int* dims /* MNVH_MAX_DIMS */, int* stream);
 int mnvh_tensor_read(void* runtime, void* tensor, float* out, size_t out_capacity);
 int mnvh_tensor_free(void* tensor);

@@ -227,6 +227,18 @@ Tensor RunNamedOp(Runner* rt, const std::string& op, const std::vector<Tensor>& 
     MNV_CHECK(n_params >= 3) << "lrn_backward takes local_size, alpha, beta";
     r = rt->LRNBackward(in[0], in[1], in[2], in[3], static_cast<int>(params[0]),
                         static_cast<float>(params[1]), static_cast<float>(params[2]));
+  } else if (op == "layer_norm_forward") {  // params: eps; inputs: x, gamma, beta
+    need(3);
+    MNV_CHECK(n_params >= 1) << "layer_norm_forward takes eps";
+    r = rt->LayerNormForward(in[0], in[1], in[2], static_cast<float>(params[0]));
+  } else if (op == "relative_bias_forward") {  // params: q_len, k_len, q_start, max_distance, both_ways
+    need(1);
+    r = rt->RelativeBiasForward(in[0], P(params, n_params, 0), P(params, n_params, 1), P(params, n_params, 2),
+                                P(params, n_params, 3), P(params, n_params, 4) != 0);
+  } else if (op == "relative_bias_backward") {  // params: buckets, q_len, k_len, q_start, max_distance, both_ways
+    need(1);
+    r = rt->RelativeBiasBackward(in[0], P(params, n_params, 0), P(params, n_params, 1), P(params, n_params, 2),
+                                 P(params, n_params, 3), P(params, n_params, 4), P(params, n_params, 5) != 0);
   } else if (op == "randn" || op == "rand_bernoulli") {  // params: mu, var | p ; then d0, d1, ...
     need(0);
     const int lead = op == "randn" ? 2 : 1;
@@ -245,6 +257,35 @@ Tensor RunNamedOp(Runner* rt, const std::string& op, const std::vector<Tensor>& 
     MNV_FATAL() << "unknown operator '" << op << "'";
   }
   return r;
+}
+
+// The same for operators with any number of results.
+std::vector<Tensor> RunNamedOps(Runner* rt, const std::string& op, const std::vector<Tensor>& in, const double* params,
+                                int n_params) {
+  const int n_inputs = static_cast<int>(in.size());
+  // attention's bias and lengths follow the other inputs, as far as params 1 and 2 say they are there
+  auto optional = [&](int fixed, Tensor* bias, Tensor* lengths) {
+    MNV_CHECK(n_params >= 3) << op << " takes scale, has_bias, has_lengths";
+    const bool has_bias = P(params, n_params, 1) != 0, has_lengths = P(params, n_params, 2) != 0;
+    MNV_CHECK_EQ(n_inputs, fixed + has_bias + has_lengths) << op << " takes " << fixed << " inputs and those it says";
+    if (has_bias) *bias = in[fixed];
+    if (has_lengths) *lengths = in[fixed + has_bias];
+  };
+  Tensor bias, lengths;
+  if (op == "layer_norm_backward") {  // params: eps; inputs: diff, x, gamma
+    MNV_CHECK_EQ(n_inputs, 3) << op << " takes 3 inputs";
+    MNV_CHECK(n_params >= 1) << "layer_norm_backward takes eps";
+    return rt->LayerNormBackward(in[0], in[1], in[2], static_cast<float>(params[0]));
+  }
+  if (op == "attention_forward") {  // inputs: q, k, v [, bias] [, lengths]
+    optional(3, &bias, &lengths);
+    return rt->AttentionForward(in[0], in[1], in[2], bias, lengths, static_cast<float>(params[0]));
+  }
+  if (op == "attention_backward") {  // inputs: diff, q, k, v, out, stats [, bias] [, lengths]
+    optional(6, &bias, &lengths);
+    return rt->AttentionBackward(in[0], in[1], in[2], in[3], in[4], in[5], bias, lengths, static_cast<float>(params[0]));
+  }
+  return {RunNamedOp(rt, op, in, params, n_params)};
 }
 
 }  // namespace
@@ -369,6 +410,23 @@ int mnvh_tensor_op(void* runtime, const char* op_name, void* const* inputs, int 
       in.push_back(*static_cast<Tensor*>(inputs[i]));
     }
     *out = new Tensor(RunNamedOp(rt, op_name, in, params, n_params));
+  });
+}
+
+int mnvh_tensor_op_list(void* runtime, const char* op_name, void* const* inputs, int n_inputs,
+                        const double* params, int n_params, void** outs, int capacity, int* n_outs) {
+  return Guard([&] {
+    Runner* rt = static_cast<Runner*>(runtime);
+    MNV_CHECK(rt && op_name && outs && n_outs) << "null argument";
+    std::vector<Tensor> in;
+    for (int i = 0; i < n_inputs; ++i) {
+      MNV_CHECK(inputs && inputs[i]) << "null input tensor";
+      in.push_back(*static_cast<Tensor*>(inputs[i]));
+    }
+    const std::vector<Tensor> r = RunNamedOps(rt, op_name, in, params, n_params);
+    MNV_CHECK(static_cast<int>(r.size()) <= capacity) << op_name << " has " << r.size() << " results, room for " << capacity;
+    for (size_t i = 0; i < r.size(); ++i) outs[i] = new Tensor(r[i]);
+    *n_outs = static_cast<int>(r.size());
   });
 }
 

@@ -9,6 +9,7 @@
 #include "device.h"
 #include "hip_fused_ops.h"
 #include "hip_ops.h"
+#include "hip_sequence_ops.h"
 #include "minerva_types.h"
 
 namespace minerva {
@@ -78,6 +79,13 @@ MNV_INSTALL_COMPUTE_FN(MatMultTransBClosure, hip::MatMultTransB)
 MNV_INSTALL_COMPUTE_FN(SgdUpdateClosure, hip::SgdUpdate)
 MNV_INSTALL_COMPUTE_FN(MatMultTransBSgdClosure, hip::MatMultTransBSgd)
 MNV_INSTALL_COMPUTE_FN(ConvBackwardFilterSgdClosure, hip::ConvBackwardFilterSgd)
+// operators of networks over sequences (hip_sequence_ops.h): no counterpart either
+MNV_INSTALL_COMPUTE_FN(LayerNormForwardClosure, hip::LayerNormForward)
+MNV_INSTALL_COMPUTE_FN(LayerNormBackwardClosure, hip::LayerNormBackward)
+MNV_INSTALL_COMPUTE_FN(AttentionForwardClosure, hip::AttentionForward)
+MNV_INSTALL_COMPUTE_FN(AttentionBackwardClosure, hip::AttentionBackward)
+MNV_INSTALL_COMPUTE_FN(RelativeBiasForwardClosure, hip::RelativeBiasForward)
+MNV_INSTALL_COMPUTE_FN(RelativeBiasBackwardClosure, hip::RelativeBiasBackward)
 MNV_INSTALL_DATAGEN_FN(ArrayLoaderClosure, hip::ArrayLoader)
 MNV_INSTALL_DATAGEN_FN(FillClosure, hip::Fill)
 MNV_INSTALL_DATAGEN_FN(RandnClosure, hip::Randn)
@@ -147,6 +155,12 @@ MNV_SIMPLE_OP(MatMultTransAOp, ComputeFnWithClosure, MatMultTransAClosure, "tran
 MNV_SIMPLE_OP(MatMultTransBOp, ComputeFnWithClosure, MatMultTransBClosure, "* trans")
 MNV_SIMPLE_OP(SgdUpdateOp, ComputeFnWithClosure, SgdUpdateClosure, "sgd update")
 MNV_SIMPLE_OP(MatMultTransBSgdOp, ComputeFnWithClosure, MatMultTransBSgdClosure, "* trans + sgd update")
+MNV_SIMPLE_OP(LayerNormForwardOp, ComputeFnWithClosure, LayerNormForwardClosure, "layer norm ff")
+MNV_SIMPLE_OP(LayerNormBackwardOp, ComputeFnWithClosure, LayerNormBackwardClosure, "layer norm bp")
+MNV_SIMPLE_OP(AttentionForwardOp, ComputeFnWithClosure, AttentionForwardClosure, "attention ff")
+MNV_SIMPLE_OP(AttentionBackwardOp, ComputeFnWithClosure, AttentionBackwardClosure, "attention bp")
+MNV_SIMPLE_OP(RelativeBiasForwardOp, ComputeFnWithClosure, RelativeBiasForwardClosure, "relative bias ff")
+MNV_SIMPLE_OP(RelativeBiasBackwardOp, ComputeFnWithClosure, RelativeBiasBackwardClosure, "relative bias bp")
 
 class MatMultBiasOp : public ComputeFnWithClosure<MatMultBiasClosure> {
  public:

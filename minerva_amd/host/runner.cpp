@@ -61,27 +61,38 @@ Runner::~Runner() {
 
 Tensor Runner::Compute(const std::vector<Tensor>& inputs, const Scale& out_size,
                        std::shared_ptr<ComputeFn> fn) {
+  return Compute(inputs, std::vector<Scale>{out_size}, std::move(fn))[0];
+}
+
+std::vector<Tensor> Runner::Compute(const std::vector<Tensor>& inputs, const std::vector<Scale>& out_sizes,
+                                    std::shared_ptr<ComputeFn> fn) {
   Task task;
   for (auto& t : inputs) {
     MNV_CHECK(t) << "null tensor";
     task.inputs.emplace_back(PhysicalData(t->size, device_->device_id(), t->id), t->id);
   }
-  Tensor out = std::make_shared<TensorNode>(this, next_id_++, out_size);
-  task.outputs.emplace_back(PhysicalData(out_size, device_->device_id(), out->id), out->id);
+  std::vector<Tensor> outs;
+  for (auto& size : out_sizes) {
+    outs.push_back(std::make_shared<TensorNode>(this, next_id_++, size));
+    task.outputs.emplace_back(PhysicalData(size, device_->device_id(), outs.back()->id), outs.back()->id);
+  }
   task.op.compute_fn = std::move(fn);
   task.op.device_id = device_->device_id();
   task.id = ops_issued_++;
   task.light = true;  // issued in program order from the caller's thread
   if (dataflow_) {
-    task.stream = out->stream = PickStream(inputs, out_size);
-    last_stream_ = task.stream;
-    out->seq = ++issued_[task.stream];
-    out->epoch = epoch_;
+    task.stream = last_stream_ = PickStream(inputs, out_sizes[0]);
+    const uint64_t seq = ++issued_[task.stream];
+    for (auto& out : outs) {
+      out->stream = task.stream;
+      out->seq = seq;
+      out->epoch = epoch_;
+    }
     ++queued_[task.stream];
   }
   device_->PushTask(&task);
-  if (retain_) retained_.push_back(out);
-  return out;
+  if (retain_) retained_.insert(retained_.end(), outs.begin(), outs.end());
+  return outs;
 }
 
 void Runner::Upload(const Tensor& t, const float* host) {
@@ -403,6 +414,76 @@ Tensor Runner::LRNBackward(const Tensor& bottom, const Tensor& top, const Tensor
   auto op = std::make_shared<LRNBackwardOp>();
   op->closure = {local_size, alpha, beta, bottom->size};
   return Compute({bottom, top, scale, top_diff}, bottom->size, op);
+}
+
+// ---------------------------------------------------------------- networks over sequences
+
+namespace {
+Scale Queries(const Tensor& q, int first) { return Scale{first, q->size[1], q->size[2], q->size[3]}; }
+void CheckAttention(const Tensor& q, const Tensor& k, const Tensor& v) {
+  MNV_CHECK(q && k && v) << "null tensor";
+  MNV_CHECK_EQ(q->size.NumDims(), 4u) << "queries are {head_dim, heads, q_len, batch}";
+  MNV_CHECK_EQ(k->size.NumDims(), 4u) << "keys are {head_dim, kv_heads, k_len, batch}";
+  MNV_CHECK(v->size == k->size) << "keys' and values' extents differ";
+}
+std::vector<Tensor> WithOptional(std::vector<Tensor> inputs, const Tensor& bias, const Tensor& lengths) {
+  if (bias) inputs.push_back(bias);
+  if (lengths) inputs.push_back(lengths);
+  return inputs;
+}
+}  // namespace
+
+Tensor Runner::LayerNormForward(const Tensor& x, const Tensor& gamma, const Tensor& beta, float eps) {
+  MNV_CHECK(x) << "null tensor";
+  auto op = std::make_shared<LayerNormForwardOp>();
+  op->closure = {eps};
+  return Compute({x, gamma, beta}, x->size, op);
+}
+
+std::vector<Tensor> Runner::LayerNormBackward(const Tensor& diff, const Tensor& x, const Tensor& gamma, float eps) {
+  MNV_CHECK(x && gamma) << "null tensor";
+  auto op = std::make_shared<LayerNormBackwardOp>();
+  op->closure = {eps};
+  return Compute({diff, x, gamma}, std::vector<Scale>{x->size, gamma->size, gamma->size}, op);
+}
+
+std::vector<Tensor> Runner::AttentionForward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias,
+                                             const Tensor& lengths, float scale) {
+  CheckAttention(q, k, v);
+  auto op = std::make_shared<AttentionForwardOp>();
+  op->closure = {scale, bias != nullptr, lengths != nullptr};
+  return Compute(WithOptional({q, k, v}, bias, lengths), std::vector<Scale>{q->size, Queries(q, 2)}, op);
+}
+
+std::vector<Tensor> Runner::AttentionBackward(const Tensor& diff, const Tensor& q, const Tensor& k, const Tensor& v,
+                                              const Tensor& out, const Tensor& stats, const Tensor& bias,
+                                              const Tensor& lengths, float scale) {
+  CheckAttention(q, k, v);
+  auto op = std::make_shared<AttentionBackwardOp>();
+  op->closure = {scale, bias != nullptr, lengths != nullptr};
+  std::vector<Scale> sizes{q->size, k->size, v->size};
+  if (bias) sizes.push_back(bias->size);
+  return Compute(WithOptional({diff, q, k, v, out, stats}, bias, lengths), sizes, op);
+}
+
+Tensor Runner::RelativeBiasForward(const Tensor& table, int q_len, int k_len, int q_start, int max_distance,
+                                   bool both_ways) {
+  MNV_CHECK(table) << "null tensor";
+  MNV_CHECK_EQ(table->size.NumDims(), 2u) << "the table is {heads, buckets}";
+  MNV_CHECK(q_len > 0 && k_len > 0 && q_len <= 0x7fffffff - k_len) << "bad lengths";
+  auto op = std::make_shared<RelativeBiasForwardOp>();
+  op->closure = {table->size[1], q_len, k_len, q_start, max_distance, both_ways};
+  return Compute({table}, Scale{q_len + k_len - 1, table->size[0]}, op);
+}
+
+Tensor Runner::RelativeBiasBackward(const Tensor& diff, int buckets, int q_len, int k_len, int q_start, int max_distance,
+                                    bool both_ways) {
+  MNV_CHECK(diff) << "null tensor";
+  MNV_CHECK_EQ(diff->size.NumDims(), 2u) << "the gradient is {q_len + k_len - 1, heads}";
+  MNV_CHECK(buckets > 0) << "bad number of buckets";
+  auto op = std::make_shared<RelativeBiasBackwardOp>();
+  op->closure = {buckets, q_len, k_len, q_start, max_distance, both_ways};
+  return Compute({diff}, Scale{diff->size[1], buckets}, op);
 }
 
 // ---------------------------------------------------------------- fused operators

@@ -53,6 +53,9 @@ class Runner : public DeviceListener {
 
   Tensor Compute(const std::vector<Tensor>& inputs, const Scale& out_size,
                  std::shared_ptr<ComputeFn> fn);
+  // The same with several results.
+  std::vector<Tensor> Compute(const std::vector<Tensor>& inputs, const std::vector<Scale>& out_sizes,
+                              std::shared_ptr<ComputeFn> fn);
   std::vector<float> Get(const Tensor& t);
   void Read(const Tensor& t, float* host);  // the same into the caller's buffer
   // Overwrites a tensor's device data in place (synchronous); its address is kept, which
@@ -126,6 +129,24 @@ class Runner : public DeviceListener {
                     float beta);
   Tensor LRNBackward(const Tensor& bottom, const Tensor& top, const Tensor& scale,
                      const Tensor& top_diff, int local_size, float alpha, float beta);
+
+  // Operators of networks over sequences (hip_sequence_ops.h).
+  // x {..., count}, gamma and beta with one value per value of a column
+  Tensor LayerNormForward(const Tensor& x, const Tensor& gamma, const Tensor& beta, float eps);
+  // {dx, dgamma, dbeta}
+  std::vector<Tensor> LayerNormBackward(const Tensor& diff, const Tensor& x, const Tensor& gamma, float eps);
+  // q {head_dim, heads, q_len, batch}, k and v {head_dim, kv_heads, k_len, batch}, bias {q_len + k_len - 1, heads} or
+  // none, lengths {batch} or none; {out, stats {2, heads, q_len, batch}}
+  std::vector<Tensor> AttentionForward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bias,
+                                       const Tensor& lengths, float scale);
+  // {dq, dk, dv} and with a bias its gradient
+  std::vector<Tensor> AttentionBackward(const Tensor& diff, const Tensor& q, const Tensor& k, const Tensor& v,
+                                        const Tensor& out, const Tensor& stats, const Tensor& bias,
+                                        const Tensor& lengths, float scale);
+  // table {heads, buckets} -> {q_len + k_len - 1, heads}, and the gradient back
+  Tensor RelativeBiasForward(const Tensor& table, int q_len, int k_len, int q_start, int max_distance, bool both_ways);
+  Tensor RelativeBiasBackward(const Tensor& diff, int buckets, int q_len, int k_len, int q_start, int max_distance,
+                              bool both_ways);
 
   // The opt-in fused operators (hip_fused_ops.h).  Each returns the bits of the pair of calls
   // named in its comment.

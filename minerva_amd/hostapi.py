@@ -104,6 +104,15 @@ class Runtime:
                                     ctypes.byref(h)), name)
         return DeviceTensor(self, h)
 
+    def top_list(self, name, inputs, params=(), most=8):
+        """The same for an operator with several results: a list of DeviceTensors."""
+        arr = (ctypes.c_void_p * max(len(inputs), 1))(*[t.h for t in inputs])
+        p = (ctypes.c_double * max(len(params), 1))(*[float(x) for x in params])
+        outs, n = (ctypes.c_void_p * most)(), ctypes.c_int()
+        _check(lib().mnvh_tensor_op_list(self.h, name.encode(), arr, len(inputs), p, len(params), outs, most,
+                                         ctypes.byref(n)), name)
+        return [DeviceTensor(self, ctypes.c_void_p(outs[i])) for i in range(n.value)]
+
     def close(self):
         if self.h:
             _check(lib().mnvh_runtime_destroy(self.h), "runtime_destroy")

@@ -121,6 +121,10 @@ class NArray(object):
         ins = [self._t] + [o._t for o in others]
         return NArray(self._rt, self._rt.top(name, ins, params))
 
+    def _ops(self, name, others=(), params=()):
+        ins = [self._t] + [o._t for o in others]
+        return [NArray(self._rt, t) for t in self._rt.top_list(name, ins, params)]
+
     def _binary(self, rhs, kind):
         """NArray (op) NArray: same shape -> element-wise; otherwise rhs is replicated along
         its dimensions of size 1 (reference narray_elewise.cpp:17-27, narray.cpp:195-214)."""
@@ -267,6 +271,39 @@ class NArray(object):
     def lrn_backward(bottom_data, top_data, scale, top_diff, local_size, alpha, beta):
         return bottom_data._op("lrn_backward", [top_data, scale, top_diff],
                                [int(local_size), float(alpha), float(beta)])
+
+    # ---- networks over sequences (not in the reference)
+    @staticmethod
+    def layer_norm_forward(x, gamma, beta, eps):
+        return x._op("layer_norm_forward", [gamma, beta], [float(eps)])
+
+    @staticmethod
+    def layer_norm_backward(diff, x, gamma, eps):
+        """[gradient of x, of gamma, of beta]"""
+        return diff._ops("layer_norm_backward", [x, gamma], [float(eps)])
+
+    @staticmethod
+    def attention_forward(q, k, v, scale, bias=None, lengths=None):
+        """[result, stats for the backward pass]"""
+        more = [a for a in (bias, lengths) if a is not None]
+        return q._ops("attention_forward", [k, v] + more, [float(scale), bias is not None, lengths is not None])
+
+    @staticmethod
+    def attention_backward(diff, q, k, v, out, stats, scale, bias=None, lengths=None):
+        """[gradient of q, of k, of v] and with a bias that of the bias"""
+        more = [a for a in (bias, lengths) if a is not None]
+        return diff._ops("attention_backward", [q, k, v, out, stats] + more,
+                         [float(scale), bias is not None, lengths is not None])
+
+    @staticmethod
+    def relative_bias_forward(table, q_len, k_len, q_start, max_distance, both_ways):
+        return table._op("relative_bias_forward", params=[int(q_len), int(k_len), int(q_start), int(max_distance),
+                                                          bool(both_ways)])
+
+    @staticmethod
+    def relative_bias_backward(diff, buckets, q_len, k_len, q_start, max_distance, both_ways):
+        return diff._op("relative_bias_backward", params=[int(buckets), int(q_len), int(k_len), int(q_start),
+                                                          int(max_distance), bool(both_ways)])
 
     # ---- reductions and shape (libowl.pyx:345-387)
     def _reduce(self, dims, kind):

@@ -11,11 +11,12 @@ import numpy as np
 
 from .. import conv as co
 from .. import elewise as ele
+from .. import sequence as seq
 from .. import from_numpy, randb, zeros, concat as _concat, slice as _slice
 
 __all__ = ["ComputeUnit", "ComputeUnitSimple", "WeightedComputeUnit", "LinearUnit", "SigmoidUnit",
            "ReluUnit", "TanhUnit", "PoolingUnit", "DropoutUnit", "SoftmaxUnit", "AccuracyUnit",
-           "LRNUnit", "ConcatUnit", "FullyConnection", "ConvConnection", "MemoryDataUnit", "Net"]
+           "LRNUnit", "LayerNormUnit", "ConcatUnit", "FullyConnection", "ConvConnection", "MemoryDataUnit", "Net"]
 
 
 class ComputeUnit(object):
@@ -321,6 +322,38 @@ class LRNUnit(ComputeUnitSimple):
 
     def __str__(self):
         return "lrn"
+
+
+class LayerNormUnit(WeightedComputeUnit):
+    """Layer norm over all values of an image (or column), with a gain (`weight`, 1 unless filled) and an
+    offset (`bias`) per value; layer_norm_param { eps, weight_filler, bias_filler }.  Not in the reference."""
+
+    def __init__(self, params):
+        super(LayerNormUnit, self).__init__(params)
+        p = params.layer_norm_param
+        self.norm = seq.LayerNorm(p.get("eps", 1e-5))
+        self.weight_filler = p.get("weight_filler", {"type": "constant", "value": 1.0})
+        self.bias_filler = p.get("bias_filler", {"type": "constant"})
+
+    def compute_size(self, from_btm, to_top):
+        self.in_shape = list(from_btm[self.btm_names[0]])
+        self.out_shape = list(self.in_shape)
+        to_top[self.top_names[0]] = list(self.out_shape)
+        self.wshape = self.bshape = [int(np.prod(self.in_shape[:-1])), 1]
+        self.fan_in = self.fan_out = self.wshape[0]
+
+    def ff(self, x, phase):
+        self.ff_x = x
+        if self.weight is None:
+            self.init_weights_with_filler()
+        return self.norm.ff(x, self.weight, self.bias)
+
+    def bp(self, y, phase):
+        dx, self.weightgrad, self.biasgrad = self.norm.bp(y, self.ff_x, self.weight)
+        return dx if self.propagate_down else None
+
+    def __str__(self):
+        return "layer norm"
 
 
 class ConcatUnit(ComputeUnit):

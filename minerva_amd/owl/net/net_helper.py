@@ -110,7 +110,7 @@ _UNIT_TYPES = {
     "MemoryData": _net.MemoryDataUnit, "InnerProduct": _net.FullyConnection,
     "Convolution": _net.ConvConnection, "Pooling": _net.PoolingUnit, "ReLU": _net.ReluUnit,
     "Sigmoid": _net.SigmoidUnit, "SoftmaxWithLoss": _net.SoftmaxUnit, "TanH": _net.TanhUnit,
-    "Dropout": _net.DropoutUnit, "LRN": _net.LRNUnit, "Concat": _net.ConcatUnit,
+    "Dropout": _net.DropoutUnit, "LRN": _net.LRNUnit, "LayerNorm": _net.LayerNormUnit, "Concat": _net.ConcatUnit,
     "Accuracy": _net.AccuracyUnit,
 }
 
