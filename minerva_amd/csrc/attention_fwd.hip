@@ -245,7 +245,8 @@ __global__ __launch_bounds__(256) void mnv_attention_join_kernel(const float* __
   for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o, MNV_WAVE);
   const float f = mnv_inverse(l);
   const unsigned long long shown = __ballot(ls != 0.f);
-  for (int d = lane % 16 * 4; d < pitch; d += 64) {
+  for (int d0 = 0; d0 < pitch; d0 += 64) {  // all lanes stay: they hand each other the parts' numbers
+    const int d = d0 + lane % 16 * 4;
     mnv_f4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < parts; s0 += 16) {
       mnv_f4 t[4];
@@ -253,7 +254,7 @@ __global__ __launch_bounds__(256) void mnv_attention_join_kernel(const float* __
       for (int u = 0; u < 4; ++u) {
         const int s = s0 + 4 * u + lane / 16;
         t[u] = mnv_f4{0.f, 0.f, 0.f, 0.f};
-        if (s < parts && (shown >> s & 1)) t[u] = *reinterpret_cast<const mnv_f4*>(part_out + (s * rows + row) * pitch + d);
+        if (d < pitch && s < parts && (shown >> s & 1)) t[u] = *reinterpret_cast<const mnv_f4*>(part_out + (s * rows + row) * pitch + d);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {

@@ -121,6 +121,9 @@ SIZES = [
     # few queries over many keys, and the reverse
     (1, 1, 1, 1, 1000, 64), (2, 4, 1, 1, 777, 128), (1, 16, 4, 2, 3001, 64), (3, 2, 2, 5, 500, 40), (1, 1, 1, 33, 2048, 64), (1, 2, 1, 700, 3, 64),
     (1, 1, 1, 1000, 40, 128),
+    # parts of a key range whose columns fill half of a lane's turn
+    (1, 2, 2, 1, 2500, 16), (2, 6, 2, 3, 1900, 80), (1, 3, 3, 20, 800, 30), (1, 4, 1, 8, 2100, 90), (1, 2, 2, 40, 1500, 20), (1, 2, 1, 300, 900, 84),
+    (1, 1, 1, 1, 2111, 31),
 ]
 
 
