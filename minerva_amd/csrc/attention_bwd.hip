@@ -77,8 +77,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
       float x[8], y[8];
       // a key that is not read may hold anything: another one stands in for it, and 0 is stored
       const size_t at = ((size_t)b * z.k_len + (shown ? j : n - 1)) * z.kv_heads + kh;
-      mnv_load8<DP>(a.k + at * z.dim, s, z.dim, x);
-      mnv_load8<DP>(a.v + at * z.dim, s, z.dim, y);
+      mnv_load8<DP, VEC>(a.k + at * z.dim, s, z.dim, x);
+      mnv_load8<DP, VEC>(a.v + at * z.dim, s, z.dim, y);
       kp[s] = mnv_cut8(x);
       vp[s] = mnv_cut8(y);
     }
@@ -313,9 +313,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       float x[8], y[8], o[8];
-      mnv_load8<DP>(a.q + row * z.dim, s, z.dim, x);
-      mnv_load8<DP>(a.dout + row * z.dim, s, z.dim, y);
-      mnv_load8<DP>(a.out + row * z.dim, s, z.dim, o);
+      mnv_load8<DP, VEC>(a.q + row * z.dim, s, z.dim, x);
+      mnv_load8<DP, VEC>(a.dout + row * z.dim, s, z.dim, y);
+      mnv_load8<DP, VEC>(a.out + row * z.dim, s, z.dim, o);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[e] *= z.scale;

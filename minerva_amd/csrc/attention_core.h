@@ -302,21 +302,22 @@ struct MnvStage {
   }
 };
 
-// The columns 16 s + 8 (l / 32)... of one row (the lane's own) as an operand, times `scale`; 0 from dim on.
-template <int DP>
+// The columns 16 s + 8 (l / 32)... of one row (the lane's own) as an operand; 0 from dim on.
+template <int DP, bool VEC>
 __device__ __forceinline__ void mnv_load8(const float* row, int s, int dim, float (&x)[8]) {
   const int d0 = s * 16 + (int)threadIdx.x % MNV_WAVE / 32 * 8;
-  if (dim == DP) {
-    const mnv_f4 a = mnv_ldx4u<false>(row + d0), b = mnv_ldx4u<false>(row + d0 + 4);
+  if (VEC) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = a[e];
-      x[4 + e] = b[e];
+    for (int h = 0; h < 2; ++h) {
+      const int d = d0 + 4 * h;
+      const mnv_f4 t = mnv_ldx4u<false>(row + (d < dim - 4 ? d : dim - 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * h + e] = d < dim ? t[e] : 0.f;
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float t = row[d0 + e < dim ? d0 + e : 0];
+      const float t = row[d0 + e < dim ? d0 + e : dim - 1];
       x[e] = d0 + e < dim ? t : 0.f;
     }
   }

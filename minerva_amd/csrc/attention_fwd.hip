@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) {
       float x[8];
-      mnv_load8<DP>(a.q + row * z.dim, s, z.dim, x);
+      mnv_load8<DP, VEC>(a.q + row * z.dim, s, z.dim, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] *= z.scale;
       qp[s] = mnv_cut8(x);
