@@ -99,7 +99,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
                               diagonal_pitch(z.q_len);
       float carry = 0.f;
       struct Rows {
-        Stage stage;
         float m, l, delta;
       };
       auto fetch_rows = [&](Rows& next, int i0) __attribute__((always_inline)) {
@@ -119,20 +118,25 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           row_stats[turn][2][threadIdx.x] = sign * next.delta;
         }
       };
+      // Behind the last tile comes that one again: no branch parts a tile's work.
+      const int last = from + (to - from - 1) / 32 * 32;
+      Stage stage;
       {
         Rows first;
         fetch_rows(first, from);
-        first.stage.fetch(qb + (size_t)from * pitch, ob + (size_t)from * pitch, pitch, z.q_len - from, z.dim);
-        first.stage.template store<true>(lds, z.scale);
+        stage.fetch(qb + (size_t)from * pitch, ob + (size_t)from * pitch, pitch, z.q_len - from, z.dim);
+        stage.template store<true>(lds, z.scale);
         store_rows(first, from, 0);
+        const int i1 = from < last ? from + 32 : last;
+        stage.fetch(qb + (size_t)i1 * pitch, ob + (size_t)i1 * pitch, pitch, z.q_len - i1, z.dim);
       }
       __syncthreads();
       int turn = 0;
       for (int i0 = from; i0 < to; i0 += 32) {
-        const bool more = i0 + 32 < to;
-        Rows next;  // behind the last tile that one again: no branch parts what follows
-        const int i1 = more ? i0 + 32 : i0;
-        fetch_rows(next, i1);
+        const bool more = i0 < last;
+        Rows next;
+        fetch_rows(next, more ? i0 + 32 : last);
+        const int i2 = i0 + 64 < last ? i0 + 64 : last;
         const char* now = lds + turn * Stage::BYTES;
         mnv_f4 add[4];
         if (BIAS) {
@@ -153,8 +157,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           }
         }
 
-        // Four products in a row, a step per operand: the scores, under which the next tile is fetched; dout v, under which the weights are made
-        // of the scores and cut; dv, under which ds is; dk, under which the next tile is cut.
+        // Four products in a row, a step per operand: the scores, under which the next tile is cut; dout v, under which
+        // the weights are made of the scores and cut; dv, under which ds is; dk, under which the tile after the
+        // next is fetched.
         mnv_f16 t, dp;
 #pragma unroll
         for (int e = 0; e < 16; ++e) t[e] = dp[e] = 0.f;
@@ -199,7 +204,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           read_rows(k + 1);
           if (k < KS) {
             step(t, kp[s]);
-            next.stage.fetch_piece(s, qb + (size_t)i1 * pitch, ob + (size_t)i1 * pitch, pitch, z.q_len - i1, z.dim);
+            stage.template store_piece<true>(s, lds + (turn ^ 1) * Stage::BYTES, z.scale);
           } else if (k < 2 * KS) {
             step(dp, vp[s]);
 #pragma unroll
@@ -228,7 +233,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
             }
           } else {
             step(dk[s % NB], sc[s / NB].parts());
-            next.stage.template store_piece<true>(s, lds + (turn ^ 1) * Stage::BYTES, z.scale);
+            stage.fetch_piece(s, qb + (size_t)i2 * pitch, ob + (size_t)i2 * pitch, pitch, z.q_len - i2, z.dim);
           }
           MNV_STEP_ORDER(6);
         }
@@ -331,17 +336,20 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     const float* vb = a.v + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
     const float* bias = BIAS ? a.bias + h * z.offsets() + (z.q_len - 1 - i) : nullptr;
 
+    // Behind the last tile comes that one again: no branch parts a tile's work.
+    const int last = begin + (n - begin - 1) / 32 * 32;
+    Stage stage;
+    stage.fetch(kb + (size_t)begin * pitch, vb + (size_t)begin * pitch, pitch, n - begin, z.dim);
+    stage.template store<false>(lds, 1.f);
     {
-      Stage first;
-      first.fetch(kb + (size_t)begin * pitch, vb + (size_t)begin * pitch, pitch, n - begin, z.dim);
-      first.template store<false>(lds, 1.f);
+      const int j1 = begin < last ? begin + 32 : last;
+      stage.fetch(kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
     }
     __syncthreads();
     char* now = lds;
     for (int j0 = begin; j0 < n; j0 += 32) {
-      const bool more = j0 + 32 < n, whole = j0 + 32 <= n;
-      Stage stage;  // behind the last tile that one again: no branch parts what follows
-      const int j1 = more ? j0 + 32 : j0;
+      const bool whole = j0 + 32 <= n;
+      const int j2 = j0 + 64 < last ? j0 + 64 : last;
       mnv_f4 add[4];
       if (BIAS) {
 #pragma unroll
@@ -355,11 +363,12 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
           }
         }
       }
+      char* then = lds + (now == lds ? Stage::BYTES : 0);
       // keys of the tile that are read: the others' weights become 0
       const int left = n - j0 - 4 * half;
 
-      // Three products in a row: the scores, under which the next tile is fetched; dout v, under which the weights are made of the scores; dq, under
-      // which the second half of ds is made and the next tile cut.
+      // Three products in a row: the scores, under which the next tile is cut; dout v, under which the weights are made
+      // of the scores; dq, under which the second half of ds is made and the tile after the next fetched.
       mnv_f16 t, dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) t[e] = dp[e] = 0.f;
@@ -375,7 +384,6 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
                : k < 2 * KS ? Stage::by_rows(now + Stage::MATRIX, s, c)
                             : Stage::by_cols(now, s % NB * 32, s / NB, c);
       };
-      char* then = lds + (now == lds ? Stage::BYTES : 0);
       MnvParts cur = {{operand(0, 0), operand(0, 1), operand(0, 2)}};
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -388,7 +396,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
         };
         if (k < KS) {
           step(t, qp[s]);
-          stage.fetch_piece(s, kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
+          stage.template store_piece<false>(s, then, 1.f);
         } else if (k < 2 * KS) {
           step(dp, op[s]);
 #pragma unroll
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
             for (int u = 0; u < (4 + NB - 1) / NB; ++u)
             if (4 + s * 4 / NB + u < 4 + (s + 1) * 4 / NB) cut_ds(4 + s * 4 / NB + u);
           }
-          stage.template store_piece<false>(s, then, 1.f);
+          stage.fetch_piece(s, kb + (size_t)j2 * pitch, vb + (size_t)j2 * pitch, pitch, n - j2, z.dim);
         }
         MNV_STEP_ORDER(6);
       }

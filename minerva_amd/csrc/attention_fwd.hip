@@ -176,30 +176,32 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
     const std::false_type cuts;
     const int last = begin + (n - begin - 1) / 32 * 32;  // behind it that tile again: no branch parts a phase
     char *now = lds, *then = lds + Stage::BYTES;
-    if (!late) {
+    const auto turn = [&] {
+      char* t_ = now;
+      now = then;
+      then = t_;
+    };
+    if (NW == 8 && !late) {
       for (int j0 = begin; j0 < n; j0 += 32) {
         scores(fetches, now, then, j0 < last ? j0 + 32 : last);
-        if (NW == 8) __syncthreads();
+        __syncthreads();
         results(cuts, now, then, j0, 0);
         __syncthreads();
-        char* t_ = now;
-        now = then;
-        then = t_;
+        turn();
       }
-      if (NW == 8) __syncthreads();
-    } else {
-      // one phase behind: cuts a tile while it makes scores, which is when the others do
-#pragma unroll
-      for (int piece = 0; piece < Stage::PIECES; ++piece) fetch(piece, last < begin + 32 ? last : begin + 32);
       __syncthreads();
+    } else {
+      // the next tile is cut under the scores, and the one after it fetched under the results; of eight wavefronts the
+      // second half is a phase behind, and so cuts when the first does
+#pragma unroll
+      for (int piece = 0; piece < Stage::PIECES; ++piece) fetch(piece, begin < last ? begin + 32 : last);
+      if (NW == 8) __syncthreads();
       for (int j0 = begin; j0 < n; j0 += 32) {
         scores(cuts, now, then, 0);
-        __syncthreads();
+        if (NW == 8) __syncthreads();
         results(fetches, now, then, j0, j0 + 64 < last ? j0 + 64 : last);
         __syncthreads();
-        char* t_ = now;
-        now = then;
-        then = t_;
+        turn();
       }
     }
     l += __shfl_xor(l, 32, MNV_WAVE);
