@@ -47,7 +47,7 @@ __host__ __device__ inline size_t key_tiles(int k_len) { return ((size_t)k_len +
 template <int DP, bool BIAS, bool VEC>
 __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kernel(BwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
-  using Stage = MnvStage<DP, 256, VEC>;  // queries (times scale) and their gradients
+  using Stage = MnvStage<DP, 256, VEC>;  // queries and their gradients
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   __shared__ __align__(16) float row_stats[2][3][32];  // m, 1 / l, delta of the tile's queries
   __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
@@ -71,6 +71,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
     if (BIAS)
       for (int e = threadIdx.x; e < 4 * 16 * 48; e += 256) turned[e] = 0.f;
     const bool shown = j < n;
+    // The matrix instruction rounds its sums down, by up to a step of the larger of sum and terms: nothing to a
+    // value, but of the same sign everywhere, and a bucket's gradient sums 10^5 ds that cancel.  So every other key's
+    // products dout v are made with the opposite sign (12 heads of 512 x 512: the table's gradient off
+    // by 4.0e-6 without, 4.8e-7 with).
+    const float sign = j % 2 ? -1.f : 1.f;
     MnvParts kp[KS], vp[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -79,6 +84,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
       const size_t at = ((size_t)b * z.k_len + (shown ? j : n - 1)) * z.kv_heads + kh;
       mnv_load8<DP, VEC>(a.k + at * z.dim, s, z.dim, x);
       mnv_load8<DP, VEC>(a.v + at * z.dim, s, z.dim, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] *= z.scale;
+        y[e] *= sign;
+      }
       kp[s] = mnv_cut8(x);
       vp[s] = mnv_cut8(y);
     }
@@ -112,10 +122,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
       };
       auto store_rows = [&](const Rows& next, int i0, int turn) __attribute__((always_inline)) {
         if (threadIdx.x < 32) {
-          const float sign = threadIdx.x % 2 ? -1.f : 1.f;
           row_stats[turn][0][threadIdx.x] = mnv_finite_max(next.m);
-          row_stats[turn][1][threadIdx.x] = i0 + (int)threadIdx.x < z.q_len ? sign * mnv_inverse(next.l) : 0.f;
-          row_stats[turn][2][threadIdx.x] = sign * next.delta;
+          row_stats[turn][1][threadIdx.x] = i0 + (int)threadIdx.x < z.q_len ? mnv_inverse(next.l) : 0.f;
+          row_stats[turn][2][threadIdx.x] = next.delta;
         }
       };
       // Behind the last tile comes that one again: no branch parts a tile's work.
@@ -125,7 +134,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
         Rows first;
         fetch_rows(first, from);
         stage.fetch(qb + (size_t)from * pitch, ob + (size_t)from * pitch, pitch, z.q_len - from, z.dim);
-        stage.template store<true>(lds, z.scale);
+        stage.store(lds);
         store_rows(first, from, 0);
         const int i1 = from < last ? from + 32 : last;
         stage.fetch(qb + (size_t)i1 * pitch, ob + (size_t)i1 * pitch, pitch, z.q_len - i1, z.dim);
@@ -204,7 +213,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           read_rows(k + 1);
           if (k < KS) {
             step(t, kp[s]);
-            stage.template store_piece<true>(s, lds + (turn ^ 1) * Stage::BYTES, z.scale);
+            stage.store_piece(s, lds + (turn ^ 1) * Stage::BYTES);
           } else if (k < 2 * KS) {
             step(dp, vp[s]);
 #pragma unroll
@@ -228,7 +237,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
               if (pair >= (s + 1) * 8 / KS) continue;
               const mnv_f2 delta = mine[0][u];
 #pragma unroll
-              for (int e = 0; e < 2; ++e) dp[2 * pair + e] = t[2 * pair + e] * (dp[2 * pair + e] - delta[e]);
+              for (int e = 0; e < 2; ++e) dp[2 * pair + e] = t[2 * pair + e] * fmaf(dp[2 * pair + e], sign, -delta[e]);
               sc[pair / 4].pair(pair % 4, dp[2 * pair], dp[2 * pair + 1]);
             }
           } else {
@@ -280,11 +289,11 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
     const size_t keys = (size_t)z.batch * z.k_len * z.kv_heads;
     float* to = a.sums + (split * keys + key) * DP;
     if (j < n) {
-      mnv_store_column<DP>(dk, 1.f, true, to, DP);
+      mnv_store_column<DP>(dk, z.scale, true, to, DP);
       mnv_store_column<DP>(dv, 1.f, true, to + a.splits * keys * DP, DP);
     }
   } else if (j < z.k_len) {
-    mnv_store_column<DP>(dk, 1.f, j < n, a.dk + key * z.dim, z.dim);
+    mnv_store_column<DP>(dk, z.scale, j < n, a.dk + key * z.dim, z.dim);
     mnv_store_column<DP>(dv, 1.f, j < n, a.dv + key * z.dim, z.dim);
   }
 }
@@ -340,7 +349,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     const int last = begin + (n - begin - 1) / 32 * 32;
     Stage stage;
     stage.fetch(kb + (size_t)begin * pitch, vb + (size_t)begin * pitch, pitch, n - begin, z.dim);
-    stage.template store<false>(lds, 1.f);
+    stage.store(lds);
     {
       const int j1 = begin < last ? begin + 32 : last;
       stage.fetch(kb + (size_t)j1 * pitch, vb + (size_t)j1 * pitch, pitch, n - j1, z.dim);
@@ -396,7 +405,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
         };
         if (k < KS) {
           step(t, qp[s]);
-          stage.template store_piece<false>(s, then, 1.f);
+          stage.store_piece(s, then);
         } else if (k < 2 * KS) {
           step(dp, op[s]);
 #pragma unroll

@@ -117,6 +117,18 @@ __device__ __forceinline__ float mnv_max_of_halves(float x) {
 // 1 / l, and 0 for a row that sees no key
 __device__ __forceinline__ float mnv_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// mnv_split_pair without a factor, its halves taken by byte permutations: those the compiler does not see through (it
+// would convert each half again), and no wait is put behind them as behind its empty asm.
+__device__ __forceinline__ void mnv_cut_pair(float x, float y, unsigned (&p)[3]) {
+#pragma unroll
+  for (int c = 0; c < 3; ++c) {
+    const mnv_bf2 t = {(__bf16)x, (__bf16)y};
+    p[c] = __builtin_bit_cast(unsigned, t);
+    x -= __builtin_bit_cast(float, __builtin_amdgcn_perm(p[c], p[c], 0x05040c0cu));
+    y -= __builtin_bit_cast(float, __builtin_amdgcn_perm(p[c], p[c], 0x07060c0cu));
+  }
+}
+
 // Eight values of one operand as three parts.
 struct MnvParts {
   mnv_bf8 p[3];
@@ -126,7 +138,7 @@ __device__ __forceinline__ MnvParts mnv_cut8(const float* x) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     unsigned t[3];
-    mnv_split_pair(x[2 * i], x[2 * i + 1], 1.f, t);
+    mnv_cut_pair(x[2 * i], x[2 * i + 1], t);
     u[0][i] = t[0];
     u[1][i] = t[1];
     u[2][i] = t[2];
@@ -173,7 +185,7 @@ struct MnvCutting {
   mnv_u4 u[3];
   __device__ __forceinline__ void pair(int i, float x, float y) {
     unsigned t[3];
-    mnv_split_pair(x, y, 1.f, t);
+    mnv_cut_pair(x, y, t);
     u[0][i] = t[0];
     u[1][i] = t[1];
     u[2][i] = t[2];
@@ -243,22 +255,17 @@ struct MnvStage {
     for (int piece = 0; piece < PIECES; ++piece) fetch_piece(piece, m0, m1, pitch, rows, dim);
   }
 
-  // Cuts the tile into its planes: the first matrix times `scale`; of the second, ODD_MINUS, the odd rows
-  // times -1.  In as many pieces, each unit written with its last.
+  // Cuts the tile into its planes, in as many pieces, each unit written with its last.
   mnv_u4 w[3];
-  template <bool ODD_MINUS>
-  __device__ __forceinline__ void store_piece(int piece, char* lds, float scale) {
+  __device__ __forceinline__ void store_piece(int piece, char* lds) {
     const int s = piece / 2;
     if (s >= SLOTS) return;
     const At a = at(s);
     if (!a.any) return;
-    // 96 columns: a unit's matrix is known at run time only; no branch
-    const float second = a.second, sign = ODD_MINUS && a.row % 2 ? -1.f : 1.f;
-    const float f = UNITS % NT == 0 ? (a.second ? sign : scale) : second * sign + (1.f - second) * scale;
 #pragma unroll
     for (int h = piece % 2 * 2; h < piece % 2 * 2 + 2; ++h) {
       unsigned t[3];
-      mnv_split_pair(v[s][h / 2][h % 2 * 2], v[s][h / 2][h % 2 * 2 + 1], f, t);
+      mnv_cut_pair(v[s][h / 2][h % 2 * 2], v[s][h / 2][h % 2 * 2 + 1], t);
 #pragma unroll
       for (int p = 0; p < 3; ++p) w[p][h] = t[p];
     }
@@ -267,10 +274,9 @@ struct MnvStage {
 #pragma unroll
     for (int p = 0; p < 3; ++p) *reinterpret_cast<mnv_u4*>(to + p * PLANE) = w[p];
   }
-  template <bool ODD_MINUS>
-  __device__ __forceinline__ void store(char* lds, float scale) {
+  __device__ __forceinline__ void store(char* lds) {
 #pragma unroll
-    for (int piece = 0; piece < PIECES; ++piece) store_piece<ODD_MINUS>(piece, lds, scale);
+    for (int piece = 0; piece < PIECES; ++piece) store_piece(piece, lds);
   }
 
   // What a row's chunk numbers are xored with.  4 rows of 64 bytes: 128 columns put all in the same banks, 64

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
     {
       Stage first;
       first.fetch(kb + (size_t)begin * pitch, vb + (size_t)begin * pitch, pitch, n - begin, z.dim);
-      first.template store<false>(lds, 1.f);
+      first.store(lds);
     }
     __syncthreads();
 
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_atten
 #pragma unroll
       for (int piece = s * EACH; piece < (s + 1) * EACH && piece < Stage::PIECES; ++piece) {
         if (decltype(fetches)::value) fetch(piece, j1);
-        else stage.template store_piece<false>(piece, then, 1.f);
+        else stage.store_piece(piece, then);
       }
     };
     // scores of the tile in `now`; `fetches`: the tile from j1 on is fetched, else that in `stage` is cut into `then`
