@@ -396,8 +396,9 @@ int mnv_lrn_bwd(const float* bottom, const float* top, const float* scale, const
  *   dx = (g - mean(g) - xh * mean(g * xh)) / sqrt(var + eps),  g = gamma * dy
  *   dgamma = sum over the columns of dy * xh,  dbeta = sum over the columns of dy
  * eps is finite and not negative.  backward works from x alone (nothing of the forward pass is kept).
- * Its workspace holds partial sums over columns; with less of it, or none, fewer workgroups run.
- * The results' bits depend on the sizes, the workspace's size and 16-byte alignment alone. ---- */
+ * Its workspace holds partial sums over columns; with less of it, or none, fewer workgroups run (one, for
+ * none).  The order of the sums, and so the results' bits, is set by the sizes, the workspace's size and the
+ * device's number of compute units. ---- */
 int mnv_layernorm_fwd(const float* x, const float* gamma, const float* beta, float* y, int features,
                       int count, float eps, mnv_stream_t stream);
 size_t mnv_layernorm_bwd_workspace_bytes(int features, int count);
@@ -420,8 +421,14 @@ int mnv_layernorm_bwd(const float* x, const float* gamma, const float* dy, float
  *   dbias[o] = sum of ds_ij with j - i + q_len - 1 = o over the batch
  * dk and dv sum over the heads that share a key, and are 0 for keys that are not read; dbias is
  * written unless `bias` is NULL (then dbias is ignored).  An infinity or a NaN among the values that are read
- * gives NaN where it has a part.  forward's workspace holds the parts of a key range that few
- * queries are spread over; backward's (`has_bias`: with the bias's gradient) partial sums. ---- */
+ * gives NaN where it has a part.  At most 2^26 rows of queries and of keys (over heads and batch),
+ * 2^22 heads over the batch, heads * head_dim 2^24, and 2^31 - 1 values in each tensor.
+ * A workspace is used if it is aligned to 16 bytes.  forward's holds the sums of parts of the key range,
+ * where queries are too few to fill the chip; backward's the same of its loops, and (`has_bias`) the sums of
+ * ds along the diagonals of every 32 keys, of at most 256 MiB of them at a time (or one entry's and key head's, if
+ * that is more).  With less of it fewer parts run; with too little for the diagonals of one entry and key head,
+ * dbias is made of scores that are computed once more, one by one, which is far slower.  The order of all sums
+ * is set by the sizes, the workspace's size and the device's number of compute units. ---- */
 size_t mnv_attention_fwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len,
                                          int head_dim);
 int mnv_attention_fwd(const float* q, const float* k, const float* v, const float* bias,

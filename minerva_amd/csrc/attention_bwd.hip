@@ -647,7 +647,6 @@ int mnv_attention_bwd(const float* q, const float* k, const float* v, const floa
   ka.parts = plan.pairs ? static_cast<float*>(workspace) : nullptr;
   ka.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.diagonal_bytes);
   const size_t at_once = plan.pairs ? plan.pairs : pairs;
-  if (ka.tiles * ka.splits * at_once > 0x7fffffff) return MNV_ERR_INVALID;
   for (size_t p = 0; p < pairs; p += at_once) {
     const unsigned now = (unsigned)(pairs - p < at_once ? pairs - p : at_once);
     ka.first_pair = (unsigned)p;
@@ -676,7 +675,6 @@ int mnv_attention_bwd(const float* q, const float* k, const float* v, const floa
   a.splits = plan.query_splits;
   a.chunk = (int)mnv_ceil_div(mnv_ceil_div(k_len, 32), a.splits);
   a.sums = static_cast<float*>(workspace);
-  if (a.tiles * a.splits * pairs > 0x7fffffff) return MNV_ERR_INVALID;
   const int rc = by_dim(head_dim, launch_dq<32>, launch_dq<64>, launch_dq<96>, launch_dq<128>, a,
                         (unsigned)(a.tiles * a.splits * pairs), s);
   if (rc || a.splits == 1) return rc;

@@ -20,6 +20,10 @@
 
 #define MNV_AT_MAX_DIM 128
 #define MNV_AT_MAX_PITCH (1 << 24)  // heads * dim: 64 rows of it are less than 2^32 bytes
+// Rows of queries or keys, and pairs of an entry and a head: every launch has fewer than 2^32 threads (a launch's
+// limit), and no number of a row rounded up to tiles and parts passes 2^31.
+#define MNV_AT_MAX_ROWS (1 << 26)
+#define MNV_AT_MAX_PAIRS (1 << 22)
 
 struct AttentionSizes {
   int batch, heads, kv_heads, q_len, k_len, dim;
@@ -32,9 +36,9 @@ struct AttentionSizes {
 static inline bool mnv_attention_sizes_ok(const AttentionSizes& z) {
   if (z.batch < 1 || z.heads < 1 || z.kv_heads < 1 || z.q_len < 1 || z.k_len < 1 || z.dim < 1) return false;
   if (z.dim > MNV_AT_MAX_DIM || z.heads % z.kv_heads || z.heads > MNV_AT_MAX_PITCH / z.dim) return false;
-  const long long most = 0x7fffffffLL, d = z.dim > 2 ? z.dim : 2;  // stats has two values where out has dim
-  if ((long long)z.batch * z.heads > most || (long long)z.batch * z.heads * z.q_len > most / d) return false;
-  if ((long long)z.batch * z.kv_heads * z.k_len > most / z.dim) return false;
+  const long long most = 0x7fffffffLL, rows = MNV_AT_MAX_ROWS < most / z.dim ? MNV_AT_MAX_ROWS : most / z.dim;
+  if ((long long)z.batch * z.heads > MNV_AT_MAX_PAIRS || (long long)z.batch * z.heads * z.q_len > rows) return false;
+  if ((long long)z.batch * z.kv_heads * z.k_len > rows) return false;
   return ((long long)z.q_len + z.k_len - 1) * z.heads <= most && fabsf(z.scale) <= 3e38f;
 }
 

@@ -294,9 +294,7 @@ int parts(const AttentionSizes& z, size_t workspace_bytes) {
 template <int DP, int NW>
 int launch(FwdArgs& a, hipStream_t s) {
   a.row_tiles = (int)mnv_ceil_div(a.rows, 32 * NW);
-  const size_t grid = (size_t)a.row_tiles * a.parts * a.z.batch * a.z.kv_heads;
-  if (grid > 0x7fffffff) return MNV_ERR_INVALID;
-  const dim3 g((unsigned)grid), b(64 * NW);
+  const dim3 g((unsigned)a.row_tiles * a.parts * a.z.batch * a.z.kv_heads), b(64 * NW);
   const bool vec = a.z.dim % 4 == 0;
   if (a.bias && vec) hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, true, true>), g, b, 0, s, a);
   else if (a.bias) hipLaunchKernelGGL((mnv_attention_fwd_kernel<DP, NW, true, false>), g, b, 0, s, a);

@@ -88,8 +88,8 @@ __device__ __forceinline__ void store4(float* p, int left, mnv_f4 v) {
   if (left > 2) p[2] = v.z;
 }
 
-// One column per GROUP threads of an NTH-thread workgroup, CACHE vectors of four values per thread.
-template <int GROUP, int CACHE, int NTH>
+// One column per GROUP threads of a workgroup, CACHE vectors of four values per thread.
+template <int GROUP, int CACHE>
 struct Column {
   mnv_f4 x[CACHE];
   float mean, r;
@@ -123,10 +123,10 @@ struct Column {
 template <int GROUP, int CACHE, int NTH, bool VEC, bool NT>
 __global__ __launch_bounds__(NTH) void mnv_layernorm_fwd_kernel(const float* __restrict__ x, const float* __restrict__ gamma,
                                                                 const float* __restrict__ beta, float* __restrict__ y,
-                                                                int features, int count, float eps) {
+                                                                int features, unsigned count, float eps) {
   __shared__ float lds[GROUP > MNV_WAVE ? NTH / MNV_WAVE : 1];
   constexpr int PER = NTH / GROUP;
-  Column<GROUP, CACHE, NTH> c;
+  Column<GROUP, CACHE> c;
   c.t = threadIdx.x % GROUP * 4;
   c.features = features;
   mnv_f4 g[CACHE], b[CACHE];
@@ -134,12 +134,12 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_fwd_kernel(const float* __r
   c.template load<VEC, false>(b, beta);
   // the next column is fetched while this one is summed (behind the last that one again)
   mnv_f4 next[CACHE];
-  const int first = blockIdx.x * PER + (PER > 1 ? threadIdx.x / GROUP : 0), step = gridDim.x * PER;
+  const unsigned first = blockIdx.x * PER + (PER > 1 ? threadIdx.x / GROUP : 0), step = gridDim.x * PER;
   if (first < count) c.template load<VEC, NT>(next, x + (size_t)first * features);
-  for (int i = first; i < count; i += step) {
+  for (unsigned i = first; i < count; i += step) {
 #pragma unroll
     for (int u = 0; u < CACHE; ++u) c.x[u] = next[u];
-    c.template load<VEC, NT>(next, x + (size_t)(i < count - step ? i + step : i) * features);
+    c.template load<VEC, NT>(next, x + (size_t)(i + step < count ? i + step : i) * features);
     c.centre(eps, lds);
     float* out = y + (size_t)i * features + c.t;
 #pragma unroll
@@ -159,11 +159,11 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
                                                                 const float* __restrict__ dy, float* __restrict__ dx,
                                                                 float* __restrict__ parts_gamma,
                                                                 float* __restrict__ parts_beta, size_t part_pitch,
-                                                                int features, int count, float eps) {
+                                                                int features, unsigned count, float eps) {
   constexpr int PER = NTH / GROUP;
   __shared__ float lds[GROUP > MNV_WAVE ? 2 * NTH / MNV_WAVE : 1];
   __shared__ mnv_f4 joined[PER > 1 ? NTH : 1];
-  Column<GROUP, CACHE, NTH> c;
+  Column<GROUP, CACHE> c;
   c.t = threadIdx.x % GROUP * 4;
   c.features = features;
   mnv_f4 g[CACHE], sg[CACHE], sb[CACHE];
@@ -173,12 +173,12 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
   // the next column is fetched while this one is summed (behind the last that one again), where registers allow
   constexpr bool AHEAD = CACHE <= 4;
   mnv_f4 next_x[CACHE], next_d[CACHE];
-  const int first = blockIdx.x * PER + (PER > 1 ? threadIdx.x / GROUP : 0), step = gridDim.x * PER;
+  const unsigned first = blockIdx.x * PER + (PER > 1 ? threadIdx.x / GROUP : 0), step = gridDim.x * PER;
   if (AHEAD && first < count) {
     c.template load<VEC, NT>(next_x, x + (size_t)first * features);
     c.template load<VEC, NT>(next_d, dy + (size_t)first * features);
   }
-  for (int i = first; i < count; i += step) {
+  for (unsigned i = first; i < count; i += step) {
     mnv_f4 d[CACHE];
     if (AHEAD) {
 #pragma unroll
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
         c.x[u] = next_x[u];
         d[u] = next_d[u];
       }
-      const size_t at = (size_t)(i < count - step ? i + step : i) * features;
+      const size_t at = (size_t)(i + step < count ? i + step : i) * features;
       c.template load<VEC, NT>(next_x, x + at);
       c.template load<VEC, NT>(next_d, dy + at);
     } else {
@@ -245,12 +245,12 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
 
 // Columns of more values than the register forms hold: each pass reads the column again.
 #define MNV_LN_WIDE 1024
-__device__ __forceinline__ void wide_stats(const float* x, int features, float eps, float* lds, float* mean, float* r) {
+__device__ __forceinline__ void wide_stats(const float* x, unsigned features, float eps, float* lds, float* mean, float* r) {
   float s = 0.f;
-  for (int f = threadIdx.x; f < features; f += MNV_LN_WIDE) s += x[f];
+  for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) s += x[f];
   *mean = group_sum<MNV_LN_WIDE>(s, lds) / features;
   s = 0.f;
-  for (int f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
+  for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
     const float d = x[f] - *mean;
     s = fmaf(d, d, s);
   }
@@ -258,30 +258,30 @@ __device__ __forceinline__ void wide_stats(const float* x, int features, float e
 }
 __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_fwd_wide_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, float* __restrict__ y,
-    int features, int count, float eps) {
+    unsigned features, unsigned count, float eps) {
   __shared__ float lds[MNV_LN_WIDE / MNV_WAVE];
-  for (int i = blockIdx.x; i < count; i += gridDim.x) {
+  for (unsigned i = blockIdx.x; i < count; i += gridDim.x) {
     const float* xc = x + (size_t)i * features;
     float* yc = y + (size_t)i * features;
     float mean, r;
     wide_stats(xc, features, eps, lds, &mean, &r);
-    for (int f = threadIdx.x; f < features; f += MNV_LN_WIDE) yc[f] = gamma[f] * ((xc[f] - mean) * r) + beta[f];
+    for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) yc[f] = gamma[f] * ((xc[f] - mean) * r) + beta[f];
   }
 }
 __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_bwd_wide_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ dy, float* __restrict__ dx,
-    float* __restrict__ parts_gamma, float* __restrict__ parts_beta, size_t part_pitch, int features, int count, float eps) {
+    float* __restrict__ parts_gamma, float* __restrict__ parts_beta, size_t part_pitch, unsigned features, unsigned count, float eps) {
   __shared__ float lds[2 * MNV_LN_WIDE / MNV_WAVE];
   float* pg = parts_gamma + blockIdx.x * part_pitch;
   float* pb = parts_beta + blockIdx.x * part_pitch;
-  for (int f = threadIdx.x; f < features; f += MNV_LN_WIDE) pg[f] = pb[f] = 0.f;
-  for (int i = blockIdx.x; i < count; i += gridDim.x) {
+  for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) pg[f] = pb[f] = 0.f;
+  for (unsigned i = blockIdx.x; i < count; i += gridDim.x) {
     const float* xc = x + (size_t)i * features;
     const float* dyc = dy + (size_t)i * features;
     float* dxc = dx + (size_t)i * features;
     float mean, r, s = 0.f, sx = 0.f;
     wide_stats(xc, features, eps, lds, &mean, &r);
-    for (int f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
+    for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
       const float gd = gamma[f] * dyc[f];
       s += gd;
       sx = fmaf(gd, (xc[f] - mean) * r, sx);
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_bwd_wide_kernel(
     group_sum2<MNV_LN_WIDE>(s, sx, lds);
     s /= features;
     sx /= features;
-    for (int f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
+    for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
       const float d = dyc[f], xh = (xc[f] - mean) * r;
       dxc[f] = r * (gamma[f] * d - s - xh * sx);
       pg[f] = fmaf(d, xh, pg[f]);  // each thread has its own features throughout
@@ -302,27 +302,29 @@ __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_bwd_wide_kernel(
 // every 64th part (2048 parts of 512 features: 8 loads in a row per chain).
 __global__ __launch_bounds__(1024) void mnv_layernorm_sums_kernel(const float* __restrict__ parts, int num,
                                                                   float* __restrict__ dgamma, float* __restrict__ dbeta,
-                                                                  int features) {
+                                                                  unsigned features) {
   __shared__ float lds[64][17];
   const int lane = threadIdx.x % 16, q = threadIdx.x / 16;
-  const int f = blockIdx.x * 16 + lane;
-  float chain[4] = {0.f, 0.f, 0.f, 0.f};
-  if (f < features) {
-    const float* p = parts + (size_t)blockIdx.y * features + f;
-    for (int i = q; i < num; i += 256) {
+  for (unsigned f0 = blockIdx.x * 16; f0 < features; f0 += gridDim.x * 16) {
+    const unsigned f = f0 + lane;
+    float chain[4] = {0.f, 0.f, 0.f, 0.f};
+    if (f < features) {
+      const float* p = parts + (size_t)blockIdx.y * features + f;
+      for (int i = q; i < num; i += 256) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (i + 64 * c < num) chain[c] += p[(size_t)(i + 64 * c) * 2 * features];
+        for (int c = 0; c < 4; ++c)
+          if (i + 64 * c < num) chain[c] += p[(size_t)(i + 64 * c) * 2 * features];
+      }
     }
-  }
-  lds[q][lane] = (chain[0] + chain[1]) + (chain[2] + chain[3]);
-  __syncthreads();
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    if (q < o) lds[q][lane] += lds[q + o][lane];
+    lds[q][lane] = (chain[0] + chain[1]) + (chain[2] + chain[3]);
     __syncthreads();
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      if (q < o) lds[q][lane] += lds[q + o][lane];
+      __syncthreads();
+    }
+    if (q == 0 && f < features) (blockIdx.y ? dbeta : dgamma)[f] = lds[0][lane];
   }
-  if (q == 0 && f < features) (blockIdx.y ? dbeta : dgamma)[f] = lds[0][lane];
 }
 
 bool sizes_ok(int features, int count, float eps) {
@@ -429,7 +431,8 @@ int mnv_layernorm_bwd(const float* x, const float* gamma, const float* dy, float
   n.groups = (unsigned)groups;
   const int rc = run(n);
   if (rc) return rc;
-  hipLaunchKernelGGL(mnv_layernorm_sums_kernel, dim3((unsigned)mnv_ceil_div(features, 16), 2), dim3(1024), 0, n.s, parts,
+  const size_t sums = mnv_ceil_div(features, 16);
+  hipLaunchKernelGGL(mnv_layernorm_sums_kernel, dim3((unsigned)(sums < 65536 ? sums : 65536), 2), dim3(1024), 0, n.s, parts,
                      (int)groups, dgamma, dbeta, features);
   return MNV_LAUNCH_STATUS();
 }

@@ -47,7 +47,13 @@ def _attend(fwd, pointers=None, scale=1.0, **sizes):
 BAD_SIZES = [{"batch": 0}, {"batch": -1}, {"heads": 0}, {"kv_heads": 0}, {"q_len": 0}, {"k_len": 0}, {"head_dim": 0},
              {"head_dim": 129}, {"heads": 3}, {"kv_heads": 8}, {"kv_heads": -2}, {"k_len": 1 << 28}, {"q_len": 1 << 27},
              {"batch": 1 << 16, "heads": 1 << 16}, {"heads": 1 << 10, "kv_heads": 1, "q_len": 1, "k_len": 1 << 22, "batch": 1},
-             {"batch": 1 << 20, "heads": 1 << 10, "kv_heads": 1 << 10, "q_len": 1, "k_len": 1, "head_dim": 1}]
+             {"batch": 1 << 20, "heads": 1 << 10, "kv_heads": 1 << 10, "q_len": 1, "k_len": 1, "head_dim": 1},
+             # more rows, heads of all entries or values to a position than the kernels count
+             {"batch": 1, "heads": 1, "kv_heads": 1, "q_len": 1, "k_len": 0x7fffffff, "head_dim": 1},
+             {"batch": 1, "heads": 1, "kv_heads": 1, "q_len": 1, "k_len": (1 << 26) + 1, "head_dim": 1},
+             {"batch": 1, "heads": 1, "kv_heads": 1, "q_len": (1 << 26) + 1, "k_len": 1, "head_dim": 1},
+             {"batch": (1 << 21) + 1, "heads": 2, "kv_heads": 1, "q_len": 1, "k_len": 1, "head_dim": 1},
+             {"batch": 1, "heads": (1 << 17) + 1, "kv_heads": 1, "q_len": 1, "k_len": 1, "head_dim": 128}]
 
 
 @pytest.mark.parametrize("fwd", [True, False])
@@ -67,6 +73,12 @@ def test_attention_sizes_that_are_refused_need_no_workspace(bad):
     z = tuple({**SIZES, **bad}.values())
     assert capi.lib().mnv_attention_fwd_workspace_bytes(*z) == 0
     assert capi.lib().mnv_attention_bwd_workspace_bytes(*z, 1) == 0
+
+
+def test_attention_takes_sizes_up_to_its_limits():
+    assert capi.lib().mnv_attention_fwd_workspace_bytes(1, 1, 1, 1, 1 << 26, 16) > 0
+    assert capi.lib().mnv_attention_bwd_workspace_bytes(1 << 22, 1, 1, 16, 16, 1, 1) > 0
+    assert capi.lib().mnv_attention_bwd_workspace_bytes(1, 1 << 17, 1, 1, 64, 128, 1) > 0
 
 
 GOOD = dict(buckets=32, heads=4, q_len=8, k_len=8, q_start=0, max_distance=128, both_ways=1)
