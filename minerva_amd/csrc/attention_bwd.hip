@@ -570,7 +570,9 @@ BwdPlan make_plan(const AttentionSizes& z, bool has_bias, size_t workspace_bytes
     p.diagonal_bytes = mnv_ceil_div(p.pairs * one, 16) * 16;
     if (p.diagonal_bytes > workspace_bytes) p.diagonal_bytes = p.pairs * one;
   }
-  const size_t left = workspace_bytes - p.diagonal_bytes, places = (size_t)mnv_cu_count() * (dp <= 32 ? 2 : 1);
+  // One workgroup to a CU: more parts, where a CU holds two, cost more to add up than they save (2 x 8 heads of 200 x 1000, 32
+  // wide: 32.7 us, 39.0 with two; 8 heads of 1 x 4096, 64 wide: 30.4 and 33.5).
+  const size_t left = workspace_bytes - p.diagonal_bytes, places = mnv_cu_count();
   // a head's diagonals are summed by one workgroup
   const size_t key_part = 2 * (size_t)z.batch * z.k_len * z.kv_heads * dp * sizeof(float);
   const size_t q_tiles = mnv_ceil_div(z.q_len, 32);

@@ -27,7 +27,7 @@ struct FwdArgs {
 };
 
 template <int DP, int NW, bool BIAS, bool VEC>
-__global__ __launch_bounds__(64 * NW, DP > 64 && NW <= 4 ? 1 : 2) void mnv_attention_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(64 * NW, DP > 64 && NW == 4 ? 1 : 2) void mnv_attention_fwd_kernel(FwdArgs a) {
   constexpr int NB = DP / 32, KS = DP / 16;
   using Stage = MnvStage<DP, 64 * NW, VEC>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
@@ -330,23 +330,26 @@ __global__ __launch_bounds__(256) void mnv_attention_join_few_kernel(const float
   if (lane < 2) stats[2 * row + lane] = lane ? l : m;
 }
 
-// Wavefronts of a workgroup: one for up to 32 rows of an entry and key head; eight, in two halves, where a
-// workgroup has the CU to itself and rows enough.
+// Wavefronts of a workgroup: eight, in two halves, where a workgroup has the CU to itself and rows enough (128 wide, 2 x 16
+// heads of 2048 x 4096: 626 us, 707 with four; 4 x 8 heads of 512 x 2048, a quarter of the chip: 99.5 and 103; 8 heads of
+// 512 x 2048: 42.7 and 39.9).  Four also for a few rows, where three of them only bring tiles: 16 heads of 4 key heads for
+// one query over 2000 keys 13.2 us, with one wavefront that does all 14.9; 128 wide, over 16384 keys 48 and 80.
 int wavefronts(const AttentionSizes& z) {
-  const long long rows = (long long)z.q_len * z.group();
-  return rows <= 32 ? 1 : z.dim > 64 && mnv_ceil_div(rows, 256) * z.batch * z.kv_heads >= (size_t)mnv_cu_count() / 2 ? 8 : 4;
+  const size_t rows = (size_t)z.q_len * z.group();
+  return z.dim > 64 && mnv_ceil_div(rows, 256) * z.batch * z.kv_heads >= (size_t)mnv_cu_count() / 4 ? 8 : 4;
 }
 size_t part_bytes(const AttentionSizes& z) { return z.q_rows() * (mnv_attention_padded(z.dim) + 2) * sizeof(float); }
 int parts(const AttentionSizes& z, bool lengths, size_t workspace_bytes) {
   const int nw = wavefronts(z);
   const size_t blocks = mnv_ceil_div((size_t)z.q_len * z.group(), 32 * nw) * z.batch * z.kv_heads;
-  // workgroups that a CU holds, by LDS and registers
-  const size_t places = (size_t)mnv_cu_count() * (nw == 1 ? (z.dim <= 64 ? 3 : 1) : nw == 4 && z.dim <= 64 ? 2 : 1);
+  // workgroups that a CU holds, by LDS (129 x 1500, 64 wide: 32.7 us, 35.7 with two; over 64 wide 28 us of 16 heads for one
+  // query over 2000 keys, 33 with two)
+  const size_t places = (size_t)mnv_cu_count() * (z.dim <= 64 ? 3 : 1);
   const auto fill = [&](size_t n) {
     return mnv_attention_parts(blocks, n, mnv_ceil_div(z.k_len, 32), 2, part_bytes(z), workspace_bytes);
   };
   // Of parts behind an entry's keys nothing is left to do, so where there are lengths twice as many even out the
-  // rest (12 heads of 129 queries, 6 entries of 0 to 1500 keys: 43 -> 35 us); not where there would be one
+  // rest (12 heads of 129 queries, 6 entries of 0 to 1500 keys: 43 us -> 35); not where there would be one
   // otherwise, which needs no joining (16 heads of 512 queries, 8 entries of 128 to 1024 keys: 80 us, of 2 parts 66 and 35
   // to join them).
   const int once = fill(places);
@@ -367,7 +370,6 @@ int launch(FwdArgs& a, hipStream_t s) {
 
 template <int DP>
 int launch_width(FwdArgs& a, int nw, hipStream_t s) {
-  if (nw == 1) return launch<DP, 1>(a, s);
   if (DP > 64 && nw == 8) return launch<DP, DP <= 64 ? 4 : 8>(a, s);
   return launch<DP, 4>(a, s);
 }

@@ -170,8 +170,9 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
   c.template load<VEC, false>(g, gamma);
 #pragma unroll
   for (int u = 0; u < CACHE; ++u) sg[u] = sb[u] = mnv_f4{0.f, 0.f, 0.f, 0.f};
-  // the next column is fetched while this one is summed (behind the last that one again), where registers allow
-  constexpr bool AHEAD = CACHE <= 4;
+  // the next column is fetched while this one is summed (behind the last that one again); of wider ones it costs registers that
+  // more workgroups to a CU use better (4096 x 8192: 85 us with, 80 without; 8192 x 1000: 38 and 32)
+  constexpr bool AHEAD = CACHE <= 2;
   mnv_f4 next_x[CACHE], next_d[CACHE];
   const unsigned first = blockIdx.x * PER + (PER > 1 ? threadIdx.x / GROUP : 0), step = gridDim.x * PER;
   if (AHEAD && first < count) {
@@ -370,7 +371,8 @@ int by_width(const Norm& n) {
   if (f <= 2048) return launch<256, 2, 256, VEC, NT>(n);
   if (f <= 4096) return launch<256, 4, 256, VEC, NT>(n);
   if (f <= 8192) return launch<512, 4, 512, VEC, NT>(n);
-  return launch<512, 8, 512, VEC, NT>(n);
+  // 16384 x 2048: forward 43 us, of 512 threads 54; backward, whose sums take registers too, 170 and 109
+  return n.dy ? launch<512, 8, 512, VEC, NT>(n) : launch<1024, 4, 1024, VEC, NT>(n);
 }
 int run(const Norm& n) {
   if (n.features > 16384) {
@@ -382,20 +384,19 @@ int run(const Norm& n) {
                          n.x, n.gamma, n.beta, n.y, n.features, n.count, n.eps);
     return MNV_LAUNCH_STATUS();
   }
+  // past the caches: 8192 x 16384 forward 176 us, 188 through them; backward 304 and 328.  4096 x 8192 fits them: 41, and 49 past them
   const bool vec = n.features % 4 == 0, nt = (size_t)n.features * n.count * sizeof(float) >= MNV_PAST_CACHE_BYTES;
   if (vec) return nt ? by_width<true, true>(n) : by_width<true, false>(n);
   return nt ? by_width<false, true>(n) : by_width<false, false>(n);
 }
 
-// Workgroups of the backward pass: what the chip holds at once, and fewer where a group would have few
-// columns to its partial sums.
+// Workgroups of the backward pass: 3 or 2 to a CU are enough to keep the memory busy, and leave fewer partial sums (512 x
+// 65536: 69 us, of 8 to a CU 77; 4096 x 8192: 69, of 4 to a CU 78), and fewer of them where a group would have few
+// columns to its sums (2048 x 1000: 14.0 us of two columns or more, 12.7 of four; 64 x 100: 8.1 and 8.6).
 unsigned bwd_workgroups(int features, int count) {
-  const size_t each = columns_at_once(features), all = mnv_ceil_div(count, each);
-  const size_t most = (size_t)mnv_cu_count() * (features <= 512 ? 8 : features <= 4096 ? 4 : 2);
-  size_t groups = mnv_ceil_div(count, each * 2);  // two columns or more to each
-  if (groups > most) groups = most;
-  if (groups > all) groups = all;
-  return (unsigned)(groups ? groups : 1);
+  const size_t most = (size_t)mnv_cu_count() * (features <= 512 ? 3 : 2);
+  const size_t groups = mnv_ceil_div(count, (size_t)columns_at_once(features) * (features <= 512 ? 2 : 4));
+  return (unsigned)(groups < most ? groups : most);
 }
 
 }  // namespace
