@@ -5,7 +5,13 @@
 // has 32 queries per wavefront, and tiles of 32 keys stream through LDS.  t^T = K Q^T, so a lane
 // has one query and a quarter of the tile's keys; exp(t - m) goes on as the operand of out^T += V^T P^T from
 // the registers it stands in (attention_core.h).  Heads that share keys are rows of the same workgroup: row r is query
-// r / group, head r % group of the key head, so their keys are read and cut once.
+// r / group, head r % group of the key head, so their keys are read and cut once.  Few rows over many keys are spread
+// over parts of the keys, which a second kernel joins.
+// Bound by the matrix cores where there are queries enough: 2 products of 6 instructions per value.  2 x 16 heads (4 key heads) of
+// 2048 x 4096, 128 wide: 0.63 ms = 219 TFLOP/s of fp32 products in calls back to back, cores busy 64% (the rest: the
+// first operands of each phase wait for LDS, the softmax between the phases); a large fp32 product of the
+// library reaches 153.  8 x 16 heads of 512 x 1024, 64 wide, lengths 128 to 1024: 79 us, the longest entry's workgroups.
+// For one query the memory bounds it: 16 heads of 4 key heads, 8 entries of 250 to 2000 keys: 12 us and 4 to join, of 18 MB.
 // A row that sees no key has m = -inf, l = 0, out = 0.  The pair (m, l) is kept and not m + ln l: where the bias is the
 // type's lowest value for a whole row, ln l would be lost in the sum.
 #include <type_traits>
@@ -267,7 +273,8 @@ __global__ __launch_bounds__(256) void mnv_attention_join_kernel(const float* __
       for (int u = 0; u < 4; ++u) {
         const int s = s0 + 4 * u + lane / 16;
         t[u] = mnv_f4{0.f, 0.f, 0.f, 0.f};
-        if (d < pitch && s < parts && (shown >> s & 1)) t[u] = *reinterpret_cast<const mnv_f4*>(part_out + (s * rows + row) * pitch + d);
+        if (d < pitch && s < parts && (shown >> s & 1))
+          t[u] = *reinterpret_cast<const mnv_f4*>(part_out + (s * rows + row) * pitch + d);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -287,9 +294,10 @@ __global__ __launch_bounds__(256) void mnv_attention_join_kernel(const float* __
   if (lane < 2) stats[2 * row + lane] = lane ? l : m;
 }
 
-// The same of up to 8 parts, 16 lanes to a row, each of which works all parts' numbers out by itself: nothing is handed
-// from lane to lane (9288 rows of 64 in 7 parts: 4.4 us, 7.0 by the kernel above).
-#define MNV_AT_FEW_PARTS 8
+// The same of up to MOST parts, 16 lanes to a row, each of which works all parts' numbers out by itself: nothing is handed
+// from lane to lane (9288 rows of 64 in 7 parts: 4.4 us, 7.0 by the kernel above; in 10 parts 5.0 and 7.0; where 8 do, 16
+// take half a microsecond longer).
+template <int MOST>
 __global__ __launch_bounds__(256) void mnv_attention_join_few_kernel(const float* __restrict__ part_out,
                                                                      const float* __restrict__ part_stats,
                                                                      float* __restrict__ out, float* __restrict__ stats,
@@ -297,30 +305,30 @@ __global__ __launch_bounds__(256) void mnv_attention_join_few_kernel(const float
   const size_t row = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
   if (row >= rows) return;
   const int lane = threadIdx.x % 16;
-  float w[MNV_AT_FEW_PARTS], ls[MNV_AT_FEW_PARTS], m = -INFINITY, l = 0.f;
+  float w[MOST], ls[MOST], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int s = 0; s < MNV_AT_FEW_PARTS; ++s) {
+  for (int s = 0; s < MOST; ++s) {
     const size_t at = (s < parts ? s : 0) * rows + row;
     w[s] = part_stats[2 * at];
     ls[s] = s < parts ? part_stats[2 * at + 1] : 0.f;
   }
 #pragma unroll
-  for (int s = 0; s < MNV_AT_FEW_PARTS; ++s) m = fmaxf(m, w[s]);
+  for (int s = 0; s < MOST; ++s) m = fmaxf(m, w[s]);
 #pragma unroll
-  for (int s = 0; s < MNV_AT_FEW_PARTS; ++s) {
+  for (int s = 0; s < MOST; ++s) {
     w[s] = ls[s] == 0.f ? 0.f : mnv_weight(w[s], mnv_finite_max(m));
     l = fmaf(ls[s], w[s], l);
   }
   const float f = mnv_inverse(l);
   for (int d = 4 * lane; d < pitch; d += 64) {
-    mnv_f4 t[MNV_AT_FEW_PARTS], acc = {0.f, 0.f, 0.f, 0.f};
+    mnv_f4 t[MOST], acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int s = 0; s < MNV_AT_FEW_PARTS; ++s) {
+    for (int s = 0; s < MOST; ++s) {
       t[s] = mnv_f4{0.f, 0.f, 0.f, 0.f};
       if (ls[s] != 0.f) t[s] = *reinterpret_cast<const mnv_f4*>(part_out + (s * rows + row) * pitch + d);
     }
 #pragma unroll
-    for (int s = 0; s < MNV_AT_FEW_PARTS; ++s)
+    for (int s = 0; s < MOST; ++s)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] = fmaf(t[s][e], w[s], acc[e]);
 #pragma unroll
@@ -403,10 +411,11 @@ int mnv_attention_fwd(const float* q, const float* k, const float* v, const floa
                  : dp == 96 ? launch_width<96>(a, nw, s)
                             : launch_width<128>(a, nw, s);
   if (rc || a.parts == 1) return rc;
-  const bool few = a.parts <= MNV_AT_FEW_PARTS;
-  hipLaunchKernelGGL(few ? mnv_attention_join_few_kernel : mnv_attention_join_kernel,
-                     dim3((unsigned)mnv_ceil_div(z.q_rows(), few ? 16 : 4)), dim3(256), 0, s, a.part_out, a.part_stats, out,
-                     stats, z.q_rows(), a.parts, head_dim, dp);
+  const auto join = a.parts <= 8    ? mnv_attention_join_few_kernel<8>
+                    : a.parts <= 16 ? mnv_attention_join_few_kernel<16>
+                                    : mnv_attention_join_kernel;
+  hipLaunchKernelGGL(join, dim3((unsigned)mnv_ceil_div(z.q_rows(), a.parts <= 16 ? 16 : 4)), dim3(256), 0, s, a.part_out,
+                     a.part_stats, out, stats, z.q_rows(), a.parts, head_dim, dp);
   return MNV_LAUNCH_STATUS();
 }
 

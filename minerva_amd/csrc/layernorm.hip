@@ -3,10 +3,14 @@
 //   dx = r * (g - mean(g) - xh * mean(g * xh)), g = gamma * dy;  dgamma = sum dy * xh;  dbeta = sum dy
 // The variance is the mean of squared differences from the mean (two passes over a column), never a
 // difference of squares, so a large mean costs no digits.
-// Roofline: HBM bandwidth, 8 bytes per element forward and 12 backward: a column of up to
-// 16384 values is held in registers between the passes, so it is read once.  backward sums dgamma and dbeta in
-// registers over the columns of a group of threads, each thread its own features, and leaves one partial sum per
-// workgroup to a second kernel.
+// Bound by HBM, 8 bytes per element forward and 12 backward: a column of up to 16384 values is held in registers
+// between the passes, so it is read once, by as few threads as hold it with 4 to 16 values each (16 lanes to 64 features,
+// 512 threads to 8192), and a group of threads goes from column to column.  backward sums dgamma and dbeta in
+// registers over the columns of a group, each thread its own features, and leaves one partial sum per
+// workgroup to a second kernel.  4096 x 8192 forward: 40.6 us again and again on the same 268 MB, which the
+// caches partly hold, 49.7 us on other data from call to call = 5.4 TB/s (a large copy: 4.7, an addition 5.9); backward of
+// 512 x 65536: 64.5 us and 6 for the second kernel, 78.5 us on other data = 5.1 TB/s; 999 x 4099: 14.4 and 4 us.
+// Small ones are a launch (256 x 4: 1.7 us).
 #include <math.h>
 
 #include "mnv_common.h"
@@ -170,8 +174,8 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
   c.template load<VEC, false>(g, gamma);
 #pragma unroll
   for (int u = 0; u < CACHE; ++u) sg[u] = sb[u] = mnv_f4{0.f, 0.f, 0.f, 0.f};
-  // the next column is fetched while this one is summed (behind the last that one again); of wider ones it costs registers that
-  // more workgroups to a CU use better (4096 x 8192: 85 us with, 80 without; 8192 x 1000: 38 and 32)
+  // the next column is fetched while this one is summed (behind the last that one again); of wider ones it costs
+  // registers that more workgroups to a CU use better (4096 x 8192: 85 us with, 80 without; 8192 x 1000: 38 and 32)
   constexpr bool AHEAD = CACHE <= 2;
   mnv_f4 next_x[CACHE], next_d[CACHE];
   const unsigned first = blockIdx.x * PER + (PER > 1 ? threadIdx.x / GROUP : 0), step = gridDim.x * PER;
@@ -384,7 +388,8 @@ int run(const Norm& n) {
                          n.x, n.gamma, n.beta, n.y, n.features, n.count, n.eps);
     return MNV_LAUNCH_STATUS();
   }
-  // past the caches: 8192 x 16384 forward 176 us, 188 through them; backward 304 and 328.  4096 x 8192 fits them: 41, and 49 past them
+  // past the caches: 8192 x 16384 forward 176 us, 188 through them; backward 304 and 328.  4096 x 8192 fits them: 41 us,
+  // and 49 past them
   const bool vec = n.features % 4 == 0, nt = (size_t)n.features * n.count * sizeof(float) >= MNV_PAST_CACHE_BYTES;
   if (vec) return nt ? by_width<true, true>(n) : by_width<true, false>(n);
   return nt ? by_width<false, true>(n) : by_width<false, false>(n);
