@@ -428,7 +428,7 @@ int mnv_layernorm_bwd(const float* x, const float* gamma, const float* dy, float
  * ds along the diagonals of every 32 keys, of at most 256 MiB of them at a time (or one entry's and key head's, if
  * that is more).  With less of it fewer parts run; with too little for the diagonals of one entry and key head,
  * dbias is made of scores that are computed once more, one by one, which is far slower.  The order of all sums
- * is set by the sizes, the workspace's size and the device's number of compute units. ---- */
+ * is set by the sizes, whether there are lengths, the workspace's size and the device's number of compute units. ---- */
 size_t mnv_attention_fwd_workspace_bytes(int batch, int heads, int kv_heads, int q_len, int k_len,
                                          int head_dim);
 int mnv_attention_fwd(const float* q, const float* k, const float* v, const float* bias,
