@@ -56,8 +56,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
   __shared__ __align__(16) float row_stats[2][3][32];  // m, 1 / l, delta of the tile's queries
   __shared__ float turned[BIAS ? 4 * 16 * 48 : 1];
   const AttentionSizes& z = a.z;
-  const MnvAttentionPlace place = mnv_attention_place(a.tiles * a.splits, a.first_pair, z, a.lengths);
-  const int split = mnv_uniform(place.tile / a.tiles), tile = place.tile - split * a.tiles;
+  const MnvAttentionPlace place =
+      mnv_attention_place(a.tiles * a.splits, a.splits, DP <= 64 ? 128 : 0, a.first_pair, z, a.lengths);
+  const int tile = mnv_uniform(place.tile / a.splits), split = place.tile - tile * a.splits;
   const int b = place.b, kh = place.kh, n = place.n, group = z.group();
   const int q_tiles = (z.q_len + 31) / 32, begin = split * a.chunk;
   const int end = begin + a.chunk < group * q_tiles ? begin + a.chunk : group * q_tiles;
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
   using Stage = MnvStage<DP, 256, VEC>;  // keys and values
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
-  const MnvAttentionPlace place = mnv_attention_place(a.tiles * a.splits, 0, z, a.lengths);
+  const MnvAttentionPlace place = mnv_attention_place(a.tiles * a.splits, 0, 0, 0, z, a.lengths);
   const int split = mnv_uniform(place.tile / a.tiles), tile = place.tile - split * a.tiles, b = place.b, kh = place.kh;
   // the part's keys
   const int begin = split * a.chunk * 32, n = place.n < begin + a.chunk * 32 ? place.n : begin + a.chunk * 32;

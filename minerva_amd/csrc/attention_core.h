@@ -81,20 +81,53 @@ __device__ __forceinline__ int mnv_visible(const float* lengths, int b, int k_le
 
 // The workgroup's place.  Workgroups go to the 8 dies in turn: all of one entry and key head go to one die, whose
 // L2 then holds the keys they share, and neighbouring heads to different ones, so that entries of different lengths
-// load all dies alike.
+// load all dies alike.  `keys`: of a pair's `tiles` workgroups the first `each` have to do with its first `keys` keys, and so
+// on, and those without keys go behind all others of the die; 0: in the pairs' order.  They end at once, but in between
+// they take their turns in the order in which CUs are given a second workgroup, while others have none (dk and dv and the rest of
+// the backward pass of 8 x 12 heads of 512 x 512, lengths 64 to 512, where 240 of 384 workgroups have keys: 131 us, 151
+// in the pairs' order; 16 x 16 heads of 1024 x 1024, 64 to 1024: 707 and 744; 128 wide, one workgroup to a CU: 482 and 454).
 struct MnvAttentionPlace {
   int tile, b, kh;
   unsigned pair;  // entry and key head, from the launch's first on
   int n;          // keys of the entry
 };
-__device__ __forceinline__ MnvAttentionPlace mnv_attention_place(unsigned tiles, unsigned first_pair,
+__device__ __forceinline__ MnvAttentionPlace mnv_attention_place(unsigned tiles, unsigned each, int keys, unsigned first_pair,
                                                                  const AttentionSizes& z, const float* lengths) {
   MnvAttentionPlace p;
-  const unsigned even = gridDim.x / tiles / 8 * 8 * tiles;  // workgroups of the pairs that fill all dies
-  if (blockIdx.x < even) {
-    const unsigned row = mnv_uniform(blockIdx.x / 8 / tiles);
-    p.pair = row * 8 + blockIdx.x % 8;
-    p.tile = blockIdx.x / 8 - row * tiles;
+  const unsigned rows = gridDim.x / tiles / 8;  // pairs of each die, but for the last few
+  if (blockIdx.x < rows * 8 * tiles) {
+    unsigned at = blockIdx.x / 8, row = at / tiles;
+    at -= row * tiles;
+    if (keys && lengths && rows > 1 && rows <= MNV_WAVE) {
+      const unsigned lane = threadIdx.x % MNV_WAVE;
+      unsigned mine = 0;  // workgroups of the lane's pair that have keys
+      if (lane < rows) {
+        const int n = mnv_visible(lengths, (first_pair + lane * 8 + blockIdx.x % 8) / z.kv_heads, z.k_len);
+        const unsigned steps = ((unsigned)n + keys - 1) / keys;
+        mine = steps < tiles / each ? steps * each : tiles;
+      }
+      unsigned before = mine;  // of the pairs up to the lane's
+#pragma unroll
+      for (int o = 1; o < MNV_WAVE; o <<= 1) {
+        const unsigned t = __shfl_up(before, o, MNV_WAVE);
+        if (lane >= (unsigned)o) before += t;
+      }
+      const unsigned all = __shfl(before, MNV_WAVE - 1, MNV_WAVE);
+      unsigned index = blockIdx.x / 8;
+      const bool none = index >= all;  // one of those without keys
+      if (none) {
+        index -= all;
+        before = (lane + 1) * tiles - before;
+        mine = tiles - mine;
+      }
+      const unsigned long long reached = __ballot(lane < rows && before > index);
+      row = __ffsll(reached) - 1;
+      const unsigned in = __shfl(mine, row, MNV_WAVE);
+      at = index - (__shfl(before, row, MNV_WAVE) - in);
+      if (none) at += tiles - in;  // behind those with keys
+    }
+    p.pair = mnv_uniform(row) * 8 + blockIdx.x % 8;
+    p.tile = mnv_uniform(at);
   } else {
     p.pair = mnv_uniform(blockIdx.x / tiles);
     p.tile = blockIdx.x - p.pair * tiles;

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW == 4 ? 1 : 2) void mnv_atten
   using Stage = MnvStage<DP, 64 * NW, VEC>;
   __shared__ __align__(16) char lds[2 * Stage::BYTES];
   const AttentionSizes& z = a.z;
-  const MnvAttentionPlace place = mnv_attention_place(a.row_tiles * a.parts, 0, z, a.lengths);
+  const MnvAttentionPlace place = mnv_attention_place(a.row_tiles * a.parts, 0, 0, 0, z, a.lengths);
   const int part = mnv_uniform(place.tile / a.row_tiles), tile = place.tile - part * a.row_tiles, b = place.b, kh = place.kh;
   // the part's keys
   const int begin = part * a.chunk, n = place.n < begin + a.chunk ? place.n : begin + a.chunk;

@@ -20,19 +20,19 @@ def gpu():
 
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("sizes", [(1, 11, 11, 70, 90, 64), (5, 4, 2, 150, 140, 128), (9, 2, 1, 33, 260, 32), (3, 3, 3, 300, 20, 96),
-                                   (17, 1, 1, 1, 400, 64)])
+                                   (17, 1, 1, 1, 400, 64), (5, 8, 4, 20, 500, 64), (33, 2, 2, 40, 300, 40), (130, 4, 4, 3, 140, 32)])
 def test_pairs_that_fill_no_round_of_the_dies(gpu, sizes, bias):
     lengths = [(37 * b) % (sizes[4] + 1) for b in range(sizes[0])]
     check(gpu, Case(*sizes, bias=bias, lengths=lengths))
 
 
-@pytest.mark.parametrize("pairs", [1, 2, 4, 5])
-@pytest.mark.parametrize("sizes", [(3, 6, 2, 40, 300, 64), (2, 4, 4, 130, 77, 100), (5, 3, 1, 1, 65, 32)])
+@pytest.mark.parametrize("sizes,pairs", [(z, n) for z in [(3, 6, 2, 40, 300, 64), (2, 4, 4, 130, 77, 100), (5, 3, 1, 1, 65, 32)]
+                                         for n in (1, 2, 4, 5)] + [((6, 8, 4, 20, 300, 64), n) for n in (16, 17, 23)])
 def test_diagonals_of_some_pairs_at_a_time(gpu, sizes, pairs):
     """A workspace that holds the diagonals' sums of `pairs` pairs of an entry and a key head, and a little more."""
     batch, heads, kv_heads, q_len, k_len, _ = sizes
     each = heads // kv_heads * -(-k_len // 32) * (-(-q_len // 32) * 32 + 32) * 4
-    c = Case(*sizes, bias=True, lengths=[k_len - 7 * b for b in range(batch)])
+    c = Case(*sizes, bias=True, lengths=[k_len * (b + 1) // batch for b in range(batch)])
     check(gpu, c, workspace=each * pairs)
     check(gpu, c, workspace=each * pairs + 20)
 
