@@ -10,7 +10,7 @@
 // Bound by the matrix cores, 7 products of 6 instructions per value: 2 x 16 heads (4 key heads) of 2048 x 4096, 128 wide: dk and dv
 // 1.28 ms (215 TFLOP/s of its 4 fp32 products, cores busy 67%), dq 1.07 ms (193 of its 3, 60%); the clock is 1.9 GHz
 // under such work.  The rest waits for LDS at the products' starts, and for vector work between dout v and dq.  8 x 16
-// heads of 512 x 1024, 64 wide, lengths 128 to 1024: 144 and 104 us, and 8 for delta.
+// heads of 512 x 1024, 64 wide, lengths 128 to 1024: 136 and 104 us, and 8 for delta.
 #include "attention_core.h"
 
 namespace {

@@ -353,8 +353,11 @@ int parts(const AttentionSizes& z, bool lengths, size_t workspace_bytes) {
   // workgroups that a CU holds, by LDS (129 x 1500, 64 wide: 32.7 us, 35.7 with two; over 64 wide 28 us of 16 heads for one
   // query over 2000 keys, 33 with two)
   const size_t places = (size_t)mnv_cu_count() * (z.dim <= 64 ? 3 : 1);
+  // Where every CU has a workgroup anyway, parts of less than 512 keys cost more to join than they even out (8 x 12 heads of 512 x
+  // 512: 51 us in two parts, 47 in one; of 384 x 1024: 74 and 80; 32 heads for each of 9 queries over 4000 keys: 127 and 191).
+  const size_t least = blocks > (size_t)mnv_cu_count() ? 16 : 2;
   const auto fill = [&](size_t n) {
-    return mnv_attention_parts(blocks, n, mnv_ceil_div(z.k_len, 32), 2, part_bytes(z), workspace_bytes);
+    return mnv_attention_parts(blocks, n, mnv_ceil_div(z.k_len, 32), least, part_bytes(z), workspace_bytes);
   };
   // Of parts behind an entry's keys nothing is left to do, so where there are lengths twice as many even out the
   // rest (12 heads of 129 queries, 6 entries of 0 to 1500 keys: 43 us -> 35); not where there would be one
