@@ -11,11 +11,28 @@ void Ok(int status, const char* what) {
   MNV_CHECK(status == MNV_OK) << what << ": " << mnv_error_string(status);
 }
 
+// The extents that say how values lie in memory: without those that are 1.
+std::vector<int> Layout(const std::vector<int>& dims) {
+  std::vector<int> r;
+  for (int d : dims)
+    if (d != 1) r.push_back(d);
+  return r;
+}
+// Whether s holds values in the order of `dims`: with these extents, or flat.
+bool LiesAs(const Scale& s, const std::vector<int>& dims) {
+  const std::vector<int> have = Layout(s.ToVector());
+  long long all = 1;
+  for (int d : dims) all *= d;
+  return have == Layout(dims) || (have.size() == 1 && have[0] == all);
+}
+
 // {features, count}: the last dimension counts the columns.
 int Columns(const Scale& s) {
   MNV_CHECK(s.NumDims() >= 2) << "(layer norm) takes features and columns";
   return s[s.NumDims() - 1];
 }
+// A value per feature, in a column's order.
+bool PerFeature(const Scale& s, const Scale& x) { return LiesAs(s, std::vector<int>(x.begin(), x.end() - 1)); }
 
 struct AttentionExtents {
   int head_dim, heads, q_len, batch, kv_heads, k_len;
@@ -37,13 +54,14 @@ AttentionExtents Extents(const char* what, const DataList& inputs, size_t fixed,
   e.k_len = k[2];
   if (has_bias) {
     const DataShard& b = inputs[fixed];
-    MNV_CHECK_EQ(static_cast<long long>(b.size_.Prod()), (static_cast<long long>(e.q_len) + e.k_len - 1) * e.heads)
-        << "(" << what << ") bias is {q_len + k_len - 1, heads}";
+    const long long offsets = static_cast<long long>(e.q_len) + e.k_len - 1;
+    MNV_CHECK(offsets <= 0x7fffffffLL && LiesAs(b.size_, {static_cast<int>(offsets), e.heads}))
+        << "(" << what << ") bias is {q_len + k_len - 1, heads}, not " << b.size_;
     e.bias = b.data_;
   }
   if (has_lengths) {
     const DataShard& l = inputs[fixed + has_bias];
-    MNV_CHECK_EQ(l.size_.Prod(), e.batch) << "(" << what << ") lengths has one value per entry of the batch";
+    MNV_CHECK(LiesAs(l.size_, {e.batch})) << "(" << what << ") lengths has one value per entry of the batch, not " << l.size_;
     e.lengths = l.data_;
   }
   return e;
@@ -55,8 +73,8 @@ void LayerNormForward(const DataList& inputs, const DataList& outputs, LayerNorm
   MNV_CHECK_EQ(inputs.size(), 3u) << "(layer norm forward) #inputs wrong";
   MNV_CHECK_EQ(outputs.size(), 1u) << "(layer norm forward) #outputs wrong";
   const int count = Columns(inputs[0].size_), features = inputs[0].size_.Prod() / count;
-  MNV_CHECK_EQ(inputs[1].size_.Prod(), features) << "(layer norm forward) gain has one value per feature";
-  MNV_CHECK_EQ(inputs[2].size_.Prod(), features) << "(layer norm forward) offset has one value per feature";
+  MNV_CHECK(PerFeature(inputs[1].size_, inputs[0].size_)) << "(layer norm forward) gain has one value per feature";
+  MNV_CHECK(PerFeature(inputs[2].size_, inputs[0].size_)) << "(layer norm forward) offset has one value per feature";
   Ok(mnv_layernorm_fwd(inputs[0].data_, inputs[1].data_, inputs[2].data_, outputs[0].data_, features, count, c.eps,
                        ctx.stream),
      "layer norm forward");
@@ -70,7 +88,7 @@ void LayerNormBackward(const DataList& inputs, const DataList& outputs, LayerNor
   const auto& gamma = inputs[2];
   const int count = Columns(x.size_), features = x.size_.Prod() / count;
   MNV_CHECK(diff.size_ == x.size_) << "(layer norm backward) extents differ";
-  MNV_CHECK_EQ(gamma.size_.Prod(), features) << "(layer norm backward) gain has one value per feature";
+  MNV_CHECK(PerFeature(gamma.size_, x.size_)) << "(layer norm backward) gain has one value per feature";
   Ok(mnv_layernorm_bwd(x.data_, gamma.data_, diff.data_, outputs[0].data_, outputs[1].data_, outputs[2].data_, features,
                        count, c.eps, ctx.workspace, ctx.workspace_bytes, ctx.stream),
      "layer norm backward");
@@ -94,8 +112,8 @@ void AttentionBackward(const DataList& inputs, const DataList& outputs, Attentio
                                      c.has_bias, c.has_lengths);
   MNV_CHECK(inputs[0].size_ == inputs[1].size_ && inputs[4].size_ == inputs[1].size_)
       << "(attention backward) queries', results' and gradients' extents differ";
-  MNV_CHECK_EQ(static_cast<long long>(inputs[5].size_.Prod()), 2ll * e.heads * e.q_len * e.batch)
-      << "(attention backward) stats are {2, heads, q_len, batch}";
+  MNV_CHECK(LiesAs(inputs[5].size_, {2, e.heads, e.q_len, e.batch}))
+      << "(attention backward) stats are {2, heads, q_len, batch}, not " << inputs[5].size_;
   Ok(mnv_attention_bwd(inputs[1].data_, inputs[2].data_, inputs[3].data_, e.bias, e.lengths, inputs[4].data_,
                        inputs[5].data_, inputs[0].data_, outputs[0].data_, outputs[1].data_, outputs[2].data_,
                        c.has_bias ? outputs[3].data_ : nullptr, e.batch, e.heads, e.kv_heads, e.q_len, e.k_len, e.head_dim,
