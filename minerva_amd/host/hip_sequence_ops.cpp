@@ -29,6 +29,7 @@ bool LiesAs(const Scale& s, const std::vector<int>& dims) {
 // {features, count}: the last dimension counts the columns.
 int Columns(const Scale& s) {
   MNV_CHECK(s.NumDims() >= 2) << "(layer norm) takes features and columns";
+  MNV_CHECK(s.Prod() > 0) << "(layer norm) of an empty array " << s;
   return s[s.NumDims() - 1];
 }
 // A value per feature, in a column's order.

@@ -1,6 +1,6 @@
 // CPU test of what the operators of networks over sequences ask of their arrays' extents
 // (minerva_amd/host/hip_sequence_ops.cpp), with entry points that only count the calls that reach them.
-// usage: sequence_extents_test mixed.  Prints "OK" and exits 0 when every check holds.
+// usage: sequence_extents_test mixed | empty.  Prints "OK" and exits 0 when every check holds.
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -94,8 +94,19 @@ static void Mixed() {
   }
 }
 
+// Of an array without values nothing is divided by its number of columns.
+static void Empty() {
+  for (const Scale& x : {Scale{4, 0}, Scale{0, 4}, Scale{0, 0}}) {
+    LayerNormForwardClosure n{1e-5f};
+    Expect(false, hip::LayerNormForward, n, {x, Scale{4}, Scale{4}}, {x}, "norm of an empty array");
+    LayerNormBackwardClosure nb{1e-5f};
+    Expect(false, hip::LayerNormBackward, nb, {x, x, Scale{4}}, {x, Scale{4}, Scale{4}}, "norm of an empty array, backward");
+  }
+}
+
 int main(int argc, char** argv) {
   if (argc == 2 && !std::strcmp(argv[1], "mixed")) Mixed();
+  else if (argc == 2 && !std::strcmp(argv[1], "empty")) Empty();
   else return 2;
   if (g_failed) return 1;
   std::printf("OK\n");

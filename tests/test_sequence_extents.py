@@ -19,7 +19,7 @@ def program(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("what", ["mixed"])
+@pytest.mark.parametrize("what", ["mixed", "empty"])
 def test_extents(program, what):
     run = subprocess.run([program, what], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and run.stdout.strip() == "OK", (run.returncode, run.stdout + run.stderr)
