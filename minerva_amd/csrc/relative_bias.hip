@@ -24,6 +24,36 @@ struct RelativeBuckets {
   int offsets;
 };
 
+// A whole number of 32 bits to a word, the lowest first, for products of powers.
+struct WholeNumber {
+  unsigned words[MNV_RB_MAX_BUCKETS / 2 + 2] = {1};  // of up to 128 factors below 2^31
+  int used = 1;
+  void times(unsigned x) {
+    unsigned long long carry = 0;
+    for (int i = 0; i < used; ++i) {
+      carry += (unsigned long long)words[i] * x;
+      words[i] = (unsigned)carry;
+      carry >>= 32;
+    }
+    if (carry) words[used++] = (unsigned)carry;
+  }
+  bool at_least(const WholeNumber& o) const {
+    if (used != o.used) return used > o.used;
+    for (int i = used; i-- > 0;)
+      if (words[i] != o.words[i]) return words[i] > o.words[i];
+    return true;
+  }
+};
+// Whether n >= exact * (max_distance / exact)^(u / steps), as powers: n^steps >= max_distance^u exact^(steps - u).
+bool reaches_border(int n, int exact, int max_distance, int u, int steps) {
+  WholeNumber a, b;
+  for (int i = 0; i < steps; ++i) {
+    a.times((unsigned)n);
+    b.times((unsigned)(i < u ? max_distance : exact));
+  }
+  return a.at_least(b);
+}
+
 // Fills b; false for arguments that the header does not allow.
 bool make_buckets(RelativeBuckets* b, int buckets, int heads, int q_len, int k_len, int q_start,
                   int max_distance, int both_ways) {
@@ -38,9 +68,12 @@ bool make_buckets(RelativeBuckets* b, int buckets, int heads, int q_len, int k_l
   for (int u = 0; u <= exact; ++u) b->from[u] = u;
   for (int u = 1; u < steps; ++u) {
     const double at = exact * pow((double)max_distance / exact, (double)u / steps);
-    // a border that is a whole number but for the rounding of pow belongs to the bucket above it
+    // next to a whole number, where the rounding of pow could put it on either side, whole numbers decide
     const double whole = rint(at);
-    b->from[exact + u] = (int)(fabs(at - whole) <= 1e-12 * at ? whole : ceil(at));
+    if (fabs(at - whole) <= 1e-12 * at)
+      b->from[exact + u] = (int)whole + (reaches_border((int)whole, exact, max_distance, u, steps) ? 0 : 1);
+    else
+      b->from[exact + u] = (int)ceil(at);
   }
   b->from[b->each] = 0x7fffffff;
   b->offsets = (int)offsets;
