@@ -76,7 +76,9 @@ __device__ __forceinline__ int mnv_visible(const float* lengths, int b, int k_le
   if (!lengths) return k_len;
   const float n = lengths[b];
   if (!(n > 0.f)) return 0;
-  return n >= (float)k_len ? k_len : (int)n;
+  if (n >= (float)MNV_AT_MAX_ROWS) return k_len;
+  // compared as whole numbers: k_len past 2^24 need not be one that fp32 holds
+  return (int)n < k_len ? (int)n : k_len;
 }
 
 // The workgroup's place.  Workgroups go to the 8 dies in turn: all of one entry and key head go to one die, whose
