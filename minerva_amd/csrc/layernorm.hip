@@ -2,7 +2,9 @@
 //   xh = (x - mean) * r, r = 1 / sqrt(var + eps);  y = gamma * xh + beta
 //   dx = r * (g - mean(g) - xh * mean(g * xh)), g = gamma * dy;  dgamma = sum dy * xh;  dbeta = sum dy
 // The variance is the mean of squared differences from the mean (two passes over a column), never a
-// difference of squares, so a large mean costs no digits.
+// difference of squares.  A mean in fp32 is off by up to half a step of its own size and a sum's roundings, far more than the
+// values' differences may bear (mean 10^5, deviation 1: results off by 0.05, those of a constant column by 1), but the
+// differences from it are exact where it is large; so their own mean is summed with their squares, and taken off.
 // Bound by HBM, 8 bytes per element forward and 12 backward: a column of up to 16384 values is held in registers
 // between the passes, so it is read once, by as few threads as hold it with 4 to 16 values each (16 lanes to 64 features,
 // 512 threads to 8192), and a group of threads goes from column to column.  backward sums dgamma and dbeta in
@@ -92,11 +94,17 @@ __device__ __forceinline__ void store4(float* p, int left, mnv_f4 v) {
   if (left > 2) p[2] = v.z;
 }
 
+// 1 / sqrt(var + eps) from the mean of squared differences from a mean that is off by d, the differences' own mean.
+__device__ __forceinline__ float inverse_deviation(float squares, float d, float eps) {
+  const float var = squares - d * d;
+  return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);
+}
+
 // One column per GROUP threads of a workgroup, CACHE vectors of four values per thread.
 template <int GROUP, int CACHE>
 struct Column {
   mnv_f4 x[CACHE];
-  float mean, r;
+  float r;
   int t, features;  // the thread's first feature, and the number of all
 
   __device__ __forceinline__ int left(int u) const { return features - (t + 4 * u * GROUP); }
@@ -111,16 +119,23 @@ struct Column {
     float s = 0.f;
 #pragma unroll
     for (int u = 0; u < CACHE; ++u) s += (x[u].x + x[u].y) + (x[u].z + x[u].w);
-    mean = group_sum<GROUP>(s, lds) / features;
-    s = 0.f;
+    const float mean = group_sum<GROUP>(s, lds) / features;
+    float d = 0.f, sq = 0.f;
 #pragma unroll
     for (int u = 0; u < CACHE; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[u][e] = left(u) > e ? x[u][e] - mean : 0.f;
-        s = fmaf(x[u][e], x[u][e], s);
+        d += x[u][e];
+        sq = fmaf(x[u][e], x[u][e], sq);
       }
-    r = 1.f / sqrtf(group_sum<GROUP>(s, lds) / features + eps);
+    group_sum2<GROUP>(d, sq, lds);
+    d /= features;
+    r = inverse_deviation(sq / features, d, eps);
+#pragma unroll
+    for (int u = 0; u < CACHE; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[u][e] = left(u) > e ? x[u][e] - d : 0.f;
   }
 };
 
@@ -128,7 +143,7 @@ template <int GROUP, int CACHE, int NTH, bool VEC, bool NT>
 __global__ __launch_bounds__(NTH) void mnv_layernorm_fwd_kernel(const float* __restrict__ x, const float* __restrict__ gamma,
                                                                 const float* __restrict__ beta, float* __restrict__ y,
                                                                 int features, unsigned count, float eps) {
-  __shared__ float lds[GROUP > MNV_WAVE ? NTH / MNV_WAVE : 1];
+  __shared__ float lds[GROUP > MNV_WAVE ? 2 * NTH / MNV_WAVE : 1];
   constexpr int PER = NTH / GROUP;
   Column<GROUP, CACHE> c;
   c.t = threadIdx.x % GROUP * 4;
@@ -250,27 +265,36 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
 
 // Columns of more values than the register forms hold: each pass reads the column again.
 #define MNV_LN_WIDE 1024
-__device__ __forceinline__ void wide_stats(const float* x, unsigned features, float eps, float* lds, float* mean, float* r) {
+// A column's mean is a first one and the mean of the differences from it.
+struct WideStats {
+  float mean, rest, r;
+  __device__ __forceinline__ float xh(float x) const { return (x - mean - rest) * r; }
+};
+__device__ __forceinline__ WideStats wide_stats(const float* x, unsigned features, float eps, float* lds) {  // lds: 2 floats per wavefront
+  WideStats w;
   float s = 0.f;
   for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) s += x[f];
-  *mean = group_sum<MNV_LN_WIDE>(s, lds) / features;
-  s = 0.f;
+  w.mean = group_sum<MNV_LN_WIDE>(s, lds) / features;
+  float sum = 0.f, sq = 0.f;
   for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
-    const float d = x[f] - *mean;
-    s = fmaf(d, d, s);
+    const float d = x[f] - w.mean;
+    sum += d;
+    sq = fmaf(d, d, sq);
   }
-  *r = 1.f / sqrtf(group_sum<MNV_LN_WIDE>(s, lds) / features + eps);
+  group_sum2<MNV_LN_WIDE>(sum, sq, lds);
+  w.rest = sum / features;
+  w.r = inverse_deviation(sq / features, w.rest, eps);
+  return w;
 }
 __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_fwd_wide_kernel(
     const float* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, float* __restrict__ y,
     unsigned features, unsigned count, float eps) {
-  __shared__ float lds[MNV_LN_WIDE / MNV_WAVE];
+  __shared__ float lds[2 * MNV_LN_WIDE / MNV_WAVE];
   for (unsigned i = blockIdx.x; i < count; i += gridDim.x) {
     const float* xc = x + (size_t)i * features;
     float* yc = y + (size_t)i * features;
-    float mean, r;
-    wide_stats(xc, features, eps, lds, &mean, &r);
-    for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) yc[f] = gamma[f] * ((xc[f] - mean) * r) + beta[f];
+    const WideStats w = wide_stats(xc, features, eps, lds);
+    for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) yc[f] = gamma[f] * w.xh(xc[f]) + beta[f];
   }
 }
 __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_bwd_wide_kernel(
@@ -284,19 +308,19 @@ __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_bwd_wide_kernel(
     const float* xc = x + (size_t)i * features;
     const float* dyc = dy + (size_t)i * features;
     float* dxc = dx + (size_t)i * features;
-    float mean, r, s = 0.f, sx = 0.f;
-    wide_stats(xc, features, eps, lds, &mean, &r);
+    const WideStats w = wide_stats(xc, features, eps, lds);
+    float s = 0.f, sx = 0.f;
     for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
       const float gd = gamma[f] * dyc[f];
       s += gd;
-      sx = fmaf(gd, (xc[f] - mean) * r, sx);
+      sx = fmaf(gd, w.xh(xc[f]), sx);
     }
     group_sum2<MNV_LN_WIDE>(s, sx, lds);
     s /= features;
     sx /= features;
     for (unsigned f = threadIdx.x; f < features; f += MNV_LN_WIDE) {
-      const float d = dyc[f], xh = (xc[f] - mean) * r;
-      dxc[f] = r * (gamma[f] * d - s - xh * sx);
+      const float d = dyc[f], xh = w.xh(xc[f]);
+      dxc[f] = w.r * (gamma[f] * d - s - xh * sx);
       pg[f] = fmaf(d, xh, pg[f]);  // each thread has its own features throughout
       pb[f] += d;
     }
