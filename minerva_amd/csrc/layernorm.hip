@@ -422,8 +422,13 @@ int run(const Norm& n) {
 // Workgroups of the backward pass: 3 or 2 to a CU are enough to keep the memory busy, and leave fewer partial sums (512 x
 // 65536: 69 us, of 8 to a CU 77; 4096 x 8192: 69, of 4 to a CU 78), and fewer of them where a group would have few
 // columns to its sums (2048 x 1000: 14.0 us of two columns or more, 12.7 of four; 64 x 100: 8.1 and 8.6).
+// Of very many columns there are more of them, so that no sum of a thread has more than MNV_LN_CHAIN terms (2^28 columns of one
+// feature, gradients of 1.1, whose additions all round the same way: dbeta off by 1.1e-5, 2.1e-4 with 21845 in a row).
+#define MNV_LN_CHAIN 1024
 unsigned bwd_workgroups(int features, int count) {
-  const size_t most = (size_t)mnv_cu_count() * (features <= 512 ? 3 : 2);
+  const size_t full = (size_t)mnv_cu_count() * (features <= 512 ? 3 : 2);
+  const size_t chains = mnv_ceil_div(count, (size_t)columns_at_once(features) * MNV_LN_CHAIN);
+  const size_t most = full > chains ? full : chains;
   const size_t groups = mnv_ceil_div(count, (size_t)columns_at_once(features) * (features <= 512 ? 2 : 4));
   return (unsigned)(groups < most ? groups : most);
 }
