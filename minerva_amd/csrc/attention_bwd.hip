@@ -125,11 +125,13 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
           next.delta = a.dq[row * z.dim];
         }
       };
+      // 1 / l is 0 for a row that sees no key, and -0 behind the last row
       auto store_rows = [&](const Rows& next, int i0, int turn) __attribute__((always_inline)) {
         if (threadIdx.x < 32) {
+          const float il = i0 + (int)threadIdx.x < z.q_len ? mnv_inverse(next.l) : -0.f;
           row_stats[turn][0][threadIdx.x] = mnv_finite_max(next.m);
-          row_stats[turn][1][threadIdx.x] = i0 + (int)threadIdx.x < z.q_len ? mnv_inverse(next.l) : 0.f;
-          row_stats[turn][2][threadIdx.x] = next.delta;
+          row_stats[turn][1][threadIdx.x] = il;
+          row_stats[turn][2][threadIdx.x] = il == 0.f ? 0.f : next.delta;
         }
       };
       // Behind the last tile comes that one again: no branch parts a tile's work.
@@ -152,6 +154,16 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
         fetch_rows(next, more ? i0 + 32 : last);
         const int i2 = i0 + 64 < last ? i0 + 64 : last;
         const char* now = lds + turn * Stage::BYTES;
+        // Rows of the tile that see no key, since the bias hides all: their weights are 0, their gradients may hold anything, and
+        // leave LDS before the two meet.  All wavefronts see the same rows.
+        if (BIAS && __builtin_expect(__any(__builtin_bit_cast(unsigned, row_stats[turn][1][lane % 32]) == 0), 0)) {
+          char* planes = lds + turn * Stage::BYTES + Stage::MATRIX;
+          const int row = threadIdx.x / 8;
+          if (row_stats[turn][1][row] == 0.f)
+            for (int at = threadIdx.x % 8 * 8; at < 3 * Stage::PITCH; at += 64)
+              *reinterpret_cast<mnv_u2*>(planes + at / Stage::PITCH * Stage::PLANE + row * Stage::PITCH + at % Stage::PITCH) = mnv_u2{0, 0};
+          __syncthreads();
+        }
         mnv_f4 add[4];
         if (BIAS) {
           if (i0 + 32 <= z.q_len) {
@@ -326,6 +338,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
 #pragma unroll
     for (int e = 0; e < 16; ++e) dq[c][e] = 0.f;
 
+  bool seen = false;
   if (n > begin) {
     MnvParts qp[KS], op[KS];
     float delta = 0.f;
@@ -345,6 +358,7 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
     }
     delta += __shfl_xor(delta, 32, MNV_WAVE);
     const float m = mnv_finite_max(a.stats[2 * row]), il = mnv_inverse(a.stats[2 * row + 1]);
+    seen = il != 0.f;  // else the row's gradient may hold anything, which weights of 0 do not hide
     const unsigned pitch = (unsigned)z.kv_heads * z.dim;
     const float* kb = a.k + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
     const float* vb = a.v + ((size_t)b * z.k_len * z.kv_heads + kh) * z.dim;
@@ -441,9 +455,9 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dq_kernel
   }
   if (r >= a.rows) return;
   if (a.splits == 1)
-    mnv_store_column<DP>(dq, z.scale, true, a.dq + row * z.dim, z.dim);
+    mnv_store_column<DP>(dq, z.scale, seen, a.dq + row * z.dim, z.dim);
   else if (n > begin)  // of a part without keys, nothing
-    mnv_store_column<DP>(dq, 1.f, true, a.sums + (split * z.q_rows() + row) * DP, DP);
+    mnv_store_column<DP>(dq, 1.f, seen, a.sums + (split * z.q_rows() + row) * DP, DP);
 }
 
 // out[row] = f * the sums of a row's parts, 0 for none; 16 lanes to a row.  blockIdx.y: dk and dv.  Of queries the parts that
@@ -540,11 +554,13 @@ __global__ __launch_bounds__(MNV_WAVE) void mnv_attention_dbias_alone_kernel(Bwd
         const int j = o + i - (z.q_len - 1);
         if (j < 0 || j >= n) continue;
         const size_t row = ((size_t)b * z.q_len + i) * z.heads + h;
+        const float il = mnv_inverse(a.stats[2 * row + 1]);
+        if (il == 0.f) continue;  // sees no key
         const float* kj = a.k + (((size_t)b * z.k_len + j) * z.kv_heads + kh) * z.dim;
         const float* vj = a.v + (((size_t)b * z.k_len + j) * z.kv_heads + kh) * z.dim;
         const float* oi = a.dout + row * z.dim;
         const float t = z.scale * dot(a.q + row * z.dim, kj, z.dim) + a.bias[at];
-        const float p = mnv_weight(t, mnv_finite_max(a.stats[2 * row])) * mnv_inverse(a.stats[2 * row + 1]);
+        const float p = mnv_weight(t, mnv_finite_max(a.stats[2 * row])) * il;
         sum += p * (dot(oi, vj, z.dim) - dot(oi, a.out + row * z.dim, z.dim));
       }
     }
