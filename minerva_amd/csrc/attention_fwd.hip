@@ -233,7 +233,8 @@ __global__ __launch_bounds__(64 * NW, DP > 64 && NW == 4 ? 1 : 2) void mnv_atten
     }
     return;
   }
-  mnv_store_column<DP>(acc, mnv_inverse(l), true, a.out + row * z.dim, z.dim);
+  // of a row that sees no key 0, and not 0 times what values hold that others see
+  mnv_store_column<DP>(acc, mnv_inverse(l), l != 0.f, a.out + row * z.dim, z.dim);
   if (half == 0) {
     a.stats[2 * row] = m;
     a.stats[2 * row + 1] = l;

@@ -34,3 +34,20 @@ def test_gradients_of_queries_that_the_bias_hides(gpu, sizes, workspace):
     for name in got:  # zeros of either sign are equal
         assert np.array_equal(got[name], clean[name]), name
     assert (got["dq"][:, blind, 1:] == 0).all()
+
+
+@pytest.mark.parametrize("workspace", [None, 0])
+@pytest.mark.parametrize("sizes", [(2, 2, 2, 40, 50, 64), (1, 2, 1, 33, 600, 64), (2, 32, 32, 260, 40, 128), (1, 3, 1, 5, 70, 33)])
+def test_results_of_queries_that_the_bias_hides(gpu, sizes, workspace):
+    """Values that are not finite reach the queries that see them, and no others."""
+    batch, heads, _, q_len, k_len, _ = sizes
+    c = Case(*sizes, bias=True)
+    hidden = min(max(1, q_len // 3), q_len - 1)
+    c.bias[:, :hidden - 1 + k_len] = -np.inf
+    blind = np.arange(q_len) > q_len - 1 - hidden
+    c.v[:, ::3, :, 1] = np.inf
+    c.v[:, 1::3, :, 2] = np.nan
+    got = Run(gpu, c, workspace=workspace).go()
+    assert (got["out"][:, blind] == 0).all() and (got["dq"][:, blind] == 0).all()
+    assert (got["stats"][:, blind] == [-np.inf, 0]).all()
+    assert np.isnan(got["out"][:, ~blind][..., 2]).any()
