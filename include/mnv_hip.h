@@ -421,7 +421,10 @@ int mnv_layernorm_bwd(const float* x, const float* gamma, const float* dy, float
  *   dbias[o] = sum of ds_ij with j - i + q_len - 1 = o over the batch
  * dk and dv sum over the heads that share a key, and are 0 for keys that are not read; dbias is
  * written unless `bias` is NULL (then dbias is ignored).  An infinity or a NaN among the values that are read
- * gives NaN where it has a part.  At most 2^26 rows of queries and of keys (over heads and batch),
+ * gives NaN where it has a part; a key that is hidden from a query by the bias alone is read for it, and may give it NaN, too.
+ * Finite values may have any size as long as scale * q, scale * k, the scores, ds and every sum (of
+ * exp(t_ij - m_i) v_j before it is divided, too) stay below 3.38e38; values are held to 2^-134, so those below 2^-110 lose
+ * digits, and weights below 2^-126 may be 0.  At most 2^26 rows of queries and of keys (over heads and batch),
  * 2^22 heads over the batch, heads * head_dim 2^24, and 2^31 - 1 values in each tensor.
  * A workspace is used if it is aligned to 16 bytes.  forward's holds the sums of parts of the key range,
  * where queries are too few to fill the chip; backward's the same of its loops, and (`has_bias`) the sums of
