@@ -591,8 +591,7 @@ BwdPlan make_plan(const AttentionSizes& z, bool has_bias, size_t workspace_bytes
     p.pairs = most / one;
     if (p.pairs == 0 && workspace_bytes >= one) p.pairs = 1;
     if (p.pairs > pairs) p.pairs = pairs;
-    p.diagonal_bytes = mnv_ceil_div(p.pairs * one, 16) * 16;
-    if (p.diagonal_bytes > workspace_bytes) p.diagonal_bytes = p.pairs * one;
+    p.diagonal_bytes = p.pairs * one;  // a multiple of 128
   }
   // One workgroup to a CU: more parts, where a CU holds two, cost more to add up than they save (2 x 8 heads of 200 x 1000, 32
   // wide: 32.7 us, 39.0 with two; 8 heads of 1 x 4096, 64 wide: 30.4 and 33.5).
