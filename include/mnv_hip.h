@@ -395,9 +395,10 @@ int mnv_lrn_bwd(const float* bottom, const float* top, const float* scale, const
  *   xh = (x - mean) / sqrt(var + eps),  y = gamma * xh + beta
  *   dx = (g - mean(g) - xh * mean(g * xh)) / sqrt(var + eps),  g = gamma * dy
  *   dgamma = sum over the columns of dy * xh,  dbeta = sum over the columns of dy
- * eps is finite and not negative.  backward works from x alone (nothing of the forward pass is kept).
+ * eps is finite and not negative, and the squares of a column's differences from its mean have a finite sum in fp32.
+ * backward works from x alone (nothing of the forward pass is kept).
  * Its workspace holds partial sums over columns; with less of it, or none, fewer workgroups run (one, for
- * none).  The order of the sums, and so the results' bits, is set by the sizes, the workspace's size and the
+ * none), and dgamma and dbeta sum more columns in a row (1024 to a thread at most with all of it).  The order of the sums, and so the results' bits, is set by the sizes, the workspace's size and the
  * device's number of compute units. ---- */
 int mnv_layernorm_fwd(const float* x, const float* gamma, const float* beta, float* y, int features,
                       int count, float eps, mnv_stream_t stream);

@@ -8,9 +8,12 @@
 // in one order: no atomics, and no partial gradients in memory unless the chip is empty otherwise.  delta waits in the
 // first value of each row of dq, which the last kernel overwrites, so no workspace is needed for it.
 // Bound by the matrix cores, 7 products of 6 instructions per value: 2 x 16 heads (4 key heads) of 2048 x 4096, 128 wide: dk and dv
-// 1.28 ms (215 TFLOP/s of its 4 fp32 products, cores busy 67%), dq 1.07 ms (193 of its 3, 60%); the clock is 1.9 GHz
-// under such work.  The rest waits for LDS at the products' starts, and for vector work between dout v and dq.  8 x 16
-// heads of 512 x 1024, 64 wide, lengths 128 to 1024: 136 and 104 us, and 8 for delta.
+// 1.24 to 1.29 ms (213 to 222 TFLOP/s of its 4 fp32 products, cores busy 66%), dq 1.00 to 1.07 ms (192 to 206 of its 3, 59%),
+// about 150 of the 5 that the algorithm needs; the clock is 1.9 GHz under such work.  The rest waits for LDS at the products'
+// starts, and for vector work between dout v and dq.  8 x 16 heads of 512 x 1024, 64 wide, lengths 128 to 1024: 137 and 106 us,
+// and 8 to 12 for delta.  Two workgroups to a CU leave the keys' kernel of 64 columns 256 registers, of which it has too
+// few: 27 (47 with a bias; 35 and 63 of odd widths) wait in scratch memory, 104 to 256 bytes a lane, in and out in every tile (8 x 16
+// heads of 512 x 1024: 81 MB written, of which 67 are results).  The other kernels of the backward pass keep theirs.
 #include "attention_core.h"
 
 namespace {
@@ -79,7 +82,8 @@ __global__ __launch_bounds__(256, DP <= 64 ? 2 : 1) void mnv_attention_dkv_kerne
     // The matrix instruction rounds its sums down, by up to a step of the larger of sum and terms: nothing to a
     // value, but of the same sign everywhere, and a bucket's gradient sums 10^5 ds that cancel.  So every other key's
     // products dout v are made with the opposite sign (12 heads of 512 x 512: the table's gradient off
-    // by 4.0e-6 without, 4.8e-7 with).
+    // by 4.0e-6 without, 4.8e-7 with).  The other products keep theirs: over 16384 keys, v and dout from a ReLU, out is
+    // off by 0.8e-7 and dv by 1.4e-7, in elementary fp32 operations by 3.4e-7 and 1.4e-7.
     const float sign = j % 2 ? -1.f : 1.f;
     MnvParts kp[KS], vp[KS];
 #pragma unroll

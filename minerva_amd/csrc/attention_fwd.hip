@@ -8,9 +8,10 @@
 // r / group, head r % group of the key head, so their keys are read and cut once.  Few rows over many keys are spread
 // over parts of the keys, which a second kernel joins.
 // Bound by the matrix cores where there are queries enough: 2 products of 6 instructions per value.  2 x 16 heads (4 key heads) of
-// 2048 x 4096, 128 wide: 0.63 ms = 219 TFLOP/s of fp32 products in calls back to back, cores busy 64% (the rest: the
-// first operands of each phase wait for LDS, the softmax between the phases); a large fp32 product of the
-// library reaches 153.  8 x 16 heads of 512 x 1024, 64 wide, lengths 128 to 1024: 79 us, the longest entry's workgroups.
+// 2048 x 4096, 128 wide: 0.61 ms = 225 TFLOP/s of fp32 products in calls back to back, 0.64 to 0.68 ms in a training step, cores
+// busy 63% (the rest: the first operands of each phase wait for LDS, the softmax between the phases; the kernel of eight
+// wavefronts and 128 columns keeps 10 to 30 registers more than there are in scratch memory); a large fp32 product of the
+// library reaches 153.  8 x 16 heads of 512 x 1024, 64 wide, lengths 128 to 1024: 81 us, the longest entry's workgroups.
 // For one query the memory bounds it: 16 heads of 4 key heads, 8 entries of 250 to 2000 keys: 12 us and 4 to join, of 18 MB.
 // A row that sees no key has m = -inf, l = 0, out = 0.  The pair (m, l) is kept and not m + ln l: where the bias is the
 // type's lowest value for a whole row, ln l would be lost in the sum.

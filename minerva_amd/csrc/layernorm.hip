@@ -7,12 +7,12 @@
 // differences from it are exact where it is large; so their own mean is summed with their squares, and taken off.
 // Bound by HBM, 8 bytes per element forward and 12 backward: a column of up to 16384 values is held in registers
 // between the passes, so it is read once, by as few threads as hold it with 4 to 16 values each (16 lanes to 64 features,
-// 512 threads to 8192), and a group of threads goes from column to column.  backward sums dgamma and dbeta in
+// 512 threads to 8192; 32 values backward of more), and a group of threads goes from column to column.  backward sums dgamma and dbeta in
 // registers over the columns of a group, each thread its own features, and leaves one partial sum per
-// workgroup to a second kernel.  4096 x 8192 forward: 40.6 us again and again on the same 268 MB, which the
-// caches partly hold, 49.7 us on other data from call to call = 5.4 TB/s (a large copy: 4.7, an addition 5.9); backward of
-// 512 x 65536: 64.5 us and 6 for the second kernel, 78.5 us on other data = 5.1 TB/s; 999 x 4099: 14.4 and 4 us.
-// Small ones are a launch (256 x 4: 1.7 us).
+// workgroup to a second kernel.  4096 x 8192 forward: 41.2 us again and again on the same 268 MB, which the
+// caches partly hold, 50.2 us on other data from call to call = 5.3 TB/s (a large copy: 4.7, an addition 5.9); backward of
+// 512 x 65536: 65.8 us and 6 for the second kernel, 79 us on other data = 5.1 TB/s; 999 x 4099: 14.9 and 4 us.
+// Small ones are a launch (256 x 4: 1.9 us).
 #include <math.h>
 
 #include "mnv_common.h"
@@ -263,7 +263,8 @@ __global__ __launch_bounds__(NTH) void mnv_layernorm_bwd_kernel(const float* __r
   }
 }
 
-// Columns of more values than the register forms hold: each pass reads the column again.
+// Columns of more values than the register forms hold: each pass reads the column again, value by value, three times forward
+// and four times backward, where the sums of dgamma and dbeta go through memory with every column (20001 x 1000: 49 and 177 us).
 #define MNV_LN_WIDE 1024
 // A column's mean is a first one and the mean of the differences from it.
 struct WideStats {
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(MNV_LN_WIDE) void mnv_layernorm_bwd_wide_kernel(
 }
 
 // dgamma, dbeta (blockIdx.y) = the sums of the workgroups' parts: 16 features to a workgroup, 64 threads to a feature, each with
-// every 64th part (2048 parts of 512 features: 8 loads in a row per chain).
+// every 64th part (768 parts of 512 features: 3 loads in a row per chain).
 __global__ __launch_bounds__(1024) void mnv_layernorm_sums_kernel(const float* __restrict__ parts, int num,
                                                                   float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                                   unsigned features) {
@@ -399,7 +400,8 @@ int by_width(const Norm& n) {
   if (f <= 2048) return launch<256, 2, 256, VEC, NT>(n);
   if (f <= 4096) return launch<256, 4, 256, VEC, NT>(n);
   if (f <= 8192) return launch<512, 4, 512, VEC, NT>(n);
-  // 16384 x 2048: forward 43 us, of 512 threads 54; backward, whose sums take registers too, 170 and 109
+  // 16384 x 2048: forward 46 us (before the differences' mean was summed 43, and 54 of 512 threads); backward, whose sums take
+  // registers too, 113 of 512 threads and 170 of 1024
   return n.dy ? launch<512, 8, 512, VEC, NT>(n) : launch<1024, 4, 1024, VEC, NT>(n);
 }
 int run(const Norm& n) {
@@ -420,7 +422,7 @@ int run(const Norm& n) {
 }
 
 // Workgroups of the backward pass: 3 or 2 to a CU are enough to keep the memory busy, and leave fewer partial sums (512 x
-// 65536: 69 us, of 8 to a CU 77; 4096 x 8192: 69, of 4 to a CU 78), and fewer of them where a group would have few
+// 65536: 72 us, of 8 to a CU 77; 4096 x 8192: 70, of 4 to a CU 78), and fewer of them where a group would have few
 // columns to its sums (2048 x 1000: 14.0 us of two columns or more, 12.7 of four; 64 x 100: 8.1 and 8.6).
 // Of very many columns there are more of them, so that no sum of a thread has more than MNV_LN_CHAIN terms (2^28 columns of one
 // feature, gradients of 1.1, whose additions all round the same way: dbeta off by 1.1e-5, 2.1e-4 with 21845 in a row).

@@ -5,8 +5,8 @@
 // borders are computed once per call on the host (in 64 bits, whole numbers afterwards) and go to the kernels
 // by value.  Forward: one thread per offset finds its bucket by bisection and copies; backward: one
 // workgroup per bucket and head sums its run in a fixed order, so the bits do not depend on chance.
-// Bound by launch latency: 16 heads of 32767 offsets are 2 MB, forward 4.1 us, backward 9.2 (a workgroup goes through the
-// 15000 offsets of the farthest bucket); 12 heads of 511 offsets 2.9 and 2.9 us.
+// Bound by launch latency: 16 heads of 32767 offsets are 2 MB, forward 4.1 us, backward 9.9 (a workgroup goes through the
+// 15000 offsets of the farthest bucket); 12 heads of 511 offsets about 3 us each.
 #include <math.h>
 
 #include "mnv_common.h"
