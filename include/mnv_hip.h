@@ -398,8 +398,9 @@ int mnv_lrn_bwd(const float* bottom, const float* top, const float* scale, const
  * eps is finite and not negative, and the squares of a column's differences from its mean have a finite sum in fp32.
  * backward works from x alone (nothing of the forward pass is kept).
  * Its workspace holds partial sums over columns; with less of it, or none, fewer workgroups run (one, for
- * none), and dgamma and dbeta sum more columns in a row (1024 to a thread at most with all of it).  The order of the sums, and so the results' bits, is set by the sizes, the workspace's size and the
- * device's number of compute units. ---- */
+ * none), and dgamma and dbeta sum more columns in a row (with all of it at most 1024 to a thread).  The order of
+ * the sums, and so the results' bits, is set by the sizes, the workspace's size and the device's number of
+ * compute units. ---- */
 int mnv_layernorm_fwd(const float* x, const float* gamma, const float* beta, float* y, int features,
                       int count, float eps, mnv_stream_t stream);
 size_t mnv_layernorm_bwd_workspace_bytes(int features, int count);
