@@ -463,6 +463,74 @@ int mnv_relative_bias_bwd(const float* dbias, float* dtable, int buckets, int he
                           int k_len, int q_start, int max_distance, int both_ways,
                           mnv_stream_t stream);
 
+/* ---- rotary positions of queries and keys (no counterpart in the reference).  x, y, dy, dx {head_dim, heads, length,
+ * batch}, their tokens `pitch` floats apart (heads * head_dim, or more where the heads lie in a wider matrix, as
+ * the queries and keys of one merged projection do).  Of each head the first rotary_dim values (even, 2 to 4096) are
+ * turned in pairs, i < rotary_dim / 2:  (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved;
+ *   (y1, y2) = magnitude * (x1 cos a - x2 sin a, x1 sin a + x2 cos a),  a = position * f_i
+ *   f_i = base^(-2 i / rotary_dim);  the gradient is the turn back, dx1 = magnitude * (dy1 cos a + dy2 sin a), ...
+ * and the values behind them are copied.  positions {length, batch}, or NULL for start + 0 ... length - 1 in every entry;
+ * any finite position is taken as it is (an infinity or NaN gives NaN).
+ * factor != 1 scales the angles for longer contexts: f_i / factor, or with high_turns > low_turns >= 0
+ *   f_i * (w + (1 - w) / factor),  w = (context * f_i / (2 pi) - low_turns) / (high_turns - low_turns) cut to 0 ... 1
+ * (frequencies of many turns within `context` positions stay as they are).  low_turns and high_turns are 0 otherwise.
+ * y may be x, and dx dy, if their pitches are equal: the values behind are then left alone.  Angles are
+ * computed in 64 bits, to about 1e-7 of a turn's cosine and sine. ---- */
+int mnv_rotary_fwd(const float* x, const float* positions, float* y, int head_dim, int heads, int length,
+                   int batch, int x_pitch, int y_pitch, int rotary_dim, int interleaved, int start,
+                   double base, double factor, int context, double low_turns, double high_turns,
+                   double magnitude, mnv_stream_t stream);
+int mnv_rotary_bwd(const float* dy, const float* positions, float* dx, int head_dim, int heads, int length,
+                   int batch, int dy_pitch, int dx_pitch, int rotary_dim, int interleaved, int start,
+                   double base, double factor, int context, double low_turns, double high_turns,
+                   double magnitude, mnv_stream_t stream);
+
+/* ---- gated feed-forward block (no counterpart in the reference).  x, y, dy, dx {features, tokens};
+ * w_in, dw_in {2 hidden, features}: the gate's rows, then the up projection's; w_out, dw_out {features, hidden}.
+ *   pre = w_in x {2 hidden, tokens},  h = act(pre_gate) * pre_up {hidden, tokens},  y = w_out h
+ *   dh = w_out' dy,  dpre = (dh * pre_up * act'(pre_gate), dh * act(pre_gate))
+ *   dx = w_in' dpre,  dw_in = dpre x',  dw_out = dy h'
+ * activation: 0 sigmoid, 1 relu (slope 0 at 0), 2 tanh, 3 silu x / (1 + exp(-x)), 4 gelu x Phi(x) with the normal distribution's Phi.
+ * forward writes h, and pre unless it is NULL (no backward pass follows); backward reads both, and writes dpre, which
+ * may be pre itself; dx may be NULL if nobody needs it.  Sums are those of the products above (mnv_sgemm_nn), whose
+ * workspace and plans they have; a workspace is used if it is aligned to 16 bytes, and without one pre == NULL costs
+ * few tokens more time.  Each matrix holds less than 2^29 values. ---- */
+size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens);
+int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y,
+                      int features, int hidden, int tokens, int activation, void* workspace,
+                      size_t workspace_bytes, mnv_stream_t stream);
+size_t mnv_gated_ffn_bwd_workspace_bytes(int features, int hidden, int tokens);
+int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, const float* pre,
+                      const float* h, const float* dy, float* dpre, float* dx, float* dw_in, float* dw_out,
+                      int features, int hidden, int tokens, int activation, void* workspace,
+                      size_t workspace_bytes, mnv_stream_t stream);
+
+/* ---- a step of Adam with decoupled weight decay over `count` tensors at once (no counterpart in the reference).
+ * The arrays of pointers, sizes and factors are host memory, read before the call returns; what they point to is on the
+ * device.  Of tensor i, with sizes[i] values (0: skipped), rate_i = rate * rates[i] and decay_i = weight_decay * decays[i]
+ * (rates, decays NULL: 1 each) and t = step, from 1 on:
+ *   g = grad_scale * grads;  m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2
+ *   p' = p - rate_i * (m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps) + decay_i * p)
+ * params_out may be params, m_out m and v_out v.  schedule: NULL, or two floats on the device, the rate and t, read when the kernel
+ * runs instead of `rate` and `step`: a recorded step is replayed with others.
+ * bits 32: m and v are as long as the tensor.  bits 8: a column {65} for every 256 of the tensor's values, the last one's
+ * rest 0: 64 floats whose bytes are the values' codes (byte j, value j), and the largest size among them, `top`;
+ *   m = top (c / 127)^3 for c from -127 to 127, v = top (c / 255)^4 for c from 0 to 255, as 32-bit numbers.
+ * m' is rounded to the nearest code.  v' of value i goes to the code above it if it is more than u of the way there,
+ * u = (i 0x85EBCA6B + t 0x9E3779B9 modulo 2^32) / 2^32 (it walks evenly through 0 to 1 from step to step, so that v moves in the mean where
+ * beta2 moves it by less than a code), and never to 0 from above it.  p' is computed before they are rounded.  Memory of
+ * zeros is the first step's m and v in either form.  An infinity or a NaN in g gives NaN for all values of its block's
+ * m and v.  mnv_adamw_moment_floats: floats of m, and of v, of a tensor of n values (0 for other bits).
+ * mnv_adamw_values: the values that the codes of 8-bit moments stand for, sizes[i] floats each. ---- */
+size_t mnv_adamw_moment_floats(size_t n, int bits);
+int mnv_adamw_step(int count, const float* const* params, const float* const* grads, const float* const* m,
+                   const float* const* v, float* const* params_out, float* const* m_out,
+                   float* const* v_out, const size_t* sizes, const float* rates, const float* decays,
+                   int bits, double rate, double beta1, double beta2, double eps, double weight_decay,
+                   double grad_scale, int step, const float* schedule, mnv_stream_t stream);
+int mnv_adamw_values(int count, const float* const* m, const float* const* v, float* const* m_values,
+                     float* const* v_values, const size_t* sizes, mnv_stream_t stream);
+
 /* ---- Concat / Slice / Select data movement (reference cuda.cpp:80-155, 644-655).
  * The reference builds Concat and Slice from one CudaPerformCopy (cuda_perform.h:20) per
  * image; here one 2-D copy per input tensor does it: `rows` rows of `row_elems` floats,

@@ -13,6 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libmnv_hip.so")
 
 c_f = ctypes.c_float
+c_d = ctypes.c_double
 c_i = ctypes.c_int
 c_sz = ctypes.c_size_t
 c_p = ctypes.c_void_p
@@ -122,6 +123,14 @@ PROTOTYPES["mnv_attention_bwd_workspace_bytes"] = [_I] * 7
 PROTOTYPES["mnv_attention_bwd"] = [_P] * 12 + [_I] * 6 + [c_f, _P, c_sz, _S]
 PROTOTYPES["mnv_relative_bias_fwd"] = [_P, _P] + [_I] * 7 + [_S]
 PROTOTYPES["mnv_relative_bias_bwd"] = [_P, _P] + [_I] * 7 + [_S]
+for _n in ("fwd", "bwd"):
+    PROTOTYPES["mnv_rotary_" + _n] = [_P] * 3 + [_I] * 9 + [c_d, c_d, _I, c_d, c_d, c_d, _S]
+    PROTOTYPES["mnv_gated_ffn_%s_workspace_bytes" % _n] = [_I] * 3
+PROTOTYPES["mnv_gated_ffn_fwd"] = [_P] * 6 + [_I] * 4 + [_P, c_sz, _S]
+PROTOTYPES["mnv_gated_ffn_bwd"] = [_P] * 10 + [_I] * 4 + [_P, c_sz, _S]
+PROTOTYPES["mnv_adamw_moment_floats"] = [c_sz, _I]
+PROTOTYPES["mnv_adamw_step"] = [_I] + [_P] * 10 + [_I] + [c_d] * 6 + [_I, _P, _S]
+PROTOTYPES["mnv_adamw_values"] = [_I] + [_P] * 5 + [_S]
 
 _RESTYPES = {
     "mnv_error_string": ctypes.c_char_p,
@@ -134,6 +143,9 @@ _RESTYPES = {
     "mnv_layernorm_bwd_workspace_bytes": c_sz,
     "mnv_attention_fwd_workspace_bytes": c_sz,
     "mnv_attention_bwd_workspace_bytes": c_sz,
+    "mnv_gated_ffn_fwd_workspace_bytes": c_sz,
+    "mnv_gated_ffn_bwd_workspace_bytes": c_sz,
+    "mnv_adamw_moment_floats": c_sz,
 }
 
 

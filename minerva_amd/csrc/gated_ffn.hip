@@ -1,0 +1,306 @@
+// The gated feed-forward block y = w_out (act(w_gate x) * (w_up x)), with both projections in one matrix
+// w_in {2 hidden, features}, and its gradients:
+//   pre = w_in x,  h = act(pre_gate) * pre_up,  y = w_out h
+//   dh = w_out' dy,  dpre = (dh * pre_up * act'(pre_gate), dh * act(pre_gate))
+//   dx = w_in' dpre,  dw_in = dpre x',  dw_out = dy h'
+// Bound by the matrix cores (6 features hidden flops a token forward, 12 backward), and for few tokens by reading the
+// weights.  All products are those of the SGEMM (sgemm_core.h); what lies between them is done where a product is
+// stored: the gate forward, where both projections of a row meet in one tile, and dpre backward, which is all that
+// is kept of dh.
+#include "sgemm_core.h"
+
+namespace {
+
+enum { ACT_SIGMOID, ACT_RELU, ACT_TANH, ACT_SILU, ACT_GELU, ACT_COUNT };
+
+// The activation of x, and its slope there.
+__device__ __forceinline__ void activate(int kind, float x, float& value, float& slope) {
+  if (kind == ACT_RELU) {
+    value = x > 0.f ? x : 0.f;
+    slope = x > 0.f ? 1.f : 0.f;
+  } else if (kind == ACT_TANH) {
+    value = tanhf(x);
+    slope = 1.f - value * value;
+  } else if (kind == ACT_GELU) {
+    // x times the normal distribution's share below x: erfc keeps the digits of a small share, 1 + erf does not
+    const float below = 0.5f * erfcf(x * -0.70710678f);
+    value = x * below;
+    slope = below + x * (0.39894228f * expf(-0.5f * x * x));
+  } else {
+    // 1 / (1 + exp(-x)) and what it lacks to 1, from the exponential that cannot overflow: neither loses digits near 0
+    const float z = expf(-fabsf(x)), near = 1.f / (1.f + z), far = z * near;
+    const float e = x < 0.f ? far : near, rest = x < 0.f ? near : far;
+    value = kind == ACT_SILU ? x * e : e;
+    slope = kind == ACT_SILU ? e + value * rest : e * rest;
+  }
+}
+__device__ __forceinline__ float gated(int kind, float gate, float up) {
+  float value, slope;
+  activate(kind, gate, value, slope);
+  return value * up;
+}
+
+// Four rows from p on, of which `left` exist.
+__device__ __forceinline__ void store_rows(float* p, int left, const float (&x)[4]) {
+  if (left >= 4) {
+    *reinterpret_cast<mnv_f4u*>(p) = mnv_f4u{x[0], x[1], x[2], x[3]};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      if (q < left) p[q] = x[q];
+  }
+}
+
+// w_in x with the gate where it is stored.  The product's rows are w_in's in runs of four, gate and up in turn, so that rows
+// 8 i .. 8 i + 3 are the gate's 4 i .. 4 i + 3 and the four behind them the up projection's.  A 16-byte fetch is still
+// one run of w_in's column, and a tile in parts gives neighbouring lanes the two runs of one column (C_ROWS_OF_FOUR):
+// they change places by a lane permutation.  Rows past `hidden` of the last run hold what follows in memory, or 0
+// past the end, and are not stored.
+template <bool K4>
+struct GatedIn {
+  static constexpr bool A_KFAST = false, B_KFAST = true;
+  static constexpr int A_NOFF = 1, B_NOFF = 1;
+  const float* __restrict__ A;
+  const float* __restrict__ B;
+  float* __restrict__ pre;  // may be null
+  float* __restrict__ h;
+  int M, N, K, total_slabs, spp, bk;
+  int hidden, act;
+  static constexpr bool N_GROUPED = true;
+  int n_group;
+  struct Res {
+    mnv_rsrc a, b;
+  };
+  struct AState {};
+  struct BState {};
+  __device__ void make_res(Res& r) const {
+    r.a = mnv_make_rsrc(A, (unsigned)K * (unsigned)hidden * 8u);
+    r.b = mnv_make_rsrc(B, (unsigned)N * (unsigned)K * 4u);
+  }
+  __device__ void a_init(const Res&, AState&, int) const {}
+  __device__ void b_init(const Res&, BState&, int) const {}
+  __device__ void a_period(const AState&, unsigned (&off)[A_NOFF], int m, int kl, int period) const {
+    const int k = period * spp * bk + kl, row = m / 8 * 4;
+    off[0] = ((row < hidden) & (k < K)) ? ((unsigned)k * (unsigned)hidden * 2u + (unsigned)(row + (m & 4 ? hidden : 0))) * 4u : MNV_OOB;
+  }
+  __device__ void a_load(const Res& r, const AState&, const unsigned (&off)[A_NOFF], int, int s, int, float (&v)[4]) const {
+    mnv_fetch_vec<A_NOFF>(r.a, off, (unsigned)s * (unsigned)bk * (unsigned)hidden * 8u, v);
+  }
+  __device__ void b_period(const BState&, unsigned (&off)[B_NOFF], int n, int kl, int period) const {
+    const int k = period * spp * bk + kl;
+    off[0] = ((n < N) & (k < K)) ? ((unsigned)n * (unsigned)K + (unsigned)k) * 4u : MNV_OOB;
+  }
+  __device__ void b_load(const Res& r, const BState&, const unsigned (&off)[B_NOFF], int, int s, int, float (&v)[4]) const {
+    mnv_fetch_vec<B_NOFF>(r.b, off, (unsigned)s * (unsigned)bk * 4u, v);
+  }
+  // as SgemmNN: a vector of the last, partial slab is cleared past K
+  static constexpr bool B_STASH_FIX = !K4;
+  __device__ void b_stash_fix(int period, int, int kl, float (&v)[4]) const {
+    if (period == (K >= bk ? 1 : 0)) {
+      const int rest = K % bk;
+#pragma unroll
+      for (int q = 1; q < 4; ++q) v[q] = kl + q < rest ? v[q] : 0.f;
+    }
+  }
+  size_t extra_lds_bytes() const { return 0; }
+  void set_bk(int b) {
+    bk = b;
+    spp = K >= b ? K / b : 1;
+    total_slabs = (K + b - 1) / b;
+  }
+  __device__ void block_init(Res&, float*, int, int) const {}
+  static constexpr bool C_STORE4 = true, C_ROWS_OF_FOUR = true;
+  __device__ void c_store4(int m, int n, const float (&x)[4]) const {
+    const int row = m / 8 * 4, left = hidden - row;
+    const bool up = m & 4;
+    float other[4], r[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)  // quad_perm 1, 0, 3, 2
+      other[q] = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x[q]), 0xb1, 0xf, 0xf, true));
+    if (pre) store_rows(pre + (size_t)n * hidden * 2 + row + (up ? hidden : 0), left, x);
+    // each lane of the pair gates two of the four rows
+#pragma unroll
+    for (int q = 0; q < 4; ++q) r[q] = gated(act, up ? other[q] : x[q], up ? x[q] : other[q]);
+    if (!up) store_rows(h + (size_t)n * hidden + row, left, r);
+  }
+};
+
+// w_out' dy, stored as dpre.  dpre may be pre itself: every element is read and written by one thread.
+template <bool K4>
+struct GatedOutBack : SgemmNN<K4, true, false> {
+  typedef SgemmNN<K4, true, false> Base;
+  const float* pre;
+  float* dpre;
+  int hidden, act;
+  __device__ void c_store(int m, int n, float dh) const {
+    const size_t at = (size_t)n * hidden * 2 + m;
+    const float gate = pre[at], up = pre[at + hidden];
+    float value, slope;
+    activate(act, gate, value, slope);
+    dpre[at] = dh * up * slope;
+    dpre[at + hidden] = dh * value;
+  }
+  __device__ void c_store4(int m, int n, const float (&dh)[4]) const {
+    if (m + 3 < this->M) {
+      const size_t at = (size_t)n * hidden * 2 + m;
+      const mnv_f4u gate = *reinterpret_cast<const mnv_f4u*>(pre + at), up = *reinterpret_cast<const mnv_f4u*>(pre + at + hidden);
+      mnv_f4u dg, du;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float value, slope;
+        activate(act, gate[q], value, slope);
+        dg[q] = dh[q] * up[q] * slope;
+        du[q] = dh[q] * value;
+      }
+      *reinterpret_cast<mnv_f4u*>(dpre + at) = dg;
+      *reinterpret_cast<mnv_f4u*>(dpre + at + hidden) = du;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (m + q < this->M) c_store(m + q, n, dh[q]);
+    }
+  }
+};
+
+// h = act(gate) * up from pre as a product of its own left it: four rows a thread.
+__global__ __launch_bounds__(256) void gate_kernel(const float* __restrict__ pre, float* __restrict__ h, int hidden, MnvFastDiv quads,
+                                                   int quads_count, size_t total, int act) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+    const int n = total <= 0x7fffffff ? mnv_fastdiv((int)i, quads) : (int)(i / quads_count);
+    const int row = (int)(i - (size_t)n * quads_count) * 4, left = hidden - row;
+    const float* p = pre + (size_t)n * hidden * 2 + row;
+    float r[4];
+    if (left >= 4) {
+      const mnv_f4u gate = *reinterpret_cast<const mnv_f4u*>(p), up = *reinterpret_cast<const mnv_f4u*>(p + hidden);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) r[q] = gated(act, gate[q], up[q]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) r[q] = q < left ? gated(act, p[q], p[hidden + q]) : 0.f;
+    }
+    store_rows(h + (size_t)n * hidden + row, left, r);
+  }
+}
+
+template <bool K4>
+int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens,
+                    int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  GatedIn<K4> p;
+  p.A = w_in; p.B = x; p.pre = pre; p.h = h;
+  p.M = (hidden + 3) / 4 * 8; p.N = tokens; p.K = features;
+  p.hidden = hidden; p.act = act;
+  p.n_group = 1;
+  p.set_bk(16);
+  return launch_split(plan, p, workspace, workspace ? workspace_bytes : 0, s);
+}
+
+// Whether the projections run as one product on tiles in bf16 parts that need no k ranges, whose store has the gate.  What a plan
+// of the plain product gives to other tiles keeps them, and a kernel of its own gates.
+bool fused(const SgemmPlan& plan) { return plan.split && plan.splits == 1 && !plan.skinny && !plan.tile; }
+
+int launch_gate(const float* pre, float* h, int hidden, int tokens, int act, hipStream_t s) {
+  const int quads = (hidden + 3) / 4;
+  const size_t total = (size_t)quads * tokens;
+  size_t blocks = mnv_ceil_div(total, 256);
+  if (blocks > MNV_MAX_STREAM_BLOCKS) blocks = MNV_MAX_STREAM_BLOCKS;
+  hipLaunchKernelGGL(gate_kernel, dim3((unsigned)blocks), dim3(256), 0, s, pre, h, hidden, mnv_fastdiv_make(quads), quads, total, act);
+  return MNV_LAUNCH_STATUS();
+}
+
+template <bool K4>
+int launch_out_back(const SgemmPlan& plan, const float* w_out, const float* dy, const float* pre, float* dpre, int features, int hidden,
+                    int tokens, int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  GatedOutBack<K4> p;
+  static_cast<SgemmNN<K4, true, false>&>(p) =
+      make_sgemm<K4, true, false>(w_out, dy, nullptr, hidden, tokens, features, SgemmEpilogue{nullptr, nullptr, 0});
+  p.pre = pre; p.dpre = dpre;
+  p.hidden = hidden; p.act = act;
+  if constexpr (K4) {
+    if (plan.skinny) return launch_skinny_columns(plan, p, workspace, s);
+    if (plan.tile) return launch_small_tiles(plan, p, s);
+  }
+  return launch_plan(plan, p, workspace, workspace_bytes, s);
+}
+
+// Products read matrices through 32-bit byte offsets.
+bool sizes_ok(int features, int hidden, int tokens, int act) {
+  const long long most = (1LL << 29) - 1;
+  return features > 0 && hidden > 0 && tokens > 0 && act >= 0 && act < ACT_COUNT && 2LL * hidden <= most / features &&
+         2LL * hidden <= most / tokens && features <= most / tokens;
+}
+
+size_t larger(size_t a, size_t b) { return a > b ? a : b; }
+// Bytes of pre where the caller keeps none and the plan does not do without it, in whole 16 bytes.
+size_t pre_bytes(int hidden, int tokens) { return ((size_t)hidden * 2 * tokens * sizeof(float) + 15) / 16 * 16; }
+
+}  // namespace
+
+extern "C" {
+
+size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens) {
+  if (!sizes_ok(features, hidden, tokens, 0)) return 0;
+  const size_t in = mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
+  const bool keeps = !fused(plan_sgemm(2 * hidden, tokens, features, in / sizeof(float)));
+  return larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (keeps ? pre_bytes(hidden, tokens) : 0);
+}
+
+int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y, int features, int hidden,
+                      int tokens, int activation, void* workspace, size_t workspace_bytes, mnv_stream_t stream) {
+  if (!x || !w_in || !w_out || !h || !y || !sizes_ok(features, hidden, tokens, activation)) return MNV_ERR_INVALID;
+  hipStream_t s = mnv_stream(stream);
+  char* ws = static_cast<char*>(workspace);
+  size_t bytes = workspace_bytes;
+  if (!ws || !mnv_aligned16(ws)) {
+    ws = nullptr;
+    bytes = 0;
+  }
+  SgemmPlan plan = plan_sgemm(2 * hidden, tokens, features, bytes / sizeof(float));
+  float* kept = pre;
+  if (!fused(plan) && !kept) {
+    const size_t want = pre_bytes(hidden, tokens);
+    if (bytes >= want) {
+      kept = reinterpret_cast<float*>(ws);
+      ws += want;
+      bytes -= want;
+      plan = plan_sgemm(2 * hidden, tokens, features, bytes / sizeof(float));
+    } else {  // nowhere to leave pre: one product, whatever its size
+      plan = SgemmPlan{false, 1};
+      plan.split = true;
+    }
+  }
+  int rc;
+  if (fused(plan)) {
+    rc = features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
+                           : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
+  } else {
+    rc = mnv_sgemm_nn(w_in, x, kept, 2 * hidden, tokens, features, ws, bytes, stream);
+    if (!rc) rc = launch_gate(kept, h, hidden, tokens, activation, s);
+  }
+  return rc ? rc : mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
+}
+
+size_t mnv_gated_ffn_bwd_workspace_bytes(int features, int hidden, int tokens) {
+  if (!sizes_ok(features, hidden, tokens, 0)) return 0;
+  return larger(larger(mnv_sgemm_nn_workspace_bytes(hidden, tokens, features), mnv_sgemm_nn_workspace_bytes(features, tokens, 2 * hidden)),
+                larger(mnv_sgemm_nn_workspace_bytes(2 * hidden, features, tokens), mnv_sgemm_nn_workspace_bytes(features, hidden, tokens)));
+}
+
+int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, const float* pre, const float* h, const float* dy, float* dpre,
+                      float* dx, float* dw_in, float* dw_out, int features, int hidden, int tokens, int activation, void* workspace,
+                      size_t workspace_bytes, mnv_stream_t stream) {
+  if (!x || !w_in || !w_out || !pre || !h || !dy || !dpre || !dw_in || !dw_out || !sizes_ok(features, hidden, tokens, activation))
+    return MNV_ERR_INVALID;
+  hipStream_t s = mnv_stream(stream);
+  void* ws = workspace && mnv_aligned16(workspace) ? workspace : nullptr;
+  const size_t bytes = ws ? workspace_bytes : 0;
+  const SgemmPlan plan = plan_sgemm(hidden, tokens, features, bytes / sizeof(float));
+  int rc = plan.skinny || plan.tile || features % 4 == 0
+               ? launch_out_back<true>(plan, w_out, dy, pre, dpre, features, hidden, tokens, activation, ws, bytes, s)
+               : launch_out_back<false>(plan, w_out, dy, pre, dpre, features, hidden, tokens, activation, ws, bytes, s);
+  if (!rc && dx) rc = mnv_sgemm_tn(w_in, dpre, nullptr, dx, features, tokens, 2 * hidden, ws, bytes, stream);
+  if (!rc) rc = mnv_sgemm_nt(dpre, x, dw_in, 2 * hidden, features, tokens, ws, bytes, stream);
+  if (!rc) rc = mnv_sgemm_nt(dy, h, dw_out, features, hidden, tokens, ws, bytes, stream);
+  return rc;
+}
+
+}  // extern "C"

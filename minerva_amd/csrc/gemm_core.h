@@ -125,6 +125,9 @@ struct MnvFetchMap {
 //        stores 16 bytes per lane, 512 contiguous bytes per column and instruction, instead of
 //        4 bytes per lane: a quarter of the store instructions.  Taken for products of at most
 //        MNV_STORE4_MAX_SLABS k-slabs.
+//   optional, for a store that needs a column's neighbouring rows together: static constexpr bool C_ROWS_OF_FOUR = true;
+//        Only c_store4 is called, and lanes 2 i and 2 i + 1 call it at the same time, for rows m and m + 4 of one column
+//        (m a multiple of 8, M too).  For tiles in bf16 parts without k ranges (a cut tail is fine).
 //   optional, for a product whose left operand depends on the column tile (batched products
 //   folded into the column index): static constexpr bool N_GROUPED = true;  int n_group;
 //        Tiles are then dealt m-tile by m-tile within groups of n_group consecutive column
@@ -174,6 +177,14 @@ struct MnvCStore4 {
 };
 template <class P>
 struct MnvCStore4<P, std::enable_if_t<P::C_STORE4>> {
+  static constexpr bool value = true;
+};
+template <class P, class = void>
+struct MnvCRowsOfFour {
+  static constexpr bool value = false;
+};
+template <class P>
+struct MnvCRowsOfFour<P, std::enable_if_t<P::C_ROWS_OF_FOUR>> {
   static constexpr bool value = true;
 };
 template <class P, class = void>
@@ -353,10 +364,15 @@ __device__ __forceinline__ void mnv_partial_store(const P& prob, int m0, int n0,
     m = m0 + wave % T::WGM * T::WM + 4 * (lane % 16);
     n = n0 + (P::B_KFAST ? block * 16 + col : block / 4 * 64 + block % 4 + 4 * col);
     if (n >= prob.N) return;
-    if (m + 0 < prob.M) prob.c_store(m + 0, n, s.x);
-    if (m + 1 < prob.M) prob.c_store(m + 1, n, s.y);
-    if (m + 2 < prob.M) prob.c_store(m + 2, n, s.z);
-    if (m + 3 < prob.M) prob.c_store(m + 3, n, s.w);
+    if constexpr (MnvCRowsOfFour<P>::value) {
+      if (m < prob.M) prob.c_store4(m, n, {s.x, s.y, s.z, s.w});
+      return;
+    } else {
+      if (m + 0 < prob.M) prob.c_store(m + 0, n, s.x);
+      if (m + 1 < prob.M) prob.c_store(m + 1, n, s.y);
+      if (m + 2 < prob.M) prob.c_store(m + 2, n, s.z);
+      if (m + 3 < prob.M) prob.c_store(m + 3, n, s.w);
+    }
   } else {
     mnv_partial_group_mn<T>(group, m, n);
     m += m0;
@@ -1198,6 +1214,7 @@ static int mnv_gemm_launch(const P& prob, int splits, void* workspace, hipStream
   if (per < 1) per = 1;
   splits = total_slabs > 0 ? (total_slabs + per - 1) / per : 1;
   if ((long long)tiles_m * tiles_n > 0x7fffffffLL || splits > 65535) return MNV_ERR_INVALID;
+  if (MnvCRowsOfFour<P>::value && splits > 1) return MNV_ERR_INVALID;  // their sums are stored one by one
   // The LDS limit of a kernel is an attribute per device; set once on each (idempotent: a
   // race only repeats the same call).
   static std::atomic<bool> attr_set[64];
@@ -1235,8 +1252,8 @@ static int mnv_gemm_launch(const P& prob, int splits, void* workspace, hipStream
       return MNV_LAUNCH_STATUS();
     }
   }
-  if (splits > 1) {
-    rc = mnv_gemm_reduce_launch(prob, reinterpret_cast<const float*>(workspace), splits, s);
+  if constexpr (!MnvCRowsOfFour<P>::value) {
+    if (splits > 1) rc = mnv_gemm_reduce_launch(prob, reinterpret_cast<const float*>(workspace), splits, s);
   }
   return rc;
 }
