@@ -54,7 +54,7 @@ __device__ __forceinline__ void store_rows(float* p, int left, const float (&x)[
 // w_in x with the gate where it is stored.  The product's rows are w_in's in runs of four, gate and up in turn, so that rows
 // 8 i .. 8 i + 3 are the gate's 4 i .. 4 i + 3 and the four behind them the up projection's.  A 16-byte fetch is still
 // one run of w_in's column, and a tile in parts gives neighbouring lanes the two runs of one column (C_ROWS_OF_FOUR):
-// they change places by a lane permutation.  Rows past `hidden` of the last run hold what follows in memory, or 0
+// they change places by a lane permutation, as do the lanes that store a small tile's sums, four rows apart.  Rows past `hidden` of the last run hold what follows in memory, or 0
 // past the end, and are not stored.
 template <bool K4>
 struct GatedIn {
@@ -65,7 +65,7 @@ struct GatedIn {
   float* __restrict__ pre;  // may be null
   float* __restrict__ h;
   int M, N, K, total_slabs, spp, bk;
-  int hidden, act;
+  int lda, ldb, hidden, act;
   static constexpr bool N_GROUPED = true;
   int n_group;
   struct Res {
@@ -109,6 +109,15 @@ struct GatedIn {
     total_slabs = (K + b - 1) / b;
   }
   __device__ void block_init(Res&, float*, int, int) const {}
+  // the small tiles' view: one row of A, and one sum of a lane, whose up or gate is four lanes away
+  __device__ int a_row(int m) const { return m / 8 * 4 + m % 4 + (m & 4 ? hidden : 0); }
+  __device__ void c_store(int m, int n, float x) const {
+    const float other = __shfl_xor(x, 4, MNV_WAVE);
+    const int row = m / 8 * 4 + m % 4;
+    if (row >= hidden) return;
+    if (pre) pre[(size_t)n * hidden * 2 + a_row(m)] = x;
+    if (!(m & 4)) h[(size_t)n * hidden + row] = gated(act, x, other);
+  }
   static constexpr bool C_STORE4 = true, C_ROWS_OF_FOUR = true;
   __device__ void c_store4(int m, int n, const float (&x)[4]) const {
     const int row = m / 8 * 4, left = hidden - row;
@@ -182,6 +191,59 @@ __global__ __launch_bounds__(256) void gate_kernel(const float* __restrict__ pre
   }
 }
 
+// The k ranges of a product of few columns (mnv_sgemm_skinny_kernel) added, and gated: `ranges` times {2 hidden, tokens}.  ZL threads
+// share a value, each adding every ZL-th range.
+template <int ZL>
+__global__ __launch_bounds__(256) void gate_ranges_kernel(const float* __restrict__ part, float* __restrict__ pre, float* __restrict__ h, int hidden,
+                                                          int tokens, int ranges, int act) {
+  constexpr int QL = 256 / ZL;
+  __shared__ float red[2][256];
+  const int tq = threadIdx.x % QL, tz = threadIdx.x / QL;
+  const size_t all = (size_t)hidden * tokens, q = (size_t)blockIdx.x * QL + tq;
+  const int n = (int)(q / hidden), m = (int)(q - (size_t)n * hidden);
+  float gate = 0.f, up = 0.f;
+  if (q < all) {
+    const float* p = part + (size_t)tz * all * 2 + (size_t)n * hidden * 2 + m;
+#pragma unroll 4
+    for (int r = tz; r < ranges; r += ZL, p += ZL * all * 2) {
+      gate += p[0];
+      up += p[hidden];
+    }
+  }
+  red[0][threadIdx.x] = gate;
+  red[1][threadIdx.x] = up;
+  __syncthreads();
+  if (tz || q >= all) return;
+#pragma unroll
+  for (int i = 1; i < ZL; ++i) {
+    gate += red[0][i * QL + tq];
+    up += red[1][i * QL + tq];
+  }
+  if (pre) {
+    pre[(size_t)n * hidden * 2 + m] = gate;
+    pre[(size_t)n * hidden * 2 + hidden + m] = up;
+  }
+  h[q] = gated(act, gate, up);
+}
+// The projections of few tokens by k ranges in the workspace, as the plan of their product has them.
+int launch_gate_ranges(const SgemmPlan& plan, const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens, int act,
+                       float* part, hipStream_t s) {
+  const auto p = make_sgemm<true>(w_in, x, (float*)nullptr, 2 * hidden, tokens, features, SgemmEpilogue{nullptr, nullptr, 0});
+  if (tokens <= 1) launch_skinny<1, false>(plan, p, part, s);
+  else if (tokens <= 2) launch_skinny<2, false>(plan, p, part, s);
+  else if (tokens <= 4) launch_skinny<4, false>(plan, p, part, s);
+  else if (tokens <= 8) launch_skinny<8, false>(plan, p, part, s);
+  else launch_skinny<MNV_SKINNY_COLUMNS, false>(plan, p, part, s);
+  const int rc = MNV_LAUNCH_STATUS();
+  if (rc) return rc;
+  const size_t all = (size_t)hidden * tokens;
+  if (plan.splits >= 16 && all < 65536)
+    hipLaunchKernelGGL(gate_ranges_kernel<8>, dim3((unsigned)mnv_ceil_div(all, 32)), dim3(256), 0, s, part, pre, h, hidden, tokens, plan.splits, act);
+  else
+    hipLaunchKernelGGL(gate_ranges_kernel<2>, dim3((unsigned)mnv_ceil_div(all, 128)), dim3(256), 0, s, part, pre, h, hidden, tokens, plan.splits, act);
+  return MNV_LAUNCH_STATUS();
+}
+
 template <bool K4>
 int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens,
                     int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
@@ -189,14 +251,19 @@ int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, fl
   p.A = w_in; p.B = x; p.pre = pre; p.h = h;
   p.M = (hidden + 3) / 4 * 8; p.N = tokens; p.K = features;
   p.hidden = hidden; p.act = act;
+  p.lda = 2 * hidden; p.ldb = features;
   p.n_group = 1;
   p.set_bk(16);
+  if constexpr (K4) {
+    if (plan.tile) return launch_small_tiles(plan, p, s);
+  }
   return launch_split(plan, p, workspace, workspace ? workspace_bytes : 0, s);
 }
 
-// Whether the projections run as one product on tiles in bf16 parts that need no k ranges, whose store has the gate.  What a plan
-// of the plain product gives to other tiles keeps them, and a kernel of its own gates.
-bool fused(const SgemmPlan& plan) { return plan.split && plan.splits == 1 && !plan.skinny && !plan.tile; }
+// Whether the projections' product by this plan gates where it stores: on tiles in bf16 parts that need no k ranges, on small tiles, and of
+// few columns by k ranges where those are added.  What the plan gives to other tiles keeps them, and a kernel of its own gates.
+bool by_ranges(const SgemmPlan& plan) { return plan.skinny && plan.splits > 1; }
+bool gates(const SgemmPlan& plan) { return by_ranges(plan) || plan.tile || (plan.split && plan.splits == 1 && !plan.skinny); }
 
 int launch_gate(const float* pre, float* h, int hidden, int tokens, int act, hipStream_t s) {
   const int quads = (hidden + 3) / 4;
@@ -240,7 +307,7 @@ extern "C" {
 size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens) {
   if (!sizes_ok(features, hidden, tokens, 0)) return 0;
   const size_t in = mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
-  const bool keeps = !fused(plan_sgemm(2 * hidden, tokens, features, in / sizeof(float)));
+  const bool keeps = !gates(plan_sgemm(2 * hidden, tokens, features, in / sizeof(float)));
   return larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (keeps ? pre_bytes(hidden, tokens) : 0);
 }
 
@@ -256,7 +323,7 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
   }
   SgemmPlan plan = plan_sgemm(2 * hidden, tokens, features, bytes / sizeof(float));
   float* kept = pre;
-  if (!fused(plan) && !kept) {
+  if (!gates(plan) && !kept) {
     const size_t want = pre_bytes(hidden, tokens);
     if (bytes >= want) {
       kept = reinterpret_cast<float*>(ws);
@@ -269,9 +336,11 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
     }
   }
   int rc;
-  if (fused(plan)) {
-    rc = features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
-                           : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
+  if (by_ranges(plan)) {
+    rc = launch_gate_ranges(plan, w_in, x, pre, h, features, hidden, tokens, activation, reinterpret_cast<float*>(ws), s);
+  } else if (gates(plan)) {
+    rc = plan.tile || features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
+                                        : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
   } else {
     rc = mnv_sgemm_nn(w_in, x, kept, 2 * hidden, tokens, features, ws, bytes, stream);
     if (!rc) rc = launch_gate(kept, h, hidden, tokens, activation, s);

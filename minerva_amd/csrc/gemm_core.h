@@ -126,8 +126,8 @@ struct MnvFetchMap {
 //        4 bytes per lane: a quarter of the store instructions.  Taken for products of at most
 //        MNV_STORE4_MAX_SLABS k-slabs.
 //   optional, for a store that needs a column's neighbouring rows together: static constexpr bool C_ROWS_OF_FOUR = true;
-//        Only c_store4 is called, and lanes 2 i and 2 i + 1 call it at the same time, for rows m and m + 4 of one column
-//        (m a multiple of 8, M too).  For tiles in bf16 parts without k ranges (a cut tail is fine).
+//        Tiles in bf16 parts call c_store4 alone, lanes 2 i and 2 i + 1 at the same time, for rows m and m + 4 of one column
+//        (m a multiple of 8, M too); they have no k ranges then (a cut tail is fine).
 //   optional, for a product whose left operand depends on the column tile (batched products
 //   folded into the column index): static constexpr bool N_GROUPED = true;  int n_group;
 //        Tiles are then dealt m-tile by m-tile within groups of n_group consecutive column

@@ -73,6 +73,7 @@ struct SgemmNN {
   }
   __device__ void a_init(const Res&, AState&, int) const {}
   __device__ void b_init(const Res&, BState&, int) const {}
+  __device__ int a_row(int m) const { return m; }  // (of an x-fast A, where it lies)
   // A[m..m+3, k] (x-fast) or, transposed, A[m, k..k+3] (k-fast)
   __device__ void a_period(const AState&, unsigned (&off)[A_NOFF], int m, int kl, int period) const {
     const int k = period * spp * bk + kl;
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(W * MNV_WAVE, 4) void mnv_sgemm_small_kernel(P prob
   prob.make_res(res);
   const unsigned lda = (unsigned)prob.lda * 4u, ldb = (unsigned)prob.ldb * 4u;
   const unsigned a_off = P::A_KFAST ? (m0 + x < prob.M ? (unsigned)(m0 + x) * lda + (unsigned)h * 16u : MNV_OOB)
-                                    : (unsigned)h * 4u * lda + (unsigned)(m0 + x) * 4u;
+                                    : (unsigned)h * 4u * lda + (unsigned)prob.a_row(m0 + x) * 4u;
   const unsigned b_off = P::B_KFAST ? (n0 + x < prob.N ? (unsigned)(n0 + x) * ldb + (unsigned)h * 16u : MNV_OOB)
                                     : (unsigned)h * 4u * ldb + (unsigned)(n0 + x) * 4u;
   auto fetch = [&](mnv_rsrc r, unsigned off, unsigned ld, auto KFAST, int k, float (&v)[VECS][4]) {
