@@ -191,8 +191,8 @@ __global__ __launch_bounds__(256) void gate_kernel(const float* __restrict__ pre
   }
 }
 
-// The k ranges of a product of few columns (mnv_sgemm_skinny_kernel) added, and gated: `ranges` times {2 hidden, tokens}.  ZL threads
-// share a value, each adding every ZL-th range.
+// The projections' k ranges added, and gated: `ranges` times {2 hidden, tokens}.  ZL threads share a value, each adding every
+// ZL-th range.
 template <int ZL>
 __global__ __launch_bounds__(256) void gate_ranges_kernel(const float* __restrict__ part, float* __restrict__ pre, float* __restrict__ h, int hidden,
                                                           int tokens, int ranges, int act) {
@@ -225,22 +225,14 @@ __global__ __launch_bounds__(256) void gate_ranges_kernel(const float* __restric
   }
   h[q] = gated(act, gate, up);
 }
-// The projections of few tokens by k ranges in the workspace, as the plan of their product has them.
-int launch_gate_ranges(const SgemmPlan& plan, const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens, int act,
-                       float* part, hipStream_t s) {
-  const auto p = make_sgemm<true>(w_in, x, (float*)nullptr, 2 * hidden, tokens, features, SgemmEpilogue{nullptr, nullptr, 0});
-  if (tokens <= 1) launch_skinny<1, false>(plan, p, part, s);
-  else if (tokens <= 2) launch_skinny<2, false>(plan, p, part, s);
-  else if (tokens <= 4) launch_skinny<4, false>(plan, p, part, s);
-  else if (tokens <= 8) launch_skinny<8, false>(plan, p, part, s);
-  else launch_skinny<MNV_SKINNY_COLUMNS, false>(plan, p, part, s);
-  const int rc = MNV_LAUNCH_STATUS();
-  if (rc) return rc;
+int launch_gate_ranges(const float* part, float* pre, float* h, int hidden, int tokens, int ranges, int act, hipStream_t s) {
   const size_t all = (size_t)hidden * tokens;
-  if (plan.splits >= 16 && all < 65536)
-    hipLaunchKernelGGL(gate_ranges_kernel<8>, dim3((unsigned)mnv_ceil_div(all, 32)), dim3(256), 0, s, part, pre, h, hidden, tokens, plan.splits, act);
+  if (ranges >= 16 && all < 65536)
+    hipLaunchKernelGGL(gate_ranges_kernel<8>, dim3((unsigned)mnv_ceil_div(all, 32)), dim3(256), 0, s, part, pre, h, hidden, tokens, ranges, act);
+  else if (ranges >= 4)
+    hipLaunchKernelGGL(gate_ranges_kernel<2>, dim3((unsigned)mnv_ceil_div(all, 128)), dim3(256), 0, s, part, pre, h, hidden, tokens, ranges, act);
   else
-    hipLaunchKernelGGL(gate_ranges_kernel<2>, dim3((unsigned)mnv_ceil_div(all, 128)), dim3(256), 0, s, part, pre, h, hidden, tokens, plan.splits, act);
+    hipLaunchKernelGGL(gate_ranges_kernel<1>, dim3((unsigned)mnv_ceil_div(all, 256)), dim3(256), 0, s, part, pre, h, hidden, tokens, ranges, act);
   return MNV_LAUNCH_STATUS();
 }
 
@@ -260,10 +252,36 @@ int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, fl
   return launch_split(plan, p, workspace, workspace ? workspace_bytes : 0, s);
 }
 
-// Whether the projections' product by this plan gates where it stores: on tiles in bf16 parts that need no k ranges, on small tiles, and of
-// few columns by k ranges where those are added.  What the plan gives to other tiles keeps them, and a kernel of its own gates.
-bool by_ranges(const SgemmPlan& plan) { return plan.skinny && plan.splits > 1; }
-bool gates(const SgemmPlan& plan) { return by_ranges(plan) || plan.tile || (plan.split && plan.splits == 1 && !plan.skinny); }
+// How the projections run.  SMALL, TILES: their product gates where it stores, on small tiles or on those in bf16 parts; RANGES: by k ranges,
+// which are gated where they are added; APART: as a plain product, and a kernel of its own gates.
+// The product's own plan decides, but for tiles in parts where it has others: those save the gating kernel, 3 us and 12 bytes a value
+// at 5 TB/s, and their cut tail, which that plan has not weighed.  us, as planned and on these tiles, both with w_out's product: 777 tokens
+// of 1001 -> 2731 158 / 130, 512 of 1024 -> 2816 99 / 91, 300 of 2048 -> 5632 219 / 191; kept: 400 of 1500 -> 1500 70 / 95, 128 of 1024 -> 4096 46 / 71.
+enum Way { SMALL, TILES, RANGES, APART };
+// Microseconds of a product on 128 x 128 tiles with a cut tail (as mnv_tail_plan prices it), or without one.
+double tiles_cost(int m, int n, int k, size_t ws_floats, int cus) {
+  const long long tiles = (long long)((m + 127) / 128) * ((n + 127) / 128);
+  const int slabs = (k + 15) / 16;
+  const MnvTailPlan t = mnv_tail_plan(tiles, slabs, 128 * 128, ws_floats, SplitPair::TAIL);
+  if (t.z <= 1) return split_cost(m, n, k, 1, cus);
+  const int rem = (int)(tiles - t.begin), per_cu = t.begin / cus, parts = (rem * t.z + cus - 1) / cus, len = (slabs + t.z - 1) / t.z;
+  return 1.3 * per_cu * ((slabs + 1) / 2) + 3.0 * ((per_cu + 1) / 2) + SplitPair::TAIL.slab * parts * len + SplitPair::TAIL.start * (parts - 1) +
+         2.0 + 0.46e-6 * sizeof(float) * rem * t.z * 128 * 128;
+}
+Way way(SgemmPlan* plan, int features, int hidden, int tokens, size_t ws_bytes) {
+  *plan = plan_sgemm(2 * hidden, tokens, features, ws_bytes / sizeof(float));
+  if (plan->tile) return SMALL;
+  if (plan->split && plan->splits == 1) return TILES;
+  if (!plan->skinny && tokens > 64) {
+    const int cus = mnv_cu_count();
+    if (tiles_cost((hidden + 3) / 4 * 8, tokens, features, ws_bytes / sizeof(float), cus) < plan->us + 3.0 + 12.0 * hidden * tokens / 5e6) {
+      *plan = SgemmPlan{false, 1};
+      plan->split = true;
+      return TILES;
+    }
+  }
+  return plan->splits > 1 ? RANGES : APART;
+}
 
 int launch_gate(const float* pre, float* h, int hidden, int tokens, int act, hipStream_t s) {
   const int quads = (hidden + 3) / 4;
@@ -306,9 +324,12 @@ extern "C" {
 
 size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens) {
   if (!sizes_ok(features, hidden, tokens, 0)) return 0;
-  const size_t in = mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
-  const bool keeps = !gates(plan_sgemm(2 * hidden, tokens, features, in / sizeof(float)));
-  return larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (keeps ? pre_bytes(hidden, tokens) : 0);
+  SgemmPlan plan;
+  const Way w = way(&plan, features, hidden, tokens, (size_t)-1);
+  const int rows = (hidden + 3) / 4 * 8;
+  size_t in = mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
+  if (w == TILES) in = sgemm_tail_bytes(plan, rows, tokens, features);
+  return larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (w == APART ? pre_bytes(hidden, tokens) : 0);
 }
 
 int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y, int features, int hidden,
@@ -321,29 +342,33 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
     ws = nullptr;
     bytes = 0;
   }
-  SgemmPlan plan = plan_sgemm(2 * hidden, tokens, features, bytes / sizeof(float));
+  SgemmPlan plan;
+  Way w = way(&plan, features, hidden, tokens, bytes);
+  int rc = MNV_OK, ranges = 1;
+  if (w == RANGES) {
+    rc = mnv_sgemm_nn_ranges(w_in, x, 2 * hidden, tokens, features, ws, bytes, &ranges, s);
+    if (rc) return rc;
+    if (ranges > 1) rc = launch_gate_ranges(reinterpret_cast<const float*>(ws), pre, h, hidden, tokens, ranges, activation, s);
+    else w = APART;
+  }
   float* kept = pre;
-  if (!gates(plan) && !kept) {
-    const size_t want = pre_bytes(hidden, tokens);
-    if (bytes >= want) {
+  if (w == APART && !kept) {
+    if (bytes >= pre_bytes(hidden, tokens)) {
       kept = reinterpret_cast<float*>(ws);
-      ws += want;
-      bytes -= want;
-      plan = plan_sgemm(2 * hidden, tokens, features, bytes / sizeof(float));
-    } else {  // nowhere to leave pre: one product, whatever its size
+      ws += pre_bytes(hidden, tokens);
+      bytes -= pre_bytes(hidden, tokens);
+    } else {  // nowhere to leave pre: on tiles, whatever the size
       plan = SgemmPlan{false, 1};
       plan.split = true;
+      w = TILES;
     }
   }
-  int rc;
-  if (by_ranges(plan)) {
-    rc = launch_gate_ranges(plan, w_in, x, pre, h, features, hidden, tokens, activation, reinterpret_cast<float*>(ws), s);
-  } else if (gates(plan)) {
-    rc = plan.tile || features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
-                                        : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
-  } else {
+  if (w == APART) {
     rc = mnv_sgemm_nn(w_in, x, kept, 2 * hidden, tokens, features, ws, bytes, stream);
     if (!rc) rc = launch_gate(kept, h, hidden, tokens, activation, s);
+  } else if (w != RANGES) {
+    rc = w == SMALL || features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
+                                         : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
   }
   return rc ? rc : mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
 }

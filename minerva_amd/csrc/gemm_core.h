@@ -128,6 +128,8 @@ struct MnvFetchMap {
 //   optional, for a store that needs a column's neighbouring rows together: static constexpr bool C_ROWS_OF_FOUR = true;
 //        Tiles in bf16 parts call c_store4 alone, lanes 2 i and 2 i + 1 at the same time, for rows m and m + 4 of one column
 //        (m a multiple of 8, M too); they have no k ranges then (a cut tail is fine).
+//   optional, for a product whose k ranges the caller adds: static constexpr bool C_LEAVES_RANGES = true;  bool leaves_ranges;
+//        If set, a launch with k ranges leaves them in the workspace, {M, N, ranges}, and nothing is stored.
 //   optional, for a product whose left operand depends on the column tile (batched products
 //   folded into the column index): static constexpr bool N_GROUPED = true;  int n_group;
 //        Tiles are then dealt m-tile by m-tile within groups of n_group consecutive column
@@ -185,6 +187,14 @@ struct MnvCRowsOfFour {
 };
 template <class P>
 struct MnvCRowsOfFour<P, std::enable_if_t<P::C_ROWS_OF_FOUR>> {
+  static constexpr bool value = true;
+};
+template <class P, class = void>
+struct MnvCLeavesRanges {
+  static constexpr bool value = false;
+};
+template <class P>
+struct MnvCLeavesRanges<P, std::enable_if_t<P::C_LEAVES_RANGES>> {
   static constexpr bool value = true;
 };
 template <class P, class = void>
@@ -1251,6 +1261,9 @@ static int mnv_gemm_launch(const P& prob, int splits, void* workspace, hipStream
                          tiles_n, tail.begin, tail.z);
       return MNV_LAUNCH_STATUS();
     }
+  }
+  if constexpr (MnvCLeavesRanges<P>::value) {
+    if (prob.leaves_ranges) return rc;
   }
   if constexpr (!MnvCRowsOfFour<P>::value) {
     if (splits > 1) rc = mnv_gemm_reduce_launch(prob, reinterpret_cast<const float*>(workspace), splits, s);

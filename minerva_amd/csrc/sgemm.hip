@@ -81,6 +81,24 @@ int sgemm_nn_large(const float* a, const float* b, float* c, int m, int n, int k
 
 }  // namespace
 
+int mnv_sgemm_nn_ranges(const float* a, const float* b, int m, int n, int k, void* workspace, size_t workspace_bytes, int* ranges, hipStream_t s) {
+  const SgemmPlan plan = plan_sgemm(m, n, k, workspace ? workspace_bytes / sizeof(float) : 0);
+  *ranges = plan.tile ? 1 : plan.splits;
+  if (*ranges == 1) return MNV_OK;
+  if (!plan.skinny) {  // as the launch rounds it: ranges of equal length
+    const int slabs = (k + 15) / 16, per = (slabs + plan.splits - 1) / plan.splits;
+    *ranges = (slabs + per - 1) / per;
+    if (*ranges == 1) return MNV_OK;
+  }
+  auto p = make_sgemm<true>(a, b, (float*)nullptr, m, n, k, SgemmEpilogue{nullptr, nullptr, 0});
+  p.leaves_ranges = true;
+  if (plan.skinny) return launch_skinny_columns(plan, p, workspace, s);
+  if (k % 4 == 0) return launch_plan(plan, p, workspace, workspace_bytes, s);
+  auto q = make_sgemm<false>(a, b, (float*)nullptr, m, n, k, SgemmEpilogue{nullptr, nullptr, 0});
+  q.leaves_ranges = true;
+  return launch_plan(plan, q, workspace, workspace_bytes, s);
+}
+
 extern "C" {
 
 size_t mnv_sgemm_nn_workspace_bytes(int m, int n, int k) {

@@ -60,6 +60,8 @@ struct SgemmNN {
   // at a time are not all the rows of one column (see launch_split).
   static constexpr bool N_GROUPED = true;
   int n_group;
+  static constexpr bool C_LEAVES_RANGES = true;
+  bool leaves_ranges;
   struct Res {
     mnv_rsrc a, b;
   };
@@ -479,6 +481,7 @@ SgemmNN<K4, TA, TB> make_sgemm(const float* a, const float* b, float* c, int m, 
   p.accumulate = e.accumulate;
   p.sgd_w = e.sgd_w; p.sgd_scale = e.sgd_scale;
   p.n_group = 1;
+  p.leaves_ranges = false;
   p.set_bk(16);
   return p;
 }
@@ -816,7 +819,7 @@ int launch_skinny_columns(const SgemmPlan& plan, const P& p, void* workspace, hi
   else if (p.N <= 8) launch_skinny<8, TB>(plan, p, part, s);
   else launch_skinny<MNV_SKINNY_COLUMNS, TB>(plan, p, part, s);
   const int rc = MNV_LAUNCH_STATUS();
-  if (rc || plan.splits == 1) return rc;
+  if (rc || plan.splits == 1 || p.leaves_ranges) return rc;
   return mnv_gemm_reduce_launch(p, part, plan.splits, s);
 }
 
@@ -882,3 +885,7 @@ int sgemm_t_impl(const float* a, const float* b, float* c, int m, int n, int k, 
 }
 
 }  // namespace
+
+// The product of mnv_sgemm_nn where its plan has k ranges, with these left in the workspace as {m, n, *ranges}, to be added by the
+// caller.  *ranges is 1, and nothing is launched, where it has none.
+int mnv_sgemm_nn_ranges(const float* a, const float* b, int m, int n, int k, void* workspace, size_t workspace_bytes, int* ranges, hipStream_t s);
