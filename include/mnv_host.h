@@ -129,6 +129,15 @@ int mnvh_tensor_op(void* runtime, const char* op, void* const* inputs, int n_inp
  *   "attention_backward" [scale, has_bias, has_lengths]
  *                                     inputs: diff, q, k, v, out, stats [, bias] [, lengths];
  *                                     results: dq, dk, dv [, dbias]
+ *   "rotary_forward" / "rotary_backward" [first, count, rotary_dim, interleaved, start, base, factor, context,
+ *                                     low_turns, high_turns, magnitude]
+ *                                     inputs: x, or the gradient [, positions]; result: its heads
+ *                                     first ... first + count - 1, turned
+ *   "gated_ffn_forward" [activation]  inputs: x, w_in, w_out; results: y, pre, h
+ *   "gated_ffn_backward" [activation] inputs: diff, x, w_in, w_out, pre, h; results: dx, dw_in, dw_out
+ *   "adamw" [bits, step, rate, beta1, beta2, eps, weight_decay, grad_scale, rates..., decays...]
+ *                                     inputs: arrays..., gradients..., m..., v...; results: arrays..., m..., v...
+ *   "adamw_values" [values of each array...]    inputs: m..., v... in 8 bits; results: m..., v...
  * (extents as in mnv_hip.h).  `outs` has room for `capacity` handles; *n_outs are written. */
 int mnvh_tensor_op_list(void* runtime, const char* op, void* const* inputs, int n_inputs,
                         const double* params, int n_params, void** outs, int capacity, int* n_outs);

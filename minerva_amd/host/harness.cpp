@@ -259,6 +259,30 @@ Tensor RunNamedOp(Runner* rt, const std::string& op, const std::vector<Tensor>& 
   return r;
 }
 
+// rotary's params: first, count, rotary_dim, interleaved, start, base, factor, context, low_turns, high_turns, magnitude
+template <class C>
+C RotaryParams(const double* p, int n) {
+  MNV_CHECK(n >= 11) << "rotary takes 11 numbers";
+  C c;
+  c.first = P(p, n, 0);
+  c.count = P(p, n, 1);
+  c.rotary_dim = P(p, n, 2);
+  c.interleaved = P(p, n, 3) != 0;
+  c.start = P(p, n, 4);
+  c.base = p[5];
+  c.factor = p[6];
+  c.context = P(p, n, 7);
+  c.low_turns = p[8];
+  c.high_turns = p[9];
+  c.magnitude = p[10];
+  return c;
+}
+GateType Gate(const double* p, int n) {
+  const int kind = P(p, n, 0);
+  MNV_CHECK(kind >= 0 && kind <= static_cast<int>(GateType::kGelu)) << "no activation " << kind;
+  return static_cast<GateType>(kind);
+}
+
 // The same for operators with any number of results.
 std::vector<Tensor> RunNamedOps(Runner* rt, const std::string& op, const std::vector<Tensor>& in, const double* params,
                                 int n_params) {
@@ -284,6 +308,46 @@ std::vector<Tensor> RunNamedOps(Runner* rt, const std::string& op, const std::ve
   if (op == "attention_backward") {  // inputs: diff, q, k, v, out, stats [, bias] [, lengths]
     optional(6, &bias, &lengths);
     return rt->AttentionBackward(in[0], in[1], in[2], in[3], in[4], in[5], bias, lengths, static_cast<float>(params[0]));
+  }
+  if (op == "rotary_forward" || op == "rotary_backward") {  // inputs: x [, positions]
+    MNV_CHECK(n_inputs == 1 || n_inputs == 2) << op << " takes 1 or 2 inputs";
+    const Tensor positions = n_inputs == 2 ? in[1] : Tensor();
+    if (op == "rotary_forward") return {rt->RotaryForward(in[0], positions, RotaryParams<RotaryForwardClosure>(params, n_params))};
+    return {rt->RotaryBackward(in[0], positions, RotaryParams<RotaryBackwardClosure>(params, n_params))};
+  }
+  if (op == "gated_ffn_forward") {  // params: activation; inputs: x, w_in, w_out
+    MNV_CHECK_EQ(n_inputs, 3) << op << " takes 3 inputs";
+    return rt->GatedFFNForward(in[0], in[1], in[2], Gate(params, n_params));
+  }
+  if (op == "gated_ffn_backward") {  // params: activation; inputs: diff, x, w_in, w_out, pre, h
+    MNV_CHECK_EQ(n_inputs, 6) << op << " takes 6 inputs";
+    return rt->GatedFFNBackward(in[0], in[1], in[2], in[3], in[4], in[5], Gate(params, n_params));
+  }
+  if (op == "adamw") {  // params: bits, step, rate, beta1, beta2, eps, weight_decay, grad_scale, a rate each, a decay each
+    MNV_CHECK(n_inputs > 0 && n_inputs % 4 == 0) << op << " takes arrays, gradients and both moments of each";
+    const int n = n_inputs / 4;
+    MNV_CHECK_EQ(n_params, 8 + 2 * n) << op << " takes 8 numbers, and a rate and a decay for every array";
+    AdamWClosure c;
+    c.bits = P(params, n_params, 0);
+    c.step = P(params, n_params, 1);
+    c.rate = params[2];
+    c.beta1 = params[3];
+    c.beta2 = params[4];
+    c.eps = params[5];
+    c.weight_decay = params[6];
+    c.grad_scale = params[7];
+    c.rates.assign(params + 8, params + 8 + n);
+    c.decays.assign(params + 8 + n, params + 8 + 2 * n);
+    return rt->AdamW(in, std::move(c));
+  }
+  if (op == "adamw_values") {  // params: values of each array; inputs: m..., v...
+    MNV_CHECK(n_params > 0 && n_inputs == 2 * n_params) << op << " takes both moments of every array, and their numbers of values";
+    std::vector<Scale> sizes;
+    for (int i = 0; i < n_params; ++i) {
+      MNV_CHECK(P(params, n_params, i) > 0) << op << ": an array without values";
+      sizes.push_back(Scale{P(params, n_params, i)});
+    }
+    return rt->AdamWValues(in, sizes);
   }
   return {RunNamedOp(rt, op, in, params, n_params)};
 }

@@ -86,6 +86,12 @@ MNV_INSTALL_COMPUTE_FN(AttentionForwardClosure, hip::AttentionForward)
 MNV_INSTALL_COMPUTE_FN(AttentionBackwardClosure, hip::AttentionBackward)
 MNV_INSTALL_COMPUTE_FN(RelativeBiasForwardClosure, hip::RelativeBiasForward)
 MNV_INSTALL_COMPUTE_FN(RelativeBiasBackwardClosure, hip::RelativeBiasBackward)
+MNV_INSTALL_COMPUTE_FN(RotaryForwardClosure, hip::RotaryForward)
+MNV_INSTALL_COMPUTE_FN(RotaryBackwardClosure, hip::RotaryBackward)
+MNV_INSTALL_COMPUTE_FN(GatedFFNForwardClosure, hip::GatedFFNForward)
+MNV_INSTALL_COMPUTE_FN(GatedFFNBackwardClosure, hip::GatedFFNBackward)
+MNV_INSTALL_COMPUTE_FN(AdamWClosure, hip::AdamWStep)
+MNV_INSTALL_COMPUTE_FN(AdamWValuesClosure, hip::AdamWValues)
 MNV_INSTALL_DATAGEN_FN(ArrayLoaderClosure, hip::ArrayLoader)
 MNV_INSTALL_DATAGEN_FN(FillClosure, hip::Fill)
 MNV_INSTALL_DATAGEN_FN(RandnClosure, hip::Randn)
@@ -161,6 +167,12 @@ MNV_SIMPLE_OP(AttentionForwardOp, ComputeFnWithClosure, AttentionForwardClosure,
 MNV_SIMPLE_OP(AttentionBackwardOp, ComputeFnWithClosure, AttentionBackwardClosure, "attention bp")
 MNV_SIMPLE_OP(RelativeBiasForwardOp, ComputeFnWithClosure, RelativeBiasForwardClosure, "relative bias ff")
 MNV_SIMPLE_OP(RelativeBiasBackwardOp, ComputeFnWithClosure, RelativeBiasBackwardClosure, "relative bias bp")
+MNV_SIMPLE_OP(RotaryForwardOp, ComputeFnWithClosure, RotaryForwardClosure, "rotary ff")
+MNV_SIMPLE_OP(RotaryBackwardOp, ComputeFnWithClosure, RotaryBackwardClosure, "rotary bp")
+MNV_SIMPLE_OP(GatedFFNForwardOp, ComputeFnWithClosure, GatedFFNForwardClosure, "gated ffn ff")
+MNV_SIMPLE_OP(GatedFFNBackwardOp, ComputeFnWithClosure, GatedFFNBackwardClosure, "gated ffn bp")
+MNV_SIMPLE_OP(AdamWOp, ComputeFnWithClosure, AdamWClosure, "adamw")
+MNV_SIMPLE_OP(AdamWValuesOp, ComputeFnWithClosure, AdamWValuesClosure, "adamw values")
 
 class MatMultBiasOp : public ComputeFnWithClosure<MatMultBiasClosure> {
  public:

@@ -486,6 +486,74 @@ Tensor Runner::RelativeBiasBackward(const Tensor& diff, int buckets, int q_len, 
   return Compute({diff}, Scale{diff->size[1], buckets}, op);
 }
 
+namespace {
+template <class C>
+Scale Turned(const Tensor& x, const C& c) {
+  MNV_CHECK(x) << "null tensor";
+  MNV_CHECK_EQ(x->size.NumDims(), 4u) << "rotary positions take {head_dim, heads, length, batch}";
+  MNV_CHECK(c.count > 0) << "bad number of heads";
+  return Scale{x->size[0], c.count, x->size[2], x->size[3]};
+}
+std::vector<Tensor> WithPositions(const Tensor& x, const Tensor& positions) {
+  return positions ? std::vector<Tensor>{x, positions} : std::vector<Tensor>{x};
+}
+}  // namespace
+
+Tensor Runner::RotaryForward(const Tensor& x, const Tensor& positions, RotaryForwardClosure c) {
+  auto op = std::make_shared<RotaryForwardOp>();
+  c.has_positions = positions != nullptr;
+  op->closure = c;
+  return Compute(WithPositions(x, positions), Turned(x, c), op);
+}
+
+Tensor Runner::RotaryBackward(const Tensor& diff, const Tensor& positions, RotaryBackwardClosure c) {
+  auto op = std::make_shared<RotaryBackwardOp>();
+  c.has_positions = positions != nullptr;
+  op->closure = c;
+  return Compute(WithPositions(diff, positions), Turned(diff, c), op);
+}
+
+std::vector<Tensor> Runner::GatedFFNForward(const Tensor& x, const Tensor& w_in, const Tensor& w_out, GateType type) {
+  MNV_CHECK(x && w_in && w_out) << "null tensor";
+  MNV_CHECK(x->size.NumDims() >= 2u && x->size[0] > 0) << "(gated ffn) takes features and tokens";
+  MNV_CHECK(w_out->size.NumDims() == 2u && w_out->size[1] > 0 && w_out->size[1] <= 0x3fffffff) << "(gated ffn) the second weights are {features, hidden}";
+  auto op = std::make_shared<GatedFFNForwardOp>();
+  op->closure = {type};
+  const int tokens = x->size.Prod() / x->size[0], hidden = w_out->size[1];
+  return Compute({x, w_in, w_out}, std::vector<Scale>{x->size, Scale{2 * hidden, tokens}, Scale{hidden, tokens}}, op);
+}
+
+std::vector<Tensor> Runner::GatedFFNBackward(const Tensor& diff, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& pre,
+                                             const Tensor& h, GateType type) {
+  MNV_CHECK(diff && x && w_in && w_out && pre && h) << "null tensor";
+  auto op = std::make_shared<GatedFFNBackwardOp>();
+  op->closure = {type};
+  std::vector<Tensor> r = Compute({diff, x, w_in, w_out, pre, h}, std::vector<Scale>{x->size, w_in->size, w_out->size, pre->size}, op);
+  r.pop_back();  // dpre
+  return r;
+}
+
+std::vector<Tensor> Runner::AdamW(const std::vector<Tensor>& inputs, AdamWClosure c) {
+  const size_t n = c.rates.size();
+  MNV_CHECK(n > 0 && inputs.size() == 4 * n) << "(adamw) takes arrays, gradients and both moments of each";
+  std::vector<Scale> sizes;
+  for (size_t k : {size_t(0), size_t(2), size_t(3)})
+    for (size_t i = 0; i < n; ++i) {
+      MNV_CHECK(inputs[k * n + i]) << "null tensor";
+      sizes.push_back(inputs[k * n + i]->size);
+    }
+  auto op = std::make_shared<AdamWOp>();
+  op->closure = std::move(c);
+  return Compute(inputs, sizes, op);
+}
+
+std::vector<Tensor> Runner::AdamWValues(const std::vector<Tensor>& inputs, const std::vector<Scale>& sizes) {
+  MNV_CHECK(!sizes.empty() && inputs.size() == 2 * sizes.size()) << "(adamw values) takes both moments of every array";
+  std::vector<Scale> outs = sizes;
+  outs.insert(outs.end(), sizes.begin(), sizes.end());
+  return Compute(inputs, outs, std::make_shared<AdamWValuesOp>());
+}
+
 // ---------------------------------------------------------------- fused operators
 
 Tensor Runner::ConvForwardRelu(const Tensor& src, const Tensor& filter, const Tensor& bias,

@@ -148,6 +148,19 @@ class Runner : public DeviceListener {
   Tensor RelativeBiasBackward(const Tensor& diff, int buckets, int q_len, int k_len, int q_start, int max_distance,
                               bool both_ways);
 
+  // heads [c.first, c.first + c.count) of x {head_dim, heads, length, batch}, with positions {length, batch} or none
+  Tensor RotaryForward(const Tensor& x, const Tensor& positions, RotaryForwardClosure c);
+  Tensor RotaryBackward(const Tensor& diff, const Tensor& positions, RotaryBackwardClosure c);
+  // x {features, ...}, w_in {2 hidden, features}, w_out {features, hidden}; {y, pre {2 hidden, tokens}, h {hidden, tokens}}
+  std::vector<Tensor> GatedFFNForward(const Tensor& x, const Tensor& w_in, const Tensor& w_out, GateType type);
+  // {dx, dw_in, dw_out}
+  std::vector<Tensor> GatedFFNBackward(const Tensor& diff, const Tensor& x, const Tensor& w_in, const Tensor& w_out, const Tensor& pre,
+                                       const Tensor& h, GateType type);
+  // inputs {params..., grads..., m..., v...}; {params..., m..., v...}
+  std::vector<Tensor> AdamW(const std::vector<Tensor>& inputs, AdamWClosure c);
+  // the values of 8-bit moments {m..., v...} of arrays of these extents; {m..., v...}
+  std::vector<Tensor> AdamWValues(const std::vector<Tensor>& inputs, const std::vector<Scale>& sizes);
+
   // The opt-in fused operators (hip_fused_ops.h).  Each returns the bits of the pair of calls
   // named in its comment.
   // ReluForward(ConvForward(src, filter, bias, info))

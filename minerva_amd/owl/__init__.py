@@ -123,7 +123,7 @@ class NArray(object):
 
     def _ops(self, name, others=(), params=()):
         ins = [self._t] + [o._t for o in others]
-        return [NArray(self._rt, t) for t in self._rt.top_list(name, ins, params)]
+        return [NArray(self._rt, t) for t in self._rt.top_list(name, ins, params, max(8, len(ins)))]
 
     def _binary(self, rhs, kind):
         """NArray (op) NArray: same shape -> element-wise; otherwise rhs is replicated along
@@ -304,6 +304,44 @@ class NArray(object):
     def relative_bias_backward(diff, buckets, q_len, k_len, q_start, max_distance, both_ways):
         return diff._op("relative_bias_backward", params=[int(buckets), int(q_len), int(k_len), int(q_start),
                                                           int(max_distance), bool(both_ways)])
+
+    @staticmethod
+    def rotary_forward(x, params, positions=None):
+        """params: as `sequence.Rotary` lists them"""
+        return x._ops("rotary_forward", [] if positions is None else [positions], params)[0]
+
+    @staticmethod
+    def rotary_backward(diff, params, positions=None):
+        return diff._ops("rotary_backward", [] if positions is None else [positions], params)[0]
+
+    @staticmethod
+    def gated_ffn_forward(x, w_in, w_out, activation):
+        """[result, and pre and h for the backward pass]"""
+        return x._ops("gated_ffn_forward", [w_in, w_out], [int(activation)])
+
+    @staticmethod
+    def gated_ffn_backward(diff, x, w_in, w_out, pre, h, activation):
+        """[gradient of x, of w_in, of w_out]"""
+        return diff._ops("gated_ffn_backward", [x, w_in, w_out, pre, h], [int(activation)])
+
+    @staticmethod
+    def adamw(arrays, grads, m, v, bits, step, rate, beta1, beta2, eps, weight_decay, grad_scale, rates, decays):
+        """[arrays], [m], [v] after one step; lists of the same length, a rate and a decay for every array"""
+        n = len(arrays)
+        if not n or not all(len(x) == n for x in (grads, m, v, rates, decays)):
+            raise ValueError("adamw: arrays, gradients, moments, rates and decays are lists of one length")
+        out = arrays[0]._ops("adamw", list(arrays[1:]) + list(grads) + list(m) + list(v),
+                             [int(bits), int(step), rate, beta1, beta2, eps, weight_decay, grad_scale] + list(rates) + list(decays))
+        return out[:n], out[n:2 * n], out[2 * n:]
+
+    @staticmethod
+    def adamw_values(m, v, sizes):
+        """[m], [v]: the values that 8-bit moments of arrays of so many values stand for"""
+        n = len(sizes)
+        if not n or len(m) != n or len(v) != n:
+            raise ValueError("adamw_values: moments and sizes are lists of one length")
+        out = m[0]._ops("adamw_values", list(m[1:]) + list(v), [int(s) for s in sizes])
+        return out[:n], out[n:]
 
     # ---- reductions and shape (libowl.pyx:345-387)
     def _reduce(self, dims, kind):

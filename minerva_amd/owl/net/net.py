@@ -3,7 +3,7 @@
 A network is a DAG of ComputeUnits.  `forward` walks it in topological order handing every
 unit the outputs of its bottom units (a dict name -> NArray), `backward` walks it in reverse
 with the sensitivities, weighted units keep `weightgrad` / `biasgrad`, and `weight_update`
-applies momentum SGD with weight decay.  Shapes follow Minerva: images are [W, H, C, N],
+applies momentum SGD with weight decay, or an AdamW step over all weights at once.  Shapes follow Minerva: images are [W, H, C, N],
 matrices [rows, N]."""
 import collections
 
@@ -536,6 +536,7 @@ class Net(object):
         self.name_to_uid = {}
         self.loss_uids = []
         self.accuracy_uids = []
+        self.optimizer = None  # a sequence.AdamW instead of the units' own momentum SGD
 
     def add_unit(self, unit):
         uid = len(self.units)
@@ -627,8 +628,21 @@ class Net(object):
                                       self.batch_size)
 
     def weight_update(self):
+        if self.optimizer is not None:
+            return self._optimizer_update()
         for uid in self.get_weighted_unit_ids():
             self.update(uid)
+
+    def _optimizer_update(self):
+        units = [self.units[uid] for uid in self.get_weighted_unit_ids()]
+        pairs = [(u, name) for u in units for name in ("weight", "bias")]
+        self.optimizer.rate, self.optimizer.weight_decay = self.current_lr, self.base_weight_decay
+        new = self.optimizer.step([getattr(u, n) for u, n in pairs], [getattr(u, n + "grad") for u, n in pairs],
+                                  [getattr(u, "lr_mult_" + n[0]) for u, n in pairs], [getattr(u, "decay_mult_" + n[0]) for u, n in pairs],
+                                  1.0 / self.batch_size)
+        for (u, n), a in zip(pairs, new):
+            setattr(u, n, a)
+            setattr(u, n + "grad", None)
 
     def init_weights(self, seed=None):
         """Applies every weighted unit's fillers (the reference does it lazily in the first

@@ -6,13 +6,15 @@ reads the same prototxt TEXT into plain message objects, which is all the builde
 The snapshot layout is the reference's: a folder `<dir>/snapshot<idx>/` holding, per weighted
 layer, `<layer>_weights.dat`, `<layer>_weightdelta.dat`, `<layer>_bias.dat` and
 `<layer>_biasdelta.dat` as raw float32 in the arrays' element order ('/' in a layer name
-becomes '_')."""
+becomes '_').  A network whose solver is AdamW also keeps `adamw_steps.dat`, the number of steps as one float32, and
+`<layer>_weights_m.dat`, `<layer>_weights_v.dat`, `<layer>_bias_m.dat` and `<layer>_bias_v.dat`, the moments as they are held."""
 import os
 import re
 
 import numpy as np
 
 from .. import from_numpy, zeros
+from .. import sequence as _seq
 from . import net as _net
 
 
@@ -136,6 +138,9 @@ class NetBuilder(object):
         owl_net.momentum = s.get("momentum", 0.0)
         owl_net.solver = s
         owl_net.lr_policy = s.get("lr_policy", "fixed")
+        if s.get("type", "SGD") == "AdamW":  # momentum is beta1, momentum2 beta2, delta what the root is guarded by
+            owl_net.optimizer = _seq.AdamW(owl_net.base_lr, s.get("momentum", 0.9), s.get("momentum2", 0.999), s.get("delta", 1e-8),
+                                           owl_net.base_weight_decay, s.get("moment_bits", 32))
         stacked_layers, top_name_to_layer = {}, {}
         owl_net.data_layers = []
         for l in self.netconfig.get_all("layer"):
@@ -194,6 +199,22 @@ def save_net_to_file(owl_net, weightpath, snapshotidx):
             if arr is None:  # no update yet: the momentum term is zero
                 arr = zeros(ref.shape)
             arr.to_numpy().astype(np.float32).ravel().tofile("%s_%s.dat" % (base, suffix))
+    opt = owl_net.optimizer
+    if opt is not None and opt.m is not None:
+        for (base, shape), m, v in zip(_moment_files(owl_net, folder), opt.m, opt.v):
+            m.to_numpy().ravel().tofile(base + "_m.dat")
+            v.to_numpy().ravel().tofile(base + "_v.dat")
+        np.array([opt.steps], np.float32).tofile(os.path.join(folder, "adamw_steps.dat"))
+
+
+def _moment_files(owl_net, folder):
+    """Of every weight and bias in the optimizer's order: the name its moments' files begin with, and its extents."""
+    out = []
+    for uid in owl_net.get_weighted_unit_ids():
+        unit = owl_net.units[uid]
+        base = os.path.join(folder, unit.name.replace("/", "_"))
+        out += [(base + "_weights", unit.wshape), (base + "_bias", unit.bshape)]
+    return out
 
 
 def init_net_from_file(owl_net, weightpath, snapshotidx):
@@ -215,4 +236,22 @@ def init_net_from_file(owl_net, weightpath, snapshotidx):
             dpath = "%s_%s.dat" % (base, delta)
             if os.path.isfile(dpath) and os.path.getsize(dpath) == 4 * want:
                 setattr(unit, delta, from_numpy(np.fromfile(dpath, np.float32)).reshape(shape))
+    if owl_net.optimizer is not None:
+        _init_moments(owl_net, folder, need_reinit)
     return need_reinit
+
+
+def _init_moments(owl_net, folder, need_reinit):
+    """The optimizer's state, all of it or none."""
+    opt = owl_net.optimizer
+    files = _moment_files(owl_net, folder)
+    sizes = [int(np.prod(shape)) for _, shape in files]
+    steps = os.path.join(folder, "adamw_steps.dat")
+    want = [(base + end, opt.moment_shape(n)) for end in ("_m.dat", "_v.dat") for (base, _), n in zip(files, sizes)]
+    if not os.path.isfile(steps) or any(not os.path.isfile(p) or os.path.getsize(p) != 4 * int(np.prod(s)) for p, s in want):
+        opt.m = opt.v = opt.sizes = None
+        opt.steps = 0
+        need_reinit.append("adamw moments")
+        return
+    held = [from_numpy(np.fromfile(p, np.float32)).reshape(s) for p, s in want]
+    opt.m, opt.v, opt.sizes, opt.steps = held[:len(files)], held[len(files):], sizes, int(np.fromfile(steps, np.float32)[0])
