@@ -492,13 +492,20 @@ int mnv_rotary_bwd(const float* dy, const float* positions, float* dx, int head_
  *   dx = w_in' dpre,  dw_in = dpre x',  dw_out = dy h'
  * activation: 0 sigmoid, 1 relu (slope 0 at 0), 2 tanh, 3 silu x / (1 + exp(-x)), 4 gelu x Phi(x) with the normal distribution's Phi.
  * forward writes h, and pre unless it is NULL (no backward pass follows); backward reads both, and writes dpre, which
- * may be pre itself; dx may be NULL if nobody needs it.  Sums are those of the products above (mnv_sgemm_nn), whose
- * workspace and plans they have; a workspace is used if it is aligned to 16 bytes, and without one pre == NULL costs
- * few tokens more time.  Each matrix holds less than 2^29 values. ---- */
+ * may be pre itself; dx may be NULL if nobody needs it.  Each matrix holds less than 2^29 values.
+ * A workspace is used if it is aligned to 16 bytes.  Large products, from 5 GFLOP on, run in pairs of fp16 numbers where the workspace
+ * holds those: every value is rounded to 22 bits, 2^-22 of itself or 2^-39 of the largest in its row of the left matrix (column of the right
+ * one; rows and columns over which the product sums), whichever is more, products are exact but for 2^-22 and summed in fp32.  The result is as near to the
+ * exact one as fp32 products' is, whose error is that of the sum.  An infinity or NaN then gives NaN in all of the results that its row has a part
+ * in.  Other products, and all of them with a workspace that is too small for it, are those of mnv_sgemm_nn.  Without a workspace pre == NULL costs
+ * few tokens more time.  mnv_gated_ffn_plan: which products run in pairs with workspaces of these sizes, as a sum of 1 pre, 2 y, 4 dh,
+ * 8 dx, 16 dw_in, 32 dw_out. ---- */
 size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens);
 int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y,
                       int features, int hidden, int tokens, int activation, void* workspace,
                       size_t workspace_bytes, mnv_stream_t stream);
+int mnv_gated_ffn_plan(int features, int hidden, int tokens, size_t fwd_workspace_bytes,
+                       size_t bwd_workspace_bytes, int* pairs);
 size_t mnv_gated_ffn_bwd_workspace_bytes(int features, int hidden, int tokens);
 int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, const float* pre,
                       const float* h, const float* dy, float* dpre, float* dx, float* dw_in, float* dw_out,

@@ -7,7 +7,9 @@
 // weights.  All products are those of the SGEMM (sgemm_core.h); what lies between them is done where a product is
 // stored: the gate forward, where both projections of a row meet in one tile, and dpre backward, which is all that
 // is kept of dh.
-#include "sgemm_core.h"
+#include <algorithm>
+
+#include "pair_gemm.h"
 
 namespace {
 
@@ -40,6 +42,7 @@ __device__ __forceinline__ float gated(int kind, float gate, float up) {
   return value * up;
 }
 
+typedef float Two __attribute__((ext_vector_type(2), aligned(4)));
 // Four rows from p on, of which `left` exist.
 __device__ __forceinline__ void store_rows(float* p, int left, const float (&x)[4]) {
   if (left >= 4) {
@@ -119,18 +122,25 @@ struct GatedIn {
     if (!(m & 4)) h[(size_t)n * hidden + row] = gated(act, x, other);
   }
   static constexpr bool C_STORE4 = true, C_ROWS_OF_FOUR = true;
+  struct Fetched {};
+  __device__ Fetched c_fetch4(int, int) const { return {}; }
+  __device__ void c_store4_with(int m, int n, const float (&x)[4], const Fetched&) const { c_store4(m, n, x); }
   __device__ void c_store4(int m, int n, const float (&x)[4]) const {
     const int row = m / 8 * 4, left = hidden - row;
     const bool up = m & 4;
-    float other[4], r[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)  // quad_perm 1, 0, 3, 2
-      other[q] = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x[q]), 0xb1, 0xf, 0xf, true));
     if (pre) store_rows(pre + (size_t)n * hidden * 2 + row + (up ? hidden : 0), left, x);
-    // each lane of the pair gates two of the four rows
+    // The lane of the gate takes rows 0 and 1, that of the up projection 2 and 3; each gives the other what it wants (quad_perm 1, 0, 3, 2).
+    float r[2];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) r[q] = gated(act, up ? other[q] : x[q], up ? x[q] : other[q]);
-    if (!up) store_rows(h + (size_t)n * hidden + row, left, r);
+    for (int q = 0; q < 2; ++q) {
+      const float give = up ? x[q] : x[q + 2];
+      const float got = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, give), 0xb1, 0xf, 0xf, true));
+      r[q] = gated(act, up ? got : x[q], up ? x[q + 2] : got);
+    }
+    float* const p = h + (size_t)n * hidden + row + (up ? 2 : 0);
+    const int rest = left - (up ? 2 : 0);
+    if (rest >= 2) *reinterpret_cast<Two*>(p) = Two{r[0], r[1]};
+    else if (rest == 1) p[0] = r[0];
   }
 };
 
@@ -149,16 +159,23 @@ struct GatedOutBack : SgemmNN<K4, true, false> {
     dpre[at] = dh * up * slope;
     dpre[at + hidden] = dh * value;
   }
-  __device__ void c_store4(int m, int n, const float (&dh)[4]) const {
+  struct Fetched {
+    mnv_f4u gate, up;
+  };
+  __device__ Fetched c_fetch4(int m, int n) const {
+    const size_t at = (size_t)n * hidden * 2 + m;
+    if (m + 3 < this->M) return {*reinterpret_cast<const mnv_f4u*>(pre + at), *reinterpret_cast<const mnv_f4u*>(pre + at + hidden)};
+    return {};
+  }
+  __device__ void c_store4_with(int m, int n, const float (&dh)[4], const Fetched& f) const {
     if (m + 3 < this->M) {
       const size_t at = (size_t)n * hidden * 2 + m;
-      const mnv_f4u gate = *reinterpret_cast<const mnv_f4u*>(pre + at), up = *reinterpret_cast<const mnv_f4u*>(pre + at + hidden);
       mnv_f4u dg, du;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         float value, slope;
-        activate(act, gate[q], value, slope);
-        dg[q] = dh[q] * up[q] * slope;
+        activate(act, f.gate[q], value, slope);
+        dg[q] = dh[q] * f.up[q] * slope;
         du[q] = dh[q] * value;
       }
       *reinterpret_cast<mnv_f4u*>(dpre + at) = dg;
@@ -169,6 +186,7 @@ struct GatedOutBack : SgemmNN<K4, true, false> {
         if (m + q < this->M) c_store(m + q, n, dh[q]);
     }
   }
+  __device__ void c_store4(int m, int n, const float (&dh)[4]) const { c_store4_with(m, n, dh, c_fetch4(m, n)); }
 };
 
 // h = act(gate) * up from pre as a product of its own left it: four rows a thread.
@@ -237,8 +255,7 @@ int launch_gate_ranges(const float* part, float* pre, float* h, int hidden, int 
 }
 
 template <bool K4>
-int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens,
-                    int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
+GatedIn<K4> make_gated_in(const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens, int act) {
   GatedIn<K4> p;
   p.A = w_in; p.B = x; p.pre = pre; p.h = h;
   p.M = (hidden + 3) / 4 * 8; p.N = tokens; p.K = features;
@@ -246,18 +263,18 @@ int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, fl
   p.lda = 2 * hidden; p.ldb = features;
   p.n_group = 1;
   p.set_bk(16);
+  return p;
+}
+template <bool K4>
+int launch_gated_in(const SgemmPlan& plan, const float* w_in, const float* x, float* pre, float* h, int features, int hidden, int tokens,
+                    int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  const GatedIn<K4> p = make_gated_in<K4>(w_in, x, pre, h, features, hidden, tokens, act);
   if constexpr (K4) {
     if (plan.tile) return launch_small_tiles(plan, p, s);
   }
   return launch_split(plan, p, workspace, workspace ? workspace_bytes : 0, s);
 }
 
-// How the projections run.  SMALL, TILES: their product gates where it stores, on small tiles or on those in bf16 parts; RANGES: by k ranges,
-// which are gated where they are added; APART: as a plain product, and a kernel of its own gates.
-// The product's own plan decides, but for tiles in parts where it has others: those save the gating kernel, 3 us and 12 bytes a value
-// at 5 TB/s, and their cut tail, which that plan has not weighed.  us, as planned and on these tiles, both with w_out's product: 777 tokens
-// of 1001 -> 2731 158 / 130, 512 of 1024 -> 2816 99 / 91, 300 of 2048 -> 5632 219 / 191; kept: 400 of 1500 -> 1500 70 / 95, 128 of 1024 -> 4096 46 / 71.
-enum Way { SMALL, TILES, RANGES, APART };
 // Microseconds of a product on 128 x 128 tiles with a cut tail (as mnv_tail_plan prices it), or without one.
 double tiles_cost(int m, int n, int k, size_t ws_floats, int cus) {
   const long long tiles = (long long)((m + 127) / 128) * ((n + 127) / 128);
@@ -268,6 +285,12 @@ double tiles_cost(int m, int n, int k, size_t ws_floats, int cus) {
   return 1.3 * per_cu * ((slabs + 1) / 2) + 3.0 * ((per_cu + 1) / 2) + SplitPair::TAIL.slab * parts * len + SplitPair::TAIL.start * (parts - 1) +
          2.0 + 0.46e-6 * sizeof(float) * rem * t.z * 128 * 128;
 }
+// How the projections run.  SMALL, TILES: their product gates where it stores, on small tiles or on those in bf16 parts; RANGES: by k ranges,
+// which are gated where they are added; APART: as a plain product, and a kernel of its own gates.
+// The product's own plan decides, but for tiles in parts where it has others: those save the gating kernel, 3 us and 12 bytes a value
+// at 5 TB/s, and their cut tail, which that plan has not weighed.  us, as planned and on these tiles, both with w_out's product: 777 tokens
+// of 1001 -> 2731 158 / 130, 512 of 1024 -> 2816 99 / 91, 300 of 2048 -> 5632 219 / 191; kept: 400 of 1500 -> 1500 70 / 95, 128 of 1024 -> 4096 46 / 71.
+enum Way { SMALL, TILES, RANGES, APART };
 Way way(SgemmPlan* plan, int features, int hidden, int tokens, size_t ws_bytes) {
   *plan = plan_sgemm(2 * hidden, tokens, features, ws_bytes / sizeof(float));
   if (plan->tile) return SMALL;
@@ -293,13 +316,18 @@ int launch_gate(const float* pre, float* h, int hidden, int tokens, int act, hip
 }
 
 template <bool K4>
-int launch_out_back(const SgemmPlan& plan, const float* w_out, const float* dy, const float* pre, float* dpre, int features, int hidden,
-                    int tokens, int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
+GatedOutBack<K4> make_out_back(const float* w_out, const float* dy, const float* pre, float* dpre, int features, int hidden, int tokens, int act) {
   GatedOutBack<K4> p;
   static_cast<SgemmNN<K4, true, false>&>(p) =
       make_sgemm<K4, true, false>(w_out, dy, nullptr, hidden, tokens, features, SgemmEpilogue{nullptr, nullptr, 0});
   p.pre = pre; p.dpre = dpre;
   p.hidden = hidden; p.act = act;
+  return p;
+}
+template <bool K4>
+int launch_out_back(const SgemmPlan& plan, const float* w_out, const float* dy, const float* pre, float* dpre, int features, int hidden,
+                    int tokens, int act, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  const GatedOutBack<K4> p = make_out_back<K4>(w_out, dy, pre, dpre, features, hidden, tokens, act);
   if constexpr (K4) {
     if (plan.skinny) return launch_skinny_columns(plan, p, workspace, s);
     if (plan.tile) return launch_small_tiles(plan, p, s);
@@ -312,6 +340,50 @@ bool sizes_ok(int features, int hidden, int tokens, int act) {
   const long long most = (1LL << 29) - 1;
   return features > 0 && hidden > 0 && tokens > 0 && act >= 0 && act < ACT_COUNT && 2LL * hidden <= most / features &&
          2LL * hidden <= most / tokens && features <= most / tokens;
+}
+
+// The six products.  Operands' rows are the result's rows (the left one's) and columns; a matrix lies with its rows contiguous.
+struct Product {
+  PairOperand a, b;
+  double store_bytes;  // that its store moves for a value
+};
+Product product_in(const float* w_in, const float* x, int features, int hidden, int tokens) {
+  return {{w_in, 2 * (size_t)hidden, (hidden + 3) / 4 * 8, features, false, hidden}, {x, (size_t)features, tokens, features, true, 0}, 6.0};
+}
+Product product_out(const float* w_out, const float* h, int features, int hidden, int tokens) {
+  return {{w_out, (size_t)features, features, hidden, false, 0}, {h, (size_t)hidden, tokens, hidden, true, 0}, 4.0};
+}
+Product product_dh(const float* w_out, const float* dy, int features, int hidden, int tokens) {
+  return {{w_out, (size_t)features, hidden, features, true, 0}, {dy, (size_t)features, tokens, features, true, 0}, 16.0};
+}
+Product product_dx(const float* w_in, const float* dpre, int features, int hidden, int tokens) {
+  return {{w_in, 2 * (size_t)hidden, features, 2 * hidden, true, 0}, {dpre, 2 * (size_t)hidden, tokens, 2 * hidden, true, 0}, 4.0};
+}
+// dw = left right', left {rows, tokens}, right {columns, tokens}
+Product product_dw(const float* left, const float* right, int rows, int columns, int tokens) {
+  return {{left, (size_t)rows, rows, tokens, false, 0}, {right, (size_t)columns, columns, tokens, false, 0}, 4.0};
+}
+// Whether a product runs in pairs: where that is estimated at less than 92% of the SGEMM's time, and the workspace holds it.  The
+// SGEMM's own estimate is 1.2 times too low where products of this size follow each other.
+bool in_pairs(const Product& p, int most_ranges, size_t ws_bytes, PairPlan* plan) {
+  // below 5 GFLOP the four launches of the packing alone take half of the time
+  if (!pair_fits(p.a, p.b) || 2.0 * p.a.rows * p.b.rows * p.a.k < 5e9) return false;
+  const int cus = mnv_cu_count();
+  *plan = pair_plan(p.a, p.b, most_ranges, p.store_bytes, cus);
+  const SgemmPlan other = plan_unlimited(p.a.rows, p.b.rows, p.a.k, cus);
+  double us = other.us;
+  if ((other.split && other.splits == 1) || p.a.gate) us = std::min(us, tiles_cost(p.a.rows, p.b.rows, p.a.k, (size_t)-1, cus));
+  return plan->us < 0.92 * 1.2 * us && plan->bytes() <= ws_bytes;
+}
+size_t pair_bytes(const Product& p, int most_ranges) {
+  PairPlan plan;
+  return in_pairs(p, most_ranges, (size_t)-1, &plan) ? plan.bytes() : 0;
+}
+constexpr int RANGES_AT_MOST = 16;
+// c = a b
+int pair_plain(const PairPlan& plan, const Product& p, float* c, char* ws, hipStream_t s) {
+  return pair_product(plan, p.a, p.b, PairStore{c, p.a.rows},
+                      make_sgemm<true>(nullptr, nullptr, c, p.a.rows, p.b.rows, 1, SgemmEpilogue{nullptr, nullptr, 0}), ws, s);
 }
 
 size_t larger(size_t a, size_t b) { return a > b ? a : b; }
@@ -329,7 +401,9 @@ size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens) {
   const int rows = (hidden + 3) / 4 * 8;
   size_t in = mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
   if (w == TILES) in = sgemm_tail_bytes(plan, rows, tokens, features);
-  return larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (w == APART ? pre_bytes(hidden, tokens) : 0);
+  const size_t others = larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (w == APART ? pre_bytes(hidden, tokens) : 0);
+  return larger(others, larger(pair_bytes(product_in(nullptr, nullptr, features, hidden, tokens), 1),
+                               pair_bytes(product_out(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST)));
 }
 
 int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y, int features, int hidden,
@@ -342,9 +416,17 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
     ws = nullptr;
     bytes = 0;
   }
+  int rc = MNV_OK, ranges = 1;
+  PairPlan pair;
+  const Product in = product_in(w_in, x, features, hidden, tokens), out = product_out(w_out, h, features, hidden, tokens);
+  if (in_pairs(in, 1, bytes, &pair)) {
+    const GatedIn<true> e = make_gated_in<true>(w_in, x, pre, h, features, hidden, tokens, activation);
+    rc = pair_product(pair, in.a, in.b, e, make_sgemm<true>(nullptr, nullptr, h, 1, 1, 1, SgemmEpilogue{nullptr, nullptr, 0}), ws, s);
+    if (!rc && in_pairs(out, RANGES_AT_MOST, bytes, &pair)) return pair_plain(pair, out, y, ws, s);
+    return rc ? rc : mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
+  }
   SgemmPlan plan;
   Way w = way(&plan, features, hidden, tokens, bytes);
-  int rc = MNV_OK, ranges = 1;
   if (w == RANGES) {
     rc = mnv_sgemm_nn_ranges(w_in, x, 2 * hidden, tokens, features, ws, bytes, &ranges, s);
     if (rc) return rc;
@@ -370,13 +452,33 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
     rc = w == SMALL || features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
                                          : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
   }
+  if (!rc && in_pairs(out, RANGES_AT_MOST, bytes, &pair)) return pair_plain(pair, out, y, ws, s);
   return rc ? rc : mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
+}
+
+int mnv_gated_ffn_plan(int features, int hidden, int tokens, size_t fwd_workspace_bytes, size_t bwd_workspace_bytes, int* pairs) {
+  if (!pairs || !sizes_ok(features, hidden, tokens, 0)) return MNV_ERR_INVALID;
+  const size_t f = fwd_workspace_bytes, b = bwd_workspace_bytes;
+  PairPlan plan;
+  *pairs = in_pairs(product_in(nullptr, nullptr, features, hidden, tokens), 1, f, &plan) << 0 |
+           in_pairs(product_out(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST, f, &plan) << 1 |
+           in_pairs(product_dh(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST, b, &plan) << 2 |
+           in_pairs(product_dx(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST, b, &plan) << 3 |
+           in_pairs(product_dw(nullptr, nullptr, 2 * hidden, features, tokens), RANGES_AT_MOST, b, &plan) << 4 |
+           in_pairs(product_dw(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST, b, &plan) << 5;
+  return MNV_OK;
 }
 
 size_t mnv_gated_ffn_bwd_workspace_bytes(int features, int hidden, int tokens) {
   if (!sizes_ok(features, hidden, tokens, 0)) return 0;
-  return larger(larger(mnv_sgemm_nn_workspace_bytes(hidden, tokens, features), mnv_sgemm_nn_workspace_bytes(features, tokens, 2 * hidden)),
-                larger(mnv_sgemm_nn_workspace_bytes(2 * hidden, features, tokens), mnv_sgemm_nn_workspace_bytes(features, hidden, tokens)));
+  const size_t others =
+      larger(larger(mnv_sgemm_nn_workspace_bytes(hidden, tokens, features), mnv_sgemm_nn_workspace_bytes(features, tokens, 2 * hidden)),
+             larger(mnv_sgemm_nn_workspace_bytes(2 * hidden, features, tokens), mnv_sgemm_nn_workspace_bytes(features, hidden, tokens)));
+  const size_t pairs = larger(larger(pair_bytes(product_dh(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST),
+                                     pair_bytes(product_dx(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST)),
+                              larger(pair_bytes(product_dw(nullptr, nullptr, 2 * hidden, features, tokens), RANGES_AT_MOST),
+                                     pair_bytes(product_dw(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST)));
+  return larger(others, pairs);
 }
 
 int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, const float* pre, const float* h, const float* dy, float* dpre,
@@ -385,15 +487,35 @@ int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, con
   if (!x || !w_in || !w_out || !pre || !h || !dy || !dpre || !dw_in || !dw_out || !sizes_ok(features, hidden, tokens, activation))
     return MNV_ERR_INVALID;
   hipStream_t s = mnv_stream(stream);
-  void* ws = workspace && mnv_aligned16(workspace) ? workspace : nullptr;
+  char* const ws = workspace && mnv_aligned16(workspace) ? static_cast<char*>(workspace) : nullptr;
   const size_t bytes = ws ? workspace_bytes : 0;
-  const SgemmPlan plan = plan_sgemm(hidden, tokens, features, bytes / sizeof(float));
-  int rc = plan.skinny || plan.tile || features % 4 == 0
-               ? launch_out_back<true>(plan, w_out, dy, pre, dpre, features, hidden, tokens, activation, ws, bytes, s)
-               : launch_out_back<false>(plan, w_out, dy, pre, dpre, features, hidden, tokens, activation, ws, bytes, s);
-  if (!rc && dx) rc = mnv_sgemm_tn(w_in, dpre, nullptr, dx, features, tokens, 2 * hidden, ws, bytes, stream);
-  if (!rc) rc = mnv_sgemm_nt(dpre, x, dw_in, 2 * hidden, features, tokens, ws, bytes, stream);
-  if (!rc) rc = mnv_sgemm_nt(dy, h, dw_out, features, hidden, tokens, ws, bytes, stream);
+  int rc;
+  PairPlan pair;
+  const Product dh = product_dh(w_out, dy, features, hidden, tokens);
+  if (in_pairs(dh, RANGES_AT_MOST, bytes, &pair)) {
+    const GatedOutBack<true> e = make_out_back<true>(w_out, dy, pre, dpre, features, hidden, tokens, activation);
+    rc = pair_product(pair, dh.a, dh.b, e, e, ws, s);
+  } else {
+    const SgemmPlan plan = plan_sgemm(hidden, tokens, features, bytes / sizeof(float));
+    rc = plan.skinny || plan.tile || features % 4 == 0
+             ? launch_out_back<true>(plan, w_out, dy, pre, dpre, features, hidden, tokens, activation, ws, bytes, s)
+             : launch_out_back<false>(plan, w_out, dy, pre, dpre, features, hidden, tokens, activation, ws, bytes, s);
+  }
+  if (!rc && dx) {
+    const Product p = product_dx(w_in, dpre, features, hidden, tokens);
+    rc = in_pairs(p, RANGES_AT_MOST, bytes, &pair) ? pair_plain(pair, p, dx, ws, s)
+                                                   : mnv_sgemm_tn(w_in, dpre, nullptr, dx, features, tokens, 2 * hidden, ws, bytes, stream);
+  }
+  if (!rc) {
+    const Product p = product_dw(dpre, x, 2 * hidden, features, tokens);
+    rc = in_pairs(p, RANGES_AT_MOST, bytes, &pair) ? pair_plain(pair, p, dw_in, ws, s)
+                                                   : mnv_sgemm_nt(dpre, x, dw_in, 2 * hidden, features, tokens, ws, bytes, stream);
+  }
+  if (!rc) {
+    const Product p = product_dw(dy, h, features, hidden, tokens);
+    rc = in_pairs(p, RANGES_AT_MOST, bytes, &pair) ? pair_plain(pair, p, dw_out, ws, s)
+                                                   : mnv_sgemm_nt(dy, h, dw_out, features, hidden, tokens, ws, bytes, stream);
+  }
   return rc;
 }
 

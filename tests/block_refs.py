@@ -103,10 +103,11 @@ def activation(kind, a):
 
 def product(a, b, ea=0.0, eb=0.0):
     """a @ b of factors that are off by ea and eb, and its bound: every product within 2 U of itself, a sum of k of
-    them rounded k - 1 times at most, in whatever order, and 4 more for sums of partial sums."""
+    them rounded k - 1 times at most, in whatever order, and 4 more for sums of partial sums.  Below 2^-126 numbers are multiples of
+    2^-149, and each of those roundings is off by up to half of that whatever the value."""
     k = a.shape[1]
     aa, ab = np.abs(a), np.abs(b)
-    bound = (k + 5) * U * (aa @ ab)
+    bound = (k + 5) * U * (aa @ ab) + (k + 4) * 2.0 ** -150
     if np.ndim(ea):
         bound = bound + ea @ ab
     if np.ndim(eb):
@@ -123,7 +124,7 @@ def ffn(x, w_in, w_out, kind):
     pre, e_pre = product(x, w_in)
     gate, up, eg, eu = pre[:, :hidden], pre[:, hidden:], e_pre[:, :hidden], e_pre[:, hidden:]
     act, e_act = activation_bound(kind, gate, eg)[:2]
-    h, e_h = act * up, e_act * (np.abs(up) + eu) + np.abs(act) * eu + U * np.abs(act * up)
+    h, e_h = act * up, e_act * (np.abs(up) + eu) + np.abs(act) * eu + U * np.abs(act * up) + 2.0 ** -150  # (the last: of results below 2^-126)
     y, e_y = product(h, w_out, ea=e_h)
     return {"pre": (pre, e_pre), "h": (h, e_h), "y": (y, e_y)}
 
@@ -158,7 +159,7 @@ def ffn_back(x, w_in, w_out, dy, kind):
     dh, e_dh = product(dy, w_out.T)
 
     def times(a, ea, b, eb):
-        return a * b, np.abs(a) * eb + np.abs(b) * ea + ea * eb + U * np.abs(a * b) * 1.01
+        return a * b, np.abs(a) * eb + np.abs(b) * ea + ea * eb + U * np.abs(a * b) * 1.01 + 2.0 ** -150
 
     dup, e_dup = times(dh, e_dh, act, e_act)
     dgate, e_dgate = times(*times(dh, e_dh, up, eu), slope, e_slope)

@@ -61,10 +61,24 @@ def test_gated_ffn_refuses_null(fwd, i):
     assert f(*[None if j == i else P for j in range(n)], 4, 4, 4, 3, None, 0, None) == INVALID
 
 
+def _plan(features, hidden, tokens, fwd=1 << 40, bwd=1 << 40):
+    mask = ctypes.c_int(-1)
+    return capi.lib().mnv_gated_ffn_plan(features, hidden, tokens, fwd, bwd, ctypes.byref(mask)), mask.value
+
+
 def test_gated_ffn_takes_sizes_up_to_its_limits():
+    assert _plan(1, 1 << 14, (1 << 14) - 1)[0] == 0 and _plan((1 << 14) - 1, 1 << 14, 1)[0] == 0
+    assert _plan((1 << 14) + 1, 1 << 14, 1)[0] == INVALID and _plan(1, 1 << 14, 1 << 14)[0] == INVALID
+    assert capi.lib().mnv_gated_ffn_plan(4, 4, 4, 0, 0, None) == INVALID
+
+
+def test_gated_ffn_products_in_pairs():
+    """Large products where the workspace holds them, each by its own; small ones never."""
     L = capi.lib()
-    assert L.mnv_gated_ffn_fwd_workspace_bytes(1, 1 << 14, (1 << 14) - 1) > 0
-    assert L.mnv_gated_ffn_bwd_workspace_bytes((1 << 14) - 1, 1 << 14, 1) > 0
+    sizes = (2048, 5632, 8192)
+    assert _plan(*sizes) == (0, 63) and _plan(*sizes, 0, 0) == (0, 0) and _plan(*sizes, 1 << 40, 0) == (0, 3) and _plan(*sizes, 0, 1 << 40) == (0, 60)
+    assert _plan(*sizes, L.mnv_gated_ffn_fwd_workspace_bytes(*sizes), L.mnv_gated_ffn_bwd_workspace_bytes(*sizes)) == (0, 63)
+    assert _plan(64, 172, 100) == (0, 0) and _plan(1024, 4096, 8) == (0, 0)
 
 
 def _adamw(count=1, sizes=(5,), pointers=None, bits=32, rate=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.1, grad_scale=1.0, step=1,
