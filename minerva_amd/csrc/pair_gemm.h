@@ -2,11 +2,14 @@
 //
 // A value x of a row (of the left operand; of the right one, of a column) whose largest size is below 2^(e + 15) is x = 2^e (h + l), with
 // h the fp16 number next to x 2^-e and l that next to what is left: 22 bits, |x - 2^e (h + l)| <= 2^-22 |x| down to 2^-17 of the row's
-// largest, and 2^-40 of that below.  A product a b is then  ah bh + al bh + ah bl,  and al bl of at most 2^-22 |a b| is left
+// largest, and 2^-39 of that below.  A product a b is then  ah bh + al bh + ah bl,  and al bl of at most 2^-22 |a b| is left
 // out.  The instruction multiplies exactly and adds in fp32; 2^(ea + eb) is put on at the end, exactly.  That is half the matrix
 // instructions of the six products of three bf16 parts (gemm_split.h), which hold all 24 bits and need no scale: a product here
 // is within 3 x 2^-22 of itself, a sum's error is set by the roundings of its fp32 additions all the same.  Measured against
-// float64 (2-norm, relative), this / six products of bf16 parts / the fp32 instruction: TODO.  An infinity or NaN gives NaN in all that its row has a part in.
+// float64 (2-norm, relative; normal values, k = 1024 / 4096 / 16384): 3.6e-7, 7.1e-7, 1.5e-6; six products of bf16 parts 1.9e-7, 4.0e-7,
+// 8.2e-7; the fp32 instruction 5.7e-7, 1.2e-6, 2.3e-6.  Sums of the two small products kept apart from the large one's bring it to
+// that of bf16 parts, but their 128 registers leave the fragments too few: 160 moves beside 192 matrix instructions, 6% of the time.  An infinity or NaN
+// gives NaN in all that its row has a part in.
 //
 // The pairs are made once for a product, not while it multiplies (the cut takes 6 vector instructions a value, and there would be
 // one for two matrix instructions): pair_pack_kernel writes them in the order in which a wavefront's lanes want them, 64 rows x 32 k
@@ -41,11 +44,25 @@ __device__ __forceinline__ int pair_source_row(int row, int gate) { return gate 
 // Bits of the largest size; infinities and NaN are larger than all others.
 __device__ __forceinline__ unsigned pair_size(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
 
-// Largest sizes of source rows, k contiguous: a wavefront to a row.  tops[row]
-__global__ __launch_bounds__(256) void pair_tops_k_kernel(const float* __restrict__ src, size_t ld, int rows, int k, unsigned* __restrict__ tops) {
-  const int lane = threadIdx.x % MNV_WAVE, row = blockIdx.x * 4 + threadIdx.x / MNV_WAVE;
-  if (row >= rows) return;
-  const float* p = src + row * ld;
+// What the kernels below do for one operand; both of a product's go into one launch, the right one's workgroups behind the left one's.
+struct PairPacking {
+  PairOperand o;
+  int source_rows, parts, per_part;  // largest sizes: tops[part][source row]
+  unsigned* tops;
+  int blocks_k, per_wave, blocks_x;  // packing: blocks_x workgroups along k, four wavefronts with per_wave blocks of 32 k each
+  char* out;
+  int* exps;                         // [row]: the row's e
+};
+struct PairBoth {
+  PairPacking p[2];
+  int first;  // the right operand's first workgroup
+};
+
+// Largest sizes of source rows, k contiguous: a wavefront to a row.
+__device__ __forceinline__ void pair_tops_k(const PairPacking& z, int block) {
+  const int lane = threadIdx.x % MNV_WAVE, row = block * 4 + threadIdx.x / MNV_WAVE, k = z.o.k;
+  if (row >= z.source_rows) return;
+  const float* p = z.o.src + row * z.o.ld;
   unsigned most = 0;
   int i = lane * 4;
   for (; i + 768 + 4 <= k; i += 1024) {
@@ -68,75 +85,81 @@ __global__ __launch_bounds__(256) void pair_tops_k_kernel(const float* __restric
       if (i + q < k) most = max(most, pair_size(p[i + q]));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, o, MNV_WAVE));
-  if (lane == 0) tops[row] = most;
+  if (lane == 0) z.tops[row] = most;
 }
-// The same, rows contiguous: a lane has four of them, a workgroup's wavefronts every fourth k of the part blockIdx.y.  tops[part][row]
-__global__ __launch_bounds__(256) void pair_tops_x_kernel(const float* __restrict__ src, size_t ld, int rows, int k, int per_part,
-                                                          unsigned* __restrict__ tops) {
-  __shared__ unsigned red[4][256];
-  const int lane = threadIdx.x % MNV_WAVE, wave = threadIdx.x / MNV_WAVE, row = blockIdx.x * 256 + lane * 4;
-  const int end = min(k, ((int)blockIdx.y + 1) * per_part);
+// The same, rows contiguous: a lane has four of them, a workgroup's wavefronts every fourth k of a part.
+__device__ __forceinline__ void pair_tops_x(const PairPacking& z, int block, unsigned (&red)[4][256]) {
+  const int blocks = (z.source_rows + 255) / 256, part = block / blocks, first = (block - part * blocks) * 256;
+  const int lane = threadIdx.x % MNV_WAVE, wave = threadIdx.x / MNV_WAVE, row = first + lane * 4, rows = z.source_rows;
+  const int end = min(z.o.k, (part + 1) * z.per_part);
   unsigned most[4] = {0, 0, 0, 0};
+  int i = part * z.per_part + wave;
   if (row + 4 <= rows) {
-    int i = blockIdx.y * per_part + wave;
     for (; i + 12 < end; i += 16) {
       mnv_f4u v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const mnv_f4u*>(src + (size_t)(i + u * 4) * ld + row);
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const mnv_f4u*>(z.o.src + (size_t)(i + u * 4) * z.o.ld + row);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int q = 0; q < 4; ++q) most[q] = max(most[q], pair_size(v[u][q]));
     }
     for (; i < end; i += 4) {
-      const mnv_f4u v = *reinterpret_cast<const mnv_f4u*>(src + (size_t)i * ld + row);
+      const mnv_f4u v = *reinterpret_cast<const mnv_f4u*>(z.o.src + (size_t)i * z.o.ld + row);
 #pragma unroll
       for (int q = 0; q < 4; ++q) most[q] = max(most[q], pair_size(v[q]));
     }
   } else {
-    for (int i = blockIdx.y * per_part + wave; i < end; i += 4)
+    for (; i < end; i += 4)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (row + q < rows) most[q] = max(most[q], pair_size(src[(size_t)i * ld + row + q]));
+        if (row + q < rows) most[q] = max(most[q], pair_size(z.o.src[(size_t)i * z.o.ld + row + q]));
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) red[wave][lane * 4 + q] = most[q];
   __syncthreads();
-  const int mine = blockIdx.x * 256 + threadIdx.x;
-  if (mine < rows) tops[(size_t)blockIdx.y * rows + mine] = max(max(red[0][threadIdx.x], red[1][threadIdx.x]), max(red[2][threadIdx.x], red[3][threadIdx.x]));
+  const int t = threadIdx.x;
+  if (first + t < rows) z.tops[(size_t)part * rows + first + t] = max(max(red[0][t], red[1][t]), max(red[2][t], red[3][t]));
+}
+__global__ __launch_bounds__(256) void pair_tops_kernel(PairBoth both) {
+  __shared__ unsigned red[4][256];
+  const bool right = (int)blockIdx.x >= both.first;
+  const PairPacking& z = both.p[right];
+  const int block = (int)blockIdx.x - (right ? both.first : 0);
+  if (z.o.k_fast) pair_tops_k(z, block);
+  else pair_tops_x(z, block, red);
 }
 
-// A wavefront packs 64 rows x 32 k at a time.  exps[row]: the row's e.
+// A wavefront packs 64 rows x 32 k at a time.
 template <bool K_FAST>
-__global__ __launch_bounds__(256) void pair_pack_kernel(PairOperand z, int source_rows, const unsigned* __restrict__ tops, int parts, int blocks_k,
-                                                        int per_wave, char* __restrict__ out, int* __restrict__ exps) {
+__device__ __forceinline__ void pair_pack(const PairPacking& z, int block) {
   const int lane = threadIdx.x % MNV_WAVE, lr = lane % 16, lq = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / MNV_WAVE));
-  const int group = blockIdx.y, row = group * PAIR_GROUP + lr * 4;
+  const int group = block / z.blocks_x, bx = block - group * z.blocks_x, row = group * PAIR_GROUP + lr * 4;
   int e[4], src_row[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    src_row[q] = pair_source_row(row + q, z.gate);
+    src_row[q] = pair_source_row(row + q, z.o.gate);
     // of the rows that fill the last run of the gate's, what is read is not stored
-    const bool on = row + q < z.rows && src_row[q] < source_rows;
+    const bool on = row + q < z.o.rows && src_row[q] < z.source_rows;
     unsigned top = 0;
     if (on)
-      for (int p = 0; p < parts; ++p) top = max(top, tops[(size_t)p * source_rows + src_row[q]]);
+      for (int p = 0; p < z.parts; ++p) top = max(top, z.tops[(size_t)p * z.source_rows + src_row[q]]);
     // 2^e below the top by 14 powers of two; of tops below 2^-112 the smallest e that a factor holds
     const int power = (int)(top >> 23) - 127;
     e[q] = top == 0 ? 0 : max(power - 14, -126);
     if (!on) src_row[q] = -1;
-    if (blockIdx.x == 0 && wave == 0 && lq == 0) exps[row + q] = e[q];
+    if (bx == 0 && wave == 0 && lq == 0) z.exps[row + q] = e[q];
   }
-  const int first = ((int)blockIdx.x * 4 + wave) * per_wave;
-  for (int kb = first; kb < first + per_wave && kb < blocks_k; ++kb) {
+  const int first = (bx * 4 + wave) * z.per_wave;
+  for (int kb = first; kb < first + z.per_wave && kb < z.blocks_k; ++kb) {
     const int k = kb * PAIR_K + lq * 8;
     float v[4][8];
     if constexpr (K_FAST) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float* p = z.src + (size_t)max(src_row[q], 0) * z.ld + k;
-        if (k + 8 <= z.k) {
+        const float* p = z.o.src + (size_t)max(src_row[q], 0) * z.o.ld + k;
+        if (k + 8 <= z.o.k) {
           const mnv_f4u a = *reinterpret_cast<const mnv_f4u*>(p), b = *reinterpret_cast<const mnv_f4u*>(p + 4);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -145,14 +168,14 @@ __global__ __launch_bounds__(256) void pair_pack_kernel(PairOperand z, int sourc
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[q][i] = k + i < z.k ? p[i] : 0.f;
+          for (int i = 0; i < 8; ++i) v[q][i] = k + i < z.o.k ? p[i] : 0.f;
         }
       }
     } else {
       const bool whole = src_row[0] >= 0 && src_row[3] == src_row[0] + 3;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float* p = z.src + (size_t)min(k + i, z.k - 1) * z.ld;
+        const float* p = z.o.src + (size_t)min(k + i, z.o.k - 1) * z.o.ld;
         if (whole) {
           const mnv_f4u a = *reinterpret_cast<const mnv_f4u*>(p + src_row[0]);
 #pragma unroll
@@ -161,12 +184,12 @@ __global__ __launch_bounds__(256) void pair_pack_kernel(PairOperand z, int sourc
 #pragma unroll
           for (int q = 0; q < 4; ++q) v[q][i] = src_row[q] >= 0 ? p[src_row[q]] : 0.f;
         }
-        if (k + i >= z.k)
+        if (k + i >= z.o.k)
 #pragma unroll
           for (int q = 0; q < 4; ++q) v[q][i] = 0.f;
       }
     }
-    char* const at = out + ((size_t)group * blocks_k + kb) * PAIR_CHUNK + lane * 16;
+    char* const at = z.out + ((size_t)group * z.blocks_k + kb) * PAIR_CHUNK + lane * 16;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       PairHalf8 h, l;
@@ -180,6 +203,13 @@ __global__ __launch_bounds__(256) void pair_pack_kernel(PairOperand z, int sourc
       *reinterpret_cast<PairHalf8*>(at + 4096 + q * 1024) = l;
     }
   }
+}
+__global__ __launch_bounds__(256) void pair_pack_kernel(PairBoth both) {
+  const bool right = (int)blockIdx.x >= both.first;
+  const PairPacking& z = both.p[right];
+  const int block = (int)blockIdx.x - (right ? both.first : 0);
+  if (z.o.k_fast) pair_pack<true>(z, block);
+  else pair_pack<false>(z, block);
 }
 
 // A plain result of M rows.
@@ -267,7 +297,7 @@ __global__ __launch_bounds__(256, 1) void pair_gemm_kernel(PairProblem<E> z) {
 #pragma unroll
     for (int i = 0; i < 24; ++i) read_one(step, s, i);
   };
-  // instruction t of 96: the small products of four fragments before their large one
+  // instruction t of 96
   auto multiply_one = [&](const Set& s, int t) {
     const int i = t / 12, part = t % 12 / 4, j = t % 4;
     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(s.b[j][part == 0], s.a[i][part == 1], acc[i][j], 0, 0, 0);
@@ -395,7 +425,7 @@ inline int pair_parts(const PairOperand& o) {
 }
 // most_ranges: 1 where the store wants whole sums.  store_bytes: what the store moves for a value.  Microseconds: 1.17 a step of 32 k and 10
 // around a tile on each CU (no other workgroup multiplies meanwhile, so that the store's bytes count in full), 12 bytes a value of either
-// operand to pack and 20 for its four launches, 8 bytes a value and range for k ranges, all bytes at 5 TB/s.
+// operand to pack and 12 for its two launches, 8 bytes a value and range for k ranges, all bytes at 5 TB/s.
 PairPlan pair_plan(const PairOperand& a, const PairOperand& b, int most_ranges, double store_bytes, int cus) {
   PairPlan p;
   p.tiles_m = (a.rows + PAIR_M - 1) / PAIR_M;
@@ -414,7 +444,7 @@ PairPlan pair_plan(const PairOperand& a, const PairOperand& b, int most_ranges, 
     }
   }
   p.ranges = (p.blocks_k + p.per_range - 1) / p.per_range;
-  p.us = best + store_bytes * 1e-6 / 5.0 * a.rows * b.rows + 20.0 + 12e-6 / 5.0 * ((double)a.rows + b.rows) * a.k;
+  p.us = best + store_bytes * 1e-6 / 5.0 * a.rows * b.rows + 12.0 + 12e-6 / 5.0 * ((double)a.rows + b.rows) * a.k;
   p.a_bytes = (size_t)p.tiles_m * 4 * p.blocks_k * PAIR_CHUNK;
   p.b_bytes = (size_t)p.tiles_n * 2 * p.blocks_k * PAIR_CHUNK;
   p.exps = pair_round(((size_t)p.tiles_m * PAIR_M + (size_t)p.tiles_n * PAIR_N) * sizeof(int));
@@ -428,24 +458,15 @@ inline bool pair_fits(const PairOperand& a, const PairOperand& b) {
   return a.k < (1 << 20) && a.rows < (1 << 21) && b.rows < (1 << 21);
 }
 
-int pair_pack(const PairOperand& o, int blocks_k, unsigned* tops, char* out, int* exps, hipStream_t s) {
-  const int source = pair_source_rows(o), parts = pair_parts(o);
-  if (o.k_fast) {
-    hipLaunchKernelGGL(pair_tops_k_kernel, dim3((source + 3) / 4), dim3(256), 0, s, o.src, o.ld, source, o.k, tops);
-  } else {
-    hipLaunchKernelGGL(pair_tops_x_kernel, dim3((source + 255) / 256, parts), dim3(256), 0, s, o.src, o.ld, source, o.k, (o.k + parts - 1) / parts,
-                       tops);
-  }
-  const int groups = (o.rows + PAIR_GROUP - 1) / PAIR_GROUP;
+PairPacking pair_packing(const PairOperand& o, int blocks_k, unsigned* tops, char* out, int* exps) {
+  const int parts = pair_parts(o), groups = (o.rows + PAIR_GROUP - 1) / PAIR_GROUP;
   long long per_wave = (long long)blocks_k * groups / (4 * 2048);  // 2048 workgroups where there is that much
   if (per_wave < 1) per_wave = 1;
-  const dim3 grid((unsigned)((blocks_k + 4 * per_wave - 1) / (4 * per_wave)), groups);
-  if (o.k_fast)
-    hipLaunchKernelGGL(pair_pack_kernel<true>, grid, dim3(256), 0, s, o, source, tops, parts, blocks_k, (int)per_wave, out, exps);
-  else
-    hipLaunchKernelGGL(pair_pack_kernel<false>, grid, dim3(256), 0, s, o, source, tops, parts, blocks_k, (int)per_wave, out, exps);
-  return MNV_LAUNCH_STATUS();
+  return {o, pair_source_rows(o), parts, (o.k + parts - 1) / parts, tops, blocks_k, (int)per_wave, (int)((blocks_k + 4 * per_wave - 1) / (4 * per_wave)),
+          out, exps};
 }
+inline int pair_tops_blocks(const PairPacking& z) { return z.o.k_fast ? (z.source_rows + 3) / 4 : (z.source_rows + 255) / 256 * z.parts; }
+inline int pair_pack_blocks(const PairPacking& z) { return (z.o.rows + PAIR_GROUP - 1) / PAIR_GROUP * z.blocks_x; }
 
 // c = a b, stored by e, or with k ranges by `reduced`, a policy of the products.  The workspace holds plan.bytes(), aligned to 16 bytes.
 template <class E, class R>
@@ -457,8 +478,14 @@ int pair_product(const PairPlan& p, const PairOperand& a, const PairOperand& b, 
   unsigned* const ta = reinterpret_cast<unsigned*>(pb + p.b_bytes + p.exps);
   unsigned* const tb = reinterpret_cast<unsigned*>(pb + p.b_bytes + p.exps + p.tops_a);
   float* const partial = p.ranges > 1 ? reinterpret_cast<float*>(pb + p.b_bytes + p.exps + p.tops_a + p.tops_b) : nullptr;
-  int rc = pair_pack(a, p.blocks_k, ta, pa, ea, s);
-  if (!rc) rc = pair_pack(b, p.blocks_k, tb, pb, eb, s);
+  PairBoth both{{pair_packing(a, p.blocks_k, ta, pa, ea), pair_packing(b, p.blocks_k, tb, pb, eb)}, 0};
+  both.first = pair_tops_blocks(both.p[0]);
+  hipLaunchKernelGGL(pair_tops_kernel, dim3(both.first + pair_tops_blocks(both.p[1])), dim3(256), 0, s, both);
+  int rc = MNV_LAUNCH_STATUS();
+  if (rc) return rc;
+  both.first = pair_pack_blocks(both.p[0]);
+  hipLaunchKernelGGL(pair_pack_kernel, dim3(both.first + pair_pack_blocks(both.p[1])), dim3(256), 0, s, both);
+  rc = MNV_LAUNCH_STATUS();
   if (rc) return rc;
   constexpr int LDS = 3 * 6 * (int)PAIR_CHUNK;
   static std::atomic<bool> attr_set[64];
