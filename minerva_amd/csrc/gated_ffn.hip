@@ -9,6 +9,7 @@
 // is kept of dh.
 #include <algorithm>
 
+#include "few_gemm.h"
 #include "pair_gemm.h"
 
 namespace {
@@ -386,6 +387,19 @@ int pair_plain(const PairPlan& plan, const Product& p, float* c, char* ws, hipSt
                       make_sgemm<true>(nullptr, nullptr, c, p.a.rows, p.b.rows, 1, SgemmEpilogue{nullptr, nullptr, 0}), ws, s);
 }
 
+// The products that read a weight matrix for few tokens.  The least values: below them the SGEMM's plans are as fast; of the one with
+// dh, whose tiles store no ranges, 12 million (1024 -> 4096 for 16 tokens 7 / 9 us, 4096 -> 4096 31 / 18).
+FewPlan few_in(int features, int hidden, int tokens, size_t ws_bytes) { return plan_few(2 * hidden, tokens, features, false, 5e6, ws_bytes); }
+FewPlan few_out(int features, int hidden, int tokens, size_t ws_bytes) { return plan_few(features, tokens, hidden, false, 2.5e6, ws_bytes); }
+FewPlan few_dh(int features, int hidden, int tokens, size_t ws_bytes) { return plan_few(hidden, tokens, features, true, 12e6, ws_bytes); }
+FewPlan few_dx(int features, int hidden, int tokens, size_t ws_bytes) { return plan_few(features, tokens, 2 * hidden, true, 2.5e6, ws_bytes); }
+template <class P>
+int run_few(const FewPlan& plan, const P& p, char* ws, hipStream_t s) {
+  float* const partial = reinterpret_cast<float*>(ws);
+  const int rc = launch_few(plan, p, partial, s);
+  return rc || plan.ranges == 1 ? rc : mnv_gemm_reduce_launch(p, partial, plan.ranges, s);
+}
+
 size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 // Bytes of pre where the caller keeps none and the plan does not do without it, in whole 16 bytes.
 size_t pre_bytes(int hidden, int tokens) { return ((size_t)hidden * 2 * tokens * sizeof(float) + 15) / 16 * 16; }
@@ -397,11 +411,13 @@ extern "C" {
 size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens) {
   if (!sizes_ok(features, hidden, tokens, 0)) return 0;
   SgemmPlan plan;
-  const Way w = way(&plan, features, hidden, tokens, (size_t)-1);
+  const FewPlan few = few_in(features, hidden, tokens, (size_t)-1), few_y = few_out(features, hidden, tokens, (size_t)-1);
+  const Way w = few.cols ? RANGES : way(&plan, features, hidden, tokens, (size_t)-1);
   const int rows = (hidden + 3) / 4 * 8;
-  size_t in = mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
+  size_t in = few.cols ? few.bytes(2 * hidden, tokens) : mnv_sgemm_nn_workspace_bytes(2 * hidden, tokens, features);
   if (w == TILES) in = sgemm_tail_bytes(plan, rows, tokens, features);
-  const size_t others = larger(in, mnv_sgemm_nn_workspace_bytes(features, tokens, hidden)) + (w == APART ? pre_bytes(hidden, tokens) : 0);
+  const size_t out = few_y.cols ? few_y.bytes(features, tokens) : mnv_sgemm_nn_workspace_bytes(features, tokens, hidden);
+  const size_t others = larger(in, out) + (w == APART ? pre_bytes(hidden, tokens) : 0);
   return larger(others, larger(pair_bytes(product_in(nullptr, nullptr, features, hidden, tokens), 1),
                                pair_bytes(product_out(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST)));
 }
@@ -419,11 +435,27 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
   int rc = MNV_OK, ranges = 1;
   PairPlan pair;
   const Product in = product_in(w_in, x, features, hidden, tokens), out = product_out(w_out, h, features, hidden, tokens);
+  const auto product_y = [&] {
+    if (in_pairs(out, RANGES_AT_MOST, bytes, &pair)) return pair_plain(pair, out, y, ws, s);
+    const FewPlan few = few_out(features, hidden, tokens, bytes);
+    if (few.cols) return run_few(few, make_sgemm<true>(w_out, h, y, features, tokens, hidden, SgemmEpilogue{nullptr, nullptr, 0}), ws, s);
+    return mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
+  };
   if (in_pairs(in, 1, bytes, &pair)) {
     const GatedIn<true> e = make_gated_in<true>(w_in, x, pre, h, features, hidden, tokens, activation);
     rc = pair_product(pair, in.a, in.b, e, make_sgemm<true>(nullptr, nullptr, h, 1, 1, 1, SgemmEpilogue{nullptr, nullptr, 0}), ws, s);
-    if (!rc && in_pairs(out, RANGES_AT_MOST, bytes, &pair)) return pair_plain(pair, out, y, ws, s);
-    return rc ? rc : mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
+    return rc ? rc : product_y();
+  }
+  const FewPlan few = few_in(features, hidden, tokens, bytes);
+  if (few.cols) {
+    if (few.ranges == 1) {
+      rc = launch_few(few, make_gated_in<true>(w_in, x, pre, h, features, hidden, tokens, activation), nullptr, s);
+    } else {
+      float* const partial = reinterpret_cast<float*>(ws);
+      rc = launch_few(few, make_sgemm<true>(w_in, x, nullptr, 2 * hidden, tokens, features, SgemmEpilogue{nullptr, nullptr, 0}), partial, s);
+      if (!rc) rc = launch_gate_ranges(partial, pre, h, hidden, tokens, few.ranges, activation, s);
+    }
+    return rc ? rc : product_y();
   }
   SgemmPlan plan;
   Way w = way(&plan, features, hidden, tokens, bytes);
@@ -452,8 +484,7 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
     rc = w == SMALL || features % 4 == 0 ? launch_gated_in<true>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s)
                                          : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
   }
-  if (!rc && in_pairs(out, RANGES_AT_MOST, bytes, &pair)) return pair_plain(pair, out, y, ws, s);
-  return rc ? rc : mnv_sgemm_nn(w_out, h, y, features, tokens, hidden, ws, bytes, stream);
+  return rc ? rc : product_y();
 }
 
 int mnv_gated_ffn_plan(int features, int hidden, int tokens, size_t fwd_workspace_bytes, size_t bwd_workspace_bytes, int* pairs) {
@@ -471,8 +502,10 @@ int mnv_gated_ffn_plan(int features, int hidden, int tokens, size_t fwd_workspac
 
 size_t mnv_gated_ffn_bwd_workspace_bytes(int features, int hidden, int tokens) {
   if (!sizes_ok(features, hidden, tokens, 0)) return 0;
+  const FewPlan few = few_dh(features, hidden, tokens, (size_t)-1), few_x = few_dx(features, hidden, tokens, (size_t)-1);
   const size_t others =
-      larger(larger(mnv_sgemm_nn_workspace_bytes(hidden, tokens, features), mnv_sgemm_nn_workspace_bytes(features, tokens, 2 * hidden)),
+      larger(larger(few.cols ? few.bytes(hidden, tokens) : mnv_sgemm_nn_workspace_bytes(hidden, tokens, features),
+                    few_x.cols ? few_x.bytes(features, tokens) : mnv_sgemm_nn_workspace_bytes(features, tokens, 2 * hidden)),
              larger(mnv_sgemm_nn_workspace_bytes(2 * hidden, features, tokens), mnv_sgemm_nn_workspace_bytes(features, hidden, tokens)));
   const size_t pairs = larger(larger(pair_bytes(product_dh(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST),
                                      pair_bytes(product_dx(nullptr, nullptr, features, hidden, tokens), RANGES_AT_MOST)),
@@ -495,6 +528,8 @@ int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, con
   if (in_pairs(dh, RANGES_AT_MOST, bytes, &pair)) {
     const GatedOutBack<true> e = make_out_back<true>(w_out, dy, pre, dpre, features, hidden, tokens, activation);
     rc = pair_product(pair, dh.a, dh.b, e, e, ws, s);
+  } else if (const FewPlan few = few_dh(features, hidden, tokens, bytes); few.cols) {
+    rc = run_few(few, make_out_back<true>(w_out, dy, pre, dpre, features, hidden, tokens, activation), ws, s);
   } else {
     const SgemmPlan plan = plan_sgemm(hidden, tokens, features, bytes / sizeof(float));
     rc = plan.skinny || plan.tile || features % 4 == 0
@@ -503,8 +538,13 @@ int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, con
   }
   if (!rc && dx) {
     const Product p = product_dx(w_in, dpre, features, hidden, tokens);
-    rc = in_pairs(p, RANGES_AT_MOST, bytes, &pair) ? pair_plain(pair, p, dx, ws, s)
-                                                   : mnv_sgemm_tn(w_in, dpre, nullptr, dx, features, tokens, 2 * hidden, ws, bytes, stream);
+    if (in_pairs(p, RANGES_AT_MOST, bytes, &pair)) {
+      rc = pair_plain(pair, p, dx, ws, s);
+    } else if (const FewPlan few = few_dx(features, hidden, tokens, bytes); few.cols) {
+      rc = run_few(few, make_sgemm<true, true>(w_in, dpre, dx, features, tokens, 2 * hidden, SgemmEpilogue{nullptr, nullptr, 0}), ws, s);
+    } else {
+      rc = mnv_sgemm_tn(w_in, dpre, nullptr, dx, features, tokens, 2 * hidden, ws, bytes, stream);
+    }
   }
   if (!rc) {
     const Product p = product_dw(dpre, x, 2 * hidden, features, tokens);
