@@ -130,21 +130,30 @@ __global__ __launch_bounds__(256) void pair_tops_kernel(PairBoth both) {
   else pair_tops_x(z, block, red);
 }
 
-// A wavefront packs 64 rows x 32 k at a time.
+// A wavefront packs 64 rows x 32 k at a time.  The workgroup's have the same rows, whose largest sizes they find together: every lane of
+// each over all parts, one load waiting for the other, took longer than the packing (5632 + 1024 rows of 4096 k 129 -> 47 us).
 template <bool K_FAST>
-__device__ __forceinline__ void pair_pack(const PairPacking& z, int block) {
+__device__ __forceinline__ void pair_pack(const PairPacking& z, int block, unsigned (&red)[4][PAIR_GROUP]) {
   const int lane = threadIdx.x % MNV_WAVE, lr = lane % 16, lq = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / MNV_WAVE));
   const int group = block / z.blocks_x, bx = block - group * z.blocks_x, row = group * PAIR_GROUP + lr * 4;
+  {
+    const int r = group * PAIR_GROUP + lane, src = pair_source_row(r, z.o.gate);
+    unsigned top = 0;
+    if (r < z.o.rows && src < z.source_rows) {
+#pragma unroll 8
+      for (int p = wave; p < z.parts; p += 4) top = max(top, z.tops[(size_t)p * z.source_rows + src]);
+    }
+    red[wave][lane] = top;
+  }
+  __syncthreads();
   int e[4], src_row[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     src_row[q] = pair_source_row(row + q, z.o.gate);
     // of the rows that fill the last run of the gate's, what is read is not stored
     const bool on = row + q < z.o.rows && src_row[q] < z.source_rows;
-    unsigned top = 0;
-    if (on)
-      for (int p = 0; p < z.parts; ++p) top = max(top, z.tops[(size_t)p * z.source_rows + src_row[q]]);
+    const unsigned top = max(max(red[0][lr * 4 + q], red[1][lr * 4 + q]), max(red[2][lr * 4 + q], red[3][lr * 4 + q]));
     // 2^e below the top by 14 powers of two; of tops below 2^-112 the smallest e that a factor holds
     const int power = (int)(top >> 23) - 127;
     e[q] = top == 0 ? 0 : max(power - 14, -126);
@@ -205,11 +214,12 @@ __device__ __forceinline__ void pair_pack(const PairPacking& z, int block) {
   }
 }
 __global__ __launch_bounds__(256) void pair_pack_kernel(PairBoth both) {
+  __shared__ unsigned red[4][PAIR_GROUP];
   const bool right = (int)blockIdx.x >= both.first;
   const PairPacking& z = both.p[right];
   const int block = (int)blockIdx.x - (right ? both.first : 0);
-  if (z.o.k_fast) pair_pack<true>(z, block);
-  else pair_pack<false>(z, block);
+  if (z.o.k_fast) pair_pack<true>(z, block, red);
+  else pair_pack<false>(z, block, red);
 }
 
 // A plain result of M rows.
