@@ -16,31 +16,55 @@ namespace {
 
 enum { ACT_SIGMOID, ACT_RELU, ACT_TANH, ACT_SILU, ACT_GELU, ACT_COUNT };
 
-// The activation of x, and its slope there.
-__device__ __forceinline__ void activate(int kind, float x, float& value, float& slope) {
+// The activation of N values, and its slopes there.  The kind is looked at once for them all, so that their instructions
+// interleave: a wavefront has its SIMD to itself where large products store (8192 tokens of 2048 -> 5632, silu, w_in's 1166 -> 1009 us, w_out's backward
+// 712 -> 611, with the reciprocal below).
+template <int N>
+__device__ __forceinline__ void activate(int kind, const float (&x)[N], float (&value)[N], float (&slope)[N]) {
   if (kind == ACT_RELU) {
-    value = x > 0.f ? x : 0.f;
-    slope = x > 0.f ? 1.f : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      value[i] = x[i] > 0.f ? x[i] : 0.f;
+      slope[i] = x[i] > 0.f ? 1.f : 0.f;
+    }
   } else if (kind == ACT_TANH) {
-    value = tanhf(x);
-    slope = 1.f - value * value;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      value[i] = tanhf(x[i]);
+      slope[i] = 1.f - value[i] * value[i];
+    }
   } else if (kind == ACT_GELU) {
     // x times the normal distribution's share below x: erfc keeps the digits of a small share, 1 + erf does not
-    const float below = 0.5f * erfcf(x * -0.70710678f);
-    value = x * below;
-    slope = below + x * (0.39894228f * expf(-0.5f * x * x));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float below = 0.5f * erfcf(x[i] * -0.70710678f);
+      value[i] = x[i] * below;
+      slope[i] = below + x[i] * (0.39894228f * expf(-0.5f * x[i] * x[i]));
+    }
   } else {
-    // 1 / (1 + exp(-x)) and what it lacks to 1, from the exponential that cannot overflow: neither loses digits near 0
-    const float z = expf(-fabsf(x)), near = 1.f / (1.f + z), far = z * near;
-    const float e = x < 0.f ? far : near, rest = x < 0.f ? near : far;
-    value = kind == ACT_SILU ? x * e : e;
-    slope = kind == ACT_SILU ? e + value * rest : e * rest;
+    // 1 / (1 + exp(-x)) and what it lacks to 1, from the exponential that cannot overflow: neither loses digits near 0.  The divisor
+    // is 1 to 2: the vector unit's reciprocal and a step of Newton's leave at most one rounding more than a division.
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float z = expf(-fabsf(x[i])), d = 1.f + z, guess = __builtin_amdgcn_rcpf(d);
+      const float near = __builtin_fmaf(__builtin_fmaf(-d, guess, 1.f), guess, guess), far = z * near;
+      const float e = x[i] < 0.f ? far : near, rest = x[i] < 0.f ? near : far;
+      value[i] = kind == ACT_SILU ? x[i] * e : e;
+      slope[i] = kind == ACT_SILU ? e + value[i] * rest : e * rest;
+    }
   }
 }
+template <int N>
+__device__ __forceinline__ void gated(int kind, const float (&gate)[N], const float (&up)[N], float (&h)[N]) {
+  float slope[N];
+  activate(kind, gate, h, slope);
+#pragma unroll
+  for (int i = 0; i < N; ++i) h[i] *= up[i];
+}
 __device__ __forceinline__ float gated(int kind, float gate, float up) {
-  float value, slope;
-  activate(kind, gate, value, slope);
-  return value * up;
+  float h[1];
+  gated<1>(kind, {gate}, {up}, h);
+  return h[0];
 }
 
 typedef float Two __attribute__((ext_vector_type(2), aligned(4)));
@@ -131,13 +155,15 @@ struct GatedIn {
     const bool up = m & 4;
     if (pre) store_rows(pre + (size_t)n * hidden * 2 + row + (up ? hidden : 0), left, x);
     // The lane of the gate takes rows 0 and 1, that of the up projection 2 and 3; each gives the other what it wants (quad_perm 1, 0, 3, 2).
-    float r[2];
+    float gate[2], high[2], r[2];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const float give = up ? x[q] : x[q + 2];
       const float got = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, give), 0xb1, 0xf, 0xf, true));
-      r[q] = gated(act, up ? got : x[q], up ? x[q + 2] : got);
+      gate[q] = up ? got : x[q];
+      high[q] = up ? x[q + 2] : got;
     }
+    gated(act, gate, high, r);
     float* const p = h + (size_t)n * hidden + row + (up ? 2 : 0);
     const int rest = left - (up ? 2 : 0);
     if (rest >= 2) *reinterpret_cast<Two*>(p) = Two{r[0], r[1]};
@@ -155,10 +181,10 @@ struct GatedOutBack : SgemmNN<K4, true, false> {
   __device__ void c_store(int m, int n, float dh) const {
     const size_t at = (size_t)n * hidden * 2 + m;
     const float gate = pre[at], up = pre[at + hidden];
-    float value, slope;
-    activate(act, gate, value, slope);
-    dpre[at] = dh * up * slope;
-    dpre[at + hidden] = dh * value;
+    float value[1], slope[1];
+    activate<1>(act, {gate}, value, slope);
+    dpre[at] = dh * up * slope[0];
+    dpre[at + hidden] = dh * value[0];
   }
   struct Fetched {
     mnv_f4u gate, up;
@@ -172,12 +198,12 @@ struct GatedOutBack : SgemmNN<K4, true, false> {
     if (m + 3 < this->M) {
       const size_t at = (size_t)n * hidden * 2 + m;
       mnv_f4u dg, du;
+      float value[4], slope[4];
+      activate<4>(act, {f.gate[0], f.gate[1], f.gate[2], f.gate[3]}, value, slope);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float value, slope;
-        activate(act, f.gate[q], value, slope);
-        dg[q] = dh[q] * f.up[q] * slope;
-        du[q] = dh[q] * value;
+        dg[q] = dh[q] * f.up[q] * slope[q];
+        du[q] = dh[q] * value[q];
       }
       *reinterpret_cast<mnv_f4u*>(dpre + at) = dg;
       *reinterpret_cast<mnv_f4u*>(dpre + at + hidden) = du;
@@ -200,8 +226,7 @@ __global__ __launch_bounds__(256) void gate_kernel(const float* __restrict__ pre
     float r[4];
     if (left >= 4) {
       const mnv_f4u gate = *reinterpret_cast<const mnv_f4u*>(p), up = *reinterpret_cast<const mnv_f4u*>(p + hidden);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) r[q] = gated(act, gate[q], up[q]);
+      gated<4>(act, {gate[0], gate[1], gate[2], gate[3]}, {up[0], up[1], up[2], up[3]}, r);
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q) r[q] = q < left ? gated(act, p[q], p[hidden + q]) : 0.f;
