@@ -465,7 +465,7 @@ int mnv_relative_bias_bwd(const float* dbias, float* dtable, int buckets, int he
 
 /* ---- rotary positions of queries and keys (no counterpart in the reference).  x, y, dy, dx {head_dim, heads, length,
  * batch}, their tokens `pitch` floats apart (heads * head_dim, or more where the heads lie in a wider matrix, as
- * the queries and keys of one merged projection do).  Of each head the first rotary_dim values (even, 2 to 4096) are
+ * the queries and keys of one merged projection do), heads * head_dim at most 2^30.  Of each head the first rotary_dim values (even, 2 to 4096) are
  * turned in pairs, i < rotary_dim / 2:  (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved;
  *   (y1, y2) = magnitude * (x1 cos a - x2 sin a, x1 sin a + x2 cos a),  a = position * f_i
  *   f_i = base^(-2 i / rotary_dim);  the gradient is the turn back, dx1 = magnitude * (dy1 cos a + dy2 sin a), ...
@@ -493,13 +493,17 @@ int mnv_rotary_bwd(const float* dy, const float* positions, float* dx, int head_
  * activation: 0 sigmoid, 1 relu (slope 0 at 0), 2 tanh, 3 silu x / (1 + exp(-x)), 4 gelu x Phi(x) with the normal distribution's Phi.
  * forward writes h, and pre unless it is NULL (no backward pass follows); backward reads both, and writes dpre, which
  * may be pre itself; dx may be NULL if nobody needs it.  Each matrix holds less than 2^29 values.
- * A workspace is used if it is aligned to 16 bytes.  Large products, from 5 GFLOP on, run in pairs of fp16 numbers where the workspace
- * holds those: every value is rounded to 22 bits, 2^-22 of itself or 2^-39 of the largest in its row of the left matrix (column of the right
- * one; rows and columns over which the product sums), whichever is more, products are exact but for 2^-22 and summed in fp32.  The result is as near to the
- * exact one as fp32 products' is, whose error is that of the sum.  An infinity or NaN then gives NaN in all of the results that its row has a part
- * in.  Other products, and all of them with a workspace that is too small for it, are those of mnv_sgemm_nn.  Without a workspace pre == NULL costs
- * few tokens more time.  mnv_gated_ffn_plan: which products run in pairs with workspaces of these sizes, as a sum of 1 pre, 2 y, 4 dh,
- * 8 dx, 16 dw_in, 32 dw_out. ---- */
+ * A workspace is used if it is aligned to 16 bytes.  Without one, pre == NULL costs few tokens more time.
+ * Products are those of mnv_sgemm_nn but for
+ *   large ones, from 5 GFLOP on, where the workspace holds their factors as pairs of fp16 numbers: every value is rounded to 22
+ *   bits, 2^-22 of itself or 2^-39 of the largest in its row of the left matrix (column of the right one; rows and columns
+ *   that the product sums over), whichever is more, products are exact but for 2^-22 and summed in fp32.  The result is as
+ *   near to the exact one as fp32 products' is, whose error is that of the sum.  An infinity or NaN then gives NaN in all
+ *   results that its row has a part in.
+ *   those of 5 to 160 tokens with weights of some million values: the fp32 instruction sums them, in eight wavefronts and up to
+ *   16 ranges.
+ * mnv_gated_ffn_plan: which products run in pairs with workspaces of these sizes, as a sum of 1 pre, 2 y, 4 dh, 8 dx,
+ * 16 dw_in, 32 dw_out. ---- */
 size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens);
 int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y,
                       int features, int hidden, int tokens, int activation, void* workspace,
@@ -518,7 +522,7 @@ int mnv_gated_ffn_bwd(const float* x, const float* w_in, const float* w_out, con
  * (rates, decays NULL: 1 each) and t = step, from 1 on:
  *   g = grad_scale * grads;  m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g^2
  *   p' = p - rate_i * (m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps) + decay_i * p)
- * params_out may be params, m_out m and v_out v.  schedule: NULL, or two floats on the device, the rate and t, read when the kernel
+ * params_out may be params, m_out m and v_out v; no result shares memory with another tensor's arrays.  schedule: NULL, or two floats on the device, the rate and t, read when the kernel
  * runs instead of `rate` and `step`: a recorded step is replayed with others.
  * bits 32: m and v are as long as the tensor.  bits 8: a column {65} for every 256 of the tensor's values, the last one's
  * rest 0: 64 floats whose bytes are the values' codes (byte j, value j), and the largest size among them, `top`;

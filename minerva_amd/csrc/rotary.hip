@@ -156,7 +156,8 @@ int rotary(const float* x, const float* positions, float* y, int head_dim, int h
            double magnitude, bool back, mnv_stream_t stream) {
   if (!x || !y || head_dim <= 0 || heads <= 0 || length <= 0 || batch <= 0) return MNV_ERR_INVALID;
   const long long tokens = (long long)length * batch, width = (long long)heads * head_dim;
-  if (width > x_pitch || width > y_pitch || tokens > 0x7fffffffLL || (x == y && x_pitch != y_pitch)) return MNV_ERR_INVALID;
+  // (a workgroup counts its vectors in 32 bits)
+  if (width > 1 << 30 || width > x_pitch || width > y_pitch || tokens > 0x7fffffffLL || (x == y && x_pitch != y_pitch)) return MNV_ERR_INVALID;
   if (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > head_dim || rotary_dim > 4096) return MNV_ERR_INVALID;
   if (!(base > 0.0) || !(factor > 0.0) || !isfinite(base) || !isfinite(factor) || !isfinite(magnitude)) return MNV_ERR_INVALID;
   if (!(low_turns >= 0.0) || !isfinite(high_turns) || context < 0) return MNV_ERR_INVALID;

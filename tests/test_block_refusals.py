@@ -125,3 +125,10 @@ def test_adamw_values_refuses():
 def test_floats_of_a_moment(n):
     f = capi.lib().mnv_adamw_moment_floats
     assert f(n, 32) == n and f(n, 8) == moment_floats(n, 8) and f(n, 16) == 0
+
+
+@pytest.mark.parametrize("name", ["mnv_rotary_fwd", "mnv_rotary_bwd"])
+@pytest.mark.parametrize("head_dim,heads", [((1 << 30) + 2, 1), (2, (1 << 29) + 1), (0x7fffffff, 1)])
+def test_rotary_refuses_heads_past_2_30_values(name, head_dim, heads):
+    wide = {**ROTARY, "head_dim": head_dim, "heads": heads, "rotary_dim": 2, "x_pitch": 0x7fffffff, "y_pitch": 0x7fffffff, "length": 1, "batch": 1}
+    assert getattr(capi.lib(), name)(P, None, ctypes.c_void_p(1 << 40), *wide.values(), None) == INVALID
