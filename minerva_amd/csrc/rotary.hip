@@ -4,6 +4,7 @@
 // it makes few turns within the old context, and kept where it makes many.
 // Angles are counted in whole turns in 64 bits (a position of 10^6 would cost 32 bits all but one digit of the
 // fastest angle) and brought to an eighth of a turn before they are 32-bit numbers.
+// Bound by HBM, 8 bytes a value: 2 x 16384 tokens of 16 heads of 128 93 us, 5.8 TB/s; few tokens by the launch (3 us).
 #include <math.h>
 
 #include "mnv_common.h"
@@ -125,8 +126,10 @@ int launch(RotaryShape z, const RotaryAngles& a, hipStream_t s) {
   z.half_div = mnv_fastdiv_make(z.half);
   z.length_div = mnv_fastdiv_make(z.length);
   const int cus = mnv_cu_count();
-  // About 8192 values to a workgroup, fewer where that leaves CUs without one: then single tokens, and parts of their heads.
-  long long per = 8192 / ((long long)z.heads * z.head_dim);
+  // About 2048 values to a workgroup, fewer where that leaves CUs without one: then single tokens, and parts of their heads.  us of both
+  // passes with 1024 / 2048 / 4096 / 8192: 2 x 16384 tokens of 16 heads of 128 185 / 185 / 189 / 195, 8 x 4096 of 20 of 24 heads of 64
+  // 118 / 118 / 125 / 133, 8 x 16384 of one 33 / 31 / 33 / 36.
+  long long per = 2048 / ((long long)z.heads * z.head_dim);
   const long long lds_most = 8192 / (2LL * z.half);  // 32 KB
   if (per > lds_most) per = lds_most;
   if (per > z.tokens / (2LL * cus)) per = z.tokens / (2LL * cus);
