@@ -393,7 +393,8 @@ Product product_dw(const float* left, const float* right, int rows, int columns,
 }
 // Whether a product runs in pairs: where that is estimated at less than the SGEMM's time, and the workspace holds it.  The
 // SGEMM's own estimate is 1.2 times too low where products of this size follow each other, and more where it is above 216 TFLOP/s: 180 of
-// them last (both passes, without / with that: 4096 tokens of 1024 -> 2816 955 / 936, 500 of 4096 -> 8192 1511 / 1462).  us, both passes, in pairs never / so: 4096 tokens
+// them last (both passes, without / with that: 4096 tokens of 1024 -> 2816 955 / 936, 500 of 4096 -> 8192 1511 / 1462).  It is one of a plain
+// product: what the store moves beyond 4 bytes comes on top (without / with: 8192 of 768 -> 2048 1089 / 1041, 16384 of 512 -> 2048 1580 / 1512).  us, both passes, in pairs never / so: 4096 tokens
 // of 1024 -> 2816 1212 / 958, 1024 of 2048 -> 5632 1203 / 921, 8192 of 2048 -> 5632 8360 / 5120, 300 of 4096 -> 8192 1202 / 1100 (all in pairs 1240).
 bool in_pairs(const Product& p, int most_ranges, size_t ws_bytes, PairPlan* plan) {
   // below 5 GFLOP the four launches of the packing alone take half of the time
@@ -403,7 +404,7 @@ bool in_pairs(const Product& p, int most_ranges, size_t ws_bytes, PairPlan* plan
   const SgemmPlan other = plan_unlimited(p.a.rows, p.b.rows, p.a.k, cus);
   double us = other.us;
   if ((other.split && other.splits == 1) || p.a.gate) us = std::min(us, tiles_cost(p.a.rows, p.b.rows, p.a.k, (size_t)-1, cus));
-  us = std::max(1.2 * us, 2e-6 * p.a.rows * p.b.rows * p.a.k / 180.0);
+  us = std::max(1.2 * us, 2e-6 * p.a.rows * p.b.rows * p.a.k / 180.0) + (p.store_bytes - 4.0) * 1e-6 / 5.0 * p.a.rows * p.b.rows;
   return plan->us < us && plan->bytes() <= ws_bytes;
 }
 size_t pair_bytes(const Product& p, int most_ranges) {
