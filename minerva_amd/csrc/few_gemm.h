@@ -9,7 +9,7 @@ namespace {
 constexpr int FEW_ROWS = 64, FEW_K = 16, FEW_WAVES = 8;
 
 // C = A B, B {K, N} with its columns contiguous, A with its rows (x-fast) or its k contiguous, through a policy's A, B, M, N, K, lda, ldb
-// (floats), a_row and c_store4.  A workgroup has 64 rows, 16 COLS columns and a k range (gridDim.z); its eight wavefronts take every eighth step of
+// (floats), a_row and c_store4.  A workgroup has 64 rows, 16 COLS columns and a k range; its eight wavefronts take every eighth step of
 // 16 k, and their sums are added through LDS in order.  Lane (i, h) = (lane % 16, lane / 16) fetches rows 4 i .. 4 i + 3 at k = 4 h + j
 // for j of 4, or k = 4 h .. 4 h + 3 of each of these rows, and k = 4 h .. 4 h + 3 of column i.  Value j of k is then what the fp32
 // instruction wants of the lane for k = {j, 4 + j, 8 + j, 12 + j}, in either order, so that the operands go from memory to the instruction without
@@ -20,17 +20,18 @@ constexpr int FEW_ROWS = 64, FEW_K = 16, FEW_WAVES = 8;
 // columns 23 / 23 / 28 / 34 / 42 us, 49 / 48 / 56 / 63 from 16 on; 92 MB, i.e. 4.0 TB/s up to 16 columns.  From 32 on the matrix
 // instruction, at 0.7 of its rate, and how the workgroups divide on the CUs bound it.
 template <class P, int COLS>
-__global__ __launch_bounds__(FEW_WAVES * MNV_WAVE, 4) void few_gemm_kernel(P prob, int blocks_m, int blocks_n, int per_range,
+__global__ __launch_bounds__(FEW_WAVES * MNV_WAVE, 4) void few_gemm_kernel(P prob, int blocks_m, int blocks_n, int ranges, int per_range,
                                                                                           float* __restrict__ partial) {
   typedef float Acc __attribute__((ext_vector_type(4)));
   constexpr int AHEAD = 5 - COLS, AT_ONCE = COLS < 2 ? COLS : 2;
   extern __shared__ __align__(16) float few_sums[];  // [wavefront][column][row]
-  // the column blocks of the same rows on one XCD, next to each other
-  const int id = blockIdx.x, block_m = id % 8 + id / (8 * blocks_n) * 8, block_n = id / 8 % blocks_n;
-  if (block_m >= blocks_m) return;
+  // an XCD has a run of these: the column blocks of the same rows next to each other, then neighbouring rows, which share lines where a
+  // column is no multiple of them (33 columns, forward, 2048 -> 5632 65 -> 57 us, 2049 -> 5633 72 -> 70), then the ranges
+  const int id = mnv_tile_remap((int)blockIdx.x, (int)gridDim.x), block_n = id % blocks_n, block_m = id / blocks_n % blocks_m;
+  const int range = id / (blocks_n * blocks_m);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / MNV_WAVE)), lane = threadIdx.x % MNV_WAVE, i = lane % 16, h = lane / 16;
   const int m0 = block_m * FEW_ROWS, n0 = block_n * COLS * 16;
-  const int steps = (prob.K + FEW_K - 1) / FEW_K, first = (int)blockIdx.z * per_range + wave, end = min(steps, ((int)blockIdx.z + 1) * per_range);
+  const int steps = (prob.K + FEW_K - 1) / FEW_K, first = range * per_range + wave, end = min(steps, (range + 1) * per_range);
   typename P::Res res;
   prob.make_res(res);
   const unsigned lda = (unsigned)prob.lda * 4u, ldb = (unsigned)prob.ldb * 4u;
@@ -114,10 +115,10 @@ __global__ __launch_bounds__(FEW_WAVES * MNV_WAVE, 4) void few_gemm_kernel(P pro
 #pragma unroll
     for (int w = 1; w < FEW_WAVES; ++w) x += *reinterpret_cast<const mnv_f4*>(few_sums + w * REGION + e * 4);
     const float v[4] = {x[0], x[1], x[2], x[3]};
-    if (gridDim.z == 1) {
+    if (ranges == 1) {
       prob.c_store4(m, n, v);
     } else {
-      float* const p = partial + ((size_t)blockIdx.z * prob.N + n) * prob.M + m;
+      float* const p = partial + ((size_t)range * prob.N + n) * prob.M + m;
       if (m + 3 < prob.M) {
         *reinterpret_cast<mnv_f4u*>(p) = mnv_f4u{x[0], x[1], x[2], x[3]};
       } else {
@@ -136,19 +137,26 @@ struct FewPlan {
 };
 
 // The plan of an m x n x k product with A's k contiguous or not, or none (cols 0).  Against the SGEMM's plans on 180 products (12 shapes of
-// 64 -> 172 up to 4096 -> 14000, 1 to 220 columns): it gains from 5 columns on, where A has `least` values (for less, other tiles cover the chip
-// sooner), up to 64 columns, or 160 of a matrix of up to 9 million values, whose tiles of the SGEMM are too few for the
-// chip; up to 48 of one with k contiguous or from 64 million values on, where the matrix instruction bounds it (4096 x 8192 at 64 columns
-// 49 / 57); one of k contiguous from there on has 12 columns read it faster in the SGEMM (4096 x 28000 87 / 100).
-// So many ranges that the workgroups are just one to a CU, of at least 128 k: 1.02 times the best number's time.
+// 64 -> 172 up to 4096 -> 14000, 1 to 220 columns) and a block's passes of 10 more, even and odd: it gains from 5 columns on, where A
+// has `least` values (for less, other tiles cover the chip sooner), up to 64 columns, or 160 of a matrix of up to 9 million values, whose tiles
+// of the SGEMM are too few for the chip; up to 48 of one with k contiguous or from 64 million values on, where the matrix instruction
+// bounds it (4096 x 8192 at 64 columns 49 / 57).  Not where the SGEMM's reads of up to 12 columns are as quick: below 9 columns from 16 million
+// values on (5 columns, forward, 3001 -> 9001 72 / 78 us), below 13 of k contiguous from 64 million on (4096 x 28000 87 / 100); nor
+// for more than 32 columns from 20 million values on in rows off the 128-byte grid, where 256 bytes take a third line (33 columns, forward,
+// 2049 -> 5633 61 / 70 us, 2048 -> 5632 72 / 57).
+// So many ranges that the workgroups are just one to a CU, of at least 128 k: 1.02 times the best number's time; two and a half for up to
+// 16 columns of rows contiguous from 8 million values on, where the fetches of one are too few for HBM (16 columns, forward, 3000 -> 9000 97 -> 83 us).
 FewPlan plan_few(int m, int n, int k, bool k_fast, double least, size_t ws_bytes) {
   const double values = (double)m * k;
-  const bool large = values >= 64e6;
+  const bool large = values >= 64e6, cut = !k_fast && values >= 20e6 && m % 32;
+  const int from = k_fast ? (large ? 13 : 5) : values >= 16e6 ? 9 : 5;
+  const int most = cut ? 32 : k_fast || large ? 48 : values <= 9e6 ? 160 : 64;
   FewPlan plan;
-  if (values < least || n < (k_fast && large ? 13 : 5) || n > (k_fast || large ? 48 : values <= 9e6 ? 160 : 64)) return plan;
+  if (values < least || n < from || n > most) return plan;
   plan.cols = n <= 16 ? 1 : n <= 32 ? 2 : n <= 48 ? 3 : n <= 64 ? 2 : (n + 47) / 48 * 3 <= (n + 31) / 32 * 2 ? 3 : 2;
-  const int blocks = (m + FEW_ROWS - 1) / FEW_ROWS * ((n + plan.cols * 16 - 1) / (plan.cols * 16));
-  plan.ranges = std::max(1, std::min(std::min(16, k / 128), mnv_cu_count() / blocks));
+  const int blocks = (m + FEW_ROWS - 1) / FEW_ROWS * ((n + plan.cols * 16 - 1) / (plan.cols * 16)), cus = mnv_cu_count();
+  const int workgroups = !k_fast && n <= 16 && values >= 8e6 ? cus * 5 / 2 : cus;
+  plan.ranges = std::max(1, std::min(std::min(16, k / 128), workgroups / blocks));
   while (plan.bytes(m, n) > ws_bytes) --plan.ranges;
   return plan;
 }
@@ -158,8 +166,8 @@ int launch_few_cols(const FewPlan& plan, const P& p, float* partial, hipStream_t
   const int blocks_m = (p.M + FEW_ROWS - 1) / FEW_ROWS, blocks_n = (p.N + COLS * 16 - 1) / (COLS * 16);
   const int steps = (p.K + FEW_K - 1) / FEW_K, per = (steps + plan.ranges - 1) / plan.ranges;
   const int lds = FEW_WAVES * (COLS < 2 ? COLS : 2) * 16 * FEW_ROWS * (int)sizeof(float);
-  hipLaunchKernelGGL((few_gemm_kernel<P, COLS>), dim3((unsigned)((blocks_m + 7) / 8 * 8 * blocks_n), 1, (unsigned)plan.ranges),
-                     dim3(FEW_WAVES * MNV_WAVE), lds, s, p, blocks_m, blocks_n, per, partial);
+  hipLaunchKernelGGL((few_gemm_kernel<P, COLS>), dim3((unsigned)blocks_m * blocks_n * plan.ranges), dim3(FEW_WAVES * MNV_WAVE), lds, s, p, blocks_m,
+                     blocks_n, plan.ranges, per, partial);
   return MNV_LAUNCH_STATUS();
 }
 // The k ranges of a plan with more than one are left in `partial`, range by range as {M, N}.
