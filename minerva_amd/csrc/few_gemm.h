@@ -21,12 +21,12 @@ constexpr int FEW_ROWS = 64, FEW_K = 16, FEW_WAVES = 8;
 // instruction, at 0.7 of its rate, and how the workgroups divide on the CUs bound it.
 template <class P, int COLS>
 __global__ __launch_bounds__(FEW_WAVES * MNV_WAVE, 4) void few_gemm_kernel(P prob, int blocks_m, int blocks_n, int ranges, int per_range,
-                                                                                          float* __restrict__ partial) {
+                                                                              float* __restrict__ partial) {
   typedef float Acc __attribute__((ext_vector_type(4)));
   constexpr int AHEAD = 5 - COLS, AT_ONCE = COLS < 2 ? COLS : 2;
   extern __shared__ __align__(16) float few_sums[];  // [wavefront][column][row]
   // an XCD has a run of these: the column blocks of the same rows next to each other, then neighbouring rows, which share lines where a
-  // column is no multiple of them (33 columns, forward, 2048 -> 5632 65 -> 57 us, 2049 -> 5633 72 -> 70), then the ranges
+  // column is no multiple of them (dealt out one by one, 33 columns, forward, 3001 -> 9001 138 -> 132 us, 5 columns 112 -> 93), then the ranges
   const int id = mnv_tile_remap((int)blockIdx.x, (int)gridDim.x), block_n = id % blocks_n, block_m = id / blocks_n % blocks_m;
   const int range = id / (blocks_n * blocks_m);
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / MNV_WAVE)), lane = threadIdx.x % MNV_WAVE, i = lane % 16, h = lane / 16;
@@ -143,7 +143,7 @@ struct FewPlan {
 // bounds it (4096 x 8192 at 64 columns 49 / 57).  Not where the SGEMM's reads of up to 12 columns are as quick: below 9 columns from 16 million
 // values on (5 columns, forward, 3001 -> 9001 72 / 78 us), below 13 of k contiguous from 64 million on (4096 x 28000 87 / 100); nor
 // for more than 32 columns from 20 million values on in rows off the 128-byte grid, where 256 bytes take a third line (33 columns, forward,
-// 2049 -> 5633 61 / 70 us, 2048 -> 5632 72 / 57).
+// 4095 -> 4097 72 / 89 us, 4096 -> 4096 76 / 60).
 // So many ranges that the workgroups are just one to a CU, of at least 128 k: 1.02 times the best number's time; two and a half for up to
 // 16 columns of rows contiguous from 8 million values on, where the fetches of one are too few for HBM (16 columns, forward, 3000 -> 9000 97 -> 83 us).
 FewPlan plan_few(int m, int n, int k, bool k_fast, double least, size_t ws_bytes) {

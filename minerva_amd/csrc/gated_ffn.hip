@@ -7,8 +7,8 @@
 // weights.  Products are those of the SGEMM (sgemm_core.h), large ones in pairs of fp16 numbers (pair_gemm.h), those of large
 // weights and few tokens of few_gemm.h; what lies between them is done where a product is stored: the gate forward, where both projections
 // of a row meet in one tile, and dpre backward, which is all that is kept of dh.
-// Both passes: 8192 tokens of 2048 -> 5632 5.1 ms (333 TFLOP/s), 4096 of 1024 -> 2816 0.95 ms (225); forward: 777 of 1001 -> 2731
-// 112 us (113), 4 of 1024 -> 4096 23 us (50 MB of weights, 2.2 TB/s over four launches).
+// Both passes: 8192 tokens of 2048 -> 5632 5.0 ms (340 TFLOP/s), 4096 of 1024 -> 2816 0.90 ms (236); forward: 777 of 1001 -> 2731
+// 110 us (115), 4 of 1024 -> 4096 23 us (50 MB of weights, 2.2 TB/s over four launches).
 #include <algorithm>
 
 #include "few_gemm.h"
