@@ -31,8 +31,8 @@ __device__ __forceinline__ void activate(int kind, const float (&x)[N], float (&
   if (kind == ACT_RELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      value[i] = x[i] > 0.f ? x[i] : 0.f;
-      slope[i] = x[i] > 0.f ? 1.f : 0.f;
+      value[i] = x[i] <= 0.f ? 0.f : x[i];  // (a NaN is not below 0: it goes on)
+      slope[i] = x[i] <= 0.f ? 0.f : x[i] > 0.f ? 1.f : x[i];
     }
   } else if (kind == ACT_TANH) {
 #pragma unroll
