@@ -475,7 +475,8 @@ int mnv_relative_bias_bwd(const float* dbias, float* dtable, int buckets, int he
  *   f_i * (w + (1 - w) / factor),  w = (context * f_i / (2 pi) - low_turns) / (high_turns - low_turns) cut to 0 ... 1
  * (frequencies of many turns within `context` positions stay as they are).  low_turns and high_turns are 0 otherwise.
  * y may be x, and dx dy, if their pitches are equal: the values behind are then left alone.  Angles are
- * computed in 64 bits, to about 1e-7 of a turn's cosine and sine. ---- */
+ * computed in 64 bits, off by some 2^-52 of themselves (1e-7 of a turn at 2^31 radians), and their cosines and sines, times
+ * the magnitude, are rounded to 32 bits once. ---- */
 int mnv_rotary_fwd(const float* x, const float* positions, float* y, int head_dim, int heads, int length,
                    int batch, int x_pitch, int y_pitch, int rotary_dim, int interleaved, int start,
                    double base, double factor, int context, double low_turns, double high_turns,

@@ -3,7 +3,7 @@
 // The gradient is the turn by -a.  For contexts longer than the angles were made for, f_i is divided by `factor` where
 // it makes few turns within the old context, and kept where it makes many.
 // Angles are counted in whole turns in 64 bits (a position of 10^6 would cost 32 bits all but one digit of the
-// fastest angle) and brought to an eighth of a turn before they are 32-bit numbers.
+// fastest angle), and their cosines and sines, times the magnitude, are rounded to 32 bits once.
 // Bound by HBM, 8 bytes a value: 2 x 16384 tokens of 16 heads of 128 93 us, 5.8 TB/s; few tokens by the launch (3 us).
 #include <math.h>
 
@@ -31,22 +31,40 @@ struct RotaryShape {
   float sign;      // -1: the gradient
 };
 
-// Turns of pair i at a position, as cosine and sine.
-__device__ __forceinline__ void turn(const RotaryAngles& a, int i, double position, float& c, float& s) {
+// Turns that a position adds to pair i.
+__device__ __forceinline__ double frequency(const RotaryAngles& a, int i) {
   double f = exp2(i * a.log2_step) * 0.15915494309189535;  // 1 / (2 pi)
   if (a.inverse_factor != 1.0) {
     double w = (a.context * f - a.low) * a.inverse_range;
     w = w < 0.0 ? 0.0 : w > 1.0 ? 1.0 : w;
     f *= w + (1.0 - w) * a.inverse_factor;
   }
-  const double turns = position * f, quarters = rint(4.0 * turns);
-  float cr, sr;
-  sincospif((float)(2.0 * (turns - 0.25 * quarters)), &sr, &cr);
+  return f;
+}
+
+// Cosine and sine of so many turns: brought to an eighth of a turn by the nearest quarter, where the series' next terms, t^17 / 17! and
+// t^16 / 16!, are below 2^-49.
+__device__ __forceinline__ void cosine_sine(double turns, double& c, double& s) {
+  const double quarters = rint(4.0 * turns), t = (turns - 0.25 * quarters) * 6.283185307179586, u = t * t;
+  double x = -1.0 / 1307674368000.0, y = -1.0 / 87178291200.0;
+  x = fma(u, x, 1.0 / 6227020800.0);
+  y = fma(u, y, 1.0 / 479001600.0);
+  x = fma(u, x, -1.0 / 39916800.0);
+  y = fma(u, y, -1.0 / 3628800.0);
+  x = fma(u, x, 1.0 / 362880.0);
+  y = fma(u, y, 1.0 / 40320.0);
+  x = fma(u, x, -1.0 / 5040.0);
+  y = fma(u, y, -1.0 / 720.0);
+  x = fma(u, x, 1.0 / 120.0);
+  y = fma(u, y, 1.0 / 24.0);
+  x = fma(u, x, -1.0 / 6.0);
+  y = fma(u, y, -0.5);
+  x = fma(u * t, x, t);
+  y = fma(u, y, 1.0);
   const int q = (int)(quarters - 4.0 * floor(0.25 * quarters));  // 0 .. 3
-  const float m = (float)a.magnitude;
-  const float cq = q & 1 ? -sr : cr, sq = q & 1 ? cr : sr;
-  c = (q & 2 ? -cq : cq) * m;
-  s = (q & 2 ? -sq : sq) * m;
+  const double cq = q & 1 ? -x : y, sq = q & 1 ? y : x;
+  c = q & 2 ? -cq : cq;
+  s = q & 2 ? -sq : sq;
 }
 
 template <int W>
@@ -66,14 +84,20 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryShape z, RotaryAngles
   const int heads = z.heads - head0 < z.head_chunk ? z.heads - head0 : z.head_chunk;
   float* const cosines = lds;
   float* const sines = lds + z.per_wg * z.half;
+  int pair = -1;
+  double f = 0.0;
   for (int e = threadIdx.x; e < count * z.half; e += 256) {
     const int t = mnv_fastdiv(e, z.half_div), i = e - t * z.half, token = token0 + t;
+    if (i != pair) {  // (a thread has the same one for all of its tokens where `half` divides 256)
+      f = frequency(angles, i);
+      pair = i;
+    }
     const double position =
         z.positions ? (double)z.positions[token] : (double)(z.start + (token - mnv_fastdiv(token, z.length_div) * z.length));
-    float c, s;
-    turn(angles, i, position, c, s);
-    cosines[e] = c;
-    sines[e] = s * z.sign;
+    double s, c;
+    cosine_sine(position * f, c, s);
+    cosines[e] = (float)(c * angles.magnitude);
+    sines[e] = (float)(s * angles.magnitude) * z.sign;
   }
   __syncthreads();
   constexpr int W = PAIRED ? 2 * V : V;  // values of a load
