@@ -79,7 +79,9 @@ struct Vec {
 template <int V, bool PAIRED, int C>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryShape z, RotaryAngles angles) {
   extern __shared__ __align__(16) float lds[];  // cosines [per_wg][half], sines
-  const int token0 = blockIdx.x * z.per_wg, head0 = blockIdx.y * z.head_chunk;
+  const long long first = ((long long)blockIdx.z * gridDim.x + blockIdx.x) * z.per_wg;
+  if (first >= z.tokens) return;
+  const int token0 = (int)first, head0 = blockIdx.y * z.head_chunk;
   const int count = z.tokens - token0 < z.per_wg ? z.tokens - token0 : z.per_wg;
   const int heads = z.heads - head0 < z.head_chunk ? z.heads - head0 : z.head_chunk;
   float* const cosines = lds;
@@ -170,9 +172,11 @@ int launch(RotaryShape z, const RotaryAngles& a, hipStream_t s) {
     if (chunk < least) chunk = least;
     if (chunk < z.head_chunk) z.head_chunk = chunk;
   }
-  const int chunks = (z.heads + z.head_chunk - 1) / z.head_chunk;
-  if (chunks > 65535 || groups > 0x7fffffffLL) return MNV_ERR_INVALID;
-  const dim3 grid((unsigned)groups, chunks);
+  // A grid has 65535 chunks at most, and less than 2^32 threads along x: groups past 2^23 are dealt out along z.
+  const int most_chunks = 65535;
+  if ((z.heads - 1) / z.head_chunk >= most_chunks) z.head_chunk = (z.heads - 1) / most_chunks + 1;
+  const long long across = groups < 1 << 23 ? groups : 1 << 23;
+  const dim3 grid((unsigned)across, (z.heads - 1) / z.head_chunk + 1, (unsigned)((groups + across - 1) / across));
   const size_t lds = (size_t)z.per_wg * z.half * 2 * sizeof(float);
   hipLaunchKernelGGL((rotary_kernel<V, PAIRED, C>), grid, dim3(256), lds, s, z, a);
   return MNV_LAUNCH_STATUS();
