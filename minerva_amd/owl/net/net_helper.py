@@ -189,6 +189,11 @@ def save_net_to_file(owl_net, weightpath, snapshotidx):
     """net_helper.py:233-270"""
     folder = _snapshot_dir(weightpath, snapshotidx)
     os.makedirs(folder, exist_ok=True)
+    # what another run left here: without the number of steps, which is written last, moments are not taken for these weights'
+    _remove(os.path.join(folder, "adamw_steps.dat"))
+    for base, _ in _moment_files(owl_net, folder):
+        _remove(base + "_m.dat")
+        _remove(base + "_v.dat")
     for uid in owl_net.get_weighted_unit_ids():
         unit = owl_net.units[uid]
         base = os.path.join(folder, unit.name.replace("/", "_"))
@@ -205,6 +210,11 @@ def save_net_to_file(owl_net, weightpath, snapshotidx):
             m.to_numpy().ravel().tofile(base + "_m.dat")
             v.to_numpy().ravel().tofile(base + "_v.dat")
         np.array([opt.steps], np.float32).tofile(os.path.join(folder, "adamw_steps.dat"))
+
+
+def _remove(path):
+    if os.path.isfile(path):
+        os.remove(path)
 
 
 def _moment_files(owl_net, folder):
@@ -242,13 +252,13 @@ def init_net_from_file(owl_net, weightpath, snapshotidx):
 
 
 def _init_moments(owl_net, folder, need_reinit):
-    """The optimizer's state, all of it or none."""
+    """The optimizer's state, all of it or none: none, too, if a weight or bias that it belongs to is not there."""
     opt = owl_net.optimizer
     files = _moment_files(owl_net, folder)
     sizes = [int(np.prod(shape)) for _, shape in files]
     steps = os.path.join(folder, "adamw_steps.dat")
     want = [(base + end, opt.moment_shape(n)) for end in ("_m.dat", "_v.dat") for (base, _), n in zip(files, sizes)]
-    if not os.path.isfile(steps) or any(not os.path.isfile(p) or os.path.getsize(p) != 4 * int(np.prod(s)) for p, s in want):
+    if need_reinit or not os.path.isfile(steps) or any(not os.path.isfile(p) or os.path.getsize(p) != 4 * int(np.prod(s)) for p, s in want):
         opt.m = opt.v = opt.sizes = None
         opt.steps = 0
         need_reinit.append("adamw moments")
