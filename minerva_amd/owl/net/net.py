@@ -624,6 +624,8 @@ class Net(object):
             self.units[u].backward(from_top, unit_to_btms[u], phase)
 
     def update(self, uid):
+        if self.optimizer is not None:
+            raise RuntimeError("AdamW steps over all arrays at once: call weight_update, not update of one unit")
         self.units[uid].weight_update(self.current_lr, self.base_weight_decay, self.momentum,
                                       self.batch_size)
 
