@@ -10,6 +10,7 @@ becomes '_').  A network whose solver is AdamW also keeps `adamw_steps.dat`, the
 `<layer>_weights_m.dat`, `<layer>_weights_v.dat`, `<layer>_bias_m.dat` and `<layer>_bias_v.dat`, the moments as they are held."""
 import os
 import re
+import warnings
 
 import numpy as np
 
@@ -138,7 +139,10 @@ class NetBuilder(object):
         owl_net.momentum = s.get("momentum", 0.0)
         owl_net.solver = s
         owl_net.lr_policy = s.get("lr_policy", "fixed")
-        if s.get("type", "SGD") == "AdamW":  # momentum is beta1, momentum2 beta2, delta what the root is guarded by
+        kind = str(s.get("type", s.get("solver_type", "SGD")))
+        if kind.upper() not in ("SGD", "ADAMW"):
+            warnings.warn("solver type %r is not implemented: momentum SGD runs in its place" % kind)
+        if kind.upper() == "ADAMW":  # momentum is beta1, momentum2 beta2, delta what the root is guarded by
             owl_net.optimizer = _seq.AdamW(owl_net.base_lr, s.get("momentum", 0.9), s.get("momentum2", 0.999), s.get("delta", 1e-8),
                                            owl_net.base_weight_decay, s.get("moment_bits", 32))
         stacked_layers, top_name_to_layer = {}, {}

@@ -1,4 +1,4 @@
-"""What a network with an optimizer of its own does with a single unit's update.  Nothing is launched, so this runs
+"""Which solver a network description gets by its type, and what a network with AdamW does with a single unit's update.  Nothing is launched, so this runs
 without a GPU."""
 import pytest
 
@@ -31,3 +31,22 @@ def test_one_units_update_is_refused_with_adamw(monkeypatch):
     net.current_lr = 0.1
     net.update(uid)
     assert called == [(0.1, 0.0, 0.8, net.batch_size)]
+
+
+@pytest.mark.parametrize("spelling", ["AdamW", "ADAMW", "adamw"])
+def test_adamw_in_any_case(spelling):
+    assert built('type: "%s"' % spelling).optimizer is not None
+
+
+@pytest.mark.parametrize("solver", ["", 'type: "SGD"', 'type: "sgd"'])
+def test_momentum_sgd_is_taken_in_silence(solver, recwarn):
+    assert built(solver).optimizer is None
+    assert not recwarn.list
+
+
+@pytest.mark.parametrize("spelling", ["Adam", "AdamW ", "Nesterov"])
+def test_other_types_are_not_taken_in_silence(spelling):
+    """They run as momentum SGD, as every type did before there was another, and say so."""
+    for name in ("type", "solver_type"):
+        with pytest.warns(UserWarning, match="momentum SGD"):
+            assert built('%s: "%s"' % (name, spelling)).optimizer is None
