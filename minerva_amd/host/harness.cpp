@@ -59,6 +59,7 @@ Scale ToScale(const mnvh_tensor& t) {
 
 int P(const double* p, int n, int i) {
   MNV_CHECK(i < n) << "missing operator parameter " << i;
+  MNV_CHECK(p[i] > -2147483649.0 && p[i] < 2147483648.0) << "operator parameter " << i << " is no whole number of 32 bits: " << p[i];
   return static_cast<int>(p[i]);
 }
 
