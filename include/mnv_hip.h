@@ -498,13 +498,18 @@ int mnv_rotary_bwd(const float* dy, const float* positions, float* dx, int head_
  * Products are those of mnv_sgemm_nn but for
  *   large ones, from 5 GFLOP on, where the workspace holds their factors as pairs of fp16 numbers: every value is rounded to 22
  *   bits, 2^-22 of itself or 2^-39 of the largest in its row of the left matrix (column of the right one; rows and columns
- *   that the product sums over), whichever is more, products are exact but for 2^-22 and summed in fp32.  The result is as
- *   near to the exact one as fp32 products' is, whose error is that of the sum.  An infinity or NaN then gives NaN in all
- *   results that its row has a part in.
+ *   that the product sums over), whichever is more, products are exact but for 2^-22 and summed in fp32.  Where values of a row
+ *   (column) are within 2^-17 of its largest, or those that are not count for little beside it, the result is as near to the exact one
+ *   as the fp32 instruction's, whose error is that of the sum, and off by up to twice as much as mnv_sgemm_nn's; where the largest
+ *   meets a 0, what 2^-39 of it hides is lost.  An infinity or NaN gives NaN in all results that its row has a part in.
+ *   mnv_gated_ffn_pairs_mode(0) switches them off: all 24 bits of every value count then.
  *   those of 5 to 160 tokens with weights of some million values: the fp32 instruction sums them, in eight wavefronts and up to
  *   16 ranges.
  * mnv_gated_ffn_plan: which products run in pairs with workspaces of these sizes, as a sum of 1 pre, 2 y, 4 dh, 8 dx,
- * 16 dw_in, 32 dw_out. ---- */
+ * 16 dw_in, 32 dw_out.
+ * mnv_gated_ffn_pairs_mode: 0 none, 1 (initial) where an estimate puts them ahead.  Process-wide; returns the previous mode; any
+ * other value only queries. ---- */
+int mnv_gated_ffn_pairs_mode(int mode);
 size_t mnv_gated_ffn_fwd_workspace_bytes(int features, int hidden, int tokens);
 int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, float* pre, float* h, float* y,
                       int features, int hidden, int tokens, int activation, void* workspace,

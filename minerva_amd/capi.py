@@ -128,6 +128,7 @@ for _n in ("fwd", "bwd"):
     PROTOTYPES["mnv_gated_ffn_%s_workspace_bytes" % _n] = [_I] * 3
 PROTOTYPES["mnv_gated_ffn_fwd"] = [_P] * 6 + [_I] * 4 + [_P, c_sz, _S]
 PROTOTYPES["mnv_gated_ffn_bwd"] = [_P] * 10 + [_I] * 4 + [_P, c_sz, _S]
+PROTOTYPES["mnv_gated_ffn_pairs_mode"] = [_I]
 PROTOTYPES["mnv_gated_ffn_plan"] = [_I] * 3 + [c_sz, c_sz, _P]
 PROTOTYPES["mnv_adamw_moment_floats"] = [c_sz, _I]
 PROTOTYPES["mnv_adamw_step"] = [_I] + [_P] * 10 + [_I] + [c_d] * 6 + [_I, _P, _S]

@@ -10,6 +10,7 @@
 // Both passes: 8192 tokens of 2048 -> 5632 5.0 ms (340 TFLOP/s), 4096 of 1024 -> 2816 0.90 ms (236); forward: 777 of 1001 -> 2731
 // 110 us (115), 4 of 1024 -> 4096 23 us (50 MB of weights, 2.2 TB/s over four launches).
 #include <algorithm>
+#include <atomic>
 
 #include "few_gemm.h"
 #include "pair_gemm.h"
@@ -401,7 +402,9 @@ Product product_dw(const float* left, const float* right, int rows, int columns,
 // them last (both passes, without / with that: 4096 tokens of 1024 -> 2816 955 / 936, 500 of 4096 -> 8192 1511 / 1462).  It is one of a plain
 // product: what the store moves beyond 4 bytes comes on top (without / with: 8192 of 768 -> 2048 1089 / 1041, 16384 of 512 -> 2048 1580 / 1512).  us, both passes, in pairs never / so: 4096 tokens
 // of 1024 -> 2816 1212 / 958, 1024 of 2048 -> 5632 1203 / 921, 8192 of 2048 -> 5632 8360 / 5120, 300 of 4096 -> 8192 1202 / 1100 (all in pairs 1240).
+std::atomic<int> g_pairs{1};  // mnv_gated_ffn_pairs_mode
 bool in_pairs(const Product& p, int most_ranges, size_t ws_bytes, PairPlan* plan) {
+  if (!g_pairs.load(std::memory_order_relaxed)) return false;
   // below 5 GFLOP the four launches of the packing alone take half of the time
   if (!pair_fits(p.a, p.b) || 2.0 * p.a.rows * p.b.rows * p.a.k < 5e9) return false;
   const int cus = mnv_cu_count();
@@ -521,6 +524,11 @@ int mnv_gated_ffn_fwd(const float* x, const float* w_in, const float* w_out, flo
                                          : launch_gated_in<false>(plan, w_in, x, pre, h, features, hidden, tokens, activation, ws, bytes, s);
   }
   return rc ? rc : product_y();
+}
+
+int mnv_gated_ffn_pairs_mode(int mode) {
+  if (mode < 0 || mode > 1) return g_pairs.load(std::memory_order_relaxed);
+  return g_pairs.exchange(mode, std::memory_order_relaxed);
 }
 
 int mnv_gated_ffn_plan(int features, int hidden, int tokens, size_t fwd_workspace_bytes, size_t bwd_workspace_bytes, int* pairs) {

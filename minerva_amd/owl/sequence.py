@@ -89,7 +89,8 @@ class gate(object):
 
 class GatedFFN(object):
     """w_out (act(w_gate x) * (w_up x)) for x {features, tokens}, w_in {2 hidden, features} (the gate's rows first) and
-    w_out {features, hidden}."""
+    w_out {features, hidden}.  Large products hold 22 bits of their factors' values, or 2^-39 of the largest in a row, unless
+    `capi.lib().mnv_gated_ffn_pairs_mode(0)` switches that off for the process."""
 
     def __init__(self, activation=gate.silu):
         self.activation = int(activation)
