@@ -491,7 +491,8 @@ int mnv_rotary_bwd(const float* dy, const float* positions, float* dx, int head_
  *   pre = w_in x {2 hidden, tokens},  h = act(pre_gate) * pre_up {hidden, tokens},  y = w_out h
  *   dh = w_out' dy,  dpre = (dh * pre_up * act'(pre_gate), dh * act(pre_gate))
  *   dx = w_in' dpre,  dw_in = dpre x',  dw_out = dy h'
- * activation: 0 sigmoid, 1 relu (slope 0 at 0; a NaN and its slope are NaN, where mnv_relu_fwd gives 0), 2 tanh, 3 silu x / (1 + exp(-x)), 4 gelu x Phi(x) with the normal distribution's Phi.
+ * activation: 0 sigmoid, 1 relu (slope 0 at 0; a NaN and its slope are NaN, where mnv_relu_fwd gives 0), 2 tanh,
+ * 3 silu x / (1 + exp(-x)), 4 gelu x Phi(x) with the normal distribution's Phi.
  * forward writes h, and pre unless it is NULL (no backward pass follows); backward reads both, and writes dpre, which
  * may be pre itself; dx may be NULL if nobody needs it.  Each matrix holds less than 2^29 values.
  * A workspace is used if it is aligned to 16 bytes.  Without one, pre == NULL costs few tokens more time.

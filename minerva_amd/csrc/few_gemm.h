@@ -16,9 +16,10 @@ constexpr int FEW_ROWS = 64, FEW_K = 16, FEW_WAVES = 8;
 // LDS, a fetch of an x-fast A brings 256 bytes of a column together, and a lane's sums are four neighbouring rows.
 // Two workgroups fit on a CU with up to 128 registers a lane: sums, and the fetches of 4, 3 or 2 steps, which are in flight under the
 // steps before (with three steps' and 141 registers for 32 columns, and so one workgroup: 2 x 5632 x 2048 for 150 columns 88 -> 103 us).
-// Measured as the projections of a gated block (and what adds the ranges), 2 x 5632 rows, 2048 k, against the SGEMM's plans: 6 / 16 / 32 / 48 / 64
-// columns 23 / 23 / 28 / 34 / 42 us, 49 / 48 / 56 / 63 from 16 on; 92 MB, i.e. 4.0 TB/s up to 16 columns.  From 32 on the matrix
-// instruction, at 0.7 of its rate, and how the workgroups divide on the CUs bound it.
+// Measured as the projections of a gated block, 2 x 5632 rows, 2048 k, with the weights read from HBM (four of them in turn, 369 MB), this
+// kernel and the SGEMM's small tiles, which leave the gate to another 3 us: 13 / 16 / 32 / 48 / 64 columns 26 / 27 / 35 / 40 / 53 us (up to 16 in k
+// ranges, and 5 to add and gate them) and 37 / 38 / 35 / 40 / 47; 92 MB, i.e. 3.5 TB/s up to 16 columns.  From 32 on the matrix instruction, at 0.7 of its rate,
+// and how the workgroups divide on the CUs bound it.
 template <class P, int COLS>
 __global__ __launch_bounds__(FEW_WAVES * MNV_WAVE, 4) void few_gemm_kernel(P prob, int blocks_m, int blocks_n, int ranges, int per_range,
                                                                               float* __restrict__ partial) {
